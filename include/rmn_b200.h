@@ -614,6 +614,90 @@ int rmn_bn_backward_coeffs(const double *d_dots, const float *d_mean, const floa
 int rmn_affine2(const void *d_a, const void *d_b, uint32_t n_rows, int channels, const float *d_c_a,
                 const float *d_c_b, const float *d_c_0, void *d_out, int dtype, void *stream);
 
+/* ------------------- layer norm over the channels of every row -------------------
+ * Replaces: torch's layer norm on the feature matrix (the reference's wrapper stands beside its batch norm,
+ * engine/nn/normalization.hpp). */
+
+/*
+ * out[r][c] = (x[r][c] - mean[r]) * inv[r] * gamma[c] + beta[c], inv = 1 / sqrt(var + eps), var the mean of the squared
+ * distances from the mean (biased); statistics in fp32. Rows of x lie ld_x elements apart, out is [n_rows, channels] without
+ * gaps (in place where d_out == d_x and ld_x == channels). gamma and beta (param_dtype; NULL: 1 and 0). d_mean and d_inv
+ * [n_rows] are what the backward pass needs (both NULL: not written). RMN_ERR_UNSUPPORTED beyond 4096 channels (16384 in fp32,
+ * 32768 in bf16 where channels, ld_x and the pointers are multiples of 16 bytes).
+ */
+int rmn_layer_norm_forward(const void *d_x, int64_t ld_x, uint32_t n_rows, int channels, const void *d_gamma,
+                           const void *d_beta, int param_dtype, float eps, void *d_out, float *d_mean, float *d_inv,
+                           int dtype, void *stream);
+/* Scratch bytes of rmn_layer_norm_backward. */
+size_t rmn_layer_norm_backward_workspace_bytes(uint32_t n_rows, int channels);
+/*
+ * Gradients of rmn_layer_norm_forward: d_dx [n_rows, channels], d_dgamma and d_dbeta [channels] (param_dtype, summed in
+ * fp32 and rounded once); each may be NULL. dy and x rows ld_dy and ld_x apart (0: one row for all). The same bits every time.
+ * d_dx may be d_dy where ld_dy == channels. RMN_ERR_UNSUPPORTED as the forward pass, and for dgamma / dbeta beyond 25600
+ * channels. d_workspace: 16-byte aligned.
+ */
+int rmn_layer_norm_backward(const void *d_dy, int64_t ld_dy, const void *d_x, int64_t ld_x, uint32_t n_rows, int channels,
+                            const void *d_gamma, int param_dtype, const float *d_mean, const float *d_inv, void *d_dx,
+                            void *d_dgamma, void *d_dbeta, int dtype, void *d_workspace, size_t workspace_bytes,
+                            void *stream);
+
+/* ------------------- attention within the samples of a batch -------------------
+ * The rows of the samples lie one behind the other in one matrix; every sample attends within itself. No counterpart in the
+ * reference. */
+
+/* Scratch bytes of rmn_sample_offsets. */
+size_t rmn_sample_offsets_workspace_bytes(uint32_t n_samples);
+/*
+ * Row ranges of the samples of a coordinate map whose rows of one batch index are adjacent: d_offsets[s] = first row of the
+ * s-th sample in row order, d_offsets[n_samples] = n_rows, and d_offsets[n_samples + 1] = the number of runs of equal batch
+ * indices (n_samples + 2 words in all). Rows are adjacent when that number is n_samples, the count of distinct batch indices;
+ * otherwise the offsets are of no use.
+ */
+int rmn_sample_offsets(const int32_t *d_coords, uint32_t n_rows, int W, uint32_t n_samples, int32_t *d_offsets,
+                       void *d_workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * One attention problem. q is [rows_q, heads, dim], k and v are [rows_k, kv_heads, dim]; channels are adjacent, rows and
+ * heads lie *_row and *_head elements apart (>= 0; 0 broadcasts). Query head h attends with key head h / (heads / kv_heads).
+ * Sample s owns query rows offsets[s] ... offsets[s + 1] - 1 and key rows kv_offsets[s] ... kv_offsets[s + 1] - 1 (device
+ * arrays [sequences + 1], ascending; kv_offsets NULL: offsets, and rows_k == rows_q then); where kv_lengths [sequences] is
+ * given, only its first kv_lengths[s] key rows are in use (a cache with room behind what it holds) and the others are never
+ * read as keys. causal: aligned at the end, query i of n sees keys 0 ... i + m - n of m. scale multiplies the scores.
+ * Offsets or lengths that do not ascend or leave the tensors are clamped to them and reported as RMN_ERR_BAD_ARG by
+ * rmn_device_status. dim <= 256 (RMN_ERR_UNSUPPORTED beyond).
+ */
+typedef struct {
+  const void *q, *k, *v;
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head;
+  uint32_t rows_q, rows_k, sequences;
+  int heads, kv_heads, dim;
+  const int32_t *offsets, *kv_offsets, *kv_lengths;
+  int causal, dtype;
+  float scale;
+} rmn_attention;
+
+/* Scratch bytes of rmn_attention_forward (may be 0). Depends on sizes only. */
+size_t rmn_attention_forward_workspace_bytes(const rmn_attention *problem);
+/*
+ * out[i, h] = sum_j softmax_j(scale q[i, h] . k[j, h']) v[j, h'] over the keys that row i sees: [rows_q, heads, dim] without
+ * gaps. A row that sees no key, and a row of no sample, is zero. d_lse [heads, rows_q] (may be NULL): logarithm of the sum of
+ * exponentials, -infinity for such a row; the backward pass needs it. Sums and softmax in fp32. A non-finite value in a
+ * row of k or v may reach every row of its own sample and head, never those of another. The workspace may be shared by calls on one
+ * stream, not by calls that run at the same time.
+ */
+int rmn_attention_forward(const rmn_attention *problem, void *d_out, float *d_lse, void *d_workspace, size_t workspace_bytes,
+                          void *stream);
+/* Scratch bytes of rmn_attention_backward. Depends on sizes only. */
+size_t rmn_attention_backward_workspace_bytes(const rmn_attention *problem);
+/*
+ * Gradients of rmn_attention_forward from its outputs (d_out, d_lse) and d_grad_out (rows and heads grad_row and grad_head
+ * elements apart): dq [rows_q, heads, dim], dk and dv [rows_k, kv_heads, dim] without gaps, summed over the query heads that share
+ * a key head; zeros in rows of no sample and in key rows not in use. No atomics: the same bits every time. d_workspace: 16-byte aligned.
+ */
+int rmn_attention_backward(const rmn_attention *problem, const void *d_out, const float *d_lse, const void *d_grad_out,
+                           int64_t grad_row, int64_t grad_head, void *d_dq, void *d_dk, void *d_dv, void *d_workspace,
+                           size_t workspace_bytes, void *stream);
+
 /* ------------------- weight-gradient all-reduce (data-parallel training) -------------------
  * Batches shard by sample: every rank hashes, maps and convolves its own samples, and the one
  * collective of a training step is the sum of the fp32 weight gradients over the ranks (NCCL over

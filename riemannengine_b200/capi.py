@@ -109,6 +109,18 @@ SIGNATURES = {
                                        c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
     "rmn_affine2": (c_int, [c_void_p, c_void_p, c_uint32, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
                             c_void_p]),
+    "rmn_layer_norm_forward": (c_int, [c_void_p, c_int64, c_uint32, c_int, c_void_p, c_void_p, c_int, ctypes.c_float,
+                                       c_void_p, c_void_p, c_void_p, c_int, c_void_p]),
+    "rmn_layer_norm_backward_workspace_bytes": (c_size_t, [c_uint32, c_int]),
+    "rmn_layer_norm_backward": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_uint32, c_int, c_void_p, c_int, c_void_p,
+                                        c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_size_t, c_void_p]),
+    "rmn_sample_offsets_workspace_bytes": (c_size_t, [c_uint32]),
+    "rmn_sample_offsets": (c_int, [c_void_p, c_uint32, c_int, c_uint32, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "rmn_attention_forward_workspace_bytes": (c_size_t, [c_void_p]),
+    "rmn_attention_forward": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "rmn_attention_backward_workspace_bytes": (c_size_t, [c_void_p]),
+    "rmn_attention_backward": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p,
+                                       c_void_p, c_void_p, c_size_t, c_void_p]),
     "rmn_comm_unique_id": (c_int, [c_void_p]),
     "rmn_comm_init": (c_int, [c_void_p, c_int, c_int, c_void_p]),
     "rmn_comm_destroy": (c_int, [c_void_p]),
@@ -130,6 +142,17 @@ SIGNATURES = {
     "rmn_pool_backward": (c_int, [c_void_p, c_uint32, c_int, c_void_p, c_int, c_uint32, c_int, c_void_p, c_void_p,
                                   c_int, c_void_p]),
 }
+
+
+class Attention(ctypes.Structure):
+    """rmn_attention of the header."""
+    _fields_ = ([(name, c_void_p) for name in ("q", "k", "v")]
+                + [(name, c_int64) for name in ("q_row", "q_head", "k_row", "k_head", "v_row", "v_head")]
+                + [(name, c_uint32) for name in ("rows_q", "rows_k", "sequences")]
+                + [(name, c_int) for name in ("heads", "kv_heads", "dim")]
+                + [(name, c_void_p) for name in ("offsets", "kv_offsets", "kv_lengths")]
+                + [("causal", c_int), ("dtype", c_int), ("scale", ctypes.c_float)])
+
 
 _lib = None
 

@@ -1,0 +1,154 @@
+// C-ABI entry points of attention within packed samples: argument checks and the choice of the kernel; and the row ranges of
+// the samples of a coordinate map.
+#include "rmn_attention.cuh"
+
+namespace rmn {
+
+const uint32_t* tc_status_device_address();  // defined in rmn_conv_tc.cu
+
+namespace {
+
+// Runs of equal batch indices: the first row of every run, in any order, and their number.
+__global__ void __launch_bounds__(256) k_sample_runs(const int32_t* __restrict__ coords, uint32_t n, int W, uint32_t most,
+                                                     int32_t* __restrict__ starts, uint32_t* __restrict__ count) {
+  after_previous_kernel();
+  for (uint32_t i = blockIdx.x * blockDim.x + threadIdx.x; i < n; i += gridDim.x * blockDim.x) {
+    if (i > 0 && __ldg(coords + (size_t)i * W) == __ldg(coords + (size_t)(i - 1) * W)) continue;
+    const uint32_t at = atomicAdd(count, 1u);
+    if (at < most) starts[at] = (int32_t)i;
+  }
+}
+// offsets = the starts in ascending order, then n, then the number of runs
+__global__ void __launch_bounds__(1024) k_sample_offsets(const int32_t* __restrict__ starts, const uint32_t* __restrict__ count,
+                                                         uint32_t n, uint32_t most, int32_t* __restrict__ offsets) {
+  after_previous_kernel();
+  const uint32_t runs = *count, have = min(runs, most);
+  for (uint32_t i = threadIdx.x; i < most; i += blockDim.x) {
+    if (i >= have) {
+      offsets[i] = (int32_t)n;
+      continue;
+    }
+    const int32_t mine = starts[i];
+    uint32_t rank = 0;
+    for (uint32_t j = 0; j < have; ++j) rank += starts[j] < mine ? 1u : 0u;
+    offsets[rank] = mine;
+  }
+  if (threadIdx.x == 0) {
+    offsets[most] = (int32_t)n;
+    offsets[most + 1] = (int32_t)min(runs, 0x7fffffffu);
+  }
+}
+
+bool stride_ok(int64_t s) { return s >= 0 && s <= (int64_t(1) << 40); }
+
+// the problem as the kernels take it; RMN_OK or what is wrong with it
+int arguments(const rmn_attention* p, AttnArgs* a) {
+  if (!p) return RMN_ERR_BAD_ARG;
+  if (p->heads < 1 || p->kv_heads < 1 || p->heads > 65536 || p->heads % p->kv_heads || p->dim < 1 ||
+      (p->dtype != RMN_F32 && p->dtype != RMN_BF16) || p->rows_q > 0x7fffffffu || p->rows_k > 0x7fffffffu ||
+      p->sequences > 0x7ffffffdu || !p->offsets)
+    return RMN_ERR_BAD_ARG;
+  if (p->dim > 256) return RMN_ERR_UNSUPPORTED;
+  const int64_t strides[6] = {p->q_row, p->q_head, p->k_row, p->k_head, p->v_row, p->v_head};
+  for (int64_t s : strides)
+    if (!stride_ok(s)) return RMN_ERR_BAD_ARG;
+  if ((p->rows_q && !p->q) || (p->rows_k && (!p->k || !p->v))) return RMN_ERR_BAD_ARG;
+  if (!p->kv_offsets && p->rows_k != p->rows_q) return RMN_ERR_BAD_ARG;
+  if (!(p->scale == p->scale)) return RMN_ERR_BAD_ARG;
+  *a = {};
+  a->q = p->q; a->k = p->k; a->v = p->v;
+  a->q_row = p->q_row; a->q_head = p->q_head;
+  a->k_row = p->k_row; a->k_head = p->k_head;
+  a->v_row = p->v_row; a->v_head = p->v_head;
+  a->rows_q = p->rows_q; a->rows_k = p->rows_k; a->sequences = p->sequences;
+  a->heads = p->heads; a->kv_heads = p->kv_heads; a->dim = p->dim;
+  a->offsets = p->offsets;
+  a->kv_offsets = p->kv_offsets ? p->kv_offsets : p->offsets;
+  a->kv_lengths = p->kv_lengths;
+  a->causal = p->causal != 0;
+  a->scale = p->scale;
+  a->status = const_cast<uint32_t*>(tc_status_device_address());
+  return a->status ? RMN_OK : RMN_ERR_CUDA;
+}
+
+}  // namespace
+}  // namespace rmn
+
+using namespace rmn;
+
+extern "C" size_t rmn_sample_offsets_workspace_bytes(uint32_t n_samples) { return ((size_t)n_samples + 4) * sizeof(int32_t); }
+
+extern "C" int rmn_sample_offsets(const int32_t* d_coords, uint32_t n_rows, int W, uint32_t n_samples, int32_t* d_offsets,
+                                  void* d_workspace, size_t workspace_bytes, void* stream_) {
+  cudaStream_t stream = (cudaStream_t)stream_;
+  if (W < 2 || W > RMN_MAX_W || n_rows > 0x7fffffffu || n_samples > 0x7ffffff0u || !d_offsets || !d_workspace ||
+      (n_rows && !d_coords) || ((uintptr_t)d_workspace & 3))
+    return RMN_ERR_BAD_ARG;
+  if (workspace_bytes < rmn_sample_offsets_workspace_bytes(n_samples)) return RMN_ERR_ALLOC;
+  uint32_t* count = static_cast<uint32_t*>(d_workspace);
+  int32_t* starts = reinterpret_cast<int32_t*>(count + 4);
+  RMN_CUDA_TRY(cudaMemsetAsync(count, 0, sizeof(uint32_t), stream));
+  if (n_rows) {
+    const uint64_t want = ((uint64_t)n_rows + 255) / 256;
+    const uint32_t grid = (uint32_t)(want < 148 * 8 ? want : 148 * 8);
+    RMN_CUDA_TRY(launch_overlapped(k_sample_runs, dim3(grid), dim3(256), 0, stream, d_coords, n_rows, W, n_samples, starts, count));
+    RMN_LAUNCH_CHECK();
+  }
+  RMN_CUDA_TRY(launch_overlapped(k_sample_offsets, dim3(1), dim3(1024), 0, stream, static_cast<const int32_t*>(starts),
+                                 static_cast<const uint32_t*>(count), n_rows, n_samples, d_offsets));
+  RMN_LAUNCH_CHECK();
+  return RMN_OK;
+}
+
+extern "C" size_t rmn_attention_forward_workspace_bytes(const rmn_attention* problem) {
+  (void)problem;
+  return 0;
+}
+
+extern "C" int rmn_attention_forward(const rmn_attention* problem, void* d_out, float* d_lse, void* d_workspace,
+                                     size_t workspace_bytes, void* stream_) {
+  (void)d_workspace;
+  (void)workspace_bytes;
+  AttnArgs a;
+  const int st = arguments(problem, &a);
+  if (st != RMN_OK) return st;
+  if (a.rows_q == 0) return RMN_OK;
+  if (!d_out) return RMN_ERR_BAD_ARG;
+  a.out = d_out;
+  a.lse = d_lse;
+  return attention_simt_forward(a, problem->dtype, (cudaStream_t)stream_);
+}
+
+extern "C" size_t rmn_attention_backward_workspace_bytes(const rmn_attention* problem) {
+  return problem && problem->heads > 0 ? (size_t)problem->heads * problem->rows_q * sizeof(float) : 0;
+}
+
+extern "C" int rmn_attention_backward(const rmn_attention* problem, const void* d_out, const float* d_lse,
+                                      const void* d_grad_out, int64_t grad_row, int64_t grad_head, void* d_dq, void* d_dk,
+                                      void* d_dv, void* d_workspace, size_t workspace_bytes, void* stream_) {
+  cudaStream_t stream = (cudaStream_t)stream_;
+  AttnArgs a;
+  const int st = arguments(problem, &a);
+  if (st != RMN_OK) return st;
+  if ((a.rows_q && !d_dq) || (a.rows_k && (!d_dk || !d_dv)) || !stride_ok(grad_row) || !stride_ok(grad_head))
+    return RMN_ERR_BAD_ARG;
+  const size_t elem = problem->dtype == RMN_F32 ? 4 : 2;
+  if (a.rows_q == 0 || a.rows_k == 0) {  // nothing attends to anything
+    if (a.rows_q) RMN_CUDA_TRY(cudaMemsetAsync(d_dq, 0, (size_t)a.rows_q * a.heads * a.dim * elem, stream));
+    if (a.rows_k) {
+      RMN_CUDA_TRY(cudaMemsetAsync(d_dk, 0, (size_t)a.rows_k * a.kv_heads * a.dim * elem, stream));
+      RMN_CUDA_TRY(cudaMemsetAsync(d_dv, 0, (size_t)a.rows_k * a.kv_heads * a.dim * elem, stream));
+    }
+    return RMN_OK;
+  }
+  if (!d_out || !d_lse || !d_grad_out || !d_workspace || ((uintptr_t)d_workspace & 15)) return RMN_ERR_BAD_ARG;
+  if (workspace_bytes < rmn_attention_backward_workspace_bytes(problem)) return RMN_ERR_ALLOC;
+  a.fwd_out = d_out;
+  a.lse = const_cast<float*>(d_lse);
+  a.grad = d_grad_out;
+  a.grad_row = grad_row;
+  a.grad_head = grad_head;
+  a.delta = static_cast<float*>(d_workspace);
+  a.dq = d_dq; a.dk = d_dk; a.dv = d_dv;
+  return attention_simt_backward(a, problem->dtype, stream);
+}

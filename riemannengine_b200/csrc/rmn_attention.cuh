@@ -1,0 +1,142 @@
+// What the attention kernels share: the arguments as the kernels take them, the samples' row ranges, and the search of the
+// tile of rows that a block works on.
+#pragma once
+
+#include "rmn_common.cuh"
+
+#include <cuda_bf16.h>
+
+namespace rmn {
+
+// One attention problem, as rmn_attention describes it, with what backward passes add.
+struct AttnArgs {
+  const void *q, *k, *v;
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head;  // strides in elements
+  uint32_t rows_q, rows_k, sequences;
+  int heads, kv_heads, dim;
+  const int32_t *offsets, *kv_offsets, *kv_lengths;     // kv_offsets never NULL here
+  int causal;
+  float scale;                                          // of the scores
+  uint32_t* status;                                     // device status word
+  void* out;                                            // [rows_q, heads, dim]
+  float* lse;                                           // [heads, rows_q], natural logarithm (forward: may be NULL)
+  // backward
+  const void* grad;                                     // of the output
+  int64_t grad_row, grad_head;
+  const void* fwd_out;
+  float* delta;                                         // [heads, rows_q]: sum over the channels of grad * out
+  void *dq, *dk, *dv;                                   // contiguous
+};
+
+// Row ranges of one sample. Every row of the tensors belongs to exactly one segment: segments 0 ... S - 1 are the samples,
+// segment S the rows behind the last sample and S + 1 those before the first; the last two have no keys to attend to, so that
+// their outputs come out as zeros by the same code.
+struct Segment {
+  int32_t q0, n_q;    // query rows
+  int32_t k0, n_k;    // key rows in use
+  int32_t k_slot;     // key rows from k0 to the next sample's
+};
+
+__device__ __forceinline__ int32_t clamp_row(int32_t v, uint32_t rows) { return max(0, min(v, (int32_t)rows)); }
+
+// Offsets that do not ascend or leave the tensor are set right here, so that no row outside the tensors is touched whatever
+// they say, and recorded in the status word.
+__device__ __forceinline__ Segment segment(const AttnArgs& a, uint32_t s) {
+  Segment g;
+  const uint32_t S = a.sequences;
+  if (s > S) {
+    g.q0 = 0;
+    g.n_q = clamp_row(a.offsets[0], a.rows_q);
+    g.k0 = 0;
+    g.k_slot = clamp_row(a.kv_offsets[0], a.rows_k);
+    g.n_k = 0;
+    return g;
+  }
+  const int32_t q_lo = a.offsets[s], k_lo = a.kv_offsets[s];
+  const int32_t q_hi = s < S ? a.offsets[s + 1] : (int32_t)a.rows_q, k_hi = s < S ? a.kv_offsets[s + 1] : (int32_t)a.rows_k;
+  g.q0 = clamp_row(q_lo, a.rows_q);
+  g.k0 = clamp_row(k_lo, a.rows_k);
+  g.n_q = max(0, clamp_row(q_hi, a.rows_q) - g.q0);
+  g.k_slot = max(0, clamp_row(k_hi, a.rows_k) - g.k0);
+  bool bad = q_lo < 0 || q_hi < q_lo || q_hi > (int32_t)a.rows_q || k_lo < 0 || k_hi < k_lo || k_hi > (int32_t)a.rows_k;
+  g.n_k = s < S ? g.k_slot : 0;
+  if (s < S && a.kv_lengths) {
+    const int32_t len = a.kv_lengths[s];
+    bad = bad || len < 0 || len > g.k_slot;
+    g.n_k = max(0, min(len, g.k_slot));
+  }
+  if (bad) atomicMax(a.status, (uint32_t)RMN_ERR_BAD_ARG);
+  return g;
+}
+
+// Keys that query row i of a segment attends to are 0 ... visible(i) - 1: all, or (causal, aligned at the end) those up to
+// its own place.
+__device__ __forceinline__ int32_t visible_keys(const Segment& g, int32_t i, int causal) {
+  return causal ? max(0, min(g.n_k, i + 1 + g.n_k - g.n_q)) : g.n_k;
+}
+// The first query row that attends to key j.
+__device__ __forceinline__ int32_t first_query(const Segment& g, int32_t j, int causal) {
+  return causal ? max(0, j - (g.n_k - g.n_q)) : 0;
+}
+
+// Tiles of `tile_rows` rows of all segments, one behind the other: finds the segment of tile `want` and the tile's number in
+// it; false where there are no so many tiles. kKeys: tiles of key rows (the whole slots), else of query rows. All threads
+// of the block call it (kThreads of them); `found` is shared memory. Every thread counts the tiles of a run of
+// segments, a scan over the block places them.
+struct FoundTile {
+  Segment g;
+  int32_t tile, tiles;  // number of the tile in its segment, and the segment's tiles
+};
+template <int kThreads, bool kKeys>
+__device__ __forceinline__ bool find_tile(const AttnArgs& a, uint32_t want, int tile_rows, FoundTile* found, int32_t* warp_sums) {
+  const uint32_t n = a.sequences + 2;
+  const uint32_t per = (n + kThreads - 1) / kThreads;
+  const uint32_t lo = threadIdx.x * per, hi = min(lo + per, n);
+  int32_t mine = 0;
+  Segment g = {};
+  for (uint32_t s = lo; s < hi; ++s) {
+    g = segment(a, s);
+    mine += ((kKeys ? g.k_slot : g.n_q) + tile_rows - 1) / tile_rows;
+  }
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int32_t upto = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int32_t t = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += t;
+  }
+  if (lane == 31) warp_sums[warp] = upto;
+  __syncthreads();
+  int32_t before = 0, total = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w < warp) before += warp_sums[w];
+    total += warp_sums[w];
+  }
+  const bool exists = want < (uint32_t)total;
+  int32_t first = before + upto - mine;
+  if (exists && (int32_t)want >= first && (int32_t)want < first + mine) {
+    for (uint32_t s = lo; s < hi; ++s) {
+      if (per > 1) g = segment(a, s);
+      const int32_t tiles = ((kKeys ? g.k_slot : g.n_q) + tile_rows - 1) / tile_rows;
+      if ((int32_t)want < first + tiles) {
+        found->g = g;
+        found->tile = (int32_t)want - first;
+        found->tiles = tiles;
+        break;
+      }
+      first += tiles;
+    }
+  }
+  __syncthreads();
+  return exists;
+}
+
+// How many tiles find_tile may be asked for at most: with valid offsets every segment's last tile may be a part of one.
+inline uint64_t most_tiles(uint64_t rows, uint64_t sequences, uint32_t tile_rows) { return rows / tile_rows + sequences + 2; }
+
+// The kernels behind rmn_attention_*: RMN_ERR_UNSUPPORTED where they do not cover the call.
+int attention_simt_forward(const AttnArgs& a, int dtype, cudaStream_t stream);
+int attention_simt_backward(const AttnArgs& a, int dtype, cudaStream_t stream);
+
+}  // namespace rmn

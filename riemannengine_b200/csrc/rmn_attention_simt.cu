@@ -1,0 +1,409 @@
+// Attention within packed samples by multiply-adds in fp32: every type, head size up to 256, stride and alignment.
+//
+// Forward: a block takes BM query rows of one head and walks over the keys they see, BM at a time, with the running maximum m
+// and sum l of each row's softmax: scores s = scale q k^T, m' = max(m, max s), p = exp(s - m'), l = l exp(m - m') + sum p,
+// o = o exp(m - m') + p v; at the end o / l and lse = m + log l. Nothing of the scores reaches memory.
+// Backward, without atomics: one kernel per query tile (delta = sum grad * out, dq = scale sum ds k) and one per key tile
+// (dv = sum p^T grad, dk = scale sum ds^T q over the query heads that share the key head), p = exp(s - lse),
+// ds = p * (grad v^T - delta); each makes the scores anew, which costs 7 products where 5 would do, and every gradient is
+// written once, in a fixed order of sums.
+//
+// Bound by the multiply-adds' operands in shared memory: a thread's 4 x 4 outputs take 8 16-byte reads per 64 multiply-adds; rows
+// are padded by 16 bytes, and a thread's columns are 16 apart, so that the reads of a warp meet no bank twice.
+#include "rmn_attention.cuh"
+
+#include <math_constants.h>
+
+namespace rmn {
+namespace {
+
+constexpr int kSimtThreads = 256;  // 16 x 16 threads over a tile
+
+template <int DP, int BM>
+struct SimtShape {
+  static constexpr int R = BM / 16;                 // rows, and columns of scores, of a thread
+  static constexpr int CW = DP >= 64 ? 4 : DP / 16; // neighbouring channels of a thread
+  static constexpr int NC = DP / (16 * CW);         // groups of them, 16 CW apart
+  static constexpr int LD = DP + 4, LP = BM + 4;
+  static constexpr size_t tile = (size_t)BM * LD * sizeof(float), square = (size_t)BM * LP * sizeof(float);
+};
+
+__device__ __forceinline__ float load_f32(const float* p) { return __ldg(p); }
+__device__ __forceinline__ float load_f32(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+__device__ __forceinline__ void store_f32(float* p, float v) { *p = v; }
+__device__ __forceinline__ void store_f32(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+
+// rows [0, n) of `from` (rows `row` elements apart) as fp32 into dst [BM][LD], times `scale`; zeros behind them and behind `dim`
+template <typename T, int DP, int BM>
+__device__ __forceinline__ void load_tile(float* dst, const T* from, int64_t row, int n, int dim, float scale) {
+  constexpr int LD = SimtShape<DP, BM>::LD, Q = DP / 4;
+  const bool wide = ((uintptr_t)from % (4 * sizeof(T))) == 0 && row % 4 == 0 && dim % 4 == 0;
+  for (int i = threadIdx.x; i < BM * Q; i += kSimtThreads) {
+    const int r = i / Q, c = (i % Q) * 4;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (r < n && c < dim) {
+      const T* p = from + (int64_t)r * row + c;
+      if (wide) {
+        if constexpr (sizeof(T) == 4) {
+          v = __ldg(reinterpret_cast<const float4*>(p));
+        } else {
+          const uint2 w = __ldg(reinterpret_cast<const uint2*>(p));
+          const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w.x));
+          const float2 b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w.y));
+          v = make_float4(a.x, a.y, b.x, b.y);
+        }
+      } else {
+        v.x = load_f32(p);
+        if (c + 1 < dim) v.y = load_f32(p + 1);
+        if (c + 2 < dim) v.z = load_f32(p + 2);
+        if (c + 3 < dim) v.w = load_f32(p + 3);
+      }
+    }
+    v.x *= scale; v.y *= scale; v.z *= scale; v.w *= scale;
+    *reinterpret_cast<float4*>(dst + r * LD + c) = v;
+  }
+}
+
+// s[i][j] = row (ty + 16 i) of a times row (tx + 16 j) of b
+template <int DP, int BM, int R = SimtShape<DP, BM>::R>
+__device__ __forceinline__ void product_rows(const float* a, const float* b, int tx, int ty, float (&s)[R][R]) {
+  constexpr int LD = SimtShape<DP, BM>::LD;
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+#pragma unroll
+    for (int j = 0; j < R; ++j) s[i][j] = 0.f;
+#pragma unroll 4
+  for (int c = 0; c < DP; c += 4) {
+    float4 x[R], y[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) x[i] = *reinterpret_cast<const float4*>(a + (ty + 16 * i) * LD + c);
+#pragma unroll
+    for (int j = 0; j < R; ++j) y[j] = *reinterpret_cast<const float4*>(b + (tx + 16 * j) * LD + c);
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+      for (int j = 0; j < R; ++j) {
+        s[i][j] = fmaf(x[i].x, y[j].x, s[i][j]);
+        s[i][j] = fmaf(x[i].y, y[j].y, s[i][j]);
+        s[i][j] = fmaf(x[i].z, y[j].z, s[i][j]);
+        s[i][j] = fmaf(x[i].w, y[j].w, s[i][j]);
+      }
+  }
+}
+
+// o[i][channels of the thread] += sum_j p[ty + 16 i][j] b[j][channels], j < n rounded up to 4 (zeros there)
+template <int DP, int BM, int R = SimtShape<DP, BM>::R, int NC = SimtShape<DP, BM>::NC, int CW = SimtShape<DP, BM>::CW>
+__device__ __forceinline__ void product_columns(const float* p, const float* b, int n, int tx, int ty, float (&o)[R][NC][CW]) {
+  constexpr int LD = SimtShape<DP, BM>::LD, LP = SimtShape<DP, BM>::LP;
+  for (int j = 0; j < n; j += 4) {
+    float4 w[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) w[i] = *reinterpret_cast<const float4*>(p + (ty + 16 * i) * LP + j);
+#pragma unroll
+    for (int jj = 0; jj < 4; ++jj) {
+      const float* row = b + (j + jj) * LD + tx * CW;
+#pragma unroll
+      for (int g = 0; g < NC; ++g) {
+        float y[CW];
+#pragma unroll
+        for (int e = 0; e < CW; ++e) y[e] = row[g * 16 * CW + e];
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+          const float f = jj == 0 ? w[i].x : jj == 1 ? w[i].y : jj == 2 ? w[i].z : w[i].w;
+#pragma unroll
+          for (int e = 0; e < CW; ++e) o[i][g][e] = fmaf(f, y[e], o[i][g][e]);
+        }
+      }
+    }
+  }
+}
+
+// o times `by` into rows [0, n) of `to`, `row` elements apart
+template <typename T, int DP, int BM, int R = SimtShape<DP, BM>::R, int NC = SimtShape<DP, BM>::NC, int CW = SimtShape<DP, BM>::CW>
+__device__ __forceinline__ void store_tile(T* to, int64_t row, int n, int dim, int tx, int ty, const float (&o)[R][NC][CW],
+                                           const float (&by)[R]) {
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    if (ty + 16 * i >= n) continue;
+#pragma unroll
+    for (int g = 0; g < NC; ++g)
+#pragma unroll
+      for (int e = 0; e < CW; ++e) {
+        const int c = g * 16 * CW + tx * CW + e;
+        if (c < dim) store_f32(to + (int64_t)(ty + 16 * i) * row + c, o[i][g][e] * by[i]);
+      }
+  }
+}
+
+template <typename T, int DP, int BM>
+__global__ void __launch_bounds__(kSimtThreads) k_attention_simt(const AttnArgs a) {
+  using S = SimtShape<DP, BM>;
+  constexpr int R = S::R, NC = S::NC, CW = S::CW;
+  extern __shared__ __align__(16) float smem[];
+  __shared__ FoundTile found;
+  __shared__ int32_t warp_sums[kSimtThreads / 32];
+  float* s_q = smem;
+  float* s_kv = s_q + BM * S::LD;
+  float* s_p = s_kv + BM * S::LD;
+  after_previous_kernel();
+  const int head = blockIdx.x % a.heads;
+  if (!find_tile<kSimtThreads, false>(a, blockIdx.x / a.heads, BM, &found, warp_sums)) return;
+  const Segment g = found.g;
+  const int first = (found.tiles - 1 - found.tile) * BM;  // the tiles with the most keys first
+  const int rows = min(BM, g.n_q - first);
+  const int kv = head / (a.heads / a.kv_heads);
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  load_tile<T, DP, BM>(s_q, static_cast<const T*>(a.q) + (int64_t)(g.q0 + first) * a.q_row + head * a.q_head, a.q_row, rows,
+                       a.dim, a.scale);
+  float o[R][NC][CW] = {}, m[R], l[R];
+  int seen[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    m[i] = -CUDART_INF_F;
+    l[i] = 0.f;
+    seen[i] = ty + 16 * i < rows ? visible_keys(g, first + ty + 16 * i, a.causal) : 0;
+  }
+  const int keys = visible_keys(g, first + rows - 1, a.causal);  // of the last row: the most
+  const T* k0 = static_cast<const T*>(a.k) + (int64_t)g.k0 * a.k_row + kv * a.k_head;
+  const T* v0 = static_cast<const T*>(a.v) + (int64_t)g.k0 * a.v_row + kv * a.v_head;
+  for (int j0 = 0; j0 < keys; j0 += BM) {
+    const int n = min(BM, keys - j0);
+    __syncthreads();  // the products with the tile before are done
+    load_tile<T, DP, BM>(s_kv, k0 + (int64_t)j0 * a.k_row, a.k_row, n, a.dim, 1.f);
+    __syncthreads();
+    float s[R][R];
+    product_rows<DP, BM>(s_q, s_kv, tx, ty, s);
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      float top = -CUDART_INF_F;
+#pragma unroll
+      for (int j = 0; j < R; ++j) {
+        if (j0 + tx + 16 * j >= seen[i]) s[i][j] = -CUDART_INF_F;
+        top = fmaxf(top, s[i][j]);
+      }
+#pragma unroll
+      for (int w = 8; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w, 16));
+      const float m_new = fmaxf(m[i], top);
+      const float base = m_new == -CUDART_INF_F ? 0.f : m_new;  // a row that sees nothing yet
+      const float shrink = expf(m[i] - base);
+      float sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < R; ++j) {
+        const float p = expf(s[i][j] - base);
+        s_p[(ty + 16 * i) * S::LP + tx + 16 * j] = p;
+        sum += p;
+      }
+#pragma unroll
+      for (int w = 8; w > 0; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w, 16);
+      l[i] = l[i] * shrink + sum;
+      m[i] = m_new;
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int e = 0; e < CW; ++e) o[i][c][e] *= shrink;
+    }
+    __syncthreads();  // the keys have been read
+    load_tile<T, DP, BM>(s_kv, v0 + (int64_t)j0 * a.v_row, a.v_row, n, a.dim, 1.f);
+    __syncthreads();
+    product_columns<DP, BM>(s_p, s_kv, n, tx, ty, o);
+  }
+  float by[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    by[i] = l[i] == 0.f ? 0.f : 1.f / l[i];
+    if (a.lse && tx == 0 && ty + 16 * i < rows)
+      a.lse[(size_t)head * a.rows_q + g.q0 + first + ty + 16 * i] = l[i] == 0.f ? -CUDART_INF_F : m[i] + logf(l[i]);
+  }
+  const int64_t out_row = (int64_t)a.heads * a.dim;
+  store_tile<T, DP, BM>(static_cast<T*>(a.out) + (int64_t)(g.q0 + first) * out_row + (int64_t)head * a.dim, out_row, rows,
+                        a.dim, tx, ty, o, by);
+}
+
+// dq of a query tile, and delta of its rows for the kernel of the key tiles
+template <typename T, int DP, int BM>
+__global__ void __launch_bounds__(kSimtThreads) k_attention_simt_dq(const AttnArgs a) {
+  using S = SimtShape<DP, BM>;
+  constexpr int R = S::R, NC = S::NC, CW = S::CW;
+  extern __shared__ __align__(16) float smem[];
+  __shared__ FoundTile found;
+  __shared__ int32_t warp_sums[kSimtThreads / 32];
+  float* s_q = smem;
+  float* s_g = s_q + BM * S::LD;
+  float* s_k = s_g + BM * S::LD;
+  float* s_v = s_k + BM * S::LD;
+  float* s_p = s_v + BM * S::LD;
+  after_previous_kernel();
+  const int head = blockIdx.x % a.heads;
+  if (!find_tile<kSimtThreads, false>(a, blockIdx.x / a.heads, BM, &found, warp_sums)) return;
+  const Segment g = found.g;
+  const int first = (found.tiles - 1 - found.tile) * BM;
+  const int rows = min(BM, g.n_q - first);
+  const int kv = head / (a.heads / a.kv_heads);
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  const int64_t out_row = (int64_t)a.heads * a.dim;
+  load_tile<T, DP, BM>(s_q, static_cast<const T*>(a.q) + (int64_t)(g.q0 + first) * a.q_row + head * a.q_head, a.q_row, rows,
+                       a.dim, a.scale);
+  load_tile<T, DP, BM>(s_g, static_cast<const T*>(a.grad) + (int64_t)(g.q0 + first) * a.grad_row + head * a.grad_head,
+                       a.grad_row, rows, a.dim, 1.f);
+  load_tile<T, DP, BM>(s_k, static_cast<const T*>(a.fwd_out) + (int64_t)(g.q0 + first) * out_row + (int64_t)head * a.dim,
+                       out_row, rows, a.dim, 1.f);
+  __syncthreads();
+  float o[R][NC][CW] = {}, delta[R], lse[R];
+  int seen[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int r = ty + 16 * i;
+    float d = 0.f;
+    for (int c = tx; c < DP; c += 16) d = fmaf(s_g[r * S::LD + c], s_k[r * S::LD + c], d);
+#pragma unroll
+    for (int w = 8; w > 0; w >>= 1) d += __shfl_xor_sync(0xffffffffu, d, w, 16);
+    delta[i] = d;
+    seen[i] = r < rows ? visible_keys(g, first + r, a.causal) : 0;
+    const size_t at = (size_t)head * a.rows_q + g.q0 + first + r;
+    lse[i] = r < rows ? __ldg(a.lse + at) : 0.f;
+    if (r < rows && tx == 0) a.delta[at] = d;
+  }
+  const int keys = visible_keys(g, first + rows - 1, a.causal);
+  const T* k0 = static_cast<const T*>(a.k) + (int64_t)g.k0 * a.k_row + kv * a.k_head;
+  const T* v0 = static_cast<const T*>(a.v) + (int64_t)g.k0 * a.v_row + kv * a.v_head;
+  for (int j0 = 0; j0 < keys; j0 += BM) {
+    const int n = min(BM, keys - j0);
+    __syncthreads();
+    load_tile<T, DP, BM>(s_k, k0 + (int64_t)j0 * a.k_row, a.k_row, n, a.dim, 1.f);
+    load_tile<T, DP, BM>(s_v, v0 + (int64_t)j0 * a.v_row, a.v_row, n, a.dim, 1.f);
+    __syncthreads();
+    float s[R][R], dp[R][R];
+    product_rows<DP, BM>(s_q, s_k, tx, ty, s);
+    product_rows<DP, BM>(s_g, s_v, tx, ty, dp);
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+      for (int j = 0; j < R; ++j) {
+        const bool see = j0 + tx + 16 * j < seen[i];
+        s_p[(ty + 16 * i) * S::LP + tx + 16 * j] = see ? expf(s[i][j] - lse[i]) * (dp[i][j] - delta[i]) : 0.f;
+      }
+    __syncthreads();
+    product_columns<DP, BM>(s_p, s_k, n, tx, ty, o);
+  }
+  float by[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) by[i] = a.scale;
+  store_tile<T, DP, BM>(static_cast<T*>(a.dq) + (int64_t)(g.q0 + first) * out_row + (int64_t)head * a.dim, out_row, rows, a.dim,
+                        tx, ty, o, by);
+}
+
+// dk and dv of a key tile: the queries of all heads that share its head
+template <typename T, int DP, int BM>
+__global__ void __launch_bounds__(kSimtThreads) k_attention_simt_dkv(const AttnArgs a) {
+  using S = SimtShape<DP, BM>;
+  constexpr int R = S::R, NC = S::NC, CW = S::CW;
+  extern __shared__ __align__(16) float smem[];
+  __shared__ FoundTile found;
+  __shared__ int32_t warp_sums[kSimtThreads / 32];
+  float* s_k = smem;
+  float* s_v = s_k + BM * S::LD;
+  float* s_q = s_v + BM * S::LD;
+  float* s_g = s_q + BM * S::LD;
+  float* s_p = s_g + BM * S::LD;
+  after_previous_kernel();
+  const int kv = blockIdx.x % a.kv_heads;
+  if (!find_tile<kSimtThreads, true>(a, blockIdx.x / a.kv_heads, BM, &found, warp_sums)) return;
+  const Segment g = found.g;
+  const int first = found.tile * BM;  // the first keys are seen by the most queries
+  const int rows = min(BM, g.k_slot - first), used = max(0, min(BM, g.n_k - first));
+  const int group = a.heads / a.kv_heads;
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  load_tile<T, DP, BM>(s_k, static_cast<const T*>(a.k) + (int64_t)(g.k0 + first) * a.k_row + kv * a.k_head, a.k_row, used,
+                       a.dim, a.scale);
+  load_tile<T, DP, BM>(s_v, static_cast<const T*>(a.v) + (int64_t)(g.k0 + first) * a.v_row + kv * a.v_head, a.v_row, used,
+                       a.dim, 1.f);
+  float dk[R][NC][CW] = {}, dv[R][NC][CW] = {};
+  const int from = used > 0 ? first_query(g, first, a.causal) / BM * BM : g.n_q;
+  for (int h = kv * group; h < (kv + 1) * group; ++h) {
+    const T* q0 = static_cast<const T*>(a.q) + (int64_t)g.q0 * a.q_row + h * a.q_head;
+    const T* g0 = static_cast<const T*>(a.grad) + (int64_t)g.q0 * a.grad_row + h * a.grad_head;
+    for (int i0 = from; i0 < g.n_q; i0 += BM) {
+      const int n = min(BM, g.n_q - i0);
+      __syncthreads();
+      load_tile<T, DP, BM>(s_q, q0 + (int64_t)i0 * a.q_row, a.q_row, n, a.dim, 1.f);
+      load_tile<T, DP, BM>(s_g, g0 + (int64_t)i0 * a.grad_row, a.grad_row, n, a.dim, 1.f);
+      __syncthreads();
+      float s[R][R], dp[R][R];
+      product_rows<DP, BM>(s_k, s_q, tx, ty, s);
+      product_rows<DP, BM>(s_v, s_g, tx, ty, dp);
+#pragma unroll
+      for (int j = 0; j < R; ++j) {
+        const int qi = tx + 16 * j;
+        const size_t at = (size_t)h * a.rows_q + g.q0 + i0 + qi;
+        const float lse = qi < n ? __ldg(a.lse + at) : 0.f, delta = qi < n ? __ldg(a.delta + at) : 0.f;
+        const int seen = qi < n ? visible_keys(g, i0 + qi, a.causal) : 0;
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+          const float p = first + ty + 16 * i < seen ? expf(s[i][j] - lse) : 0.f;
+          s[i][j] = p;
+          dp[i][j] = p == 0.f ? 0.f : p * (dp[i][j] - delta);
+          s_p[(ty + 16 * i) * S::LP + qi] = p;
+        }
+      }
+      __syncthreads();
+      product_columns<DP, BM>(s_p, s_g, n, tx, ty, dv);
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < R; ++i)
+#pragma unroll
+        for (int j = 0; j < R; ++j) s_p[(ty + 16 * i) * S::LP + tx + 16 * j] = dp[i][j];
+      __syncthreads();
+      product_columns<DP, BM>(s_p, s_q, n, tx, ty, dk);
+    }
+  }
+  float by_k[R], by_v[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    by_k[i] = a.scale;
+    by_v[i] = 1.f;
+  }
+  const int64_t kv_row = (int64_t)a.kv_heads * a.dim, at = (int64_t)(g.k0 + first) * kv_row + (int64_t)kv * a.dim;
+  store_tile<T, DP, BM>(static_cast<T*>(a.dk) + at, kv_row, rows, a.dim, tx, ty, dk, by_k);
+  store_tile<T, DP, BM>(static_cast<T*>(a.dv) + at, kv_row, rows, a.dim, tx, ty, dv, by_v);
+}
+
+template <class Kernel>
+int launch_simt(Kernel kern, SmemOptIn& opt_in, const AttnArgs& a, uint64_t blocks, size_t smem, cudaStream_t stream) {
+  if (blocks > 0x7fffffffull) return RMN_ERR_UNSUPPORTED;
+  if (smem > 48 * 1024 - 1024) RMN_CUDA_TRY(opt_in.apply(reinterpret_cast<const void*>(kern), smem));
+  RMN_CUDA_TRY(launch_overlapped(kern, dim3((uint32_t)blocks), dim3(kSimtThreads), smem, stream, a));
+  RMN_LAUNCH_CHECK();
+  return RMN_OK;
+}
+
+template <typename T, int DP, int BM>
+int forward(const AttnArgs& a, cudaStream_t stream) {
+  using S = SimtShape<DP, BM>;
+  static SmemOptIn opt_in;
+  return launch_simt(k_attention_simt<T, DP, BM>, opt_in, a, most_tiles(a.rows_q, a.sequences, BM) * a.heads,
+                     2 * S::tile + S::square, stream);
+}
+template <typename T, int DP, int BM>
+int backward(const AttnArgs& a, cudaStream_t stream) {
+  using S = SimtShape<DP, BM>;
+  static SmemOptIn opt_q, opt_kv;
+  const int st = launch_simt(k_attention_simt_dq<T, DP, BM>, opt_q, a, most_tiles(a.rows_q, a.sequences, BM) * a.heads,
+                             4 * S::tile + S::square, stream);
+  if (st != RMN_OK) return st;
+  return launch_simt(k_attention_simt_dkv<T, DP, BM>, opt_kv, a, most_tiles(a.rows_k, a.sequences, BM) * a.kv_heads,
+                     4 * S::tile + S::square, stream);
+}
+
+}  // namespace
+
+#define RMN_SIMT_SHAPES(F)                                                             \
+  if (a.dim <= 32) return dtype == RMN_F32 ? F<float, 32, 64>(a, stream) : F<__nv_bfloat16, 32, 64>(a, stream);     \
+  if (a.dim <= 64) return dtype == RMN_F32 ? F<float, 64, 64>(a, stream) : F<__nv_bfloat16, 64, 64>(a, stream);     \
+  if (a.dim <= 128) return dtype == RMN_F32 ? F<float, 128, 64>(a, stream) : F<__nv_bfloat16, 128, 64>(a, stream);  \
+  if (a.dim <= 256) return dtype == RMN_F32 ? F<float, 256, 32>(a, stream) : F<__nv_bfloat16, 256, 32>(a, stream);  \
+  return RMN_ERR_UNSUPPORTED;
+
+int attention_simt_forward(const AttnArgs& a, int dtype, cudaStream_t stream) { RMN_SIMT_SHAPES(forward) }
+int attention_simt_backward(const AttnArgs& a, int dtype, cudaStream_t stream) { RMN_SIMT_SHAPES(backward) }
+
+}  // namespace rmn

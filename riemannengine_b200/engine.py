@@ -233,6 +233,7 @@ class CoordinateManager:
         self._kernel_maps: Dict[tuple, KernelMap] = {}
         self._fields: Dict[Tuple[Tuple[int, ...], str], torch.Tensor] = {}
         self._field_to_sparse: Dict[tuple, Tuple[torch.Tensor, torch.Tensor]] = {}
+        self._sample_offsets: Dict[Tuple[Tuple[int, ...], str], torch.Tensor] = {}
 
     # -- introspection -------------------------------------------------------------------
     @property
@@ -382,6 +383,24 @@ class CoordinateManager:
         in_map, out_map = self._map(in_key), self._map(out_key)
         aligned = ops.coords_stride(in_map.coords, out_map.tensor_stride)
         return ops.table_find(out_map.table, aligned)
+
+    def sample_offsets(self, key: CoordinateMapKey) -> torch.Tensor:
+        """int32 [samples + 1] on the device: the first row of every sample of a map in row order, and the number of rows: the
+        ``offsets`` of packed_attention. Made once per map (it waits for the device then). The rows of a sample have to be
+        adjacent, as they are where the coordinates were inserted sample by sample. No counterpart in the reference."""
+        hit = self._sample_offsets.get(key.get_key())
+        if hit is None:
+            coords = self._map(key).coords
+            samples = 0
+            if coords.size(0):
+                batch = coords.clone()
+                batch[:, 1:] = 0
+                samples = ops.table_build(batch).n_unique
+            found = ops.sample_offsets(coords, samples)
+            if samples and int(found[samples + 1]) != samples:
+                raise RuntimeError("sample_offsets needs the rows of a sample to be adjacent")
+            hit = self._sample_offsets[key.get_key()] = found[:samples + 1]
+        return hit
 
     # -- kernel maps -----------------------------------------------------------------------
     def kernel_map(self, in_key: CoordinateMapKey, out_key: CoordinateMapKey, kernel_size: Sequence[int],
@@ -1022,6 +1041,101 @@ class RiemannBatchNorm(torch.nn.Module):
 
 
 RiemannSyncBatchNorm = RiemannBatchNorm  # the reference's alias (engine/nn/normalization.hpp:36-37)
+
+
+class _LayerNormFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps: float):
+        train = builtins.any(ctx.needs_input_grad)
+        out, mean, inv = ops.layer_norm_forward(x, weight, bias, eps, want_stats=train)
+        ctx.save_for_backward(x, weight, mean, inv)
+        ctx.bias_dtype = bias.dtype if bias is not None else None
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_out):
+        x, weight, mean, inv = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        return (*ops.layer_norm_backward(grad_out, x, weight, mean, inv, need[0], need[1], need[2], ctx.bias_dtype), None)
+
+
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+               eps: float = 1e-5) -> torch.Tensor:
+    """Layer norm over the channels of a feature matrix [N, C], differentiable in all three."""
+    return _LayerNormFunction.apply(x, weight, bias, eps)
+
+
+class RiemannLayerNorm(torch.nn.Module):
+    """Layer norm over the channels of every row of a SparseTensor. ``normalization`` is the torch layer that holds the
+    parameters (as in RiemannBatchNorm); the pass runs on the library's kernels."""
+
+    def __init__(self, num_features: int, eps: float = 1e-5, elementwise_affine: bool = True):
+        super().__init__()
+        self.normalization = torch.nn.LayerNorm(num_features, eps=eps, elementwise_affine=elementwise_affine)
+
+    def forward(self, input: "SparseTensor") -> "SparseTensor":
+        n = self.normalization
+        if input.F.size(1) != n.normalized_shape[0]:
+            raise RuntimeError("Input channel count does not match layer norm")
+        return SparseTensor(layer_norm(input.F, n.weight, n.bias, n.eps), input.coordinate_map_key, input.coordinate_manager)
+
+
+class _PackedAttentionFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, offsets, kv_offsets, kv_lengths, causal: bool, scale):
+        train = builtins.any(ctx.needs_input_grad)
+        out, lse = ops.attention_forward(q, k, v, offsets, kv_offsets, kv_lengths, causal, scale, want_lse=train)
+        ctx.save_for_backward(q, k, v, out, lse, offsets, kv_offsets, kv_lengths)
+        ctx.causal, ctx.scale = causal, scale
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_out):
+        q, k, v, out, lse, offsets, kv_offsets, kv_lengths = ctx.saved_tensors
+        return (*ops.attention_backward(grad_out, q, k, v, out, lse, offsets, kv_offsets, kv_lengths, ctx.causal, ctx.scale),
+                None, None, None, None, None)
+
+
+def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: torch.Tensor,
+                     kv_offsets: Optional[torch.Tensor] = None, kv_lengths: Optional[torch.Tensor] = None,
+                     causal: bool = False, scale: Optional[float] = None) -> torch.Tensor:
+    """softmax(scale q k^T) v within packed samples, differentiable in q, k and v. ``q`` [rows, heads, channels], ``k`` and
+    ``v`` [key rows, key heads, channels] (heads a multiple of key heads); ``offsets`` int32 [samples + 1]: first row of
+    every sample and the end of the last. ``kv_offsets`` where the keys' rows are others than the queries', ``kv_lengths``
+    [samples] where only the first rows of a sample's keys are in use (a cache). ``causal`` is aligned at the end of the keys.
+    ``scale``: channels ** -0.5 unless given. Rows of no sample, and rows that see no key, are zero."""
+    return _PackedAttentionFunction.apply(q, k, v, offsets, kv_offsets, kv_lengths, bool(causal), scale)
+
+
+class RiemannSelfAttention(torch.nn.Module):
+    """Self-attention of the rows of a SparseTensor within their sample: ``qkv`` projects the features to queries, keys and
+    values, packed_attention runs on the row ranges of CoordinateManager.sample_offsets, ``projection`` mixes the heads. The
+    key heads may be fewer than the query heads. No counterpart in the reference."""
+
+    def __init__(self, channels: int, num_heads: int, num_kv_heads: Optional[int] = None, causal: bool = False,
+                 bias: bool = True):
+        super().__init__()
+        kv = num_heads if num_kv_heads is None else num_kv_heads
+        if channels <= 0 or num_heads <= 0 or channels % num_heads:
+            raise RuntimeError("Attention channels must be a positive multiple of the number of heads")
+        if kv <= 0 or num_heads % kv:
+            raise RuntimeError("the number of query heads must be a multiple of the number of key heads")
+        self.channels, self.num_heads, self.num_kv_heads, self.causal = channels, num_heads, kv, causal
+        self.dim = channels // num_heads
+        self.qkv = torch.nn.Linear(channels, (num_heads + 2 * kv) * self.dim, bias=bias)
+        self.projection = torch.nn.Linear(channels, channels, bias=bias)
+
+    def forward(self, input: "SparseTensor") -> "SparseTensor":
+        if input.F.size(1) != self.channels:
+            raise RuntimeError("Input channel count does not match attention")
+        offsets = input.coordinate_manager.sample_offsets(input.coordinate_map_key)
+        h, kv = self.num_heads, self.num_kv_heads
+        q, k, v = self.qkv(input.F).view(-1, h + 2 * kv, self.dim).split([h, kv, kv], 1)
+        out = packed_attention(q, k, v, offsets, causal=self.causal)
+        return SparseTensor(self.projection(out.reshape(-1, self.channels)), input.coordinate_map_key,
+                            input.coordinate_manager)
 
 
 class RiemannConvolutionBase(torch.nn.Module):

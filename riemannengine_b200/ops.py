@@ -558,3 +558,176 @@ def field_splat(field: torch.Tensor, feats: torch.Tensor):
         capi.check(capi.lib().rmn_field_splat(_ptr(field), _ptr(feats), _dtype_code(feats), n, w, c, _ptr(out_c),
                                               _ptr(out_f), _stream()), "rmn_field_splat")
     return out_c, out_f
+
+
+def _rows(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
+    """``t`` [N, C] with adjacent channels and the distance of its rows; a copy where its strides are others."""
+    if (t.size(1) > 1 and t.stride(1) != 1) or t.stride(0) < 0:
+        t = t.contiguous()
+    return t, int(t.stride(0)) if t.size(0) > 1 else int(t.size(1))
+
+
+def _check_norm_params(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor]) -> int:
+    """The parameters' dtype code."""
+    _require_cuda(x, "features")
+    if x.dim() != 2 or x.size(1) < 1:
+        raise RuntimeError("features must be [N, C]")
+    _dtype_code(x)
+    code = None
+    for name, p in (("weight", weight), ("bias", bias)):
+        if p is None:
+            continue
+        _require_cuda(p, name)
+        if p.dim() != 1 or p.size(0) != x.size(1):
+            raise RuntimeError(f"layer norm {name} must have one entry per channel")
+        if p.device != x.device:
+            raise RuntimeError(f"layer norm {name} must be on the features' device")
+        if code is not None and _dtype_code(p) != code:
+            raise RuntimeError("layer norm weight and bias must have the same dtype")
+        code = _dtype_code(p)
+    return capi.F32 if code is None else code
+
+
+def layer_norm_forward(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+                       eps: float = 1e-5, want_stats: bool = False):
+    """Layer norm over the channels of ``x`` [N, C] (rmn_layer_norm_forward): returns (out, mean, inv), the last two
+    float32 [N] (None unless ``want_stats``), which the backward pass needs."""
+    code = _check_norm_params(x, weight, bias)
+    x, ld = _rows(x)
+    weight = weight.contiguous() if weight is not None else None
+    bias = bias.contiguous() if bias is not None else None
+    n, c = int(x.size(0)), int(x.size(1))
+    out = torch.empty((n, c), dtype=x.dtype, device=x.device)
+    stats = torch.empty((2, n), dtype=torch.float32, device=x.device) if want_stats else None
+    mean, inv = (stats[0], stats[1]) if want_stats else (None, None)
+    with torch.cuda.device(x.device):
+        capi.check(capi.lib().rmn_layer_norm_forward(_ptr(x), ld, n, c, _ptr(weight), _ptr(bias), code, float(eps), _ptr(out),
+                                                     _ptr(mean), _ptr(inv), _dtype_code(x), _stream()),
+                   "rmn_layer_norm_forward")
+    return out, mean, inv
+
+
+def layer_norm_backward(grad_out: torch.Tensor, x: torch.Tensor, weight: Optional[torch.Tensor], mean: torch.Tensor,
+                        inv: torch.Tensor, want_input: bool = True, want_weight: bool = True, want_bias: bool = True,
+                        param_dtype: Optional[torch.dtype] = None):
+    """Gradients of layer_norm_forward (rmn_layer_norm_backward): (dx, dweight, dbias), None where not wanted; the
+    parameters' gradients in ``param_dtype`` (default: the weight's, or float32)."""
+    code = _check_norm_params(x, weight, None)
+    if param_dtype is not None and weight is None:
+        code = capi.BF16 if param_dtype == torch.bfloat16 else capi.F32
+    ptype = torch.bfloat16 if code == capi.BF16 else torch.float32
+    if grad_out.shape != x.shape or grad_out.dtype != x.dtype or grad_out.device != x.device:
+        raise RuntimeError("the output gradient must have the features' shape, dtype and device")
+    x, ld_x = _rows(x)
+    dy, ld_dy = _rows(grad_out)
+    weight = weight.contiguous() if weight is not None else None
+    n, c = int(x.size(0)), int(x.size(1))
+    dx = torch.empty((n, c), dtype=x.dtype, device=x.device) if want_input else None
+    dw = torch.empty(c, dtype=ptype, device=x.device) if want_weight else None
+    db = torch.empty(c, dtype=ptype, device=x.device) if want_bias else None
+    lib = capi.lib()
+    wbytes = lib.rmn_layer_norm_backward_workspace_bytes(n, c)
+    ws = torch.empty(wbytes, dtype=torch.uint8, device=x.device)
+    with torch.cuda.device(x.device):
+        capi.check(lib.rmn_layer_norm_backward(_ptr(dy), ld_dy, _ptr(x), ld_x, n, c, _ptr(weight), code, _ptr(mean), _ptr(inv),
+                                               _ptr(dx), _ptr(dw), _ptr(db), _dtype_code(x), _ptr(ws), wbytes, _stream()),
+                   "rmn_layer_norm_backward")
+    return dx, dw, db
+
+
+def sample_offsets(coords: torch.Tensor, n_samples: int) -> torch.Tensor:
+    """int32 [n_samples + 2]: first row of every sample of ``coords``, the number of rows, and the number of runs of equal
+    batch indices (rmn_sample_offsets)."""
+    _check_coords(coords)
+    lib = capi.lib()
+    out = torch.empty(n_samples + 2, dtype=torch.int32, device=coords.device)
+    wbytes = lib.rmn_sample_offsets_workspace_bytes(n_samples)
+    ws = torch.empty(wbytes, dtype=torch.uint8, device=coords.device)
+    with torch.cuda.device(coords.device):
+        capi.check(lib.rmn_sample_offsets(_ptr(coords), int(coords.size(0)), int(coords.size(1)), n_samples, _ptr(out), _ptr(ws),
+                                          wbytes, _stream()), "rmn_sample_offsets")
+    return out
+
+
+def _heads(t: torch.Tensor) -> torch.Tensor:
+    """``t`` [N, H, D] with adjacent channels; a copy where its strides are others (other shapes are refused later)."""
+    return t if t.dim() != 3 or t.size(2) == 1 or t.stride(2) == 1 else t.contiguous()
+
+
+def _attention(q, k, v, offsets, kv_offsets, kv_lengths, causal, scale) -> capi.Attention:
+    """The checked problem; q, k and v have adjacent channels (``_heads``)."""
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        _require_cuda(t, name)
+        if t.dim() != 3 or t.size(2) < 1:
+            raise RuntimeError(f"{name} must be [rows, heads, channels]")
+        if t.dtype != q.dtype or t.device != q.device:
+            raise RuntimeError("q, k and v must have the same dtype and device")
+    if k.shape != v.shape or k.size(2) != q.size(2):
+        raise RuntimeError("k and v must have the same shape, and q's channels")
+    if q.size(1) < 1 or k.size(1) < 1 or q.size(1) % k.size(1):
+        raise RuntimeError("the number of query heads must be a multiple of the number of key heads")
+    for name, t in (("offsets", offsets), ("kv_offsets", kv_offsets), ("kv_lengths", kv_lengths)):
+        if t is None:
+            continue
+        _require_cuda(t, name)
+        if t.dim() != 1 or t.dtype != torch.int32 or not t.is_contiguous() or t.device != q.device:
+            raise RuntimeError(f"{name} must be a contiguous 1-D int32 tensor on q's device")
+    n = int(offsets.numel()) - 1
+    if n < 0:
+        raise RuntimeError("offsets must hold one entry more than there are samples")
+    if kv_offsets is not None and kv_offsets.numel() != n + 1:
+        raise RuntimeError("kv_offsets must have as many entries as offsets")
+    if kv_lengths is not None and kv_lengths.numel() != n:
+        raise RuntimeError("kv_lengths must have one entry per sample")
+    if kv_offsets is None and k.size(0) != q.size(0):
+        raise RuntimeError("q and k must have the same rows unless kv_offsets are given")
+    p = capi.Attention()
+    p.q, p.k, p.v = (t.data_ptr() if t.numel() else None for t in (q, k, v))
+    p.q_row, p.q_head, p.k_row, p.k_head, p.v_row, p.v_head = (int(t.stride(i)) for t in (q, k, v) for i in (0, 1))
+    p.rows_q, p.rows_k, p.sequences = int(q.size(0)), int(k.size(0)), n
+    p.heads, p.kv_heads, p.dim = int(q.size(1)), int(k.size(1)), int(q.size(2))
+    p.offsets = offsets.data_ptr()
+    p.kv_offsets = kv_offsets.data_ptr() if kv_offsets is not None else None
+    p.kv_lengths = kv_lengths.data_ptr() if kv_lengths is not None and n else None
+    p.causal, p.dtype = int(bool(causal)), _dtype_code(q)
+    p.scale = float(q.size(2)) ** -0.5 if scale is None else float(scale)
+    return p
+
+
+def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: torch.Tensor,
+                      kv_offsets: Optional[torch.Tensor] = None, kv_lengths: Optional[torch.Tensor] = None,
+                      causal: bool = False, scale: Optional[float] = None, want_lse: bool = False):
+    """Attention within packed samples (rmn_attention_forward): ``q`` [rows, heads, channels], ``k`` and ``v``
+    [key rows, key heads, channels], any row and head strides; returns (out, lse), lse float32 [heads, rows] or None."""
+    q, k, v = _heads(q), _heads(k), _heads(v)
+    p = _attention(q, k, v, offsets, kv_offsets, kv_lengths, causal, scale)
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    lse = torch.empty((p.heads, p.rows_q), dtype=torch.float32, device=q.device) if want_lse else None
+    lib = capi.lib()
+    with torch.cuda.device(q.device):
+        wbytes = lib.rmn_attention_forward_workspace_bytes(ctypes.byref(p))
+        ws = torch.empty(wbytes, dtype=torch.uint8, device=q.device) if wbytes else None
+        capi.check(lib.rmn_attention_forward(ctypes.byref(p), _ptr(out), _ptr(lse), _ptr(ws), wbytes, _stream()),
+                   "rmn_attention_forward")
+    return out, lse
+
+
+def attention_backward(grad_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor,
+                       lse: torch.Tensor, offsets: torch.Tensor, kv_offsets: Optional[torch.Tensor] = None,
+                       kv_lengths: Optional[torch.Tensor] = None, causal: bool = False, scale: Optional[float] = None):
+    """(dq, dk, dv) of attention_forward (rmn_attention_backward)."""
+    q, k, v, grad_out = _heads(q), _heads(k), _heads(v), _heads(grad_out)
+    p = _attention(q, k, v, offsets, kv_offsets, kv_lengths, causal, scale)
+    if grad_out.shape != q.shape or grad_out.dtype != q.dtype or grad_out.device != q.device:
+        raise RuntimeError("the output gradient must have q's shape, dtype and device")
+    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    dk = torch.empty(k.shape, dtype=k.dtype, device=q.device)
+    dv = torch.empty(v.shape, dtype=v.dtype, device=q.device)
+    lib = capi.lib()
+    with torch.cuda.device(q.device):
+        wbytes = lib.rmn_attention_backward_workspace_bytes(ctypes.byref(p))
+        ws = torch.empty(wbytes, dtype=torch.uint8, device=q.device)
+        capi.check(lib.rmn_attention_backward(ctypes.byref(p), _ptr(out), _ptr(lse), _ptr(grad_out), int(grad_out.stride(0)),
+                                              int(grad_out.stride(1)), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(ws), wbytes,
+                                              _stream()), "rmn_attention_backward")
+    return dq, dk, dv

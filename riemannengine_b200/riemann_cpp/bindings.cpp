@@ -25,6 +25,30 @@ void bind_pool(py::module_& m, const char* name) {
            py::call_guard<py::gil_scoped_release>());
 }
 
+// a layer with parameters of torch layers
+template <typename Impl>
+py::class_<Impl, std::shared_ptr<Impl>> bind_layer(py::module_& m, const char* name) {
+  py::class_<Impl, std::shared_ptr<Impl>> cls(m, name);
+  cls.def("forward", [](Impl& self, const SparseTensor& input) { return self.forward(input); }, py::arg("input"),
+          py::call_guard<py::gil_scoped_release>());
+  cls.def("__call__", [](Impl& self, const SparseTensor& input) { return self.forward(input); }, py::arg("input"),
+          py::call_guard<py::gil_scoped_release>());
+  cls.def("parameters", [](Impl& self) { return self.parameters(); });
+  cls.def("named_parameters", [](Impl& self) {
+    py::dict out;
+    for (auto& p : self.named_parameters()) out[py::str(p.key())] = p.value();
+    return out;
+  });
+  cls.def("to", [](Impl& self, py::object dtype_or_device) {
+    if (THPDtype_Check(dtype_or_device.ptr()))
+      self.to(reinterpret_cast<THPDtype*>(dtype_or_device.ptr())->scalar_type);
+    else
+      self.to(torch::Device(py::cast<std::string>(py::str(dtype_or_device))));
+  });
+  cls.def("zero_grad", [](Impl& self) { self.zero_grad(); });
+  return cls;
+}
+
 template <typename Impl>
 py::class_<Impl, std::shared_ptr<Impl>> bind_conv(py::module_& m, const char* name) {
   py::class_<Impl, std::shared_ptr<Impl>> cls(m, name);
@@ -101,6 +125,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
            py::arg("string_id") = "")
       .def("stride", &CoordinateManager::stride, py::arg("in_key"), py::arg("kernel_stride"),
            py::arg("string_id") = "")
+      .def("sample_offsets", &CoordinateManager::sample_offsets, py::arg("key"), py::call_guard<py::gil_scoped_release>())
       .def("union_map",
            [](CoordinateManager& self, const std::vector<CoordinateMapKey>& in_keys) {
              CoordinateMapKey out_key(in_keys.empty() ? 0 : in_keys.front().get_coordinate_size());
@@ -277,6 +302,42 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
       else
         self.to(torch::Device(py::cast<std::string>(py::str(dtype_or_device))));
     });
+  }
+
+  // layer norm and attention within packed samples
+  m.def(
+      "layer_norm",
+      [](const at::Tensor& x, const c10::optional<at::Tensor>& weight, const c10::optional<at::Tensor>& bias, double eps) {
+        return layer_norm(x, weight.value_or(at::Tensor()), bias.value_or(at::Tensor()), eps);
+      },
+      py::arg("x"), py::arg("weight") = py::none(), py::arg("bias") = py::none(), py::arg("eps") = 1e-5,
+      py::call_guard<py::gil_scoped_release>());
+  m.def(
+      "packed_attention",
+      [](const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& offsets,
+         const c10::optional<at::Tensor>& kv_offsets, const c10::optional<at::Tensor>& kv_lengths, bool causal,
+         c10::optional<double> scale) {
+        return packed_attention(q, k, v, offsets, kv_offsets.value_or(at::Tensor()), kv_lengths.value_or(at::Tensor()), causal,
+                                scale);
+      },
+      py::arg("q"), py::arg("k"), py::arg("v"), py::arg("offsets"), py::arg("kv_offsets") = py::none(),
+      py::arg("kv_lengths") = py::none(), py::arg("causal") = false, py::arg("scale") = py::none(),
+      py::call_guard<py::gil_scoped_release>());
+  {
+    using LN = RiemannLayerNormImpl;
+    auto cls = bind_layer<LN>(m, "RiemannLayerNorm");
+    cls.def(py::init([](int64_t num_features, double eps, bool elementwise_affine) {
+              return std::make_shared<LN>(num_features, eps, elementwise_affine);
+            }),
+            py::arg("num_features"), py::arg("eps") = 1e-5, py::arg("elementwise_affine") = true);
+    cls.def_property_readonly("weight", [](LN& self) { return self.normalization()->weight; });
+    cls.def_property_readonly("bias", [](LN& self) { return self.normalization()->bias; });
+    bind_layer<RiemannSelfAttentionImpl>(m, "RiemannSelfAttention")
+        .def(py::init([](int64_t channels, int64_t num_heads, int64_t num_kv_heads, bool causal, bool bias) {
+               return std::make_shared<RiemannSelfAttentionImpl>(channels, num_heads, num_kv_heads, causal, bias);
+             }),
+             py::arg("channels"), py::arg("num_heads"), py::arg("num_kv_heads") = 0, py::arg("causal") = false,
+             py::arg("bias") = true);
   }
 
   // the example encoder/decoder of networks.hpp (the network the benchmark trains)

@@ -447,6 +447,29 @@ std::pair<CoordinateMapKey, bool> CoordinateManager::origin() {
   return {CoordinateMapKey(static_cast<size_type>(D + 1), origin_key), created};
 }
 
+at::Tensor CoordinateManager::sample_offsets(const CoordinateMapKey& key) {
+  auto hit = sample_offsets_.find(key.get_key());
+  if (hit != sample_offsets_.end()) return hit->second;
+  const Map& map = find(key);
+  c10::cuda::CUDAGuard guard(map.coords.device());
+  uint32_t samples = 0;
+  if (map.size) {
+    auto zeroed = at::zeros_like(map.coords);
+    zeroed.select(1, 0).copy_(map.coords.select(1, 0));
+    samples = build(zeroed, stride_type(map.tensor_stride.size(), 0), nullptr, nullptr, true).size;
+  }
+  auto found = at::empty({static_cast<int64_t>(samples) + 2}, map.coords.options());
+  const size_t ws_bytes = rmn_sample_offsets_workspace_bytes(samples);
+  auto ws = at::empty({static_cast<int64_t>(ws_bytes)}, map.coords.options().dtype(at::kByte));
+  check(rmn_sample_offsets(static_cast<const int32_t*>(ptr(map.coords)), map.size, static_cast<int>(map.coords.size(1)), samples,
+                           static_cast<int32_t*>(ptr(found)), ptr(ws), ws_bytes, current_stream()),
+        "rmn_sample_offsets");
+  if (samples)
+    TORCH_CHECK(found[static_cast<int64_t>(samples) + 1].item<int>() == static_cast<int>(samples),
+                "sample_offsets needs the rows of a sample to be adjacent");
+  return sample_offsets_[key.get_key()] = found.narrow(0, 0, static_cast<int64_t>(samples) + 1);
+}
+
 std::vector<at::Tensor> CoordinateManager::union_map(const std::vector<CoordinateMapKey>& in_keys,
                                                      CoordinateMapKey& out_key) {
   if (in_keys.empty()) throw std::runtime_error("union_map needs at least one map");
@@ -1779,6 +1802,241 @@ SparseTensor RiemannBatchNormImpl::forward(const SparseTensor& input) {
     values = bn->forward(input.F());  // evaluation mode and shapes without a streaming kernel: torch's layer
   }
   return SparseTensor(std::move(values), input.coordinate_map_key(), input.coordinate_manager());
+}
+
+// ---------------------------------------------------------------------------------------------
+// Layer norm and attention within packed samples
+// ---------------------------------------------------------------------------------------------
+namespace {
+bool wants_gradient(std::initializer_list<at::Tensor> tensors) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (auto const& t : tensors)
+    if (t.defined() && t.requires_grad()) return true;
+  return false;
+}
+// The kernels read memory, so wrappers (vmap) and forward-mode derivatives cannot go through them.
+void check_plain(const at::Tensor& t, const char* what) {
+  TORCH_CHECK(t.is_cuda(), what, " must be a CUDA tensor: this library has no CPU path");
+  TORCH_CHECK(plain_autograd(t), what, " must be a plain tensor without forward-mode derivatives");
+}
+void check_once(const at::Tensor& grad, const char* what) {
+  TORCH_CHECK(!(at::GradMode::is_enabled() && grad.requires_grad()), what, " is differentiable once only");
+}
+
+// rows of x and their distance; a copy where its channels are not adjacent
+std::pair<at::Tensor, int64_t> norm_rows(const at::Tensor& x) {
+  auto y = x.size(1) > 1 && x.stride(1) != 1 ? x.contiguous() : x;
+  return {y, y.size(0) > 1 ? y.stride(0) : y.size(1)};
+}
+
+// out, and mean and 1 / sqrt(var + eps) as one float32 [2, N] where `stats` is given
+at::Tensor layer_norm_forward(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& bias, double eps, at::Tensor* stats) {
+  c10::cuda::CUDAGuard guard(x.device());
+  auto [rows, ld] = norm_rows(x);
+  const int64_t n = x.size(0);
+  auto out = at::empty({n, x.size(1)}, x.options());
+  if (stats) *stats = at::empty({2, n}, x.options().dtype(at::kFloat));
+  float* mean = stats ? static_cast<float*>(ptr(*stats)) : nullptr;
+  const auto& any = weight.defined() ? weight : bias;
+  auto w = weight.defined() ? weight.contiguous() : weight, b = bias.defined() ? bias.contiguous() : bias;
+  check(rmn_layer_norm_forward(ptr(rows), ld, static_cast<uint32_t>(n), static_cast<int>(x.size(1)), ptr(w), ptr(b),
+                               any.defined() ? dtype_code(any) : RMN_F32, static_cast<float>(eps), ptr(out), mean,
+                               mean ? mean + n : nullptr, dtype_code(x), current_stream()),
+        "rmn_layer_norm_forward");
+  return out;
+}
+
+class LayerNormAutograd : public torch::autograd::Function<LayerNormAutograd> {
+public:
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, at::Tensor x, at::Tensor weight, at::Tensor bias, double eps) {
+    at::Tensor stats;
+    auto out = layer_norm_forward(x, weight.numel() ? weight : at::Tensor(), bias.numel() ? bias : at::Tensor(), eps, &stats);
+    ctx->save_for_backward({x, weight, stats});
+    ctx->saved_data["bf16"] = (weight.numel() ? weight : bias.numel() ? bias : stats).scalar_type() == at::kBFloat16;
+    return out;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grad_outputs) {
+    auto saved = ctx->get_saved_variables();
+    const auto &x = saved[0], &stats = saved[2];
+    auto weight = saved[1].contiguous();
+    check_once(grad_outputs[0], "layer norm");
+    c10::cuda::CUDAGuard guard(x.device());
+    auto [rows, ld_x] = norm_rows(x);
+    auto [dy, ld_dy] = norm_rows(grad_outputs[0]);
+    const int64_t n = x.size(0), c = x.size(1);
+    const bool bf16 = ctx->saved_data["bf16"].toBool();
+    at::Tensor dx, dw, db;
+    auto params = x.options().dtype(bf16 ? at::kBFloat16 : at::kFloat);
+    if (ctx->needs_input_grad(0)) dx = at::empty({n, c}, x.options());
+    if (ctx->needs_input_grad(1)) dw = at::empty({c}, params);
+    if (ctx->needs_input_grad(2)) db = at::empty({c}, params);
+    const size_t ws_bytes = rmn_layer_norm_backward_workspace_bytes(static_cast<uint32_t>(n), static_cast<int>(c));
+    auto ws = at::empty({static_cast<int64_t>(ws_bytes)}, x.options().dtype(at::kByte));
+    const float* mean = static_cast<const float*>(ptr(stats));
+    check(rmn_layer_norm_backward(ptr(dy), ld_dy, ptr(rows), ld_x, static_cast<uint32_t>(n), static_cast<int>(c),
+                                  ptr(weight), bf16 ? RMN_BF16 : RMN_F32, mean, mean ? mean + n : nullptr, ptr(dx), ptr(dw),
+                                  ptr(db), dtype_code(x), ptr(ws), ws_bytes, current_stream()),
+          "rmn_layer_norm_backward");
+    return {dx, dw, db, at::Tensor()};
+  }
+};
+
+// q, k or v [rows, heads, channels] with adjacent channels; a copy where they are not
+at::Tensor head_rows(const at::Tensor& t) { return t.size(2) > 1 && t.stride(2) != 1 ? t.contiguous() : t; }
+
+struct AttentionInputs {
+  at::Tensor q, k, v, offsets, kv_offsets, kv_lengths;  // an absent one of the last two: undefined or empty
+  bool causal;
+  double scale;
+  rmn_attention problem() const {
+    rmn_attention p = {};
+    p.q = ptr(q); p.k = ptr(k); p.v = ptr(v);
+    p.q_row = q.stride(0); p.q_head = q.stride(1);
+    p.k_row = k.stride(0); p.k_head = k.stride(1);
+    p.v_row = v.stride(0); p.v_head = v.stride(1);
+    p.rows_q = static_cast<uint32_t>(q.size(0));
+    p.rows_k = static_cast<uint32_t>(k.size(0));
+    p.sequences = static_cast<uint32_t>(offsets.numel() - 1);
+    p.heads = static_cast<int>(q.size(1));
+    p.kv_heads = static_cast<int>(k.size(1));
+    p.dim = static_cast<int>(q.size(2));
+    p.offsets = static_cast<const int32_t*>(ptr(offsets));
+    p.kv_offsets = static_cast<const int32_t*>(ptr(kv_offsets));
+    p.kv_lengths = static_cast<const int32_t*>(ptr(kv_lengths));
+    p.causal = causal ? 1 : 0;
+    p.dtype = dtype_code(q);
+    p.scale = static_cast<float>(scale);
+    return p;
+  }
+};
+
+// out, and where `lse` is given the logarithms of the sums of exponentials, float32 [heads, rows]
+at::Tensor attention_forward(const AttentionInputs& in, at::Tensor* lse) {
+  c10::cuda::CUDAGuard guard(in.q.device());
+  const rmn_attention p = in.problem();
+  auto out = at::empty(in.q.sizes(), in.q.options());
+  if (lse) *lse = at::empty({in.q.size(1), in.q.size(0)}, in.q.options().dtype(at::kFloat));
+  const size_t ws_bytes = rmn_attention_forward_workspace_bytes(&p);
+  at::Tensor ws;
+  if (ws_bytes) ws = at::empty({static_cast<int64_t>(ws_bytes)}, in.q.options().dtype(at::kByte));
+  check(rmn_attention_forward(&p, ptr(out), lse ? static_cast<float*>(ptr(*lse)) : nullptr, ptr(ws), ws_bytes, current_stream()),
+        "rmn_attention_forward");
+  return out;
+}
+
+class PackedAttentionAutograd : public torch::autograd::Function<PackedAttentionAutograd> {
+public:
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor offsets,
+                            at::Tensor kv_offsets, at::Tensor kv_lengths, bool causal, double scale) {
+    at::Tensor lse;
+    auto out = attention_forward({q, k, v, offsets, kv_offsets, kv_lengths, causal, scale}, &lse);
+    ctx->save_for_backward({q, k, v, offsets, kv_offsets, kv_lengths, out, lse});
+    ctx->saved_data["causal"] = causal;
+    ctx->saved_data["scale"] = scale;
+    return out;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grad_outputs) {
+    auto saved = ctx->get_saved_variables();
+    check_once(grad_outputs[0], "packed_attention");
+    const AttentionInputs in{saved[0], saved[1], saved[2], saved[3], saved[4], saved[5], ctx->saved_data["causal"].toBool(),
+                             ctx->saved_data["scale"].toDouble()};
+    c10::cuda::CUDAGuard guard(in.q.device());
+    auto grad = head_rows(grad_outputs[0]);
+    const rmn_attention p = in.problem();
+    auto dq = at::empty(in.q.sizes(), in.q.options()), dk = at::empty(in.k.sizes(), in.k.options());
+    auto dv = at::empty(in.v.sizes(), in.v.options());
+    const size_t ws_bytes = rmn_attention_backward_workspace_bytes(&p);
+    auto ws = at::empty({static_cast<int64_t>(ws_bytes)}, in.q.options().dtype(at::kByte));
+    check(rmn_attention_backward(&p, ptr(saved[6]), static_cast<const float*>(ptr(saved[7])), ptr(grad), grad.stride(0),
+                                 grad.stride(1), ptr(dq), ptr(dk), ptr(dv), ptr(ws), ws_bytes, current_stream()),
+          "rmn_attention_backward");
+    return {dq, dk, dv, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+  }
+};
+}  // namespace
+
+at::Tensor layer_norm(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& bias, double eps) {
+  check_plain(x, "features");
+  TORCH_CHECK(x.dim() == 2 && x.size(1) >= 1, "features must be [N, C]");
+  dtype_code(x);
+  for (auto const& [p, name] : {std::pair<const at::Tensor&, const char*>{weight, "weight"}, {bias, "bias"}}) {
+    if (!p.defined()) continue;
+    check_plain(p, name);
+    TORCH_CHECK(p.dim() == 1 && p.size(0) == x.size(1), "layer norm ", name, " must have one entry per channel");
+    TORCH_CHECK(p.device() == x.device(), "layer norm ", name, " must be on the features' device");
+    dtype_code(p);
+  }
+  TORCH_CHECK(!weight.defined() || !bias.defined() || weight.scalar_type() == bias.scalar_type(),
+              "layer norm weight and bias must have the same dtype");
+  if (!wants_gradient({x, weight, bias})) return layer_norm_forward(x, weight, bias, eps, nullptr);
+  auto none = at::empty({0}, x.options());
+  return LayerNormAutograd::apply(x, weight.defined() ? weight : none, bias.defined() ? bias : none, eps);
+}
+
+RiemannLayerNormImpl::RiemannLayerNormImpl(int64_t num_features, double eps, bool elementwise_affine)
+    : normalization_(register_module(
+          "normalization",
+          torch::nn::LayerNorm(torch::nn::LayerNormOptions({num_features}).eps(eps).elementwise_affine(elementwise_affine)))) {}
+
+SparseTensor RiemannLayerNormImpl::forward(const SparseTensor& input) {
+  auto& n = normalization_;
+  TORCH_CHECK(input.F().size(1) == n->options.normalized_shape()[0], "Input channel count does not match layer norm");
+  return SparseTensor(layer_norm(input.F(), n->weight, n->bias, n->options.eps()), input.coordinate_map_key(),
+                      input.coordinate_manager());
+}
+
+at::Tensor packed_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& offsets,
+                            const at::Tensor& kv_offsets, const at::Tensor& kv_lengths, bool causal,
+                            c10::optional<double> scale) {
+  for (auto const& [t, name] : {std::pair<const at::Tensor&, const char*>{q, "q"}, {k, "k"}, {v, "v"}}) {
+    check_plain(t, name);
+    TORCH_CHECK(t.dim() == 3 && t.size(2) >= 1, name, " must be [rows, heads, channels]");
+    TORCH_CHECK(t.scalar_type() == q.scalar_type() && t.device() == q.device(), "q, k and v must have the same dtype and device");
+  }
+  dtype_code(q);
+  TORCH_CHECK(k.sizes() == v.sizes() && k.size(2) == q.size(2), "k and v must have the same shape, and q's channels");
+  TORCH_CHECK(q.size(1) >= 1 && k.size(1) >= 1 && q.size(1) % k.size(1) == 0,
+              "the number of query heads must be a multiple of the number of key heads");
+  for (auto const& [t, name] : {std::pair<const at::Tensor&, const char*>{offsets, "offsets"},
+                                {kv_offsets, "kv_offsets"}, {kv_lengths, "kv_lengths"}}) {
+    if (!t.defined() && &t != &offsets) continue;
+    TORCH_CHECK(t.defined() && t.is_cuda() && t.dim() == 1 && t.scalar_type() == at::kInt && t.is_contiguous() &&
+                    t.device() == q.device(),
+                name, " must be a contiguous 1-D int32 tensor on q's device");
+  }
+  const int64_t n = offsets.numel() - 1;
+  TORCH_CHECK(n >= 0, "offsets must hold one entry more than there are samples");
+  TORCH_CHECK(!kv_offsets.defined() || kv_offsets.numel() == n + 1, "kv_offsets must have as many entries as offsets");
+  TORCH_CHECK(!kv_lengths.defined() || kv_lengths.numel() == n, "kv_lengths must have one entry per sample");
+  TORCH_CHECK(kv_offsets.defined() || k.size(0) == q.size(0), "q and k must have the same rows unless kv_offsets are given");
+  const double by = scale.value_or(1.0 / std::sqrt(static_cast<double>(q.size(2))));
+  if (!wants_gradient({q, k, v}))
+    return attention_forward({head_rows(q), head_rows(k), head_rows(v), offsets, kv_offsets, kv_lengths, causal, by}, nullptr);
+  auto none = at::empty({0}, offsets.options());
+  return PackedAttentionAutograd::apply(head_rows(q), head_rows(k), head_rows(v), offsets, kv_offsets.defined() ? kv_offsets : none,
+                                        kv_lengths.defined() ? kv_lengths : none, causal, by);
+}
+
+RiemannSelfAttentionImpl::RiemannSelfAttentionImpl(int64_t channels, int64_t num_heads, int64_t num_kv_heads, bool causal,
+                                                   bool bias)
+    : channels_(channels), heads_(num_heads), kv_heads_(num_kv_heads ? num_kv_heads : num_heads), causal_(causal) {
+  TORCH_CHECK(channels > 0 && num_heads > 0 && channels % num_heads == 0,
+              "Attention channels must be a positive multiple of the number of heads");
+  TORCH_CHECK(kv_heads_ > 0 && heads_ % kv_heads_ == 0,
+              "the number of query heads must be a multiple of the number of key heads");
+  dim_ = channels / num_heads;
+  qkv_ = register_module("qkv", torch::nn::Linear(torch::nn::LinearOptions(channels, (heads_ + 2 * kv_heads_) * dim_).bias(bias)));
+  projection_ = register_module("projection", torch::nn::Linear(torch::nn::LinearOptions(channels, channels).bias(bias)));
+}
+
+SparseTensor RiemannSelfAttentionImpl::forward(const SparseTensor& input) {
+  TORCH_CHECK(input.F().size(1) == channels_, "Input channel count does not match attention");
+  auto offsets = input.coordinate_manager()->sample_offsets(input.coordinate_map_key());
+  auto parts = qkv_->forward(input.F()).view({-1, heads_ + 2 * kv_heads_, dim_}).split_with_sizes({heads_, kv_heads_, kv_heads_}, 1);
+  auto out = packed_attention(parts[0], parts[1], parts[2], offsets, {}, {}, causal_);
+  return SparseTensor(projection_->forward(out.reshape({-1, channels_})), input.coordinate_map_key(), input.coordinate_manager());
 }
 
 RiemannConvolutionImpl::RiemannConvolutionImpl(int in_channels, int out_channels, int kernel_size, int stride,

@@ -171,6 +171,10 @@ public:
   // (zeros, ""). Returns the key and whether the map was created by this call. Rows are numbered by first
   // occurrence of the batch index in the seed map (the reference numbers them in hash-iteration order).
   std::pair<CoordinateMapKey, bool> origin();
+  // int32 [samples + 1] on the device: the first row of every sample of a map in row order, and the number of rows: the offsets of
+  // packed_attention. Made once per map (it waits for the device then). The rows of a sample have to be adjacent, as they
+  // are where the coordinates were inserted sample by sample.
+  at::Tensor sample_offsets(const CoordinateMapKey& key);
   // Union of maps of one tensor stride (engine/grid/space.hpp:862-863, space_impl.hpp:896-914): sets out_key to the
   // merged map and returns one int64 [2, N_i] tensor per input map (row in that map, row in the merged map).
   std::vector<at::Tensor> union_map(const std::vector<CoordinateMapKey>& in_keys, CoordinateMapKey& out_key);
@@ -234,7 +238,7 @@ private:
   CoordinateMapBackend::Type map_type_;
   std::map<coordinate_map_key_type, Map> maps_;
   std::map<std::string, std::shared_ptr<KernelMap>> kernel_maps_, ordered_maps_;
-  std::map<coordinate_map_key_type, at::Tensor> fields_;
+  std::map<coordinate_map_key_type, at::Tensor> fields_, sample_offsets_;
 };
 
 class SparseTensor {
@@ -437,6 +441,47 @@ private:
 TORCH_MODULE(RiemannBatchNorm);
 using RiemannSyncBatchNormImpl = RiemannBatchNormImpl;  // as in the reference (normalization.hpp:36-37)
 using RiemannSyncBatchNorm = RiemannBatchNorm;
+
+// Layer norm over the channels of a feature matrix [N, C], differentiable (once) in all three; weight and bias may be undefined.
+at::Tensor layer_norm(const at::Tensor& x, const at::Tensor& weight = {}, const at::Tensor& bias = {}, double eps = 1e-5);
+
+// Layer norm over the channels of every row. `normalization` is the torch layer that holds the parameters, as in
+// RiemannBatchNorm; the pass runs on the library's kernels.
+class RiemannLayerNormImpl : public torch::nn::Module {
+public:
+  RiemannLayerNormImpl(int64_t num_features, double eps = 1e-5, bool elementwise_affine = true);
+  SparseTensor forward(const SparseTensor& input);
+  torch::nn::LayerNorm normalization() { return normalization_; }
+
+private:
+  torch::nn::LayerNorm normalization_{nullptr};
+};
+TORCH_MODULE(RiemannLayerNorm);
+
+// softmax(scale q k^T) v within packed samples, differentiable (once) in q, k and v. q [rows, heads, channels], k and v
+// [key rows, key heads, channels] with any row and head strides, heads a multiple of key heads; offsets int32 [samples + 1]: first
+// row of every sample and the end of the last. kv_offsets where the keys' rows are others than the queries', kv_lengths [samples]
+// where only the first rows of a sample's keys are in use (a cache). causal is aligned at the end of the keys. scale: channels ^ -1/2
+// unless given. Rows of no sample, and rows that see no key, are zero.
+at::Tensor packed_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& offsets,
+                            const at::Tensor& kv_offsets = {}, const at::Tensor& kv_lengths = {}, bool causal = false,
+                            c10::optional<double> scale = c10::nullopt);
+
+// Self-attention of the rows of a SparseTensor within their sample: `qkv` projects the features to queries, keys and values,
+// packed_attention runs on CoordinateManager::sample_offsets, `projection` mixes the heads. num_kv_heads 0: as many as heads.
+class RiemannSelfAttentionImpl : public torch::nn::Module {
+public:
+  RiemannSelfAttentionImpl(int64_t channels, int64_t num_heads, int64_t num_kv_heads = 0, bool causal = false, bool bias = true);
+  SparseTensor forward(const SparseTensor& input);
+  torch::nn::Linear qkv() { return qkv_; }
+  torch::nn::Linear projection() { return projection_; }
+
+private:
+  int64_t channels_, heads_, kv_heads_, dim_;
+  bool causal_;
+  torch::nn::Linear qkv_{nullptr}, projection_{nullptr};
+};
+TORCH_MODULE(RiemannSelfAttention);
 
 // Inference-only conv -> batch norm -> ReLU as one kernel; `bn` may be an empty holder (bias + ReLU only).
 SparseTensor fused_conv_bn_relu(const SparseTensor& input, RiemannConvolutionBaseImpl& conv,

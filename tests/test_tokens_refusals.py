@@ -1,0 +1,93 @@
+"""Layer norm and packed attention: what the C ABI refuses before it touches a GPU, and what the hosts refuse of CPU tensors."""
+import ctypes
+
+import pytest
+import torch
+
+from riemannengine_b200 import capi, engine
+
+
+def test_layer_norm_arguments():
+    lib = capi.lib()
+    p = ctypes.c_void_p(16)  # never read: every call below is refused or has nothing to do
+    ok = dict(x=p, ld=64, n=4, c=64, g=p, b=p, pt=0, eps=1e-5, out=p, mean=None, inv=None, dt=0)
+
+    def forward(**change):
+        a = {**ok, **change}
+        return lib.rmn_layer_norm_forward(a["x"], a["ld"], a["n"], a["c"], a["g"], a["b"], a["pt"], a["eps"], a["out"], a["mean"],
+                                          a["inv"], a["dt"], None)
+
+    for change in (dict(c=0), dict(c=65537), dict(dt=2), dict(pt=7), dict(x=None), dict(out=None), dict(mean=p), dict(inv=p),
+                   dict(ld=-1), dict(eps=-1.0), dict(eps=float("nan")), dict(n=1 << 31)):
+        assert forward(**change) == capi.ERR_BAD_ARG, change
+    assert forward(n=0, x=None, out=None) == capi.OK
+    assert forward(c=40_000) == capi.ERR_UNSUPPORTED
+    assert forward(c=4097, ld=4097) == capi.ERR_UNSUPPORTED
+    assert lib.rmn_layer_norm_backward_workspace_bytes(10, 64) == 10 * 2 * 64 * 4
+    assert lib.rmn_layer_norm_backward_workspace_bytes(1 << 20, 64) == 592 * 2 * 64 * 4
+
+    def backward(dy=p, x=p, n=4, c=64, mean=p, inv=p, dx=p, dg=p, db=p, ws=p, nbytes=1 << 20, dt=0):
+        return lib.rmn_layer_norm_backward(dy, 64, x, 64, n, c, p, 0, mean, inv, dx, dg, db, dt, ws, nbytes, None)
+
+    assert backward(dy=None) == backward(x=None) == backward(mean=None) == backward(inv=None) == capi.ERR_BAD_ARG
+    assert backward(ws=None) == backward(ws=ctypes.c_void_p(20)) == backward(dt=3) == capi.ERR_BAD_ARG
+    assert backward(nbytes=100) == capi.ERR_ALLOC
+    assert backward(dx=None, dg=None, db=None) == capi.OK
+
+
+def _problem(**change):
+    p = capi.Attention()
+    for name in ("q", "k", "v", "offsets"):
+        setattr(p, name, 16)
+    p.q_row = p.k_row = p.v_row = 128
+    p.q_head = p.k_head = p.v_head = 32
+    p.rows_q = p.rows_k = 10
+    p.sequences, p.heads, p.kv_heads, p.dim, p.scale = 2, 4, 4, 32, 0.1
+    for name, value in change.items():
+        setattr(p, name, value)
+    return p
+
+
+def test_attention_arguments():
+    lib = capi.lib()
+    p = ctypes.c_void_p(16)
+    bad = (dict(heads=0), dict(kv_heads=0), dict(kv_heads=3), dict(heads=65537), dict(dim=0), dict(dtype=2), dict(offsets=None),
+           dict(q=None), dict(k=None), dict(v=None), dict(q_row=-1), dict(v_head=-3), dict(rows_k=11), dict(scale=float("nan")),
+           dict(rows_q=1 << 31), dict(rows_k=1 << 31), dict(sequences=(1 << 32) - 1))
+    for change in bad:
+        problem = _problem(**change)
+        assert lib.rmn_attention_forward(ctypes.byref(problem), p, None, p, 1 << 30, None) == capi.ERR_BAD_ARG, change
+        assert lib.rmn_attention_backward(ctypes.byref(problem), p, p, p, 128, 32, p, p, p, p, 1 << 30, None) == capi.ERR_BAD_ARG
+    assert lib.rmn_attention_forward(None, p, None, p, 0, None) == capi.ERR_BAD_ARG
+    assert lib.rmn_attention_forward(ctypes.byref(_problem(dim=257)), p, None, p, 1 << 30, None) == capi.ERR_UNSUPPORTED
+
+
+def test_sample_offsets_arguments():
+    lib = capi.lib()
+    p = ctypes.c_void_p(16)
+    nbytes = lib.rmn_sample_offsets_workspace_bytes(3)
+    assert lib.rmn_sample_offsets(p, 5, 1, 3, p, p, nbytes, None) == capi.ERR_BAD_ARG
+    assert lib.rmn_sample_offsets(None, 5, 4, 3, p, p, nbytes, None) == capi.ERR_BAD_ARG
+    assert lib.rmn_sample_offsets(p, 5, 4, 3, None, p, nbytes, None) == capi.ERR_BAD_ARG
+    assert lib.rmn_sample_offsets(p, 5, 4, 3, p, None, nbytes, None) == capi.ERR_BAD_ARG
+    assert lib.rmn_sample_offsets(p, 5, 4, 3, p, p, nbytes - 1, None) == capi.ERR_ALLOC
+
+
+def _hosts():
+    from riemannengine_b200 import cpp
+    return (engine, cpp.load())
+
+
+def test_hosts_refuse_cpu_tensors_and_bad_layers():
+    x, o = torch.zeros(4, 2, 8), torch.tensor([0, 4], dtype=torch.int32)
+    for host in _hosts():
+        with pytest.raises(RuntimeError, match="CUDA"):
+            host.layer_norm(torch.zeros(3, 8))
+        with pytest.raises(RuntimeError, match="CUDA"):
+            host.packed_attention(x, x, x, o)
+        with pytest.raises(RuntimeError, match="multiple"):
+            host.RiemannSelfAttention(30, 4)
+        with pytest.raises(RuntimeError, match="multiple"):
+            host.RiemannSelfAttention(32, 4, 3)
+        layer = host.RiemannSelfAttention(32, 4, 2)
+        assert tuple(dict(layer.named_parameters())["qkv.weight"].shape) == (64, 32)
