@@ -117,9 +117,9 @@ SIGNATURES = {
     "rmn_sample_offsets_workspace_bytes": (c_size_t, [c_uint32]),
     "rmn_sample_offsets": (c_int, [c_void_p, c_uint32, c_int, c_uint32, c_void_p, c_void_p, c_size_t, c_void_p]),
     "rmn_attention_forward_workspace_bytes": (c_size_t, [c_void_p]),
-    "rmn_attention_forward": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "rmn_attention_forward": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
     "rmn_attention_backward_workspace_bytes": (c_size_t, [c_void_p]),
-    "rmn_attention_backward": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p,
+    "rmn_attention_backward": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p,
                                        c_void_p, c_void_p, c_size_t, c_void_p]),
     "rmn_comm_unique_id": (c_int, [c_void_p]),
     "rmn_comm_init": (c_int, [c_void_p, c_int, c_int, c_void_p]),

@@ -105,8 +105,9 @@ extern "C" size_t rmn_attention_forward_workspace_bytes(const rmn_attention* pro
   return 0;
 }
 
-extern "C" int rmn_attention_forward(const rmn_attention* problem, void* d_out, float* d_lse, void* d_workspace,
+extern "C" int rmn_attention_forward(const rmn_attention* problem, void* d_out, void* d_low, float* d_lse, void* d_workspace,
                                      size_t workspace_bytes, void* stream_) {
+  cudaStream_t stream = (cudaStream_t)stream_;
   (void)d_workspace;
   (void)workspace_bytes;
   AttnArgs a;
@@ -115,15 +116,20 @@ extern "C" int rmn_attention_forward(const rmn_attention* problem, void* d_out, 
   if (a.rows_q == 0) return RMN_OK;
   if (!d_out) return RMN_ERR_BAD_ARG;
   a.out = d_out;
+  a.low = problem->dtype == RMN_BF16 ? d_low : nullptr;
   a.lse = d_lse;
-  return attention_simt_forward(a, problem->dtype, (cudaStream_t)stream_);
+  if (problem->dtype == RMN_BF16) {
+    const int tc = attention_tc_forward(a, stream);
+    if (tc != RMN_ERR_UNSUPPORTED) return tc;
+  }
+  return attention_simt_forward(a, problem->dtype, stream);
 }
 
 extern "C" size_t rmn_attention_backward_workspace_bytes(const rmn_attention* problem) {
   return problem && problem->heads > 0 ? (size_t)problem->heads * problem->rows_q * sizeof(float) : 0;
 }
 
-extern "C" int rmn_attention_backward(const rmn_attention* problem, const void* d_out, const float* d_lse,
+extern "C" int rmn_attention_backward(const rmn_attention* problem, const void* d_out, const void* d_low, const float* d_lse,
                                       const void* d_grad_out, int64_t grad_row, int64_t grad_head, void* d_dq, void* d_dk,
                                       void* d_dv, void* d_workspace, size_t workspace_bytes, void* stream_) {
   cudaStream_t stream = (cudaStream_t)stream_;
@@ -144,6 +150,7 @@ extern "C" int rmn_attention_backward(const rmn_attention* problem, const void* 
   if (!d_out || !d_lse || !d_grad_out || !d_workspace || ((uintptr_t)d_workspace & 15)) return RMN_ERR_BAD_ARG;
   if (workspace_bytes < rmn_attention_backward_workspace_bytes(problem)) return RMN_ERR_ALLOC;
   a.fwd_out = d_out;
+  a.low = problem->dtype == RMN_BF16 ? const_cast<void*>(d_low) : nullptr;
   a.lse = const_cast<float*>(d_lse);
   a.grad = d_grad_out;
   a.grad_row = grad_row;

@@ -19,6 +19,7 @@ struct AttnArgs {
   float scale;                                          // of the scores
   uint32_t* status;                                     // device status word
   void* out;                                            // [rows_q, heads, dim]
+  void* low;                                            // what rounding took from out (bf16; may be NULL)
   float* lse;                                           // [heads, rows_q], natural logarithm (forward: may be NULL)
   // backward
   const void* grad;                                     // of the output
@@ -138,5 +139,6 @@ inline uint64_t most_tiles(uint64_t rows, uint64_t sequences, uint32_t tile_rows
 // The kernels behind rmn_attention_*: RMN_ERR_UNSUPPORTED where they do not cover the call.
 int attention_simt_forward(const AttnArgs& a, int dtype, cudaStream_t stream);
 int attention_simt_backward(const AttnArgs& a, int dtype, cudaStream_t stream);
+int attention_tc_forward(const AttnArgs& a, cudaStream_t stream);  // bf16
 
 }  // namespace rmn

@@ -215,8 +215,23 @@ __global__ void __launch_bounds__(kSimtThreads) k_attention_simt(const AttnArgs 
       a.lse[(size_t)head * a.rows_q + g.q0 + first + ty + 16 * i] = l[i] == 0.f ? -CUDART_INF_F : m[i] + logf(l[i]);
   }
   const int64_t out_row = (int64_t)a.heads * a.dim;
-  store_tile<T, DP, BM>(static_cast<T*>(a.out) + (int64_t)(g.q0 + first) * out_row + (int64_t)head * a.dim, out_row, rows,
-                        a.dim, tx, ty, o, by);
+  const int64_t at = (int64_t)(g.q0 + first) * out_row + (int64_t)head * a.dim;
+  store_tile<T, DP, BM>(static_cast<T*>(a.out) + at, out_row, rows, a.dim, tx, ty, o, by);
+  if constexpr (sizeof(T) == 2) {
+    if (!a.low) return;
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int e = 0; e < CW; ++e) {
+          const float x = o[i][c][e] * by[i];
+          o[i][c][e] = x - __bfloat162float(__float2bfloat16_rn(x));
+        }
+#pragma unroll
+    for (int i = 0; i < R; ++i) by[i] = 1.f;
+    store_tile<T, DP, BM>(static_cast<T*>(a.low) + at, out_row, rows, a.dim, tx, ty, o, by);
+  }
 }
 
 // dq of a query tile, and delta of its rows for the kernel of the key tiles
@@ -247,6 +262,9 @@ __global__ void __launch_bounds__(kSimtThreads) k_attention_simt_dq(const AttnAr
                        a.grad_row, rows, a.dim, 1.f);
   load_tile<T, DP, BM>(s_k, static_cast<const T*>(a.fwd_out) + (int64_t)(g.q0 + first) * out_row + (int64_t)head * a.dim,
                        out_row, rows, a.dim, 1.f);
+  if (a.low)
+    load_tile<T, DP, BM>(s_v, static_cast<const T*>(a.low) + (int64_t)(g.q0 + first) * out_row + (int64_t)head * a.dim, out_row,
+                         rows, a.dim, 1.f);
   __syncthreads();
   float o[R][NC][CW] = {}, delta[R], lse[R];
   int seen[R];
@@ -254,7 +272,8 @@ __global__ void __launch_bounds__(kSimtThreads) k_attention_simt_dq(const AttnAr
   for (int i = 0; i < R; ++i) {
     const int r = ty + 16 * i;
     float d = 0.f;
-    for (int c = tx; c < DP; c += 16) d = fmaf(s_g[r * S::LD + c], s_k[r * S::LD + c], d);
+    for (int c = tx; c < DP; c += 16)
+      d = fmaf(s_g[r * S::LD + c], s_k[r * S::LD + c] + (a.low ? s_v[r * S::LD + c] : 0.f), d);
 #pragma unroll
     for (int w = 8; w > 0; w >>= 1) d += __shfl_xor_sync(0xffffffffu, d, w, 16);
     delta[i] = d;

@@ -1,0 +1,109 @@
+// What the tensor-core attention kernels share.
+#pragma once
+
+#include "rmn_attention.cuh"
+#include "rmn_tma.cuh"
+
+namespace rmn {
+
+void count_tc_launch();  // defined in rmn_conv_tc.cu
+
+namespace tc {
+
+constexpr uint32_t kAtomBytes = 128 * 128;  // 128 rows of 64 bf16: one 128-byte swizzled box
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+__device__ __forceinline__ float exp2_approx(float x) {  // 2 ulp; results below 2^-126 are zero
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&b);
+}
+
+#define RMN_TC_REGS16(r, o)                                                                                               \
+  "r"(r[o + 0]), "r"(r[o + 1]), "r"(r[o + 2]), "r"(r[o + 3]), "r"(r[o + 4]), "r"(r[o + 5]), "r"(r[o + 6]), "r"(r[o + 7]), \
+      "r"(r[o + 8]), "r"(r[o + 9]), "r"(r[o + 10]), "r"(r[o + 11]), "r"(r[o + 12]), "r"(r[o + 13]), "r"(r[o + 14]),       \
+      "r"(r[o + 15])
+// 16 (32) columns of the warp's 32 lanes: register i of thread t is column i of lane t
+template <int FIRST, int N>
+__device__ __forceinline__ void tc_st16(uint32_t taddr, const uint32_t (&r)[N]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16};" ::"r"(taddr),
+      RMN_TC_REGS16(r, FIRST)
+      : "memory");
+}
+template <int FIRST, int N>
+__device__ __forceinline__ void tc_st32(uint32_t taddr, const uint32_t (&r)[N]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      RMN_TC_REGS16(r, FIRST), RMN_TC_REGS16(r, FIRST + 16)
+      : "memory");
+}
+#undef RMN_TC_REGS16
+
+// 32 columns into r[FIRST ... FIRST + 31]
+template <int FIRST, int N>
+__device__ __forceinline__ void tc_ld32_at(uint32_t taddr, uint32_t (&r)[N]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[FIRST + 0]), "=r"(r[FIRST + 1]), "=r"(r[FIRST + 2]), "=r"(r[FIRST + 3]), "=r"(r[FIRST + 4]),
+        "=r"(r[FIRST + 5]), "=r"(r[FIRST + 6]), "=r"(r[FIRST + 7]), "=r"(r[FIRST + 8]), "=r"(r[FIRST + 9]),
+        "=r"(r[FIRST + 10]), "=r"(r[FIRST + 11]), "=r"(r[FIRST + 12]), "=r"(r[FIRST + 13]), "=r"(r[FIRST + 14]),
+        "=r"(r[FIRST + 15]), "=r"(r[FIRST + 16]), "=r"(r[FIRST + 17]), "=r"(r[FIRST + 18]), "=r"(r[FIRST + 19]),
+        "=r"(r[FIRST + 20]), "=r"(r[FIRST + 21]), "=r"(r[FIRST + 22]), "=r"(r[FIRST + 23]), "=r"(r[FIRST + 24]),
+        "=r"(r[FIRST + 25]), "=r"(r[FIRST + 26]), "=r"(r[FIRST + 27]), "=r"(r[FIRST + 28]), "=r"(r[FIRST + 29]),
+        "=r"(r[FIRST + 30]), "=r"(r[FIRST + 31])
+      : "r"(taddr)
+      : "memory");
+}
+
+// D[128, n] (+)= A[128, 16 steps] B[n, 16 steps]^T, both K-major tiles of kAtomBytes atoms in shared memory
+__device__ __forceinline__ void mma_rows(uint32_t d_tmem, uint32_t a_s, uint32_t b_s, uint32_t idesc, int steps) {
+  constexpr uint64_t DESC = smem_desc_sw_const(16, 1024, 2u);
+  for (int j = 0; j < steps; ++j) {
+    const uint32_t at = (uint32_t)(j >> 2) * kAtomBytes + (uint32_t)(j & 3) * 32u;
+    tc_mma_bf16_elect(d_tmem, DESC + ((a_s + at) >> 4), DESC + ((b_s + at) >> 4), idesc, j != 0);
+  }
+}
+// D[128, n] (+)= A[128, 128] B[128, n]: A in tensor memory, B a tile whose rows are the 128 summed over (MN-major)
+__device__ __forceinline__ void mma_columns(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_s, uint32_t idesc, bool accumulate) {
+  constexpr uint64_t DESC = smem_desc_sw_const(kAtomBytes, 1024, 2u);
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    tc_mma_bf16_ta_elect(d_tmem, a_tmem + j * 8, DESC + ((b_s + (uint32_t)j * 2048u) >> 4), idesc, accumulate || j != 0);
+}
+
+// One warp: rows [from, 128) of a tile of `atoms` atoms become zeros (a masked weight of zero times what lies there must be zero)
+__device__ __forceinline__ void zero_rows(uint32_t tile_s, int from, int atoms) {
+  const int lane = threadIdx.x & 31;
+  for (int a = 0; a < atoms; ++a)
+    for (uint32_t at = (uint32_t)from * 128u + lane * 16u; at < kAtomBytes; at += 512u)
+      asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(tile_s + a * kAtomBytes + at), "r"(0u) : "memory");
+  fence_proxy_async();
+  __syncwarp();
+}
+
+// [rows, heads, dim] bf16 as a tensor map with boxes of 64 channels of one head in 128 rows; columns behind `dim` and rows
+// behind `rows` read as zeros. False where strides or alignment do not allow it.
+inline bool make_head_map(CUtensorMap* map, const void* base, uint32_t rows, int heads, int dim, int64_t row, int64_t head) {
+  EncodeTiledFn fn = encode_tiled_fn();
+  if (heads == 1) head = dim;
+  if (rows == 1) row = dim;
+  if (!fn || ((uintptr_t)base & 15) || dim % 8 || row % 8 || head % 8 || row <= 0 || head <= 0) return false;
+  const cuuint64_t dims[3] = {(cuuint64_t)dim, (cuuint64_t)heads, (cuuint64_t)rows};
+  const cuuint64_t strides[2] = {(cuuint64_t)head * 2, (cuuint64_t)row * 2};
+  const cuuint32_t box[3] = {64, 1, 128}, estr[3] = {1, 1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+}  // namespace tc
+}  // namespace rmn

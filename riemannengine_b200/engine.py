@@ -1085,16 +1085,16 @@ class _PackedAttentionFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, offsets, kv_offsets, kv_lengths, causal: bool, scale):
         train = builtins.any(ctx.needs_input_grad)
-        out, lse = ops.attention_forward(q, k, v, offsets, kv_offsets, kv_lengths, causal, scale, want_lse=train)
-        ctx.save_for_backward(q, k, v, out, lse, offsets, kv_offsets, kv_lengths)
+        out, low, lse = ops.attention_forward(q, k, v, offsets, kv_offsets, kv_lengths, causal, scale, want_stats=train)
+        ctx.save_for_backward(q, k, v, out, low, lse, offsets, kv_offsets, kv_lengths)
         ctx.causal, ctx.scale = causal, scale
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_out):
-        q, k, v, out, lse, offsets, kv_offsets, kv_lengths = ctx.saved_tensors
-        return (*ops.attention_backward(grad_out, q, k, v, out, lse, offsets, kv_offsets, kv_lengths, ctx.causal, ctx.scale),
+        q, k, v, out, low, lse, offsets, kv_offsets, kv_lengths = ctx.saved_tensors
+        return (*ops.attention_backward(grad_out, q, k, v, out, low, lse, offsets, kv_offsets, kv_lengths, ctx.causal, ctx.scale),
                 None, None, None, None, None)
 
 

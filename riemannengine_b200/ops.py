@@ -696,24 +696,26 @@ def _attention(q, k, v, offsets, kv_offsets, kv_lengths, causal, scale) -> capi.
 
 def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: torch.Tensor,
                       kv_offsets: Optional[torch.Tensor] = None, kv_lengths: Optional[torch.Tensor] = None,
-                      causal: bool = False, scale: Optional[float] = None, want_lse: bool = False):
+                      causal: bool = False, scale: Optional[float] = None, want_stats: bool = False):
     """Attention within packed samples (rmn_attention_forward): ``q`` [rows, heads, channels], ``k`` and ``v``
-    [key rows, key heads, channels], any row and head strides; returns (out, lse), lse float32 [heads, rows] or None."""
+    [key rows, key heads, channels], any row and head strides; returns (out, low, lse). Unless ``want_stats`` the last two are
+    None; else what the backward pass needs: lse float32 [heads, rows], and for bfloat16 low, what rounding took from out."""
     q, k, v = _heads(q), _heads(k), _heads(v)
     p = _attention(q, k, v, offsets, kv_offsets, kv_lengths, causal, scale)
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty((p.heads, p.rows_q), dtype=torch.float32, device=q.device) if want_lse else None
+    lse = torch.empty((p.heads, p.rows_q), dtype=torch.float32, device=q.device) if want_stats else None
+    low = torch.empty_like(out) if want_stats and out.dtype == torch.bfloat16 else None
     lib = capi.lib()
     with torch.cuda.device(q.device):
         wbytes = lib.rmn_attention_forward_workspace_bytes(ctypes.byref(p))
         ws = torch.empty(wbytes, dtype=torch.uint8, device=q.device) if wbytes else None
-        capi.check(lib.rmn_attention_forward(ctypes.byref(p), _ptr(out), _ptr(lse), _ptr(ws), wbytes, _stream()),
+        capi.check(lib.rmn_attention_forward(ctypes.byref(p), _ptr(out), _ptr(low), _ptr(lse), _ptr(ws), wbytes, _stream()),
                    "rmn_attention_forward")
-    return out, lse
+    return out, low, lse
 
 
 def attention_backward(grad_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor,
-                       lse: torch.Tensor, offsets: torch.Tensor, kv_offsets: Optional[torch.Tensor] = None,
+                       low: Optional[torch.Tensor], lse: torch.Tensor, offsets: torch.Tensor, kv_offsets: Optional[torch.Tensor] = None,
                        kv_lengths: Optional[torch.Tensor] = None, causal: bool = False, scale: Optional[float] = None):
     """(dq, dk, dv) of attention_forward (rmn_attention_backward)."""
     q, k, v, grad_out = _heads(q), _heads(k), _heads(v), _heads(grad_out)
@@ -727,7 +729,7 @@ def attention_backward(grad_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor,
     with torch.cuda.device(q.device):
         wbytes = lib.rmn_attention_backward_workspace_bytes(ctypes.byref(p))
         ws = torch.empty(wbytes, dtype=torch.uint8, device=q.device)
-        capi.check(lib.rmn_attention_backward(ctypes.byref(p), _ptr(out), _ptr(lse), _ptr(grad_out), int(grad_out.stride(0)),
-                                              int(grad_out.stride(1)), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(ws), wbytes,
-                                              _stream()), "rmn_attention_backward")
+        capi.check(lib.rmn_attention_backward(ctypes.byref(p), _ptr(out), _ptr(low), _ptr(lse), _ptr(grad_out),
+                                              int(grad_out.stride(0)), int(grad_out.stride(1)), _ptr(dq), _ptr(dk), _ptr(dv),
+                                              _ptr(ws), wbytes, _stream()), "rmn_attention_backward")
     return dq, dk, dv

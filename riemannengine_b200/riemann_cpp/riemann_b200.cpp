@@ -1911,16 +1911,19 @@ struct AttentionInputs {
   }
 };
 
-// out, and where `lse` is given the logarithms of the sums of exponentials, float32 [heads, rows]
-at::Tensor attention_forward(const AttentionInputs& in, at::Tensor* lse) {
+// out; for a backward pass also the logarithms of the sums of exponentials, float32 [heads, rows], and in bf16 what rounding took
+// from out
+at::Tensor attention_forward(const AttentionInputs& in, at::Tensor* low, at::Tensor* lse) {
   c10::cuda::CUDAGuard guard(in.q.device());
   const rmn_attention p = in.problem();
   auto out = at::empty(in.q.sizes(), in.q.options());
   if (lse) *lse = at::empty({in.q.size(1), in.q.size(0)}, in.q.options().dtype(at::kFloat));
+  if (low) *low = at::empty(in.q.scalar_type() == at::kBFloat16 ? in.q.sizes() : at::IntArrayRef({0}), in.q.options());
   const size_t ws_bytes = rmn_attention_forward_workspace_bytes(&p);
   at::Tensor ws;
   if (ws_bytes) ws = at::empty({static_cast<int64_t>(ws_bytes)}, in.q.options().dtype(at::kByte));
-  check(rmn_attention_forward(&p, ptr(out), lse ? static_cast<float*>(ptr(*lse)) : nullptr, ptr(ws), ws_bytes, current_stream()),
+  check(rmn_attention_forward(&p, ptr(out), low ? ptr(*low) : nullptr, lse ? static_cast<float*>(ptr(*lse)) : nullptr, ptr(ws),
+                              ws_bytes, current_stream()),
         "rmn_attention_forward");
   return out;
 }
@@ -1929,9 +1932,9 @@ class PackedAttentionAutograd : public torch::autograd::Function<PackedAttention
 public:
   static at::Tensor forward(torch::autograd::AutogradContext* ctx, at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor offsets,
                             at::Tensor kv_offsets, at::Tensor kv_lengths, bool causal, double scale) {
-    at::Tensor lse;
-    auto out = attention_forward({q, k, v, offsets, kv_offsets, kv_lengths, causal, scale}, &lse);
-    ctx->save_for_backward({q, k, v, offsets, kv_offsets, kv_lengths, out, lse});
+    at::Tensor low, lse;
+    auto out = attention_forward({q, k, v, offsets, kv_offsets, kv_lengths, causal, scale}, &low, &lse);
+    ctx->save_for_backward({q, k, v, offsets, kv_offsets, kv_lengths, out, low, lse});
     ctx->saved_data["causal"] = causal;
     ctx->saved_data["scale"] = scale;
     return out;
@@ -1949,8 +1952,8 @@ public:
     auto dv = at::empty(in.v.sizes(), in.v.options());
     const size_t ws_bytes = rmn_attention_backward_workspace_bytes(&p);
     auto ws = at::empty({static_cast<int64_t>(ws_bytes)}, in.q.options().dtype(at::kByte));
-    check(rmn_attention_backward(&p, ptr(saved[6]), static_cast<const float*>(ptr(saved[7])), ptr(grad), grad.stride(0),
-                                 grad.stride(1), ptr(dq), ptr(dk), ptr(dv), ptr(ws), ws_bytes, current_stream()),
+    check(rmn_attention_backward(&p, ptr(saved[6]), ptr(saved[7]), static_cast<const float*>(ptr(saved[8])), ptr(grad),
+                                 grad.stride(0), grad.stride(1), ptr(dq), ptr(dk), ptr(dv), ptr(ws), ws_bytes, current_stream()),
           "rmn_attention_backward");
     return {dq, dk, dv, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
   }
@@ -2013,7 +2016,8 @@ at::Tensor packed_attention(const at::Tensor& q, const at::Tensor& k, const at::
   TORCH_CHECK(kv_offsets.defined() || k.size(0) == q.size(0), "q and k must have the same rows unless kv_offsets are given");
   const double by = scale.value_or(1.0 / std::sqrt(static_cast<double>(q.size(2))));
   if (!wants_gradient({q, k, v}))
-    return attention_forward({head_rows(q), head_rows(k), head_rows(v), offsets, kv_offsets, kv_lengths, causal, by}, nullptr);
+    return attention_forward({head_rows(q), head_rows(k), head_rows(v), offsets, kv_offsets, kv_lengths, causal, by}, nullptr,
+                             nullptr);
   auto none = at::empty({0}, offsets.options());
   return PackedAttentionAutograd::apply(head_rows(q), head_rows(k), head_rows(v), offsets, kv_offsets.defined() ? kv_offsets : none,
                                         kv_lengths.defined() ? kv_lengths : none, causal, by);

@@ -56,10 +56,10 @@ def test_attention_arguments():
            dict(rows_q=1 << 31), dict(rows_k=1 << 31), dict(sequences=(1 << 32) - 1))
     for change in bad:
         problem = _problem(**change)
-        assert lib.rmn_attention_forward(ctypes.byref(problem), p, None, p, 1 << 30, None) == capi.ERR_BAD_ARG, change
-        assert lib.rmn_attention_backward(ctypes.byref(problem), p, p, p, 128, 32, p, p, p, p, 1 << 30, None) == capi.ERR_BAD_ARG
-    assert lib.rmn_attention_forward(None, p, None, p, 0, None) == capi.ERR_BAD_ARG
-    assert lib.rmn_attention_forward(ctypes.byref(_problem(dim=257)), p, None, p, 1 << 30, None) == capi.ERR_UNSUPPORTED
+        assert lib.rmn_attention_forward(ctypes.byref(problem), p, None, None, p, 1 << 30, None) == capi.ERR_BAD_ARG, change
+        assert lib.rmn_attention_backward(ctypes.byref(problem), p, None, p, p, 128, 32, p, p, p, p, 1 << 30, None) == capi.ERR_BAD_ARG
+    assert lib.rmn_attention_forward(None, p, None, None, p, 0, None) == capi.ERR_BAD_ARG
+    assert lib.rmn_attention_forward(ctypes.byref(_problem(dim=257)), p, None, None, p, 1 << 30, None) == capi.ERR_UNSUPPORTED
 
 
 def test_sample_offsets_arguments():
