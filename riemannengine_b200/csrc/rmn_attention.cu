@@ -157,5 +157,9 @@ extern "C" int rmn_attention_backward(const rmn_attention* problem, const void* 
   a.grad_head = grad_head;
   a.delta = static_cast<float*>(d_workspace);
   a.dq = d_dq; a.dk = d_dk; a.dv = d_dv;
+  if (problem->dtype == RMN_BF16) {
+    const int tc = attention_tc_backward(a, stream);
+    if (tc != RMN_ERR_UNSUPPORTED) return tc;
+  }
   return attention_simt_backward(a, problem->dtype, stream);
 }

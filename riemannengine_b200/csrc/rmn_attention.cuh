@@ -140,5 +140,6 @@ inline uint64_t most_tiles(uint64_t rows, uint64_t sequences, uint32_t tile_rows
 int attention_simt_forward(const AttnArgs& a, int dtype, cudaStream_t stream);
 int attention_simt_backward(const AttnArgs& a, int dtype, cudaStream_t stream);
 int attention_tc_forward(const AttnArgs& a, cudaStream_t stream);  // bf16
+int attention_tc_backward(const AttnArgs& a, cudaStream_t stream);
 
 }  // namespace rmn

@@ -72,12 +72,15 @@ __device__ __forceinline__ void mma_rows(uint32_t d_tmem, uint32_t a_s, uint32_t
     tc_mma_bf16_elect(d_tmem, DESC + ((a_s + at) >> 4), DESC + ((b_s + at) >> 4), idesc, j != 0);
   }
 }
-// D[128, n] (+)= A[128, 128] B[128, n]: A in tensor memory, B a tile whose rows are the 128 summed over (MN-major)
+// D[128, n] (+)= A[128, 128] B[128, n]: A in tensor memory, its two halves of 32 columns HALF apart, B a tile whose rows are the
+// 128 summed over (MN-major)
+template <int HALF = 32>
 __device__ __forceinline__ void mma_columns(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_s, uint32_t idesc, bool accumulate) {
   constexpr uint64_t DESC = smem_desc_sw_const(kAtomBytes, 1024, 2u);
 #pragma unroll
   for (int j = 0; j < 8; ++j)
-    tc_mma_bf16_ta_elect(d_tmem, a_tmem + j * 8, DESC + ((b_s + (uint32_t)j * 2048u) >> 4), idesc, accumulate || j != 0);
+    tc_mma_bf16_ta_elect(d_tmem, a_tmem + (j >> 2) * HALF + (j & 3) * 8, DESC + ((b_s + (uint32_t)j * 2048u) >> 4), idesc,
+                         accumulate || j != 0);
 }
 
 // One warp: rows [from, 128) of a tile of `atoms` atoms become zeros (a masked weight of zero times what lies there must be zero)
