@@ -676,15 +676,16 @@ typedef struct {
   float scale;
 } rmn_attention;
 
-/* Scratch bytes of rmn_attention_forward (may be 0). Depends on sizes only. */
+/* Scratch bytes of rmn_attention_forward (often 0; few query rows a sample are summed over chunks of their keys there). Depends on
+ * sizes only. */
 size_t rmn_attention_forward_workspace_bytes(const rmn_attention *problem);
 /*
  * out[i, h] = sum_j softmax_j(scale q[i, h] . k[j, h']) v[j, h'] over the keys that row i sees: [rows_q, heads, dim] without
  * gaps. A row that sees no key, and a row of no sample, is zero. d_lse [heads, rows_q] (may be NULL): logarithm of the sum of
  * exponentials, -infinity for such a row; the backward pass needs it. d_low (bf16; may be NULL, and is not written in fp32): what
  * rounding took from out, as bf16 [rows_q, heads, dim]; with it the backward pass is as exact as with an unrounded output. Sums and softmax in fp32. A non-finite value in a
- * row of k or v may reach every row of its own sample and head, never those of another. The workspace may be shared by calls on one
- * stream, not by calls that run at the same time.
+ * row of k or v may reach every row of its own sample and head, never those of another. d_workspace: 16-byte aligned; it may be
+ * shared by calls on one stream, not by calls that run at the same time.
  */
 int rmn_attention_forward(const rmn_attention *problem, void *d_out, void *d_low, float *d_lse, void *d_workspace,
                           size_t workspace_bytes, void *stream);

@@ -67,6 +67,9 @@ int arguments(const rmn_attention* p, AttnArgs* a) {
   a->kv_lengths = p->kv_lengths;
   a->causal = p->causal != 0;
   a->scale = p->scale;
+  return RMN_OK;
+}
+int find_status(AttnArgs* a) {
   a->status = const_cast<uint32_t*>(tc_status_device_address());
   return a->status ? RMN_OK : RMN_ERR_CUDA;
 }
@@ -100,24 +103,30 @@ extern "C" int rmn_sample_offsets(const int32_t* d_coords, uint32_t n_rows, int 
   return RMN_OK;
 }
 
-extern "C" size_t rmn_attention_forward_workspace_bytes(const rmn_attention* problem) {
-  (void)problem;
-  return 0;
+extern "C" size_t rmn_attention_forward_workspace_bytes(const rmn_attention* p) {
+  if (!p || p->heads < 1 || p->kv_heads < 1 || p->heads % p->kv_heads || p->dim < 1) return 0;
+  return attention_rows_workspace(p->rows_q, p->rows_k, p->sequences, p->heads, p->kv_heads, p->dim, p->dtype);
 }
 
 extern "C" int rmn_attention_forward(const rmn_attention* problem, void* d_out, void* d_low, float* d_lse, void* d_workspace,
                                      size_t workspace_bytes, void* stream_) {
   cudaStream_t stream = (cudaStream_t)stream_;
-  (void)d_workspace;
-  (void)workspace_bytes;
   AttnArgs a;
   const int st = arguments(problem, &a);
   if (st != RMN_OK) return st;
   if (a.rows_q == 0) return RMN_OK;
-  if (!d_out) return RMN_ERR_BAD_ARG;
+  const size_t need = rmn_attention_forward_workspace_bytes(problem);
+  if (!d_out || (need && (!d_workspace || ((uintptr_t)d_workspace & 15)))) return RMN_ERR_BAD_ARG;
+  if (workspace_bytes < need) return RMN_ERR_ALLOC;
+  const int found = find_status(&a);
+  if (found != RMN_OK) return found;
   a.out = d_out;
   a.low = problem->dtype == RMN_BF16 ? d_low : nullptr;
   a.lse = d_lse;
+  if (need) {
+    const int rows = attention_rows_forward(a, problem->dtype, d_workspace, stream);
+    if (rows != RMN_ERR_UNSUPPORTED) return rows;
+  }
   if (problem->dtype == RMN_BF16) {
     const int tc = attention_tc_forward(a, stream);
     if (tc != RMN_ERR_UNSUPPORTED) return tc;
@@ -149,6 +158,8 @@ extern "C" int rmn_attention_backward(const rmn_attention* problem, const void* 
   }
   if (!d_out || !d_lse || !d_grad_out || !d_workspace || ((uintptr_t)d_workspace & 15)) return RMN_ERR_BAD_ARG;
   if (workspace_bytes < rmn_attention_backward_workspace_bytes(problem)) return RMN_ERR_ALLOC;
+  const int found = find_status(&a);
+  if (found != RMN_OK) return found;
   a.fwd_out = d_out;
   a.low = problem->dtype == RMN_BF16 ? const_cast<void*>(d_low) : nullptr;
   a.lse = const_cast<float*>(d_lse);

@@ -80,57 +80,82 @@ __device__ __forceinline__ int32_t first_query(const Segment& g, int32_t j, int 
   return causal ? max(0, j - (g.n_k - g.n_q)) : 0;
 }
 
-// Tiles of `tile_rows` rows of all segments, one behind the other: finds the segment of tile `want` and the tile's number in
-// it; false where there are no so many tiles. kKeys: tiles of key rows (the whole slots), else of query rows. All threads
-// of the block call it (kThreads of them); `found` is shared memory. Every thread counts the tiles of a run of
-// segments, a scan over the block places them.
+// Tiles of `tile_rows` rows of all segments, one behind the other: of query rows, of key rows (whole slots), or of keys in use.
+enum class TilesOf { kQueries, kSlots, kKeys };
+template <TilesOf kOf>
+__device__ __forceinline__ int32_t segment_tiles(const Segment& g, int tile_rows) {
+  const int32_t rows = kOf == TilesOf::kQueries ? g.n_q : kOf == TilesOf::kSlots ? g.k_slot : g.n_k;
+  return (rows + tile_rows - 1) / tile_rows;
+}
 struct FoundTile {
   Segment g;
   int32_t tile, tiles;  // number of the tile in its segment, and the segment's tiles
+  uint32_t segment;
 };
-template <int kThreads, bool kKeys>
-__device__ __forceinline__ bool find_tile(const AttnArgs& a, uint32_t want, int tile_rows, FoundTile* found, int32_t* warp_sums) {
+// All threads of the block (kThreads) count: each a run of segments, a scan over the block places them.
+struct TileScan {
+  uint32_t lo, hi;            // this thread's segments
+  int32_t first, mine, total; // tiles before them, theirs, all
+  Segment g;                  // the last of them
+};
+template <int kThreads, TilesOf kOf>
+__device__ __forceinline__ TileScan scan_tiles(const AttnArgs& a, int tile_rows, int32_t* warp_sums) {
+  TileScan t;
   const uint32_t n = a.sequences + 2;
   const uint32_t per = (n + kThreads - 1) / kThreads;
-  const uint32_t lo = threadIdx.x * per, hi = min(lo + per, n);
-  int32_t mine = 0;
-  Segment g = {};
-  for (uint32_t s = lo; s < hi; ++s) {
-    g = segment(a, s);
-    mine += ((kKeys ? g.k_slot : g.n_q) + tile_rows - 1) / tile_rows;
+  t.lo = min(threadIdx.x * per, n);
+  t.hi = min(t.lo + per, n);
+  t.mine = 0;
+  t.g = {};
+  for (uint32_t s = t.lo; s < t.hi; ++s) {
+    t.g = segment(a, s);
+    t.mine += segment_tiles<kOf>(t.g, tile_rows);
   }
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int32_t upto = mine;
+  int32_t upto = t.mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int32_t t = __shfl_up_sync(0xffffffffu, upto, o);
-    if (lane >= o) upto += t;
+    const int32_t v = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += v;
   }
   if (lane == 31) warp_sums[warp] = upto;
   __syncthreads();
-  int32_t before = 0, total = 0;
+  t.first = upto - t.mine;
+  t.total = 0;
 #pragma unroll
   for (int w = 0; w < kThreads / 32; ++w) {
-    if (w < warp) before += warp_sums[w];
-    total += warp_sums[w];
+    if (w < warp) t.first += warp_sums[w];
+    t.total += warp_sums[w];
   }
-  const bool exists = want < (uint32_t)total;
-  int32_t first = before + upto - mine;
-  if (exists && (int32_t)want >= first && (int32_t)want < first + mine) {
-    for (uint32_t s = lo; s < hi; ++s) {
-      if (per > 1) g = segment(a, s);
-      const int32_t tiles = ((kKeys ? g.k_slot : g.n_q) + tile_rows - 1) / tile_rows;
-      if ((int32_t)want < first + tiles) {
+  return t;
+}
+// The segment of tile `want` (below t.total) into shared memory.
+template <TilesOf kOf>
+__device__ __forceinline__ void pick_tile(const AttnArgs& a, const TileScan& t, int32_t want, int tile_rows, FoundTile* found) {
+  int32_t first = t.first;
+  if (want >= first && want < first + t.mine) {
+    for (uint32_t s = t.lo; s < t.hi; ++s) {
+      const Segment g = t.hi - t.lo > 1 ? segment(a, s) : t.g;
+      const int32_t tiles = segment_tiles<kOf>(g, tile_rows);
+      if (want < first + tiles) {
         found->g = g;
-        found->tile = (int32_t)want - first;
+        found->tile = want - first;
         found->tiles = tiles;
+        found->segment = s;
         break;
       }
       first += tiles;
     }
   }
   __syncthreads();
-  return exists;
+}
+// Both; false where there are no so many tiles.
+template <int kThreads, TilesOf kOf>
+__device__ __forceinline__ bool find_tile(const AttnArgs& a, uint32_t want, int tile_rows, FoundTile* found, int32_t* warp_sums) {
+  const TileScan t = scan_tiles<kThreads, kOf>(a, tile_rows, warp_sums);
+  if (want >= (uint32_t)max(t.total, 0)) return false;
+  pick_tile<kOf>(a, t, (int32_t)want, tile_rows, found);
+  return true;
 }
 
 // How many tiles find_tile may be asked for at most: with valid offsets every segment's last tile may be a part of one.
@@ -141,5 +166,8 @@ int attention_simt_forward(const AttnArgs& a, int dtype, cudaStream_t stream);
 int attention_simt_backward(const AttnArgs& a, int dtype, cudaStream_t stream);
 int attention_tc_forward(const AttnArgs& a, cudaStream_t stream);  // bf16
 int attention_tc_backward(const AttnArgs& a, cudaStream_t stream);
+// few query rows a sample: chunks of the keys, then their sum. Scratch bytes, 0 where this form is not meant for the sizes
+size_t attention_rows_workspace(uint32_t rows_q, uint32_t rows_k, uint32_t sequences, int heads, int kv_heads, int dim, int dtype);
+int attention_rows_forward(const AttnArgs& a, int dtype, void* workspace, cudaStream_t stream);
 
 }  // namespace rmn

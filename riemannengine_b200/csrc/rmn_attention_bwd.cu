@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   bool timed_out = false;
 
   const int head = blockIdx.x % a.heads;
-  const bool exists = find_tile<kBwdThreads, false>(a, blockIdx.x / a.heads, 128, &tail->found, tail->warp_sums);
+  const bool exists = find_tile<kBwdThreads, TilesOf::kQueries>(a, blockIdx.x / a.heads, 128, &tail->found, tail->warp_sums);
   const Segment g = tail->found.g;
   const int first = (tail->found.tiles - 1 - tail->found.tile) * 128;  // the tiles that see the most keys first
   const int rows = min(128, g.n_q - first);
@@ -313,7 +313,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   bool timed_out = false;
 
   const int kv = blockIdx.x % a.kv_heads, group = a.heads / a.kv_heads;
-  const bool exists = find_tile<kBwdThreads, true>(a, blockIdx.x / a.kv_heads, 128, &tail->found, tail->warp_sums);
+  const bool exists = find_tile<kBwdThreads, TilesOf::kSlots>(a, blockIdx.x / a.kv_heads, 128, &tail->found, tail->warp_sums);
   const Segment g = tail->found.g;
   const int first = tail->found.tile * 128;  // the first keys are seen by the most queries
   // query tiles of each head that see any of these keys

@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(FwdShape<DP, NQ>::THREADS, NQ == 2 ? 1 : 2)
   bool timed_out = false;
 
   const int head = blockIdx.x % a.heads;
-  const bool exists = find_tile<C::THREADS, false>(a, blockIdx.x / a.heads, 128 * NQ, &found, warp_sums);
+  const bool exists = find_tile<C::THREADS, TilesOf::kQueries>(a, blockIdx.x / a.heads, 128 * NQ, &found, warp_sums);
   const Segment g = found.g;
   const int first = (found.tiles - 1 - found.tile) * 128 * NQ;  // the tiles that see the most keys first
   // key tiles of each query tile

@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(kSimtThreads) k_attention_simt(const AttnArgs 
   float* s_p = s_kv + BM * S::LD;
   after_previous_kernel();
   const int head = blockIdx.x % a.heads;
-  if (!find_tile<kSimtThreads, false>(a, blockIdx.x / a.heads, BM, &found, warp_sums)) return;
+  if (!find_tile<kSimtThreads, TilesOf::kQueries>(a, blockIdx.x / a.heads, BM, &found, warp_sums)) return;
   const Segment g = found.g;
   const int first = (found.tiles - 1 - found.tile) * BM;  // the tiles with the most keys first
   const int rows = min(BM, g.n_q - first);
@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(kSimtThreads) k_attention_simt_dq(const AttnAr
   float* s_p = s_v + BM * S::LD;
   after_previous_kernel();
   const int head = blockIdx.x % a.heads;
-  if (!find_tile<kSimtThreads, false>(a, blockIdx.x / a.heads, BM, &found, warp_sums)) return;
+  if (!find_tile<kSimtThreads, TilesOf::kQueries>(a, blockIdx.x / a.heads, BM, &found, warp_sums)) return;
   const Segment g = found.g;
   const int first = (found.tiles - 1 - found.tile) * BM;
   const int rows = min(BM, g.n_q - first);
@@ -326,7 +326,7 @@ __global__ void __launch_bounds__(kSimtThreads) k_attention_simt_dkv(const AttnA
   float* s_p = s_g + BM * S::LD;
   after_previous_kernel();
   const int kv = blockIdx.x % a.kv_heads;
-  if (!find_tile<kSimtThreads, true>(a, blockIdx.x / a.kv_heads, BM, &found, warp_sums)) return;
+  if (!find_tile<kSimtThreads, TilesOf::kSlots>(a, blockIdx.x / a.kv_heads, BM, &found, warp_sums)) return;
   const Segment g = found.g;
   const int first = found.tile * BM;  // the first keys are seen by the most queries
   const int rows = min(BM, g.k_slot - first), used = max(0, min(BM, g.n_k - first));

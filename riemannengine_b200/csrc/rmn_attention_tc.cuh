@@ -93,18 +93,20 @@ __device__ __forceinline__ void zero_rows(uint32_t tile_s, int from, int atoms) 
   __syncwarp();
 }
 
-// [rows, heads, dim] bf16 as a tensor map with boxes of 64 channels of one head in 128 rows; columns behind `dim` and rows
-// behind `rows` read as zeros. False where strides or alignment do not allow it.
-inline bool make_head_map(CUtensorMap* map, const void* base, uint32_t rows, int heads, int dim, int64_t row, int64_t head) {
+// [rows, heads, dim] (bf16, or fp32 where elem is 4) as a tensor map with boxes of 128 bytes of channels of one head in box_rows
+// rows; columns behind `dim` and rows behind `rows` read as zeros. False where strides or alignment do not allow it.
+inline bool make_head_map(CUtensorMap* map, const void* base, uint32_t rows, int heads, int dim, int64_t row, int64_t head,
+                          int box_rows = 128, int elem = 2) {
   EncodeTiledFn fn = encode_tiled_fn();
   if (heads == 1) head = dim;
   if (rows == 1) row = dim;
-  if (!fn || ((uintptr_t)base & 15) || dim % 8 || row % 8 || head % 8 || row <= 0 || head <= 0) return false;
+  const int unit = 16 / elem;
+  if (!fn || ((uintptr_t)base & 15) || dim % unit || row % unit || head % unit || row <= 0 || head <= 0) return false;
   const cuuint64_t dims[3] = {(cuuint64_t)dim, (cuuint64_t)heads, (cuuint64_t)rows};
-  const cuuint64_t strides[2] = {(cuuint64_t)head * 2, (cuuint64_t)row * 2};
-  const cuuint32_t box[3] = {64, 1, 128}, estr[3] = {1, 1, 1};
-  return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
-            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+  const cuuint64_t strides[2] = {(cuuint64_t)head * elem, (cuuint64_t)row * elem};
+  const cuuint32_t box[3] = {(cuuint32_t)(128 / elem), 1, (cuuint32_t)box_rows}, estr[3] = {1, 1, 1};
+  return fn(map, elem == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims,
+            strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 

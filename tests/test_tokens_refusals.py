@@ -59,6 +59,14 @@ def test_attention_arguments():
         assert lib.rmn_attention_forward(ctypes.byref(problem), p, None, None, p, 1 << 30, None) == capi.ERR_BAD_ARG, change
         assert lib.rmn_attention_backward(ctypes.byref(problem), p, None, p, p, 128, 32, p, p, p, p, 1 << 30, None) == capi.ERR_BAD_ARG
     assert lib.rmn_attention_forward(None, p, None, None, p, 0, None) == capi.ERR_BAD_ARG
+    # few query rows a sample ask for scratch
+    few = _problem(rows_q=2, rows_k=100_000, kv_offsets=16)
+    need = lib.rmn_attention_forward_workspace_bytes(ctypes.byref(few))
+    assert need > 0
+    assert lib.rmn_attention_forward(ctypes.byref(few), p, None, None, None, need, None) == capi.ERR_BAD_ARG
+    assert lib.rmn_attention_forward(ctypes.byref(few), p, None, None, ctypes.c_void_p(20), need, None) == capi.ERR_BAD_ARG
+    assert lib.rmn_attention_forward(ctypes.byref(few), p, None, None, p, need - 1, None) == capi.ERR_ALLOC
+    assert lib.rmn_attention_forward_workspace_bytes(ctypes.byref(_problem(rows_q=10_000, rows_k=10_000))) == 0
     assert lib.rmn_attention_forward(ctypes.byref(_problem(dim=257)), p, None, None, p, 1 << 30, None) == capi.ERR_UNSUPPORTED
 
 
