@@ -16,6 +16,8 @@
 
 #include <math_constants.h>
 
+#include <atomic>
+
 namespace rmn {
 namespace tc {
 namespace {
@@ -26,7 +28,10 @@ struct FwdShape {
   static constexpr uint32_t TILE = ATOMS * kAtomBytes;
   static constexpr bool kAlias = DP == 128;  // P in the columns of S
   static constexpr int SLOTS = DP == 128 ? (NQ == 2 ? 5 : 2) : (NQ == 2 ? 6 : 4);
-  static constexpr int THREADS = NQ * 128 + 64;
+  static constexpr int THREADS = NQ * 128 + 128;
+  // registers of a softmax thread and of the others: what the block is launched with, dealt out anew
+  static constexpr int SOFTMAX_REGS = NQ == 2 ? 216 : 200, OTHER_REGS = NQ == 2 ? 64 : 56;
+  static constexpr int ALL_REGS = NQ * 128 * SOFTMAX_REGS + 128 * OTHER_REGS;
   static constexpr uint32_t COLUMNS = NQ * 256;
   static constexpr uint32_t S0 = 0, P0 = kAlias ? 0 : NQ * 128, O0 = kAlias ? NQ * 128 : NQ * 192;
   static constexpr uint32_t P_STEP = kAlias ? 128 : 64;
@@ -35,6 +40,8 @@ struct FwdShape {
 };
 
 constexpr float kRescale = 8.f;  // log2 of how far a row's maximum may rise before O is scaled
+constexpr int kOneTile = 4;      // softmax warps
+constexpr int kTwoTiles = 8;
 
 template <int DP, int NQ>
 __global__ void __launch_bounds__(FwdShape<DP, NQ>::THREADS, NQ == 2 ? 1 : 2)
@@ -105,102 +112,7 @@ __global__ void __launch_bounds__(FwdShape<DP, NQ>::THREADS, NQ == 2 ? 1 : 2)
     most = max(most, key_tiles[t]);
   }
 
-  if (!exists) {
-    // nothing to do
-  } else if (warp == kCopyWarp) {
-    // ------------------------------ bulk copies ----------------------------------------
-    if (lane == 0) {
-      const int kv = head / (a.heads / a.kv_heads);
-#pragma unroll
-      for (int t = 0; t < NQ; ++t) {
-        if (key_tiles[t] == 0) continue;
-        mbar_arrive_expect_tx(&q_full[t], C::TILE);
-#pragma unroll
-        for (int c = 0; c < C::ATOMS; ++c)
-          tma_load_3d(smem_base + t * C::TILE + c * kAtomBytes, &map_q, &q_full[t], c * 64, head, g.q0 + first + t * 128);
-      }
-      const uint32_t loads = 2u * (uint32_t)most;
-      uint32_t i = 0;
-      for (; i < loads; ++i) {  // K 0, V 0, K 1, V 1, ...
-        const uint32_t s = i % SLOTS;
-        if (!mbar_wait(&empty[s], ((i / SLOTS) & 1u) ^ 1u)) { timed_out = true; break; }
-        mbar_arrive_expect_tx(&full[s], C::TILE);
-        const CUtensorMap* map = (i & 1u) ? &map_v : &map_k;
-#pragma unroll
-        for (int c = 0; c < C::ATOMS; ++c)
-          tma_load_3d(slots + s * C::TILE + c * kAtomBytes, map, &full[s], c * 64, kv, g.k0 + (int)(i >> 1) * 128);
-      }
-      if (timed_out) {  // no copy may be in flight when the block ends
-        for (uint32_t k = i > SLOTS ? i - SLOTS : 0; k < i; ++k) mbar_wait(&full[k % SLOTS], (k / SLOTS) & 1u);
-        for (int t = 0; t < NQ; ++t)
-          if (key_tiles[t]) mbar_wait(&q_full[t], 0);
-      }
-    }
-  } else if (warp == kMmaWarp) {
-    // ------------------------------ products -------------------------------------------
-    const int steps = (a.dim + 15) / 16;
-    const uint32_t idesc_s = instr_desc(128, 128, false);
-    const uint32_t idesc_o = instr_desc(128, 0, true) | ((uint32_t)(steps * 2) << 17);
-    auto ready = [&](uint32_t i) {  // load i has arrived
-      if (!mbar_wait(&full[i % SLOTS], (i / SLOTS) & 1u)) timed_out = true;
-      return !timed_out;
-    };
-    auto scores = [&](int t, int j) {
-      tc_fence_after();
-      mma_rows(tmem + C::S0 + t * 128, smem_base + t * C::TILE, slots + (2u * j) % SLOTS * C::TILE, idesc_s, steps);
-      tc_commit_elect(&s_full[t]);
-    };
-    if (most > 0 && ready(0)) {
-#pragma unroll
-      for (int t = 0; t < NQ; ++t) {
-        if (key_tiles[t] == 0 || timed_out) continue;
-        if (!mbar_wait(&q_full[t], 0)) { timed_out = true; break; }
-        scores(t, 0);
-      }
-      if (!timed_out) tc_commit_elect(&empty[0]);
-    }
-    for (int j = 0; j < most && !timed_out; ++j) {
-      const uint32_t ph = (uint32_t)j & 1u;
-      const uint32_t v_s = slots + (2u * j + 1u) % SLOTS * C::TILE;
-      bool v_here = false;
-      // O of tile t += P V
-      auto output = [&](int t) {
-        if (!mbar_wait(&p_full[t], ph)) { timed_out = true; return; }
-        if (!v_here) {
-          if (!ready(2u * j + 1u)) return;
-          v_here = true;
-          if (g.n_k - j * 128 < 128) zero_rows(v_s, g.n_k - j * 128, C::ATOMS);
-        }
-        tc_fence_after();
-        mma_columns(tmem + C::O0 + t * DP, tmem + C::P0 + t * C::P_STEP, v_s, idesc_o, j > 0);
-        tc_commit_elect(&o_done[t]);
-      };
-      if (j + 1 < most && !ready(2u * j + 2u)) break;
-      if constexpr (C::kAlias) {
-#pragma unroll
-        for (int t = 0; t < NQ; ++t) {
-          if (j >= key_tiles[t] || timed_out) continue;
-          output(t);
-          if (timed_out || j + 1 >= key_tiles[t]) continue;
-          if (!mbar_wait(&o_done[t], ph)) { timed_out = true; break; }  // P has been read
-          scores(t, j + 1);
-        }
-      } else {
-#pragma unroll
-        for (int t = 0; t < NQ; ++t) {
-          if (j + 1 >= key_tiles[t] || timed_out) continue;
-          if (!mbar_wait(&s_free[t], ph)) { timed_out = true; break; }
-          scores(t, j + 1);
-        }
-#pragma unroll
-        for (int t = 0; t < NQ; ++t)
-          if (j < key_tiles[t] && !timed_out) output(t);
-      }
-      if (timed_out) break;
-      tc_commit_elect(&empty[(2u * j + 1u) % SLOTS]);
-      if (j + 1 < most) tc_commit_elect(&empty[(2u * j + 2u) % SLOTS]);
-    }
-  } else {
+  auto softmax = [&] {
     // ------------------------------ softmax --------------------------------------------
     const int t = warp >> 2;
     const uint32_t lanes = ((uint32_t)(warp & 3) * 32u) << 16;
@@ -236,9 +148,8 @@ __global__ void __launch_bounds__(FwdShape<DP, NQ>::THREADS, NQ == 2 ? 1 : 2)
 #pragma unroll
       for (int c = 0; c < 128; c += 8)
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          top[k] = fmaxf(top[k], fmaxf(__uint_as_float(r[c + 2 * k]), __uint_as_float(r[c + 2 * k + 1])));
-      const float m_new = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale);
+        for (int k = 0; k < 4; ++k) top[k] = max3(top[k], __uint_as_float(r[c + 2 * k]), __uint_as_float(r[c + 2 * k + 1]));
+      const float m_new = fmaxf(m, fmaxf(max3(top[0], top[1], top[2]), top[3]) * scale);
       const bool rise = m_new > m + kRescale;  // (from -infinity: always, unless nothing is seen yet)
       float shrink = 1.f;
       if (rise) {
@@ -247,20 +158,19 @@ __global__ void __launch_bounds__(FwdShape<DP, NQ>::THREADS, NQ == 2 ? 1 : 2)
         m = m_new;
       }
       const float base = m == -CUDART_INF_F ? 0.f : m;
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      const Pair by = make_pair(scale, scale), minus = make_pair(-base, -base);
+      Pair sum[2] = {make_pair(0.f, 0.f), make_pair(0.f, 0.f)};
       uint32_t p[64];
 #pragma unroll
-      for (int c = 0; c < 128; c += 4) {
-        float e[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          e[k] = exp2_approx(fmaf(__uint_as_float(r[c + k]), scale, -base));
-          sum[k] += e[k];
-        }
-        p[c / 2] = pack_bf16(e[0], e[1]);
-        p[c / 2 + 1] = pack_bf16(e[2], e[3]);
+      for (int c = 0; c < 128; c += 2) {
+        float x, y;
+        parts(fma(pair_of(r[c], r[c + 1]), by, minus), x, y);
+        x = exp2_approx(x);
+        y = exp2_approx(y);
+        sum[(c >> 1) & 1] = add(sum[(c >> 1) & 1], make_pair(x, y));
+        p[c / 2] = pack_bf16(x, y);
       }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      l += total(add(sum[0], sum[1]));
       if (j > 0) {
         // P and O of the tile before are free (kAlias: these scores were made behind that)
         if constexpr (!C::kAlias) {
@@ -321,6 +231,121 @@ __global__ void __launch_bounds__(FwdShape<DP, NQ>::THREADS, NQ == 2 ? 1 : 2)
       if (mine && a.lse)
         a.lse[(size_t)head * a.rows_q + g.q0 + row] = l == 0.f ? -CUDART_INF_F : (m + log2f(l)) * kLn2;
     }
+  };
+  auto others = [&] {
+    if (warp == kCopyWarp) {
+      // ------------------------------ bulk copies ----------------------------------------
+      if (lane == 0) {
+        const int kv = head / (a.heads / a.kv_heads);
+#pragma unroll
+        for (int t = 0; t < NQ; ++t) {
+          if (key_tiles[t] == 0) continue;
+          mbar_arrive_expect_tx(&q_full[t], C::TILE);
+#pragma unroll
+          for (int c = 0; c < C::ATOMS; ++c)
+            tma_load_3d(smem_base + t * C::TILE + c * kAtomBytes, &map_q, &q_full[t], c * 64, head, g.q0 + first + t * 128);
+        }
+        const uint32_t loads = 2u * (uint32_t)most;
+        uint32_t i = 0;
+        for (; i < loads; ++i) {  // K 0, V 0, K 1, V 1, ...
+          const uint32_t s = i % SLOTS;
+          if (!mbar_wait(&empty[s], ((i / SLOTS) & 1u) ^ 1u)) { timed_out = true; break; }
+          mbar_arrive_expect_tx(&full[s], C::TILE);
+          const CUtensorMap* map = (i & 1u) ? &map_v : &map_k;
+#pragma unroll
+          for (int c = 0; c < C::ATOMS; ++c)
+            tma_load_3d(slots + s * C::TILE + c * kAtomBytes, map, &full[s], c * 64, kv, g.k0 + (int)(i >> 1) * 128);
+        }
+        if (timed_out) {  // no copy may be in flight when the block ends
+          for (uint32_t k = i > SLOTS ? i - SLOTS : 0; k < i; ++k) mbar_wait(&full[k % SLOTS], (k / SLOTS) & 1u);
+          for (int t = 0; t < NQ; ++t)
+            if (key_tiles[t]) mbar_wait(&q_full[t], 0);
+        }
+      }
+    } else if (warp == kMmaWarp) {
+      // ------------------------------ products -------------------------------------------
+      const int steps = (a.dim + 15) / 16;
+      const uint32_t idesc_s = instr_desc(128, 128, false);
+      const uint32_t idesc_o = instr_desc(128, 0, true) | ((uint32_t)(steps * 2) << 17);
+      auto ready = [&](uint32_t i) {  // load i has arrived
+        if (!mbar_wait(&full[i % SLOTS], (i / SLOTS) & 1u)) timed_out = true;
+        return !timed_out;
+      };
+      auto scores = [&](int t, int j) {
+        tc_fence_after();
+        mma_rows(tmem + C::S0 + t * 128, smem_base + t * C::TILE, slots + (2u * j) % SLOTS * C::TILE, idesc_s, steps);
+        tc_commit_elect(&s_full[t]);
+      };
+      if (most > 0 && ready(0)) {
+#pragma unroll
+        for (int t = 0; t < NQ; ++t) {
+          if (key_tiles[t] == 0 || timed_out) continue;
+          if (!mbar_wait(&q_full[t], 0)) { timed_out = true; break; }
+          scores(t, 0);
+        }
+        if (!timed_out) tc_commit_elect(&empty[0]);
+      }
+      for (int j = 0; j < most && !timed_out; ++j) {
+        const uint32_t ph = (uint32_t)j & 1u;
+        const uint32_t v_s = slots + (2u * j + 1u) % SLOTS * C::TILE;
+        bool v_here = false;
+        // O of tile t += P V
+        auto output = [&](int t) {
+          if (!mbar_wait(&p_full[t], ph)) { timed_out = true; return; }
+          if (!v_here) {
+            if (!ready(2u * j + 1u)) return;
+            v_here = true;
+            if (g.n_k - j * 128 < 128) zero_rows(v_s, g.n_k - j * 128, C::ATOMS);
+          }
+          tc_fence_after();
+          mma_columns(tmem + C::O0 + t * DP, tmem + C::P0 + t * C::P_STEP, v_s, idesc_o, j > 0);
+          tc_commit_elect(&o_done[t]);
+        };
+        if (j + 1 < most && !ready(2u * j + 2u)) break;
+        if constexpr (C::kAlias) {
+#pragma unroll
+          for (int t = 0; t < NQ; ++t) {
+            if (j >= key_tiles[t] || timed_out) continue;
+            output(t);
+            if (timed_out || j + 1 >= key_tiles[t]) continue;
+            if (!mbar_wait(&o_done[t], ph)) { timed_out = true; break; }  // P has been read
+            scores(t, j + 1);
+          }
+        } else {
+#pragma unroll
+          for (int t = 0; t < NQ; ++t) {
+            if (j + 1 >= key_tiles[t] || timed_out) continue;
+            if (!mbar_wait(&s_free[t], ph)) { timed_out = true; break; }
+            scores(t, j + 1);
+          }
+#pragma unroll
+          for (int t = 0; t < NQ; ++t)
+            if (j < key_tiles[t] && !timed_out) output(t);
+        }
+        if (timed_out) break;
+        tc_commit_elect(&empty[(2u * j + 1u) % SLOTS]);
+        if (j + 1 < most) tc_commit_elect(&empty[(2u * j + 2u) % SLOTS]);
+      }
+    }
+  };
+  if (exists) {
+    if constexpr (NQ == 2) {
+      if (warp < kTwoTiles) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::SOFTMAX_REGS));
+        softmax();
+      } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::OTHER_REGS));
+        others();
+      }
+    } else {
+      if (warp < kOneTile) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::SOFTMAX_REGS));
+        softmax();
+      } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::OTHER_REGS));
+        others();
+      }
+    }
   }
 
   if (timed_out) atomicExch(a.status, (uint32_t)RMN_ERR_TIMEOUT);
@@ -339,6 +364,14 @@ int launch_fwd(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
   auto kern = k_attention_fwd<DP, NQ>;
   const uint64_t blocks = most_tiles(a.rows_q, a.sequences, 128 * NQ) * a.heads;
   if (blocks > 0x7fffffffull) return RMN_ERR_UNSUPPORTED;
+  // the registers dealt out have to be there: asked for once
+  static std::atomic<int> enough{0};
+  if (!enough.load(std::memory_order_relaxed)) {
+    cudaFuncAttributes attr;
+    RMN_CUDA_TRY(cudaFuncGetAttributes(&attr, reinterpret_cast<const void*>(kern)));
+    enough.store(attr.numRegs * C::THREADS >= C::ALL_REGS ? 1 : 2, std::memory_order_relaxed);
+  }
+  if (enough.load(std::memory_order_relaxed) != 1) return RMN_ERR_UNSUPPORTED;
   RMN_CUDA_TRY(opt_in.apply(reinterpret_cast<const void*>(kern), C::SMEM));
   RMN_CUDA_TRY(launch_overlapped(kern, dim3((uint32_t)blocks), dim3(C::THREADS), C::SMEM, stream, q, k, v, a));
   RMN_LAUNCH_CHECK();

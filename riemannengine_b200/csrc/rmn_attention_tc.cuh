@@ -2,6 +2,7 @@
 #pragma once
 
 #include "rmn_attention.cuh"
+#include "rmn_pair.cuh"
 #include "rmn_tma.cuh"
 
 namespace rmn {
@@ -18,6 +19,12 @@ __device__ __forceinline__ float exp2_approx(float x) {  // 2 ulp; results below
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ Pair pair_of(uint32_t x, uint32_t y) { return make_pair(__uint_as_float(x), __uint_as_float(y)); }
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&b);

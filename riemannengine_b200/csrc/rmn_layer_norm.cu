@@ -10,6 +10,7 @@
 // it visits: gamma and beta are loaded once, and dgamma and dbeta are sums in its registers, which are added up over the block in a
 // fixed order; a second kernel adds the blocks' sums in order: no atomics, the same bits every time.
 #include "rmn_common.cuh"
+#include "rmn_pair.cuh"
 
 #include <cuda_bf16.h>
 
@@ -30,37 +31,8 @@ struct alignas(sizeof(T) * V) Pack {
   T v[V];
 };
 
-// Two fp32 numbers that one instruction works on (in bf16 the arithmetic bounds as much as memory: 1.2 M x 64 forward 74 us with
-// single ones, 62.5 with pairs); rows read one number at a time use plain floats in their place.
-struct Pair {
-  unsigned long long v;
-};
-__device__ __forceinline__ Pair make_pair(float x, float y) {
-  Pair p;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(p.v) : "f"(x), "f"(y));
-  return p;
-}
-__device__ __forceinline__ void parts(Pair p, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(p.v)); }
-__device__ __forceinline__ Pair add(Pair a, Pair b) {
-  Pair p;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(p.v) : "l"(a.v), "l"(b.v));
-  return p;
-}
-__device__ __forceinline__ Pair mul(Pair a, Pair b) {
-  Pair p;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(p.v) : "l"(a.v), "l"(b.v));
-  return p;
-}
-__device__ __forceinline__ Pair fma(Pair a, Pair b, Pair c) {
-  Pair p;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(p.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-  return p;
-}
-__device__ __forceinline__ float total(Pair a) {
-  float x, y;
-  parts(a, x, y);
-  return x + y;
-}
+// The arithmetic is on pairs of fp32 numbers (in bf16 it bounds as much as memory: 1.2 M x 64 forward 74 us with single ones, 62.5
+// with pairs); rows read one number at a time use plain floats in their place.
 __device__ __forceinline__ float add(float a, float b) { return a + b; }
 __device__ __forceinline__ float mul(float a, float b) { return a * b; }
 __device__ __forceinline__ float fma(float a, float b, float c) { return fmaf(a, b, c); }
