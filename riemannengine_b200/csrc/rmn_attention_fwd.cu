@@ -9,9 +9,11 @@
 //
 // Warps: NQ groups of four for the softmax of one query tile each, one for the bulk copies, one that issues the products.
 // Keys and values arrive as 128-row tiles in a ring of shared-memory slots. Bound by the exponentials: 16 a clock and SM, 1024
-// clocks a 128 x 128 tile, against 4 * head size clocks of both products on the tensor cores.
-// Head sizes up to 64: P has columns of its own, and the next scores are made while the exponentials of these run. Above, tensor
-// memory has no room for it: P takes the place of S, and the next scores wait until P has been used.
+// clocks a 128 x 128 tile, against 8 * head size clocks of both products on the tensor cores.
+// Head sizes up to 64: one query tile and two blocks an SM, P has columns of its own, and the next scores are made while the
+// exponentials of these run (8192 rows, 16 heads of 64: 414 us; two tiles and one block 433: their softmax groups fall into step).
+// Above, tensor memory has no room for it: P takes the place of S, and the next scores wait until P has been used (a softmax
+// thread waits about half of the time then, while the other tile's works: 8192 rows, 16 heads of 128: 514 us, 1070 TFLOP/s).
 #include "rmn_attention_tc.cuh"
 
 #include <math_constants.h>
@@ -27,7 +29,7 @@ struct FwdShape {
   static constexpr int ATOMS = DP / 64;
   static constexpr uint32_t TILE = ATOMS * kAtomBytes;
   static constexpr bool kAlias = DP == 128;  // P in the columns of S
-  static constexpr int SLOTS = DP == 128 ? (NQ == 2 ? 5 : 2) : (NQ == 2 ? 6 : 4);
+  static constexpr int SLOTS = DP == 128 ? (NQ == 2 ? 5 : 2) : 4;
   static constexpr int THREADS = NQ * 128 + 128;
   // registers of a softmax thread and of the others: what the block is launched with, dealt out anew
   static constexpr int SOFTMAX_REGS = NQ == 2 ? 216 : 200, OTHER_REGS = NQ == 2 ? 64 : 56;
@@ -291,12 +293,12 @@ __global__ void __launch_bounds__(FwdShape<DP, NQ>::THREADS, NQ == 2 ? 1 : 2)
         bool v_here = false;
         // O of tile t += P V
         auto output = [&](int t) {
-          if (!mbar_wait(&p_full[t], ph)) { timed_out = true; return; }
           if (!v_here) {
             if (!ready(2u * j + 1u)) return;
             v_here = true;
             if (g.n_k - j * 128 < 128) zero_rows(v_s, g.n_k - j * 128, C::ATOMS);
           }
+          if (!mbar_wait(&p_full[t], ph)) { timed_out = true; return; }
           tc_fence_after();
           mma_columns(tmem + C::O0 + t * DP, tmem + C::P0 + t * C::P_STEP, v_s, idesc_o, j > 0);
           tc_commit_elect(&o_done[t]);
@@ -391,8 +393,10 @@ int attention_tc_forward(const AttnArgs& a, cudaStream_t stream) {
       !make_head_map(&k, a.k, a.rows_k, a.kv_heads, a.dim, a.k_row, a.k_head) ||
       !make_head_map(&v, a.v, a.rows_k, a.kv_heads, a.dim, a.v_row, a.v_head))
     return RMN_ERR_UNSUPPORTED;
-  const bool two = a.rows_q / 256 >= a.sequences;
-  if (a.dim <= 64) return two ? launch_fwd<64, 2>(q, k, v, a, stream) : launch_fwd<64, 1>(q, k, v, a, stream);
+  if (a.dim <= 64) return launch_fwd<64, 1>(q, k, v, a, stream);
+  // two query tiles a block read the keys half as often, one leaves two blocks an SM: 16 heads of 128, one causal sample of 8192
+  // rows 249 us with two and 260 with one; 100 samples of 256 rows, 8 heads, 76 and 66.5; 12 of 2048 the same
+  const bool two = a.rows_q / 2048 >= a.sequences;
   return two ? launch_fwd<128, 2>(q, k, v, a, stream) : launch_fwd<128, 1>(q, k, v, a, stream);
 }
 

@@ -71,31 +71,38 @@ __device__ __forceinline__ void tc_ld32_at(uint32_t taddr, uint32_t (&r)[N]) {
       : "memory");
 }
 
-// D[128, n] (+)= A[128, 16 steps] B[n, 16 steps]^T, both K-major tiles of kAtomBytes atoms in shared memory
+// The address field of a shared-memory descriptor. In a block of a cluster other than its first, addresses have bits above the
+// block's own window, which would run into the next field.
+__device__ __forceinline__ uint64_t desc_address(uint32_t addr) { return (addr >> 4) & 0x3FFFu; }
+// D[128, n] (+)= A[128, 16 steps] B[n, 16 steps]^T, both K-major tiles in shared memory: A of 128 rows, B of B_ROWS, as atoms of 64
+// channels (128-byte swizzled lines)
+template <int B_ROWS = 128>
 __device__ __forceinline__ void mma_rows(uint32_t d_tmem, uint32_t a_s, uint32_t b_s, uint32_t idesc, int steps) {
   constexpr uint64_t DESC = smem_desc_sw_const(16, 1024, 2u);
   for (int j = 0; j < steps; ++j) {
-    const uint32_t at = (uint32_t)(j >> 2) * kAtomBytes + (uint32_t)(j & 3) * 32u;
-    tc_mma_bf16_elect(d_tmem, DESC + ((a_s + at) >> 4), DESC + ((b_s + at) >> 4), idesc, j != 0);
+    const uint32_t in = (uint32_t)(j & 3) * 32u;
+    tc_mma_bf16_elect(d_tmem, DESC + desc_address(a_s + (uint32_t)(j >> 2) * kAtomBytes + in),
+                      DESC + desc_address(b_s + (uint32_t)(j >> 2) * (B_ROWS * 128u) + in), idesc, j != 0);
   }
 }
-// D[128, n] (+)= A[128, 128] B[128, n]: A in tensor memory, its two halves of 32 columns HALF apart, B a tile whose rows are the
-// 128 summed over (MN-major)
-template <int HALF = 32>
+// D[128, n] (+)= A[128, ROWS] B[ROWS, n]: A in tensor memory, its pieces of 32 columns (64 values) HALF apart, B a tile whose ROWS
+// rows are summed over (MN-major)
+template <int ROWS = 128, int HALF = 32>
 __device__ __forceinline__ void mma_columns(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_s, uint32_t idesc, bool accumulate) {
-  constexpr uint64_t DESC = smem_desc_sw_const(kAtomBytes, 1024, 2u);
+  constexpr uint64_t DESC = smem_desc_sw_const(ROWS * 128, 1024, 2u);
 #pragma unroll
-  for (int j = 0; j < 8; ++j)
-    tc_mma_bf16_ta_elect(d_tmem, a_tmem + (j >> 2) * HALF + (j & 3) * 8, DESC + ((b_s + (uint32_t)j * 2048u) >> 4), idesc,
+  for (int j = 0; j < ROWS / 16; ++j)
+    tc_mma_bf16_ta_elect(d_tmem, a_tmem + (j >> 2) * HALF + (j & 3) * 8, DESC + desc_address(b_s + (uint32_t)j * 2048u), idesc,
                          accumulate || j != 0);
 }
 
-// One warp: rows [from, 128) of a tile of `atoms` atoms become zeros (a masked weight of zero times what lies there must be zero)
+// One warp: rows [from, ROWS) of a tile of `atoms` atoms become zeros (a masked weight of zero times what lies there must be zero)
+template <int ROWS = 128>
 __device__ __forceinline__ void zero_rows(uint32_t tile_s, int from, int atoms) {
   const int lane = threadIdx.x & 31;
   for (int a = 0; a < atoms; ++a)
-    for (uint32_t at = (uint32_t)from * 128u + lane * 16u; at < kAtomBytes; at += 512u)
-      asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(tile_s + a * kAtomBytes + at), "r"(0u) : "memory");
+    for (uint32_t at = (uint32_t)from * 128u + lane * 16u; at < ROWS * 128u; at += 512u)
+      asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(tile_s + a * (ROWS * 128u) + at), "r"(0u) : "memory");
   fence_proxy_async();
   __syncwarp();
 }

@@ -225,6 +225,25 @@ cudaError_t launch_overlapped(void (*kernel)(P...), dim3 grid, dim3 block, size_
   config.numAttrs = 1;
   return cudaLaunchKernelEx(&config, kernel, static_cast<P>(args)...);
 }
+// The same with clusters of `cluster` blocks.
+template <typename... P, typename... A>
+cudaError_t launch_overlapped_clusters(void (*kernel)(P...), uint32_t cluster, dim3 grid, dim3 block, size_t smem,
+                                       cudaStream_t stream, A&&... args) {
+  cudaLaunchAttribute attr[2] = {};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = grid;
+  config.blockDim = block;
+  config.dynamicSmemBytes = smem;
+  config.stream = stream;
+  config.attrs = attr;
+  config.numAttrs = cluster > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&config, kernel, static_cast<P>(args)...);
+}
 #ifdef __CUDACC__
 // max(v, 0) that keeps a NaN, as torch's relu does (fmaxf would turn it into 0): a diverged network shows in its output.
 __device__ __forceinline__ float relu_f32(float v) {

@@ -78,6 +78,16 @@ def test_head_sizes(d, dtype):
     _check("cpp", q, k, v, grad, _offsets(lens), causal=True, what=f"dim {d}")
 
 
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("h,hk,d", [(3, 1, 64), (6, 1, 128), (5, 1, 32), (16, 2, 64), (14, 2, 80), (32, 2, 40), (11, 1, 16), (22, 2, 128)])
+def test_many_query_heads_to_a_key_head(h, hk, d, dtype, causal):
+    """Groups of every kind: that divide into up to eight blocks, and (11 heads) that do not."""
+    lens = [40, 0, 257, 130]
+    q, k, v, grad = _inputs(427, 427, h, hk, d, TYPES[dtype])
+    _check("cpp", q, k, v, grad, _offsets(lens), causal=causal)
+
+
 @pytest.mark.parametrize("host", ["python", "cpp"])
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("d", [32, 64, 128])
