@@ -158,6 +158,43 @@ __device__ __forceinline__ bool find_tile(const AttnArgs& a, uint32_t want, int 
   return true;
 }
 
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t n;
+  asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(n));
+  return n;
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+}
+// 16 bytes at this address of another block's shared memory
+__device__ __forceinline__ float4 load_of_block(uint32_t addr, uint32_t rank) {
+  float4 v;
+  asm volatile(
+      "{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %4, %5;\n\t"
+      "ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [a];\n\t}"
+      : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+      : "r"(addr), "r"(rank)
+      : "memory");
+  return v;
+}
+
+// the number at this place of another block's shared memory
+__device__ __forceinline__ float float_of_block(const float* p, uint32_t rank) {
+  float v;
+  asm volatile(
+      "{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.f32 %0, [a];\n\t}"
+      : "=f"(v)
+      : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank)
+      : "memory");
+  return v;
+}
+
 // How many tiles find_tile may be asked for at most: with valid offsets every segment's last tile may be a part of one.
 inline uint64_t most_tiles(uint64_t rows, uint64_t sequences, uint32_t tile_rows) { return rows / tile_rows + sequences + 2; }
 

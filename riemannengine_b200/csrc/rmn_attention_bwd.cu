@@ -76,32 +76,6 @@ __device__ __forceinline__ void store32(uint32_t taddr, float by, __nv_bfloat16*
   }
 }
 
-__device__ __forceinline__ uint32_t cluster_size() {
-  uint32_t n;
-  asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(n));
-  return n;
-}
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release;" ::: "memory");
-  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
-}
-// 16 bytes at this address of another block's shared memory
-__device__ __forceinline__ float4 load_of_block(uint32_t addr, uint32_t rank) {
-  float4 v;
-  asm volatile(
-      "{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %4, %5;\n\t"
-      "ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [a];\n\t}"
-      : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-      : "r"(addr), "r"(rank)
-      : "memory");
-  return v;
-}
-
 // the barriers, the same in both kernels
 template <int DP>
 __device__ __forceinline__ void init_barriers(BwdTail* tail) {

@@ -8,9 +8,12 @@
 // ds = p * (grad v^T - delta); each makes the scores anew, which costs 7 products where 5 would do, and every gradient is
 // written once, in a fixed order of sums.
 //
-// Bound by the multiply-adds' operands in shared memory: a thread's 4 x 4 outputs take 8 16-byte reads per 64 multiply-adds; rows
-// are padded by 16 bytes, and a thread's columns are 16 apart, so that the reads of a warp meet no bank twice.
+// Bound by the multiply-adds and their operands in shared memory: a thread's 4 x 4 outputs take 8 16-byte reads per 32 multiply-adds
+// of pairs; rows are padded by 16 bytes, and a thread's columns are 16 apart, so that the reads of a warp meet no bank twice.
+// Where the tiles are fewer than the GPU has room for, a cluster of blocks shares one: each walks over every second or fourth tile of
+// the other side, and their parts are joined through shared memory, in the order of the blocks.
 #include "rmn_attention.cuh"
+#include "rmn_pair.cuh"
 
 #include <math_constants.h>
 
@@ -64,14 +67,18 @@ __device__ __forceinline__ void load_tile(float* dst, const T* from, int64_t row
   }
 }
 
+__device__ __forceinline__ Pair low_pair(const float4& v) { return make_pair(v.x, v.y); }
+__device__ __forceinline__ Pair high_pair(const float4& v) { return make_pair(v.z, v.w); }
+
 // s[i][j] = row (ty + 16 i) of a times row (tx + 16 j) of b
 template <int DP, int BM, int R = SimtShape<DP, BM>::R>
 __device__ __forceinline__ void product_rows(const float* a, const float* b, int tx, int ty, float (&s)[R][R]) {
   constexpr int LD = SimtShape<DP, BM>::LD;
+  Pair t[R][R];
 #pragma unroll
   for (int i = 0; i < R; ++i)
 #pragma unroll
-    for (int j = 0; j < R; ++j) s[i][j] = 0.f;
+    for (int j = 0; j < R; ++j) t[i][j] = make_pair(0.f, 0.f);
 #pragma unroll 4
   for (int c = 0; c < DP; c += 4) {
     float4 x[R], y[R];
@@ -83,17 +90,19 @@ __device__ __forceinline__ void product_rows(const float* a, const float* b, int
     for (int i = 0; i < R; ++i)
 #pragma unroll
       for (int j = 0; j < R; ++j) {
-        s[i][j] = fmaf(x[i].x, y[j].x, s[i][j]);
-        s[i][j] = fmaf(x[i].y, y[j].y, s[i][j]);
-        s[i][j] = fmaf(x[i].z, y[j].z, s[i][j]);
-        s[i][j] = fmaf(x[i].w, y[j].w, s[i][j]);
+        t[i][j] = fma(low_pair(x[i]), low_pair(y[j]), t[i][j]);
+        t[i][j] = fma(high_pair(x[i]), high_pair(y[j]), t[i][j]);
       }
   }
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+#pragma unroll
+    for (int j = 0; j < R; ++j) s[i][j] = total(t[i][j]);
 }
 
 // o[i][channels of the thread] += sum_j p[ty + 16 i][j] b[j][channels], j < n rounded up to 4 (zeros there)
 template <int DP, int BM, int R = SimtShape<DP, BM>::R, int NC = SimtShape<DP, BM>::NC, int CW = SimtShape<DP, BM>::CW>
-__device__ __forceinline__ void product_columns(const float* p, const float* b, int n, int tx, int ty, float (&o)[R][NC][CW]) {
+__device__ __forceinline__ void product_columns(const float* p, const float* b, int n, int tx, int ty, Pair (&o)[R][NC][CW / 2]) {
   constexpr int LD = SimtShape<DP, BM>::LD, LP = SimtShape<DP, BM>::LP;
   for (int j = 0; j < n; j += 4) {
     float4 w[R];
@@ -102,29 +111,90 @@ __device__ __forceinline__ void product_columns(const float* p, const float* b, 
 #pragma unroll
     for (int jj = 0; jj < 4; ++jj) {
       const float* row = b + (j + jj) * LD + tx * CW;
+      Pair y[NC][CW / 2];
 #pragma unroll
       for (int g = 0; g < NC; ++g) {
-        float y[CW];
-#pragma unroll
-        for (int e = 0; e < CW; ++e) y[e] = row[g * 16 * CW + e];
-#pragma unroll
-        for (int i = 0; i < R; ++i) {
-          const float f = jj == 0 ? w[i].x : jj == 1 ? w[i].y : jj == 2 ? w[i].z : w[i].w;
-#pragma unroll
-          for (int e = 0; e < CW; ++e) o[i][g][e] = fmaf(f, y[e], o[i][g][e]);
+        if constexpr (CW == 4) {
+          const float4 v = *reinterpret_cast<const float4*>(row + g * 16 * CW);
+          y[g][0] = low_pair(v);
+          y[g][1] = high_pair(v);
+        } else {
+          const float2 v = *reinterpret_cast<const float2*>(row + g * 16 * CW);
+          y[g][0] = make_pair(v.x, v.y);
         }
+      }
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        const float f = jj == 0 ? w[i].x : jj == 1 ? w[i].y : jj == 2 ? w[i].z : w[i].w;
+        const Pair ff = make_pair(f, f);
+#pragma unroll
+        for (int g = 0; g < NC; ++g)
+#pragma unroll
+          for (int e = 0; e < CW / 2; ++e) o[i][g][e] = fma(ff, y[g][e], o[i][g][e]);
       }
     }
   }
 }
+template <int R, int NC, int H>
+__device__ __forceinline__ void clear(Pair (&o)[R][NC][H]) {
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+#pragma unroll
+    for (int g = 0; g < NC; ++g)
+#pragma unroll
+      for (int e = 0; e < H; ++e) o[i][g][e] = make_pair(0.f, 0.f);
+}
+// the pairs as single numbers
+template <int R, int NC, int H>
+__device__ __forceinline__ void singles(const Pair (&o)[R][NC][H], float (&x)[R][NC][2 * H]) {
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+#pragma unroll
+    for (int g = 0; g < NC; ++g)
+#pragma unroll
+      for (int e = 0; e < H; ++e) parts(o[i][g][e], x[i][g][2 * e], x[i][g][2 * e + 1]);
+}
 
-// o times `by` into rows [0, n) of `to`, `row` elements apart
-template <typename T, int DP, int BM, int R = SimtShape<DP, BM>::R, int NC = SimtShape<DP, BM>::NC, int CW = SimtShape<DP, BM>::CW>
-__device__ __forceinline__ void store_tile(T* to, int64_t row, int n, int dim, int tx, int ty, const float (&o)[R][NC][CW],
-                                           const float (&by)[R]) {
+// A cluster's parts of a tile, each in its block's shared memory at `part` [BM][LD]: puts this block's there. Behind a cluster_sync,
+// sum_parts adds up those of rows ty + 16 i with i % blocks == rank, times weight(i, block).
+template <int DP, int BM, int R = SimtShape<DP, BM>::R, int NC = SimtShape<DP, BM>::NC, int CW = SimtShape<DP, BM>::CW>
+__device__ __forceinline__ void put_part(float* part, int tx, int ty, const float (&x)[R][NC][CW]) {
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+#pragma unroll
+    for (int g = 0; g < NC; ++g)
+#pragma unroll
+      for (int e = 0; e < CW; ++e) part[(ty + 16 * i) * SimtShape<DP, BM>::LD + g * 16 * CW + tx * CW + e] = x[i][g][e];
+}
+template <int DP, int BM, class Weight, int R = SimtShape<DP, BM>::R, int NC = SimtShape<DP, BM>::NC, int CW = SimtShape<DP, BM>::CW>
+__device__ __forceinline__ void sum_parts(const float* part, int tx, int ty, int rank, int blocks, float (&x)[R][NC][CW],
+                                          Weight&& weight) {
 #pragma unroll
   for (int i = 0; i < R; ++i) {
-    if (ty + 16 * i >= n) continue;
+    if (i % blocks != rank) continue;
+#pragma unroll
+    for (int g = 0; g < NC; ++g)
+#pragma unroll
+      for (int e = 0; e < CW; ++e) x[i][g][e] = 0.f;
+    for (int k = 0; k < blocks; ++k) {
+      const float f = weight(i, k);
+#pragma unroll
+      for (int g = 0; g < NC; ++g)
+#pragma unroll
+        for (int e = 0; e < CW; ++e)
+          x[i][g][e] = fmaf(float_of_block(part + (ty + 16 * i) * SimtShape<DP, BM>::LD + g * 16 * CW + tx * CW + e, (uint32_t)k), f,
+                            x[i][g][e]);
+    }
+  }
+}
+
+// o times `by` into rows [0, n) of `to`, `row` elements apart: those of this block of the cluster
+template <typename T, int DP, int BM, int R = SimtShape<DP, BM>::R, int NC = SimtShape<DP, BM>::NC, int CW = SimtShape<DP, BM>::CW>
+__device__ __forceinline__ void store_tile(T* to, int64_t row, int n, int dim, int tx, int ty, int rank, int blocks,
+                                           const float (&o)[R][NC][CW], const float (&by)[R]) {
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    if (ty + 16 * i >= n || i % blocks != rank) continue;
 #pragma unroll
     for (int g = 0; g < NC; ++g)
 #pragma unroll
@@ -146,8 +216,9 @@ __global__ void __launch_bounds__(kSimtThreads) k_attention_simt(const AttnArgs 
   float* s_kv = s_q + BM * S::LD;
   float* s_p = s_kv + BM * S::LD;
   after_previous_kernel();
-  const int head = blockIdx.x % a.heads;
-  if (!find_tile<kSimtThreads, TilesOf::kQueries>(a, blockIdx.x / a.heads, BM, &found, warp_sums)) return;
+  const int blocks = (int)cluster_size(), rank = (int)cluster_rank(), tile = blockIdx.x / blocks;
+  const int head = tile % a.heads;
+  if (!find_tile<kSimtThreads, TilesOf::kQueries>(a, tile / a.heads, BM, &found, warp_sums)) return;
   const Segment g = found.g;
   const int first = (found.tiles - 1 - found.tile) * BM;  // the tiles with the most keys first
   const int rows = min(BM, g.n_q - first);
@@ -155,7 +226,9 @@ __global__ void __launch_bounds__(kSimtThreads) k_attention_simt(const AttnArgs 
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   load_tile<T, DP, BM>(s_q, static_cast<const T*>(a.q) + (int64_t)(g.q0 + first) * a.q_row + head * a.q_head, a.q_row, rows,
                        a.dim, a.scale);
-  float o[R][NC][CW] = {}, m[R], l[R];
+  Pair o[R][NC][CW / 2];
+  clear(o);
+  float m[R], l[R];
   int seen[R];
 #pragma unroll
   for (int i = 0; i < R; ++i) {
@@ -166,7 +239,7 @@ __global__ void __launch_bounds__(kSimtThreads) k_attention_simt(const AttnArgs 
   const int keys = visible_keys(g, first + rows - 1, a.causal);  // of the last row: the most
   const T* k0 = static_cast<const T*>(a.k) + (int64_t)g.k0 * a.k_row + kv * a.k_head;
   const T* v0 = static_cast<const T*>(a.v) + (int64_t)g.k0 * a.v_row + kv * a.v_head;
-  for (int j0 = 0; j0 < keys; j0 += BM) {
+  for (int j0 = rank * BM; j0 < keys; j0 += blocks * BM) {
     const int n = min(BM, keys - j0);
     __syncthreads();  // the products with the tile before are done
     load_tile<T, DP, BM>(s_kv, k0 + (int64_t)j0 * a.k_row, a.k_row, n, a.dim, 1.f);
@@ -200,38 +273,71 @@ __global__ void __launch_bounds__(kSimtThreads) k_attention_simt(const AttnArgs 
 #pragma unroll
       for (int c = 0; c < NC; ++c)
 #pragma unroll
-        for (int e = 0; e < CW; ++e) o[i][c][e] *= shrink;
+        for (int e = 0; e < CW / 2; ++e) o[i][c][e] = mul(o[i][c][e], make_pair(shrink, shrink));
     }
     __syncthreads();  // the keys have been read
     load_tile<T, DP, BM>(s_kv, v0 + (int64_t)j0 * a.v_row, a.v_row, n, a.dim, 1.f);
     __syncthreads();
     product_columns<DP, BM>(s_p, s_kv, n, tx, ty, o);
   }
-  float by[R];
+  float x[R][NC][CW], by[R];
+  singles(o, x);
+  if (blocks > 1) {
+    __shared__ float s_m[BM], s_l[BM];
+    __syncthreads();  // q has been read
+    put_part<DP, BM>(s_q, tx, ty, x);
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+      if (tx == 0) {
+        s_m[ty + 16 * i] = m[i];
+        s_l[ty + 16 * i] = l[i];
+      }
+    cluster_sync();
+    float m_of[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int r = ty + 16 * i;
+      float top = -CUDART_INF_F;
+      for (int k = 0; k < blocks; ++k) top = fmaxf(top, float_of_block(s_m + r, (uint32_t)k));
+      l[i] = 0.f;
+      for (int k = 0; k < blocks; ++k) {
+        // (a block without a visible key has summed nothing; one with NaN scores has no maximum, but a sum that is NaN)
+        const float mk = float_of_block(s_m + r, (uint32_t)k), lk = float_of_block(s_l + r, (uint32_t)k);
+        l[i] += mk == -CUDART_INF_F ? lk : lk * expf(mk - top);
+      }
+      m_of[i] = top;
+    }
+    sum_parts<DP, BM>(s_q, tx, ty, rank, blocks, x, [&](int i, int k) {
+      const float mk = float_of_block(s_m + ty + 16 * i, (uint32_t)k);
+      return mk == -CUDART_INF_F ? 0.f : expf(mk - m_of[i]);
+    });
+#pragma unroll
+    for (int i = 0; i < R; ++i) m[i] = m_of[i];
+  }
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     by[i] = l[i] == 0.f ? 0.f : 1.f / l[i];
-    if (a.lse && tx == 0 && ty + 16 * i < rows)
+    if (a.lse && tx == 0 && ty + 16 * i < rows && i % blocks == rank)
       a.lse[(size_t)head * a.rows_q + g.q0 + first + ty + 16 * i] = l[i] == 0.f ? -CUDART_INF_F : m[i] + logf(l[i]);
   }
   const int64_t out_row = (int64_t)a.heads * a.dim;
   const int64_t at = (int64_t)(g.q0 + first) * out_row + (int64_t)head * a.dim;
-  store_tile<T, DP, BM>(static_cast<T*>(a.out) + at, out_row, rows, a.dim, tx, ty, o, by);
-  if constexpr (sizeof(T) == 2) {
-    if (!a.low) return;
+  store_tile<T, DP, BM>(static_cast<T*>(a.out) + at, out_row, rows, a.dim, tx, ty, rank, blocks, x, by);
+  if (sizeof(T) == 2 && a.low) {
 #pragma unroll
     for (int i = 0; i < R; ++i)
 #pragma unroll
       for (int c = 0; c < NC; ++c)
 #pragma unroll
         for (int e = 0; e < CW; ++e) {
-          const float x = o[i][c][e] * by[i];
-          o[i][c][e] = x - __bfloat162float(__float2bfloat16_rn(x));
+          const float v = x[i][c][e] * by[i];
+          x[i][c][e] = v - __bfloat162float(__float2bfloat16_rn(v));
         }
 #pragma unroll
     for (int i = 0; i < R; ++i) by[i] = 1.f;
-    store_tile<T, DP, BM>(static_cast<T*>(a.low) + at, out_row, rows, a.dim, tx, ty, o, by);
+    store_tile<T, DP, BM>(static_cast<T*>(a.low) + at, out_row, rows, a.dim, tx, ty, rank, blocks, x, by);
   }
+  if (blocks > 1) cluster_sync();  // no block leaves while another reads its part
 }
 
 // dq of a query tile, and delta of its rows for the kernel of the key tiles
@@ -248,8 +354,9 @@ __global__ void __launch_bounds__(kSimtThreads) k_attention_simt_dq(const AttnAr
   float* s_v = s_k + BM * S::LD;
   float* s_p = s_v + BM * S::LD;
   after_previous_kernel();
-  const int head = blockIdx.x % a.heads;
-  if (!find_tile<kSimtThreads, TilesOf::kQueries>(a, blockIdx.x / a.heads, BM, &found, warp_sums)) return;
+  const int blocks = (int)cluster_size(), rank = (int)cluster_rank(), tile = blockIdx.x / blocks;
+  const int head = tile % a.heads;
+  if (!find_tile<kSimtThreads, TilesOf::kQueries>(a, tile / a.heads, BM, &found, warp_sums)) return;
   const Segment g = found.g;
   const int first = (found.tiles - 1 - found.tile) * BM;
   const int rows = min(BM, g.n_q - first);
@@ -266,7 +373,9 @@ __global__ void __launch_bounds__(kSimtThreads) k_attention_simt_dq(const AttnAr
     load_tile<T, DP, BM>(s_v, static_cast<const T*>(a.low) + (int64_t)(g.q0 + first) * out_row + (int64_t)head * a.dim, out_row,
                          rows, a.dim, 1.f);
   __syncthreads();
-  float o[R][NC][CW] = {}, delta[R], lse[R];
+  Pair o[R][NC][CW / 2];
+  clear(o);
+  float delta[R], lse[R];
   int seen[R];
 #pragma unroll
   for (int i = 0; i < R; ++i) {
@@ -280,12 +389,12 @@ __global__ void __launch_bounds__(kSimtThreads) k_attention_simt_dq(const AttnAr
     seen[i] = r < rows ? visible_keys(g, first + r, a.causal) : 0;
     const size_t at = (size_t)head * a.rows_q + g.q0 + first + r;
     lse[i] = r < rows ? __ldg(a.lse + at) : 0.f;
-    if (r < rows && tx == 0) a.delta[at] = d;
+    if (r < rows && tx == 0 && rank == 0) a.delta[at] = d;
   }
   const int keys = visible_keys(g, first + rows - 1, a.causal);
   const T* k0 = static_cast<const T*>(a.k) + (int64_t)g.k0 * a.k_row + kv * a.k_head;
   const T* v0 = static_cast<const T*>(a.v) + (int64_t)g.k0 * a.v_row + kv * a.v_head;
-  for (int j0 = 0; j0 < keys; j0 += BM) {
+  for (int j0 = rank * BM; j0 < keys; j0 += blocks * BM) {
     const int n = min(BM, keys - j0);
     __syncthreads();
     load_tile<T, DP, BM>(s_k, k0 + (int64_t)j0 * a.k_row, a.k_row, n, a.dim, 1.f);
@@ -304,11 +413,19 @@ __global__ void __launch_bounds__(kSimtThreads) k_attention_simt_dq(const AttnAr
     __syncthreads();
     product_columns<DP, BM>(s_p, s_k, n, tx, ty, o);
   }
-  float by[R];
+  float x[R][NC][CW], by[R];
+  singles(o, x);
+  if (blocks > 1) {
+    __syncthreads();  // q has been read
+    put_part<DP, BM>(s_q, tx, ty, x);
+    cluster_sync();
+    sum_parts<DP, BM>(s_q, tx, ty, rank, blocks, x, [](int, int) { return 1.f; });
+  }
 #pragma unroll
   for (int i = 0; i < R; ++i) by[i] = a.scale;
   store_tile<T, DP, BM>(static_cast<T*>(a.dq) + (int64_t)(g.q0 + first) * out_row + (int64_t)head * a.dim, out_row, rows, a.dim,
-                        tx, ty, o, by);
+                        tx, ty, rank, blocks, x, by);
+  if (blocks > 1) cluster_sync();  // no block leaves while another reads its part
 }
 
 // dk and dv of a key tile: the queries of all heads that share its head
@@ -325,8 +442,9 @@ __global__ void __launch_bounds__(kSimtThreads) k_attention_simt_dkv(const AttnA
   float* s_g = s_q + BM * S::LD;
   float* s_p = s_g + BM * S::LD;
   after_previous_kernel();
-  const int kv = blockIdx.x % a.kv_heads;
-  if (!find_tile<kSimtThreads, TilesOf::kSlots>(a, blockIdx.x / a.kv_heads, BM, &found, warp_sums)) return;
+  const int blocks = (int)cluster_size(), rank = (int)cluster_rank(), tile = blockIdx.x / blocks;
+  const int kv = tile % a.kv_heads;
+  if (!find_tile<kSimtThreads, TilesOf::kSlots>(a, tile / a.kv_heads, BM, &found, warp_sums)) return;
   const Segment g = found.g;
   const int first = found.tile * BM;  // the first keys are seen by the most queries
   const int rows = min(BM, g.k_slot - first), used = max(0, min(BM, g.n_k - first));
@@ -336,12 +454,16 @@ __global__ void __launch_bounds__(kSimtThreads) k_attention_simt_dkv(const AttnA
                        a.dim, a.scale);
   load_tile<T, DP, BM>(s_v, static_cast<const T*>(a.v) + (int64_t)(g.k0 + first) * a.v_row + kv * a.v_head, a.v_row, used,
                        a.dim, 1.f);
-  float dk[R][NC][CW] = {}, dv[R][NC][CW] = {};
+  Pair dk[R][NC][CW / 2], dv[R][NC][CW / 2];
+  clear(dk);
+  clear(dv);
+  int turn = 0;  // tiles of queries, over all heads: every block of the cluster takes its own
   const int from = used > 0 ? first_query(g, first, a.causal) / BM * BM : g.n_q;
   for (int h = kv * group; h < (kv + 1) * group; ++h) {
     const T* q0 = static_cast<const T*>(a.q) + (int64_t)g.q0 * a.q_row + h * a.q_head;
     const T* g0 = static_cast<const T*>(a.grad) + (int64_t)g.q0 * a.grad_row + h * a.grad_head;
-    for (int i0 = from; i0 < g.n_q; i0 += BM) {
+    for (int i0 = from; i0 < g.n_q; i0 += BM, ++turn) {
+      if (turn % blocks != rank) continue;
       const int n = min(BM, g.n_q - i0);
       __syncthreads();
       load_tile<T, DP, BM>(s_q, q0 + (int64_t)i0 * a.q_row, a.q_row, n, a.dim, 1.f);
@@ -375,22 +497,42 @@ __global__ void __launch_bounds__(kSimtThreads) k_attention_simt_dkv(const AttnA
       product_columns<DP, BM>(s_p, s_q, n, tx, ty, dk);
     }
   }
-  float by_k[R], by_v[R];
+  float x[R][NC][CW], y[R][NC][CW], by_k[R], by_v[R];
+  singles(dk, x);
+  singles(dv, y);
+  if (blocks > 1) {
+    __syncthreads();  // the tiles have been read
+    put_part<DP, BM>(s_q, tx, ty, x);
+    put_part<DP, BM>(s_g, tx, ty, y);
+    cluster_sync();
+    sum_parts<DP, BM>(s_q, tx, ty, rank, blocks, x, [](int, int) { return 1.f; });
+    sum_parts<DP, BM>(s_g, tx, ty, rank, blocks, y, [](int, int) { return 1.f; });
+  }
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     by_k[i] = a.scale;
     by_v[i] = 1.f;
   }
   const int64_t kv_row = (int64_t)a.kv_heads * a.dim, at = (int64_t)(g.k0 + first) * kv_row + (int64_t)kv * a.dim;
-  store_tile<T, DP, BM>(static_cast<T*>(a.dk) + at, kv_row, rows, a.dim, tx, ty, dk, by_k);
-  store_tile<T, DP, BM>(static_cast<T*>(a.dv) + at, kv_row, rows, a.dim, tx, ty, dv, by_v);
+  store_tile<T, DP, BM>(static_cast<T*>(a.dk) + at, kv_row, rows, a.dim, tx, ty, rank, blocks, x, by_k);
+  store_tile<T, DP, BM>(static_cast<T*>(a.dv) + at, kv_row, rows, a.dim, tx, ty, rank, blocks, y, by_v);
+  if (blocks > 1) cluster_sync();  // no block leaves while another reads its part
+}
+
+// Blocks that share a tile: twice as many as long as they fit the GPU at once and each has a tile of the other side (`other`: its
+// rows a sample, over all heads) to walk over; at most the rows of a thread, which divide them at the end.
+int blocks_a_tile(uint64_t rows, int heads, uint64_t other, int BM) {
+  int n = 1;
+  while (2 * n <= BM / 16 && rows / BM * heads * 2 * n <= 148 * 2 && (other + BM - 1) / BM >= 2 * (uint64_t)n) n *= 2;
+  return n;
 }
 
 template <class Kernel>
-int launch_simt(Kernel kern, SmemOptIn& opt_in, const AttnArgs& a, uint64_t blocks, size_t smem, cudaStream_t stream) {
+int launch_simt(Kernel kern, SmemOptIn& opt_in, const AttnArgs& a, uint64_t tiles, int cluster, size_t smem, cudaStream_t stream) {
+  const uint64_t blocks = tiles * cluster;
   if (blocks > 0x7fffffffull) return RMN_ERR_UNSUPPORTED;
   if (smem > 48 * 1024 - 1024) RMN_CUDA_TRY(opt_in.apply(reinterpret_cast<const void*>(kern), smem));
-  RMN_CUDA_TRY(launch_overlapped(kern, dim3((uint32_t)blocks), dim3(kSimtThreads), smem, stream, a));
+  RMN_CUDA_TRY(launch_overlapped_clusters(kern, (uint32_t)cluster, dim3((uint32_t)blocks), dim3(kSimtThreads), smem, stream, a));
   RMN_LAUNCH_CHECK();
   return RMN_OK;
 }
@@ -399,18 +541,20 @@ template <typename T, int DP, int BM>
 int forward(const AttnArgs& a, cudaStream_t stream) {
   using S = SimtShape<DP, BM>;
   static SmemOptIn opt_in;
+  const uint64_t samples = a.sequences ? a.sequences : 1;
   return launch_simt(k_attention_simt<T, DP, BM>, opt_in, a, most_tiles(a.rows_q, a.sequences, BM) * a.heads,
-                     2 * S::tile + S::square, stream);
+                     blocks_a_tile(a.rows_q, a.heads, a.rows_k / samples, BM), 2 * S::tile + S::square, stream);
 }
 template <typename T, int DP, int BM>
 int backward(const AttnArgs& a, cudaStream_t stream) {
   using S = SimtShape<DP, BM>;
   static SmemOptIn opt_q, opt_kv;
+  const uint64_t samples = a.sequences ? a.sequences : 1, group = a.heads / a.kv_heads;
   const int st = launch_simt(k_attention_simt_dq<T, DP, BM>, opt_q, a, most_tiles(a.rows_q, a.sequences, BM) * a.heads,
-                             4 * S::tile + S::square, stream);
+                             blocks_a_tile(a.rows_q, a.heads, a.rows_k / samples, BM), 4 * S::tile + S::square, stream);
   if (st != RMN_OK) return st;
   return launch_simt(k_attention_simt_dkv<T, DP, BM>, opt_kv, a, most_tiles(a.rows_k, a.sequences, BM) * a.kv_heads,
-                     4 * S::tile + S::square, stream);
+                     blocks_a_tile(a.rows_k, a.kv_heads, a.rows_q / samples * group, BM), 4 * S::tile + S::square, stream);
 }
 
 }  // namespace
