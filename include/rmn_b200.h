@@ -645,7 +645,7 @@ int rmn_layer_norm_backward(const void *d_dy, int64_t ld_dy, const void *d_x, in
  * The rows of the samples lie one behind the other in one matrix; every sample attends within itself. No counterpart in the
  * reference. */
 
-/* Scratch bytes of rmn_sample_offsets. */
+/* Scratch bytes of rmn_sample_offsets (the same for any number of samples). */
 size_t rmn_sample_offsets_workspace_bytes(uint32_t n_samples);
 /*
  * Row ranges of the samples of a coordinate map whose rows of one batch index are adjacent: d_offsets[s] = first row of the
@@ -664,7 +664,7 @@ int rmn_sample_offsets(const int32_t *d_coords, uint32_t n_rows, int W, uint32_t
  * given, only its first kv_lengths[s] key rows are in use (a cache with room behind what it holds) and the others are never
  * read as keys. causal: aligned at the end, query i of n sees keys 0 ... i + m - n of m. scale multiplies the scores.
  * Offsets or lengths that do not ascend or leave the tensors are clamped to them and reported as RMN_ERR_BAD_ARG by
- * rmn_device_status. dim <= 256 (RMN_ERR_UNSUPPORTED beyond).
+ * rmn_device_status; outputs are of no use then, and need not be written. dim <= 256 (RMN_ERR_UNSUPPORTED beyond).
  */
 typedef struct {
   const void *q, *k, *v;
@@ -683,22 +683,24 @@ size_t rmn_attention_forward_workspace_bytes(const rmn_attention *problem);
  * out[i, h] = sum_j softmax_j(scale q[i, h] . k[j, h']) v[j, h'] over the keys that row i sees: [rows_q, heads, dim] without
  * gaps. A row that sees no key, and a row of no sample, is zero. d_lse [heads, rows_q] (may be NULL): logarithm of the sum of
  * exponentials, -infinity for such a row; the backward pass needs it. d_low (bf16; may be NULL, and is not written in fp32): what
- * rounding took from out, as bf16 [rows_q, heads, dim]; with it the backward pass is as exact as with an unrounded output. Sums and softmax in fp32. A non-finite value in a
- * row of k or v may reach every row of its own sample and head, never those of another. d_workspace: 16-byte aligned; it may be
- * shared by calls on one stream, not by calls that run at the same time.
+ * rounding took from out, as bf16 [rows_q, heads, dim]; with it the backward pass is as exact as with an unrounded output. Sums and
+ * softmax in fp32. A non-finite value in a row of k or v may reach every row of its own sample and head (those that do not see it,
+ * too), never those of another. d_workspace: 16-byte aligned; it may be shared by calls on one stream, not by calls that run at
+ * the same time.
  */
 int rmn_attention_forward(const rmn_attention *problem, void *d_out, void *d_low, float *d_lse, void *d_workspace,
                           size_t workspace_bytes, void *stream);
 /* Scratch bytes of rmn_attention_backward. Depends on sizes only. */
 size_t rmn_attention_backward_workspace_bytes(const rmn_attention *problem);
 /*
- * Gradients of rmn_attention_forward from its outputs (d_out, d_low, which may be NULL, and d_lse) and d_grad_out (rows and heads grad_row and grad_head
- * elements apart): dq [rows_q, heads, dim], dk and dv [rows_k, kv_heads, dim] without gaps, summed over the query heads that share
- * a key head; zeros in rows of no sample and in key rows not in use. No atomics: the same bits every time. d_workspace: 16-byte aligned.
+ * Gradients of rmn_attention_forward from its outputs (d_out, d_low, which may be NULL, and d_lse) and d_grad_out (rows and heads
+ * grad_row and grad_head elements apart): dq [rows_q, heads, dim], dk and dv [rows_k, kv_heads, dim] without gaps, summed over the
+ * query heads that share a key head; zeros in rows of no sample and in key rows not in use. No atomics: the same bits every time.
+ * d_workspace: 16-byte aligned.
  */
 int rmn_attention_backward(const rmn_attention *problem, const void *d_out, const void *d_low, const float *d_lse,
-                           const void *d_grad_out, int64_t grad_row, int64_t grad_head, void *d_dq, void *d_dk, void *d_dv, void *d_workspace,
-                           size_t workspace_bytes, void *stream);
+                           const void *d_grad_out, int64_t grad_row, int64_t grad_head, void *d_dq, void *d_dk, void *d_dv,
+                           void *d_workspace, size_t workspace_bytes, void *stream);
 
 /* ------------------- weight-gradient all-reduce (data-parallel training) -------------------
  * Batches shard by sample: every rank hashes, maps and convolves its own samples, and the one

@@ -8,34 +8,73 @@ const uint32_t* tc_status_device_address();  // defined in rmn_conv_tc.cu
 
 namespace {
 
-// Runs of equal batch indices: the first row of every run, in any order, and their number.
-__global__ void __launch_bounds__(256) k_sample_runs(const int32_t* __restrict__ coords, uint32_t n, int W, uint32_t most,
-                                                     int32_t* __restrict__ starts, uint32_t* __restrict__ count) {
-  after_previous_kernel();
-  for (uint32_t i = blockIdx.x * blockDim.x + threadIdx.x; i < n; i += gridDim.x * blockDim.x) {
-    if (i > 0 && __ldg(coords + (size_t)i * W) == __ldg(coords + (size_t)(i - 1) * W)) continue;
-    const uint32_t at = atomicAdd(count, 1u);
-    if (at < most) starts[at] = (int32_t)i;
-  }
+// Runs of equal batch indices: every block counts those that begin in its share of the rows, then places them behind the counts of
+// the blocks before it. The rows are read twice, whatever the number of runs.
+constexpr int kRunBlocks = 148 * 4, kRunThreads = 256;
+
+__device__ __forceinline__ bool begins_run(const int32_t* __restrict__ coords, uint32_t i, int W) {
+  return i == 0 || __ldg(coords + (size_t)i * W) != __ldg(coords + (size_t)(i - 1) * W);
 }
-// offsets = the starts in ascending order, then n, then the number of runs
-__global__ void __launch_bounds__(1024) k_sample_offsets(const int32_t* __restrict__ starts, const uint32_t* __restrict__ count,
-                                                         uint32_t n, uint32_t most, int32_t* __restrict__ offsets) {
+__device__ __forceinline__ uint32_t share_of(uint32_t n, uint32_t block) { return (uint32_t)((uint64_t)n * block / kRunBlocks); }
+
+__global__ void __launch_bounds__(kRunThreads) k_count_runs(const int32_t* __restrict__ coords, uint32_t n, int W,
+                                                            uint32_t* __restrict__ counts) {
   after_previous_kernel();
-  const uint32_t runs = *count, have = min(runs, most);
-  for (uint32_t i = threadIdx.x; i < most; i += blockDim.x) {
-    if (i >= have) {
-      offsets[i] = (int32_t)n;
-      continue;
-    }
-    const int32_t mine = starts[i];
-    uint32_t rank = 0;
-    for (uint32_t j = 0; j < have; ++j) rank += starts[j] < mine ? 1u : 0u;
-    offsets[rank] = mine;
+  const uint32_t end = share_of(n, blockIdx.x + 1);
+  uint32_t mine = 0;
+  for (uint32_t first = share_of(n, blockIdx.x); first < end; first += kRunThreads) {
+    const uint32_t i = first + threadIdx.x;
+    mine += (uint32_t)__syncthreads_count(i < end && begins_run(coords, i, W));
   }
-  if (threadIdx.x == 0) {
+  if (threadIdx.x == 0) counts[blockIdx.x] = mine;
+}
+// offsets = the first row of every run (`most` of them: n behind the last), n, the number of runs
+__global__ void __launch_bounds__(kRunThreads) k_sample_offsets(const int32_t* __restrict__ coords, uint32_t n, int W, uint32_t most,
+                                                                const uint32_t* __restrict__ counts, int32_t* __restrict__ offsets) {
+  constexpr int kWarps = kRunThreads / 32;
+  __shared__ uint32_t s_before[kWarps], s_all[kWarps], s_warp[2][kWarps];
+  after_previous_kernel();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  uint32_t before = 0, all = 0;
+  for (uint32_t b = threadIdx.x; b < kRunBlocks; b += kRunThreads) {
+    const uint32_t c = counts[b];
+    all += c;
+    if (b < blockIdx.x) before += c;
+  }
+  for (int o = 16; o > 0; o >>= 1) {
+    before += __shfl_xor_sync(0xffffffffu, before, o);
+    all += __shfl_xor_sync(0xffffffffu, all, o);
+  }
+  if (lane == 0) {
+    s_before[warp] = before;
+    s_all[warp] = all;
+  }
+  __syncthreads();
+  before = all = 0;
+  for (int w = 0; w < kWarps; ++w) {
+    before += s_before[w];
+    all += s_all[w];
+  }
+  const uint32_t end = share_of(n, blockIdx.x + 1);
+  uint32_t turn = 0;
+  for (uint32_t first = share_of(n, blockIdx.x); first < end; first += kRunThreads, turn ^= 1u) {
+    const uint32_t i = first + threadIdx.x;
+    const bool begins = i < end && begins_run(coords, i, W);
+    const uint32_t votes = __ballot_sync(0xffffffffu, begins);
+    if (lane == 0) s_warp[turn][warp] = (uint32_t)__popc(votes);
+    __syncthreads();
+    uint32_t at = before + (uint32_t)__popc(votes & ((1u << lane) - 1u));
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) at += s_warp[turn][w];
+      before += s_warp[turn][w];
+    }
+    if (begins && at < most) offsets[at] = (int32_t)i;
+  }
+  for (uint64_t i = (uint64_t)all + blockIdx.x * kRunThreads + threadIdx.x; i < most; i += kRunBlocks * kRunThreads)
+    offsets[i] = (int32_t)n;
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
     offsets[most] = (int32_t)n;
-    offsets[most + 1] = (int32_t)min(runs, 0x7fffffffu);
+    offsets[most + 1] = (int32_t)min(all, 0x7fffffffu);
   }
 }
 
@@ -79,7 +118,7 @@ int find_status(AttnArgs* a) {
 
 using namespace rmn;
 
-extern "C" size_t rmn_sample_offsets_workspace_bytes(uint32_t n_samples) { return ((size_t)n_samples + 4) * sizeof(int32_t); }
+extern "C" size_t rmn_sample_offsets_workspace_bytes(uint32_t) { return kRunBlocks * sizeof(uint32_t); }
 
 extern "C" int rmn_sample_offsets(const int32_t* d_coords, uint32_t n_rows, int W, uint32_t n_samples, int32_t* d_offsets,
                                   void* d_workspace, size_t workspace_bytes, void* stream_) {
@@ -88,17 +127,11 @@ extern "C" int rmn_sample_offsets(const int32_t* d_coords, uint32_t n_rows, int 
       (n_rows && !d_coords) || ((uintptr_t)d_workspace & 3))
     return RMN_ERR_BAD_ARG;
   if (workspace_bytes < rmn_sample_offsets_workspace_bytes(n_samples)) return RMN_ERR_ALLOC;
-  uint32_t* count = static_cast<uint32_t*>(d_workspace);
-  int32_t* starts = reinterpret_cast<int32_t*>(count + 4);
-  RMN_CUDA_TRY(cudaMemsetAsync(count, 0, sizeof(uint32_t), stream));
-  if (n_rows) {
-    const uint64_t want = ((uint64_t)n_rows + 255) / 256;
-    const uint32_t grid = (uint32_t)(want < 148 * 8 ? want : 148 * 8);
-    RMN_CUDA_TRY(launch_overlapped(k_sample_runs, dim3(grid), dim3(256), 0, stream, d_coords, n_rows, W, n_samples, starts, count));
-    RMN_LAUNCH_CHECK();
-  }
-  RMN_CUDA_TRY(launch_overlapped(k_sample_offsets, dim3(1), dim3(1024), 0, stream, static_cast<const int32_t*>(starts),
-                                 static_cast<const uint32_t*>(count), n_rows, n_samples, d_offsets));
+  uint32_t* counts = static_cast<uint32_t*>(d_workspace);
+  RMN_CUDA_TRY(launch_overlapped(k_count_runs, dim3(kRunBlocks), dim3(kRunThreads), 0, stream, d_coords, n_rows, W, counts));
+  RMN_LAUNCH_CHECK();
+  RMN_CUDA_TRY(launch_overlapped(k_sample_offsets, dim3(kRunBlocks), dim3(kRunThreads), 0, stream, d_coords, n_rows, W, n_samples,
+                                 static_cast<const uint32_t*>(counts), d_offsets));
   RMN_LAUNCH_CHECK();
   return RMN_OK;
 }

@@ -41,8 +41,8 @@ struct Segment {
 __device__ __forceinline__ int32_t clamp_row(int32_t v, uint32_t rows) { return max(0, min(v, (int32_t)rows)); }
 
 // Offsets that do not ascend or leave the tensor are set right here, so that no row outside the tensors is touched whatever
-// they say, and recorded in the status word.
-__device__ __forceinline__ Segment segment(const AttnArgs& a, uint32_t s) {
+// they say, and recorded in the status word. descends: set where a sample's rows would lie before those of the one before it.
+__device__ __forceinline__ Segment segment(const AttnArgs& a, uint32_t s, bool* descends = nullptr) {
   Segment g;
   const uint32_t S = a.sequences;
   if (s > S) {
@@ -57,8 +57,11 @@ __device__ __forceinline__ Segment segment(const AttnArgs& a, uint32_t s) {
   const int32_t q_hi = s < S ? a.offsets[s + 1] : (int32_t)a.rows_q, k_hi = s < S ? a.kv_offsets[s + 1] : (int32_t)a.rows_k;
   g.q0 = clamp_row(q_lo, a.rows_q);
   g.k0 = clamp_row(k_lo, a.rows_k);
-  g.n_q = max(0, clamp_row(q_hi, a.rows_q) - g.q0);
-  g.k_slot = max(0, clamp_row(k_hi, a.rows_k) - g.k0);
+  g.n_q = clamp_row(q_hi, a.rows_q) - g.q0;
+  g.k_slot = clamp_row(k_hi, a.rows_k) - g.k0;
+  if (descends) *descends = *descends || g.n_q < 0 || g.k_slot < 0;
+  g.n_q = max(0, g.n_q);
+  g.k_slot = max(0, g.k_slot);
   bool bad = q_lo < 0 || q_hi < q_lo || q_hi > (int32_t)a.rows_q || k_lo < 0 || k_hi < k_lo || k_hi > (int32_t)a.rows_k;
   g.n_k = s < S ? g.k_slot : 0;
   if (s < S && a.kv_lengths) {
@@ -73,90 +76,108 @@ __device__ __forceinline__ Segment segment(const AttnArgs& a, uint32_t s) {
 // Keys that query row i of a segment attends to are 0 ... visible(i) - 1: all, or (causal, aligned at the end) those up to
 // its own place.
 __device__ __forceinline__ int32_t visible_keys(const Segment& g, int32_t i, int causal) {
-  return causal ? max(0, min(g.n_k, i + 1 + g.n_k - g.n_q)) : g.n_k;
+  return causal ? max(0, min(g.n_k, i + 1 - (g.n_q - g.n_k))) : g.n_k;
 }
 // The first query row that attends to key j.
 __device__ __forceinline__ int32_t first_query(const Segment& g, int32_t j, int causal) {
   return causal ? max(0, j - (g.n_k - g.n_q)) : 0;
 }
 
-// Tiles of `tile_rows` rows of all segments, one behind the other: of query rows, of key rows (whole slots), or of keys in use.
-enum class TilesOf { kQueries, kSlots, kKeys };
-template <TilesOf kOf>
-__device__ __forceinline__ int32_t segment_tiles(const Segment& g, int tile_rows) {
-  const int32_t rows = kOf == TilesOf::kQueries ? g.n_q : kOf == TilesOf::kSlots ? g.k_slot : g.n_k;
-  return (rows + tile_rows - 1) / tile_rows;
+__device__ __forceinline__ int32_t tiles_of(int32_t rows, int tile_rows) {
+  return (int32_t)(((uint32_t)rows + (uint32_t)tile_rows - 1) / (uint32_t)tile_rows);
 }
+
+// The tile of `tile_rows` rows that a block works on: of query rows, or of key rows (whole slots, in use or not).
+enum class TilesOf { kQueries, kSlots };
 struct FoundTile {
   Segment g;
   int32_t tile, tiles;  // number of the tile in its segment, and the segment's tiles
-  uint32_t segment;
 };
-// All threads of the block (kThreads) count: each a run of segments, a scan over the block places them.
-struct TileScan {
-  uint32_t lo, hi;            // this thread's segments
-  int32_t first, mine, total; // tiles before them, theirs, all
-  Segment g;                  // the last of them
-};
-template <int kThreads, TilesOf kOf>
-__device__ __forceinline__ TileScan scan_tiles(const AttnArgs& a, int tile_rows, int32_t* warp_sums) {
-  TileScan t;
-  const uint32_t n = a.sequences + 2;
-  const uint32_t per = (n + kThreads - 1) / kThreads;
-  t.lo = min(threadIdx.x * per, n);
-  t.hi = min(t.lo + per, n);
-  t.mine = 0;
-  t.g = {};
-  for (uint32_t s = t.lo; s < t.hi; ++s) {
-    t.g = segment(a, s);
-    t.mine += segment_tiles<kOf>(t.g, tile_rows);
-  }
+template <TilesOf kOf>
+__device__ __forceinline__ int32_t segment_tiles(const Segment& g, int tile_rows) {
+  return tiles_of(kOf == TilesOf::kQueries ? g.n_q : g.k_slot, tile_rows);
+}
+// Sums stop at the largest number: offsets that descend may give a row to many samples.
+__device__ __forceinline__ int32_t add_tiles(int32_t a, int32_t b) { return (int32_t)min((uint32_t)a + (uint32_t)b, 0x7fffffffu); }
+// The inclusive sum of the threads before (`first`) and of all (`all`), for all kThreads threads of a block; `any`: of a flag.
+template <int kThreads>
+__device__ __forceinline__ void scan_block(int32_t mine, int32_t* warp_sums, int32_t& first, int32_t& all, bool& any) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int32_t upto = t.mine;
+  int32_t upto = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int32_t v = __shfl_up_sync(0xffffffffu, upto, o);
-    if (lane >= o) upto += v;
+    if (lane >= o) upto = add_tiles(upto, v);
   }
   if (lane == 31) warp_sums[warp] = upto;
-  __syncthreads();
-  t.first = upto - t.mine;
-  t.total = 0;
+  any = __syncthreads_or(any);
+  first = __shfl_up_sync(0xffffffffu, upto, 1);
+  if (lane == 0) first = 0;
+  all = 0;
 #pragma unroll
   for (int w = 0; w < kThreads / 32; ++w) {
-    if (w < warp) t.first += warp_sums[w];
-    t.total += warp_sums[w];
+    if (w < warp) first = add_tiles(first, warp_sums[w]);
+    all = add_tiles(all, warp_sums[w]);
   }
-  return t;
 }
-// The segment of tile `want` (below t.total) into shared memory.
-template <TilesOf kOf>
-__device__ __forceinline__ void pick_tile(const AttnArgs& a, const TileScan& t, int32_t want, int tile_rows, FoundTile* found) {
-  int32_t first = t.first;
-  if (want >= first && want < first + t.mine) {
-    for (uint32_t s = t.lo; s < t.hi; ++s) {
-      const Segment g = t.hi - t.lo > 1 ? segment(a, s) : t.g;
-      const int32_t tiles = segment_tiles<kOf>(g, tile_rows);
-      if (want < first + tiles) {
-        found->g = g;
-        found->tile = want - first;
-        found->tiles = tiles;
-        found->segment = s;
-        break;
-      }
-      first += tiles;
-    }
-  }
-  __syncthreads();
-}
-// Both; false where there are no so many tiles.
+
+// Up to kCountedSamples samples: every thread counts the tiles of a run of segments, a scan over the block places them, and the
+// numbers behind the last tile are of no tile. Beyond, counting would cost the square of the samples: segment j in the order of the
+// rows (those before the first sample, the samples, those behind) begins at row b(j) and has the numbers from b(j) / tile_rows + j
+// on, as many as it has tiles or one more, which is of no tile; every warp searches for its number, 32 places at a time. Numbers
+// without a tile cost a block each, and the search leaves them among the others. 8 heads of 64, backward, with counts and with the
+// search: 128 samples of 96 rows 81 and 94 us; 256, 512, 1024, 4096 samples of 64 rows 115 and 122, 240 and 238, 523 and 476,
+// 3650 and 1885.
+constexpr uint32_t kCountedSamples = 384;
 template <int kThreads, TilesOf kOf>
 __device__ __forceinline__ bool find_tile(const AttnArgs& a, uint32_t want, int tile_rows, FoundTile* found, int32_t* warp_sums) {
-  const TileScan t = scan_tiles<kThreads, kOf>(a, tile_rows, warp_sums);
-  if (want >= (uint32_t)max(t.total, 0)) return false;
-  pick_tile<kOf>(a, t, (int32_t)want, tile_rows, found);
+  const uint32_t n = a.sequences + 2;
+  if (a.sequences <= kCountedSamples) {
+    const uint32_t per = (n + kThreads - 1) / kThreads;
+    const uint32_t lo = min(threadIdx.x * per, n), hi = min(lo + per, n);
+    int32_t mine = 0, first, all;
+    Segment g = {};
+    for (uint32_t s = lo; s < hi; ++s) {
+      g = segment(a, s);
+      mine = add_tiles(mine, segment_tiles<kOf>(g, tile_rows));
+    }
+    bool unused = false;
+    scan_block<kThreads>(mine, warp_sums, first, all, unused);
+    if (want >= (uint32_t)all) return false;
+    if ((int32_t)want >= first && (int32_t)want - first < mine) {
+      for (uint32_t s = lo; s < hi; ++s) {
+        if (hi - lo > 1) g = segment(a, s);
+        const int32_t tiles = segment_tiles<kOf>(g, tile_rows);
+        if ((int32_t)want - first < tiles) {
+          *found = {g, (int32_t)want - first, tiles};
+          break;
+        }
+        first += tiles;
+      }
+    }
+  } else {
+    const int32_t* at = kOf == TilesOf::kQueries ? a.offsets : a.kv_offsets;
+    const uint32_t rows = kOf == TilesOf::kQueries ? a.rows_q : a.rows_k, lane = threadIdx.x & 31;
+    if (want < n && threadIdx.x == 0) segment(a, want);  // every segment is looked at: the search may step over some that are wrong
+    auto number = [&](uint32_t j) { return j == 0 ? 0u : (uint32_t)clamp_row(__ldg(at + j - 1), rows) / (uint32_t)tile_rows + j; };
+    uint32_t lo = 0, len = n;  // number(lo) <= want
+    while (len > 1) {
+      const uint32_t step = (len + 31) / 32, p = lane * step;
+      const uint32_t below = __ballot_sync(0xffffffffu, p < len && number(lo + p) <= want);
+      const uint32_t skip = (31 - __clz((int)(below | 1u))) * step;
+      lo += skip;
+      len = min(step, len - skip);
+    }
+    const Segment g = segment(a, lo == 0 ? a.sequences + 1 : lo - 1);
+    const int32_t tiles = segment_tiles<kOf>(g, tile_rows), tile = (int32_t)(want - number(lo));
+    if (tile < 0 || tile >= tiles) return false;
+    if (threadIdx.x == 0) *found = {g, tile, tiles};
+  }
+  __syncthreads();
   return true;
 }
+// How many tile numbers there are at most.
+inline uint64_t most_tiles(uint64_t rows, uint64_t sequences, uint32_t tile_rows) { return rows / tile_rows + sequences + 2; }
 
 __device__ __forceinline__ uint32_t cluster_size() {
   uint32_t n;
@@ -194,9 +215,6 @@ __device__ __forceinline__ float float_of_block(const float* p, uint32_t rank) {
       : "memory");
   return v;
 }
-
-// How many tiles find_tile may be asked for at most: with valid offsets every segment's last tile may be a part of one.
-inline uint64_t most_tiles(uint64_t rows, uint64_t sequences, uint32_t tile_rows) { return rows / tile_rows + sequences + 2; }
 
 // The kernels behind rmn_attention_*: RMN_ERR_UNSUPPORTED where they do not cover the call.
 int attention_simt_forward(const AttnArgs& a, int dtype, cudaStream_t stream);

@@ -26,6 +26,8 @@ namespace rmn {
 namespace tc {
 namespace {
 
+constexpr uint32_t kTailBytes = 2560;  // of BwdTail
+
 template <int DP>
 struct BwdShape {
   static constexpr int ATOMS = DP / 64;
@@ -38,7 +40,7 @@ struct BwdShape {
   static constexpr uint32_t TILE = ATOMS * STEP * 128;           // a tile of a step
   static constexpr int SLOTS = DP == 64 ? 8 : 5;
   static constexpr uint32_t RING = 2 * HELD, TAIL = RING + SLOTS * TILE;  // two resident tiles, the ring, the rest
-  static constexpr size_t SMEM = TAIL + 3072;
+  static constexpr size_t SMEM = TAIL + kTailBytes;
 };
 constexpr int kStats = 2;  // steps whose queries' statistics are in shared memory
 
@@ -51,7 +53,7 @@ struct BwdTail {
   alignas(16) float lse[kStats][128];   // negative, times log2 e
   alignas(16) float delta[kStats][128]; // negative
 };
-static_assert(sizeof(BwdTail) <= 3072, "tail");
+static_assert(sizeof(BwdTail) <= kTailBytes, "tail");
 
 __device__ __forceinline__ void tc_ld64(uint32_t taddr, uint32_t (&r)[64]) {
   tc_ld32_at<0>(taddr, r);

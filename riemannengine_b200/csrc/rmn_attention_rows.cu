@@ -27,6 +27,7 @@ using namespace tc;
 
 constexpr int kSumWarps = 8, kSumThreads = kSumWarps * 32;
 constexpr int kTileKeys = 64;
+constexpr int kMostRows = 32;    // of a sample and a key head (queries times heads): on average, and for the sum of pieces
 constexpr float kRescale = 8.f;  // log2 of how far a row's maximum may rise before the output is scaled
 
 __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -74,17 +75,57 @@ struct RowsShape {
 
 struct RowsWork {  // scratch, and how the keys are cut
   int blocks;           // of the first kernel, for each key head
-  int most_queries;     // rows of a sample whose pieces are summed by the second kernel; more are walked through by one block
+  int most_queries;     // rows of a sample whose pieces are summed by the second kernel
   int32_t* starts;      // [blocks][3]: the sample that a block of the first head begins in, the tiles before that; all tiles
   float* sums;          // [piece][group * most_queries][2]: maximum (log 2), sum
   float* parts;         // [piece][group * most_queries][dim]: not yet divided by the sum
 };
 // Of `tiles` tiles, block b of a head takes those from first_of(b) to first_of(b + 1).
 __device__ __forceinline__ int64_t first_of(const RowsWork& w, int64_t tiles, int64_t block) { return tiles * block / w.blocks; }
-// Places of row r (of group * n_q) of the piece that a head's block has of sample s. A step to the next piece is a step to the next
-// block, to the next sample, or both, so no two pieces have the same number.
-__device__ __forceinline__ size_t part_at(const AttnArgs& a, const RowsWork& w, int64_t block, int kv, uint32_t s, int r) {
-  const int64_t piece = (int64_t)kv * ((int64_t)w.blocks + a.sequences) + block + s;
+// The tile that a block begins with, by counts over all samples.
+struct Begin {
+  int32_t all;          // tiles; 0 where the samples' rows are out of order
+  Segment g;            // of the tile, its sample, its number in it, the sample's tiles
+  uint32_t s;
+  int32_t tile, tiles;
+};
+// All threads of the block count: each a run of samples, a scan over the block places them.
+template <int kThreads>
+__device__ __forceinline__ void find_begin(const AttnArgs& a, const RowsWork& w, int block, Begin* found, int32_t* warp_sums, bool* in_order) {
+  const uint32_t per = (a.sequences + kThreads - 1) / kThreads;
+  const uint32_t lo = min(threadIdx.x * per, a.sequences), hi = min(lo + per, a.sequences);
+  int32_t mine = 0;
+  Segment g = {};
+  bool descends = false;
+  for (uint32_t s = lo; s < hi; ++s) {
+    g = segment(a, s, &descends);
+    mine = add_tiles(mine, tiles_of(g.n_k, kTileKeys));
+  }
+  int32_t first, all;
+  scan_block<kThreads>(mine, warp_sums, first, all, descends);
+  *in_order = !descends;
+  const int32_t want = all ? (int32_t)first_of(w, all, block) : 0;
+  if (*in_order && want >= first && want - first < mine) {
+    for (uint32_t s = lo; s < hi; ++s) {
+      if (hi - lo > 1) g = segment(a, s);
+      const int32_t tiles = tiles_of(g.n_k, kTileKeys);
+      if (want - first < tiles) {
+        *found = {all, g, s, want - first, tiles};
+        break;
+      }
+      first += tiles;
+    }
+  }
+  if (threadIdx.x == 0 && (all == 0 || !*in_order)) found->all = 0;
+  __syncthreads();
+}
+// The block whose run holds a tile.
+__device__ __forceinline__ int32_t block_of(const RowsWork& w, int64_t tiles, int64_t tile) {
+  return (int32_t)(((tile + 1) * w.blocks - 1) / tiles);
+}
+// Places of row r (of group * n_q) of a piece: of a block's run only the first piece and the last can be parts of a sample.
+__device__ __forceinline__ size_t part_at(const AttnArgs& a, const RowsWork& w, int64_t block, int kv, bool first, int r) {
+  const int64_t piece = 2 * ((int64_t)kv * w.blocks + block) + (first ? 0 : 1);
   return (size_t)piece * (a.heads / a.kv_heads * w.most_queries) + r;
 }
 
@@ -93,33 +134,48 @@ struct Piece {
   Segment g;
   uint32_t s;
   int32_t tile, tiles;  // the next tile of the sample, and its tiles
-  int64_t left;         // tiles of the block's run from there on
-  // rows of keys that belong to this piece
-  int32_t from, to;     // tiles
+  int32_t left;         // tiles of the block's run from there on
+  bool first;           // of the block's run
+  // what belongs to this piece
+  int32_t from, to;     // tiles of keys
+  uint32_t row, step;   // the first of its rows, sixteen at a time, and how far the next sixteen are
   bool skip, split;
 
-  __device__ __forceinline__ void set(const RowsWork& w) {
+  // (all: the number of tiles)
+  __device__ __forceinline__ void set(const RowsWork& w, int32_t all, int block) {
     from = tile;
-    to = (int32_t)min((int64_t)tiles, tile + left);
+    to = tile + min(tiles - tile, left);
     split = to - from < tiles;
     skip = g.n_q == 0;
-    if (split && g.n_q > w.most_queries) {  // no room for its pieces: whole, by the block that has its first tile
+    row = 0;
+    step = 16;
+    if (split && g.n_q > w.most_queries) {
+      // no room for its pieces: the blocks that share its tiles walk over all of them, and take its rows in turn
       split = false;
-      skip = skip || tile > 0;
       from = 0;
       to = tiles;
+      if (all < w.blocks) {  // (a tile to a block then, and blocks without)
+        row = 16 * (uint32_t)tile;
+        step = 16 * (uint32_t)tiles;
+      } else {
+        const int64_t at = first_of(w, all, block + 1) - left - tile;  // its first tile
+        const int32_t b = block_of(w, all, at);
+        row = 16 * (uint32_t)(block - b);
+        step = 16 * (uint32_t)(block_of(w, all, at + tiles - 1) - b + 1);
+      }
     }
   }
-  __device__ __forceinline__ bool next(const AttnArgs& a, const RowsWork& w) {
-    left -= min((int64_t)tiles - tile, left);
+  __device__ __forceinline__ bool next(const AttnArgs& a, const RowsWork& w, int32_t all, int block) {
+    left -= min(tiles - tile, left);
     if (left <= 0) return false;
     do {
       if (++s >= a.sequences) return false;
       g = segment(a, s);
-      tiles = segment_tiles<TilesOf::kKeys>(g, kTileKeys);
+      tiles = tiles_of(g.n_k, kTileKeys);
     } while (tiles == 0);
     tile = 0;
-    set(w);
+    first = false;
+    set(w, all, block);
     return true;
   }
 };
@@ -146,7 +202,9 @@ __global__ void __launch_bounds__(RowsShape<T, DP>::THREADS, RowsShape<T, DP>::B
   constexpr int VJ = kF32 ? 4 : 8;              // column tiles of a value load
   constexpr int E = 16 / sizeof(T);
   constexpr int LD = DP + 4, WARPS = C::WARPS;
-  __shared__ FoundTile found;
+  __shared__ int s_timed_out;
+  __shared__ Begin found;
+  __shared__ Piece s_piece[WARPS + 1];
   __shared__ int32_t warp_sums[WARPS + 1];
   __shared__ float s_m[WARPS][16], s_l[WARPS][16];
   extern __shared__ uint8_t smem_raw[];
@@ -155,6 +213,7 @@ __global__ void __launch_bounds__(RowsShape<T, DP>::THREADS, RowsShape<T, DP>::B
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::TAIL);
   uint64_t* empty = full + C::SLOTS;
   if (threadIdx.x == 0) {
+    s_timed_out = 0;
     for (int i = 0; i < C::SLOTS; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 4);
@@ -166,10 +225,15 @@ __global__ void __launch_bounds__(RowsShape<T, DP>::THREADS, RowsShape<T, DP>::B
   const int kv = blockIdx.x % a.kv_heads, block = blockIdx.x / a.kv_heads;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gr = lane >> 2, c = lane & 3;
   const int group = a.heads / a.kv_heads;
-  // rows of segments without keys become zeros: a warp looks at 32 segments at a time
-  for (uint32_t s0 = (uint32_t)(block * (WARPS + 1) + warp) * 32; s0 < a.sequences + 2; s0 += (uint32_t)w.blocks * (WARPS + 1) * 32) {
+  bool in_order;
+  find_begin<C::THREADS>(a, w, block, &found, warp_sums, &in_order);
+  if (kv == 0 && threadIdx.x == 0) w.starts[3 * block + 2] = found.all;
+  if (!in_order) return;  // (rows of several samples: no bound on the work)
+  // rows of segments without keys become zeros, while the first copies are on their way: a warp looks at 32 segments at a time
+  const uint32_t looked_at = warp < WARPS ? a.sequences + 2 : 0;
+  for (uint32_t s0 = (uint32_t)(block * WARPS + warp) * 32; s0 < looked_at; s0 += (uint32_t)w.blocks * WARPS * 32) {
     Segment g = {};
-    if (s0 + lane < a.sequences + 2) g = segment(a, s0 + lane);
+    if (s0 + lane < looked_at) g = segment(a, s0 + lane);
     for (uint32_t some = __ballot_sync(0xffffffffu, g.n_k == 0 && g.n_q > 0); some; some &= some - 1) {
       const int from = __ffs(some) - 1, q0 = __shfl_sync(0xffffffffu, g.q0, from), n_q = __shfl_sync(0xffffffffu, g.n_q, from);
       for (int r = 0; r < group * n_q; ++r) {
@@ -179,28 +243,25 @@ __global__ void __launch_bounds__(RowsShape<T, DP>::THREADS, RowsShape<T, DP>::B
       }
     }
   }
-  Piece piece;
-  {
-    const TileScan scan = scan_tiles<C::THREADS, TilesOf::kKeys>(a, kTileKeys, warp_sums);
-    if (scan.total <= 0) {
-      if (kv == 0 && threadIdx.x == 0) w.starts[3 * block + 2] = 0;
-      return;
-    }
-    const int32_t want = (int32_t)first_of(w, scan.total, block);
-    piece.left = first_of(w, scan.total, block + 1) - want;
-    pick_tile<TilesOf::kKeys>(a, scan, want, kTileKeys, &found);
-    if (kv == 0 && threadIdx.x == 0) {
-      w.starts[3 * block] = (int32_t)found.segment;
-      w.starts[3 * block + 1] = want - found.tile;
-      w.starts[3 * block + 2] = scan.total;
-    }
-    if (piece.left <= 0) return;
+  if (found.all == 0) return;
+  const int32_t want = (int32_t)first_of(w, found.all, block), end = (int32_t)first_of(w, found.all, block + 1);
+  if (kv == 0 && threadIdx.x == 0) {
+    w.starts[3 * block] = (int32_t)found.s;
+    w.starts[3 * block + 1] = want - found.tile;
+  }
+  if (want == end) return;
+  // in shared memory, a copy for every warp: registers are short
+  Piece& piece = s_piece[warp];
+  if (lane == 0) {
     piece.g = found.g;
-    piece.s = found.segment;
+    piece.s = found.s;
     piece.tile = found.tile;
     piece.tiles = found.tiles;
-    piece.set(w);
+    piece.left = end - want;
+    piece.first = true;
+    piece.set(w, found.all, block);
   }
+  __syncwarp();
 
   const float scale = a.scale * kLog2e;
   const uint32_t ring = smem_u32(smem);
@@ -210,9 +271,9 @@ __global__ void __launch_bounds__(RowsShape<T, DP>::THREADS, RowsShape<T, DP>::B
   if (warp == WARPS) {
     // ------------------------------ bulk copies ----------------------------------------
     if (lane == 0) {
-      for (bool more = true; more && !timed_out; more = piece.next(a, w)) {
+      for (bool more = true; more && !timed_out; more = piece.next(a, w, found.all, block)) {
         if (piece.skip) continue;
-        for (int r0 = 0; r0 < group * piece.g.n_q && !timed_out; r0 += 16) {
+        for (uint32_t r = piece.row; r < (uint32_t)(group * piece.g.n_q) && !timed_out; r += piece.step) {
           for (int t = piece.from; t < piece.to; ++t, ++it) {
             const uint32_t s = it % C::SLOTS;
             if (!mbar_wait(&empty[s], ((it / C::SLOTS) & 1u) ^ 1u)) { timed_out = true; break; }
@@ -235,12 +296,20 @@ __global__ void __launch_bounds__(RowsShape<T, DP>::THREADS, RowsShape<T, DP>::B
 
   auto sync_warps = [] { asm volatile("bar.sync 1, %0;" ::"n"(WARPS * 32) : "memory"); };  // those that compute
   const int mine16 = (warp & 3) * 16;                                                      // this warp's keys of a tile
-  for (bool more = true; more && !timed_out; more = piece.next(a, w)) {
+  auto next_piece = [&] {
+    __syncwarp();
+    bool more = false;
+    if (lane == 0) more = piece.next(a, w, found.all, block);
+    return __any_sync(0xffffffffu, more) != 0;  // (a barrier of the warp, too)
+  };
+  for (bool more = true; more && !timed_out; more = next_piece()) {
+    __syncwarp();
     if (piece.skip) continue;
     const Segment& g = piece.g;
-    const int hi = g.n_k;
+    const int hi = g.n_k, first_tile = piece.from, last_tile = piece.to;
     const int rows = group * g.n_q;
-    for (int r0 = 0; r0 < rows; r0 += 16) {
+    for (uint32_t from = piece.row; from < (uint32_t)rows && !timed_out; from += piece.step) {
+      const int r0 = (int)from;
       // q of rows gr and gr + 8 as operands
       uint32_t q[kF32 ? 1 : 2 * KC][4];
       int see[2];
@@ -286,10 +355,13 @@ __global__ void __launch_bounds__(RowsShape<T, DP>::THREADS, RowsShape<T, DP>::B
         for (int e = 0; e < 4; ++e) o[j][e] = 0.f;
       float m[2] = {-CUDART_INF_F, -CUDART_INF_F}, l[2] = {0.f, 0.f};
 
-      for (int t64 = piece.from + warp / 4; t64 < piece.to; t64 += WARPS / 4) {
-        const uint32_t load = it + (uint32_t)(t64 - piece.from), slot = load % C::SLOTS;
-        if (!timed_out && !mbar_wait(&full[slot], (load / C::SLOTS) & 1u)) timed_out = true;
-        if (timed_out) break;
+      for (int t64 = first_tile + warp / 4; t64 < last_tile; t64 += WARPS / 4) {
+        const uint32_t load = it + (uint32_t)(t64 - first_tile), slot = load % C::SLOTS;
+        const bool here = mbar_wait(&full[slot], (load / C::SLOTS) & 1u);
+        if (!__all_sync(0xffffffffu, here)) {
+          timed_out = true;
+          break;
+        }
         const int k0 = t64 * kTileKeys + mine16;
         const uint8_t* s_k = smem + slot * C::SLOT;
         // row and 16-byte piece of a tile, swizzled
@@ -419,7 +491,7 @@ __global__ void __launch_bounds__(RowsShape<T, DP>::THREADS, RowsShape<T, DP>::B
         l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
         l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
       }
-      it += (uint32_t)(piece.to - piece.from);
+      it += (uint32_t)(last_tile - first_tile);
       // the warps, joined in their order
 #pragma unroll
       for (int e = 0; e < 2; ++e)
@@ -427,7 +499,9 @@ __global__ void __launch_bounds__(RowsShape<T, DP>::THREADS, RowsShape<T, DP>::B
           s_m[warp][gr + 8 * e] = m[e];
           s_l[warp][gr + 8 * e] = l[e];
         }
+      if (timed_out) s_timed_out = 1;
       sync_warps();
+      timed_out = s_timed_out != 0;  // all warps leave together
       float mine[2];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
@@ -474,7 +548,7 @@ __global__ void __launch_bounds__(RowsShape<T, DP>::THREADS, RowsShape<T, DP>::B
           // (a warp without a visible key has summed nothing; one with NaN scores has no maximum either, but a sum that is NaN)
           sum += s_m[k][r] == -CUDART_INF_F ? s_l[k][r] : s_l[k][r] * exp2f(s_m[k][r] - top);
         const int i = (r0 + r) / group, h = kv * group + (r0 + r) % group;
-        const size_t part = piece.split ? part_at(a, w, block, kv, piece.s, r0 + r) : 0;
+        const size_t part = piece.split ? part_at(a, w, block, kv, piece.first, r0 + r) : 0;
         const size_t at = ((size_t)(g.q0 + i) * a.heads + h) * a.dim;
         for (int d = lane; d < a.dim; d += 32) {
           const float v = s_o[r * LD + d];
@@ -509,9 +583,10 @@ __global__ void __launch_bounds__(kSumThreads) k_attention_rows_sum(const AttnAr
   if (all <= 0 || first_of(w, all, block) == at0 || first_of(w, all, block - 1) > at0) return;
   const Segment g = segment(a, s);
   if (g.n_q > w.most_queries) return;  // stored by the first kernel
-  const int32_t end = at0 + segment_tiles<TilesOf::kKeys>(g, kTileKeys);
+  const int32_t end = at0 + tiles_of(g.n_k, kTileKeys);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int first = block - 1;
+  const bool whole = first_of(w, all, first) == at0;  // its run begins with this sample
   // the blocks k with first_of(k) < end
   const int64_t past = ((int64_t)end * w.blocks + all - 1) / all;
   const int pieces = (int)min(past, (int64_t)w.blocks) - first;
@@ -521,7 +596,7 @@ __global__ void __launch_bounds__(kSumThreads) k_attention_rows_sum(const AttnAr
     const int r = i * group + h % group;
     float top = -CUDART_INF_F, sum = 0.f;
     for (int k = warp * 32 + lane; k < pieces; k += kSumThreads) {
-      if (!has_none(first + k)) top = fmaxf(top, __ldg(w.sums + part_at(a, w, first + k, kv, s, r) * 2));
+      if (!has_none(first + k)) top = fmaxf(top, __ldg(w.sums + part_at(a, w, first + k, kv, k > 0 || whole, r) * 2));
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -534,7 +609,7 @@ __global__ void __launch_bounds__(kSumThreads) k_attention_rows_sum(const AttnAr
 #pragma unroll 4
     for (int k = warp; k < pieces; k += kSumWarps) {
       if (has_none(first + k)) continue;
-      const size_t part = part_at(a, w, first + k, kv, s, r);
+      const size_t part = part_at(a, w, first + k, kv, k > 0 || whole, r);
       const float mk = __ldg(w.sums + part * 2), lk = __ldg(w.sums + part * 2 + 1);
       const float by = mk == -CUDART_INF_F ? 0.f : exp2f(mk - top);
       sum += mk == -CUDART_INF_F ? lk : lk * by;
@@ -566,12 +641,12 @@ struct RowsSizes {
   size_t sums_at, parts_at, total;
 };
 // As many blocks as fit the SMs at once, but two tiles for each at least.
-RowsSizes rows_sizes(uint32_t rows_q, uint32_t rows_k, uint32_t sequences, int heads, int kv_heads, int dim, int dtype) {
+RowsSizes rows_sizes(uint32_t rows_k, int heads, int kv_heads, int dim, int dtype) {
   RowsSizes z;
   const uint64_t pairs = ((uint64_t)rows_k / kTileKeys + 1) / 2, fit = 148 * (dtype == RMN_F32 ? 1 : 2) / kv_heads;
   z.blocks = (int)std::max<uint64_t>(1, std::min(pairs, fit));
-  z.most_queries = (int)((rows_q + sequences - 1) / sequences);
-  const size_t parts = ((size_t)z.blocks + sequences) * heads * z.most_queries;
+  z.most_queries = std::max(1, kMostRows / (heads / kv_heads));
+  const size_t parts = (size_t)z.blocks * 2 * heads * z.most_queries;
   auto up = [](size_t v) { return (v + 255) / 256 * 256; };
   z.sums_at = up((size_t)z.blocks * 3 * sizeof(int32_t));
   z.parts_at = up(z.sums_at + parts * 2 * sizeof(float));
@@ -598,9 +673,9 @@ int launch_rows(const CUtensorMap& k, const CUtensorMap& v, const AttnArgs& a, c
 size_t attention_rows_workspace(uint32_t rows_q, uint32_t rows_k, uint32_t sequences, int heads, int kv_heads, int dim, int dtype) {
   if (!rows_q || !rows_k || !sequences || dim > 128 || dim % (dtype == RMN_F32 ? 4 : 8)) return 0;
   const uint64_t rows = ((uint64_t)rows_q + sequences - 1) / sequences * (heads / kv_heads);
-  if (rows > 32) return 0;
+  if (rows > kMostRows) return 0;
   if ((uint64_t)rows_q * heads > 0x7fffffffull) return 0;
-  return rows_sizes(rows_q, rows_k, sequences, heads, kv_heads, dim, dtype).total;
+  return rows_sizes(rows_k, heads, kv_heads, dim, dtype).total;
 }
 
 int attention_rows_forward(const AttnArgs& a, int dtype, void* workspace, cudaStream_t stream) {
@@ -610,7 +685,7 @@ int attention_rows_forward(const AttnArgs& a, int dtype, void* workspace, cudaSt
   if (!make_head_map(&k, a.k, a.rows_k, a.kv_heads, a.dim, a.k_row, a.k_head, kTileKeys, elem) ||
       !make_head_map(&v, a.v, a.rows_k, a.kv_heads, a.dim, a.v_row, a.v_head, kTileKeys, elem))
     return RMN_ERR_UNSUPPORTED;
-  const RowsSizes z = rows_sizes(a.rows_q, a.rows_k, a.sequences, a.heads, a.kv_heads, a.dim, dtype);
+  const RowsSizes z = rows_sizes(a.rows_k, a.heads, a.kv_heads, a.dim, dtype);
   char* base = static_cast<char*>(workspace);
   const RowsWork w = {z.blocks, z.most_queries, reinterpret_cast<int32_t*>(base), reinterpret_cast<float*>(base + z.sums_at),
                       reinterpret_cast<float*>(base + z.parts_at)};

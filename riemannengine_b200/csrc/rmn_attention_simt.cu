@@ -37,8 +37,6 @@ struct SimtShape {
   static constexpr size_t tile = (size_t)BM * LD * sizeof(float), square = (size_t)BM * LP * sizeof(float);
 };
 
-__device__ __forceinline__ float load_f32(const float* p) { return __ldg(p); }
-__device__ __forceinline__ float load_f32(const __nv_bfloat16* p) { return __bfloat162float(*p); }
 __device__ __forceinline__ void store_f32(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store_f32(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 

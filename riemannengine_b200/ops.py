@@ -560,6 +560,9 @@ def field_splat(field: torch.Tensor, feats: torch.Tensor):
     return out_c, out_f
 
 
+_INT32_MAX = (1 << 31) - 1  # (the C ABI would take what is left of a larger size)
+
+
 def _rows(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
     """``t`` [N, C] with adjacent channels and the distance of its rows; a copy where its strides are others."""
     if (t.size(1) > 1 and t.stride(1) != 1) or t.stride(0) < 0:
@@ -572,6 +575,8 @@ def _check_norm_params(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Op
     _require_cuda(x, "features")
     if x.dim() != 2 or x.size(1) < 1:
         raise RuntimeError("features must be [N, C]")
+    if max(x.shape) > _INT32_MAX:
+        raise RuntimeError("layer norm takes fewer than 2^31 rows and channels")
     _dtype_code(x)
     code = None
     for name, p in (("weight", weight), ("bias", bias)):
@@ -639,6 +644,8 @@ def sample_offsets(coords: torch.Tensor, n_samples: int) -> torch.Tensor:
     """int32 [n_samples + 2]: first row of every sample of ``coords``, the number of rows, and the number of runs of equal
     batch indices (rmn_sample_offsets)."""
     _check_coords(coords)
+    if not 0 <= n_samples <= _INT32_MAX - 16 or coords.size(0) > _INT32_MAX:
+        raise RuntimeError("sample_offsets takes fewer than 2^31 rows and samples")
     lib = capi.lib()
     out = torch.empty(n_samples + 2, dtype=torch.int32, device=coords.device)
     wbytes = lib.rmn_sample_offsets_workspace_bytes(n_samples)
@@ -662,6 +669,8 @@ def _attention(q, k, v, offsets, kv_offsets, kv_lengths, causal, scale) -> capi.
             raise RuntimeError(f"{name} must be [rows, heads, channels]")
         if t.dtype != q.dtype or t.device != q.device:
             raise RuntimeError("q, k and v must have the same dtype and device")
+        if max(t.shape) > _INT32_MAX:
+            raise RuntimeError(f"{name} must have fewer than 2^31 rows, heads and channels")
     if k.shape != v.shape or k.size(2) != q.size(2):
         raise RuntimeError("k and v must have the same shape, and q's channels")
     if q.size(1) < 1 or k.size(1) < 1 or q.size(1) % k.size(1):
@@ -673,8 +682,8 @@ def _attention(q, k, v, offsets, kv_offsets, kv_lengths, causal, scale) -> capi.
         if t.dim() != 1 or t.dtype != torch.int32 or not t.is_contiguous() or t.device != q.device:
             raise RuntimeError(f"{name} must be a contiguous 1-D int32 tensor on q's device")
     n = int(offsets.numel()) - 1
-    if n < 0:
-        raise RuntimeError("offsets must hold one entry more than there are samples")
+    if not 0 <= n < _INT32_MAX:
+        raise RuntimeError("offsets must hold one entry more than there are samples, fewer than 2^31")
     if kv_offsets is not None and kv_offsets.numel() != n + 1:
         raise RuntimeError("kv_offsets must have as many entries as offsets")
     if kv_lengths is not None and kv_lengths.numel() != n:

@@ -13,6 +13,7 @@
 #include <cmath>
 #include <cstdlib>
 #include <cstring>
+#include <limits>
 #include <map>
 #include <mutex>
 #include <stdexcept>
@@ -1819,6 +1820,12 @@ void check_plain(const at::Tensor& t, const char* what) {
   TORCH_CHECK(t.is_cuda(), what, " must be a CUDA tensor: this library has no CPU path");
   TORCH_CHECK(plain_autograd(t), what, " must be a plain tensor without forward-mode derivatives");
 }
+// every size (the C ABI would take what is left of a larger one)
+bool fits_int32(const at::Tensor& t) {
+  for (int64_t n : t.sizes())
+    if (n > std::numeric_limits<int32_t>::max()) return false;
+  return true;
+}
 void check_once(const at::Tensor& grad, const char* what) {
   TORCH_CHECK(!(at::GradMode::is_enabled() && grad.requires_grad()), what, " is differentiable once only");
 }
@@ -1963,6 +1970,7 @@ public:
 at::Tensor layer_norm(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& bias, double eps) {
   check_plain(x, "features");
   TORCH_CHECK(x.dim() == 2 && x.size(1) >= 1, "features must be [N, C]");
+  TORCH_CHECK(fits_int32(x), "layer norm takes fewer than 2^31 rows and channels");
   dtype_code(x);
   for (auto const& [p, name] : {std::pair<const at::Tensor&, const char*>{weight, "weight"}, {bias, "bias"}}) {
     if (!p.defined()) continue;
@@ -1997,6 +2005,7 @@ at::Tensor packed_attention(const at::Tensor& q, const at::Tensor& k, const at::
     check_plain(t, name);
     TORCH_CHECK(t.dim() == 3 && t.size(2) >= 1, name, " must be [rows, heads, channels]");
     TORCH_CHECK(t.scalar_type() == q.scalar_type() && t.device() == q.device(), "q, k and v must have the same dtype and device");
+    TORCH_CHECK(fits_int32(t), name, " must have fewer than 2^31 rows, heads and channels");
   }
   dtype_code(q);
   TORCH_CHECK(k.sizes() == v.sizes() && k.size(2) == q.size(2), "k and v must have the same shape, and q's channels");
@@ -2010,7 +2019,7 @@ at::Tensor packed_attention(const at::Tensor& q, const at::Tensor& k, const at::
                 name, " must be a contiguous 1-D int32 tensor on q's device");
   }
   const int64_t n = offsets.numel() - 1;
-  TORCH_CHECK(n >= 0, "offsets must hold one entry more than there are samples");
+  TORCH_CHECK(n >= 0 && fits_int32(offsets), "offsets must hold one entry more than there are samples, fewer than 2^31");
   TORCH_CHECK(!kv_offsets.defined() || kv_offsets.numel() == n + 1, "kv_offsets must have as many entries as offsets");
   TORCH_CHECK(!kv_lengths.defined() || kv_lengths.numel() == n, "kv_lengths must have one entry per sample");
   TORCH_CHECK(kv_offsets.defined() || k.size(0) == q.size(0), "q and k must have the same rows unless kv_offsets are given");

@@ -296,6 +296,22 @@ def test_many_samples(dtype):
     P.check(_host("cpp")(q, k, v, offsets, _offsets(nk), causal=True), P.attention(q, k, v, offsets, _offsets(nk), causal=True)["out"])
 
 
+@pytest.mark.parametrize("samples", [383, 384, 385, 1100])
+def test_samples_counted_and_searched_for(samples):
+    """Rows before the first sample and behind the last, slots longer than what is in use, samples without rows."""
+    lens = [(i * 7) % 13 if i % 50 else 140 for i in range(samples)]
+    slots = [(i * 5) % 17 if i % 40 else 150 for i in range(samples)]
+    used = torch.tensor([max(0, n - i % 3) for i, n in enumerate(slots)], dtype=torch.int32, device=DEV)
+    offsets, kv_offsets = _offsets(lens, 9), _offsets(slots, 300)
+    q, _, _, grad = _inputs(sum(lens) + 9 + 260, 1, 1, 1, 40, torch.bfloat16)
+    k, v = _inputs(sum(slots) + 300 + 5, sum(slots) + 300 + 5, 1, 1, 40, torch.bfloat16)[1:3]
+    out, dq, dk, dv = _check("cpp", q, k, v, grad, offsets, kv_offsets, used, True)
+    for t, a, b in ((out, 9, offsets[-1]), (dq, 9, offsets[-1]), (dk, 300, kv_offsets[-1]), (dv, 300, kv_offsets[-1])):
+        assert not t[:a].any() and not t[b:].any()
+    x = [t.float() for t in (q, k, v, grad)]
+    _check("cpp", *x, offsets, kv_offsets, used, True)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_offsets_that_leave_the_tensors_are_reported(dtype):
     from riemannengine_b200 import capi
@@ -395,6 +411,67 @@ def test_refusals(host):
     with pytest.raises(RuntimeError, match="once|differentiate twice"):
         (g,) = torch.autograd.grad(f(a, k, v, o), a, w, create_graph=True)
         g.sum().backward()
+
+
+@pytest.mark.parametrize("host", ["python", "cpp"])
+def test_sizes_that_do_not_fit_are_refused(host):
+    f = _host(host)
+    q, o = torch.zeros(1, 1, 8, device=DEV), _offsets([1])
+    for many in (q.expand(2**32 + 1, 1, 8), q.expand(1, 2**32 + 1, 8)):
+        with pytest.raises(RuntimeError, match="2\\^31"):
+            f(many, q, q, o, o)
+        with pytest.raises(RuntimeError, match="2\\^31"):
+            f(q, many, many, o, o)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("h,hk,d", [(4, 4, 32), (4, 2, 128), (16, 2, 64)])
+def test_uneven_new_rows_against_long_keys(dtype, h, hk, d):
+    """Few new rows on average, many of some samples, whose keys several blocks share; and fewer tiles of keys than blocks."""
+    nq, nk = [150, 0, 7, 20] + [1] * 60, [3000, 700, 2500, 1000] + [64, 1, 130] * 20
+    slots = [n + 3 for n in nk]
+    q, k, v, _ = _inputs(sum(nq), sum(slots), h, hk, d, TYPES[dtype], seed=3)
+    offsets, kv_offsets = _offsets(nq), _offsets(slots)
+    few = [0] * len(nk)
+    few[0], few[2], few[3] = 200, 130, 64
+    for used in (nk, few):
+        lengths = torch.tensor(used, dtype=torch.int32, device=DEV)
+        for causal in (False, True):
+            want = P.attention(q, k, v, offsets, kv_offsets, lengths, causal)["out"]
+            for host in ("python", "cpp"):
+                P.check(_host(host)(q, k, v, offsets, kv_offsets, lengths, causal), want, f"{used[:4]} {causal} {host}")
+
+
+def test_offsets_that_give_rows_to_many_samples():
+    """2^17 samples that each claim all rows: more tiles than 32 bits count. The call reports it and touches only its tensors."""
+    from riemannengine_b200 import capi
+    lib = capi.lib()
+    stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    n = 1 << 21
+    offsets = torch.tensor([0, n], dtype=torch.int32, device=DEV).repeat(1 << 16)
+    lengths = torch.zeros(offsets.numel() - 1, dtype=torch.int32, device=DEV)
+    for heads in (1, 4):
+        q = torch.zeros(n, heads, 8, dtype=torch.bfloat16, device=DEV)
+        out = _host("cpp")(q, q[:, :1], q[:, :1], offsets, None, lengths, True)
+        assert lib.rmn_device_status(stream) == capi.ERR_BAD_ARG
+        del out
+    assert lib.rmn_device_status(stream) == capi.OK
+
+
+@pytest.mark.parametrize("n,runs", [(0, 0), (1, 1), (255, 3), (1000, 1000), (300_001, 7), (300_001, 100_000), (2_000_000, 1_999_999)])
+def test_sample_offsets(n, runs):
+    from riemannengine_b200 import ops
+    g = _gen(n + runs)
+    starts = torch.sort(torch.randperm(max(n - 1, 0), generator=g, device=DEV)[:max(runs - 1, 0)] + 1).values
+    batch = torch.zeros(n, dtype=torch.int32, device=DEV)
+    batch[starts] = 1
+    coords = torch.zeros(n, 4, dtype=torch.int32, device=DEV)
+    coords[:, 0] = batch.cumsum(0) * 37 % 65521  # neighbours differ
+    coords[:, 1] = torch.randint(0, 9, (n,), generator=g, device=DEV)
+    first = torch.cat([torch.zeros(min(n, 1), dtype=torch.int64, device=DEV), starts]).tolist()
+    for room in sorted({runs, max(runs - 1, 0), runs + 3}):
+        want = (first + [n] * 3)[:room] + [n, runs]
+        assert ops.sample_offsets(coords, room).tolist() == want
 
 
 def _cloud(host, order):

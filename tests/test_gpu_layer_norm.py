@@ -1,4 +1,6 @@
 """Layer norm over the channels of every row: both hosts against 64 bits, forward and backward."""
+import ctypes
+
 import pytest
 import torch
 
@@ -196,6 +198,34 @@ def test_on_a_stream_and_captured(host):
         want = P.layer_norm(x2, w2, b2, 1e-5, dy2)
         for name, got in (("y", y), ("dx", grads[0]), ("dw", grads[1]), ("db", grads[2])):
             P.check(got, want[name], name)
+
+
+@pytest.mark.parametrize("host", ["python", "cpp"])
+def test_sizes_that_do_not_fit_are_refused(host):
+    with pytest.raises(RuntimeError, match="2\\^31"):
+        _host(host)(torch.zeros(1, 8, device=DEV).expand(2**32 + 1, 8), None, None, 1e-5)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n,c", [(5, 3), (1000, 64), (300, 1024), (7, 5000)])
+def test_in_place(dtype, n, c):
+    """The C calls may write over x and over dy."""
+    from riemannengine_b200 import capi, ops
+    x, w, b, dy = _inputs(n, c, TYPES[dtype])
+    want = P.layer_norm(x, w, b, 1e-5, dy)
+    code, pcode = (capi.F32 if t.dtype == torch.float32 else capi.BF16 for t in (x, w))
+    lib, p = capi.lib(), lambda t: ctypes.c_void_p(t.data_ptr())  # noqa: E731
+    stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    y, stats = x.clone(), torch.empty(2, n, device=DEV)
+    assert lib.rmn_layer_norm_forward(p(y), c, n, c, p(w), p(b), pcode, 1e-5, p(y), p(stats[0]), p(stats[1]), code, stream) == 0
+    P.check(y, want["y"], "y")
+    dx, dw, db = dy.clone(), torch.empty_like(w), torch.empty_like(b)
+    nbytes = lib.rmn_layer_norm_backward_workspace_bytes(n, c)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=DEV)
+    assert lib.rmn_layer_norm_backward(p(dx), c, p(x), c, n, c, p(w), pcode, p(stats[0]), p(stats[1]), p(dx), p(dw), p(db), code,
+                                       p(ws), nbytes, stream) == 0
+    for name, got in (("dx", dx), ("dw", dw), ("db", db)):
+        P.check(got, want[name], name)
 
 
 @pytest.mark.parametrize("host", ["python", "cpp"])
