@@ -60,12 +60,15 @@ const char *rmn_status_string(int status);
 /* Number of CUDA kernels this library has launched in this process so far
  * (telemetry for benchmarks; no counterpart in the reference). */
 unsigned long long rmn_launch_count(void);
-/* Of those, launches of the tcgen05 convolution kernels (forward, input gradient, weight gradient): tells a
- * host that a convolution ran on the tensor cores and not on the SIMT kernels. No counterpart in the reference. */
+/* Of those, launches of the tcgen05 kernels of convolutions (forward, input gradient, weight gradient) and of attention (forward,
+ * one; backward, two): tells a host that a call ran on the tensor cores and not on the SIMT kernels. No counterpart in the
+ * reference. */
 unsigned long long rmn_tensor_core_launch_count(void);
 /* Synchronises `stream` and returns the device-side status of the convolution
- * kernels: RMN_OK, or RMN_ERR_TIMEOUT when a bounded wait inside a kernel ran
- * out (the kernel then returned early and its output is invalid). The status
+ * and attention kernels: RMN_OK, or RMN_ERR_TIMEOUT when a bounded wait inside a
+ * kernel ran out (the kernel then returned early and its output is invalid), or
+ * RMN_ERR_BAD_ARG when attention met offsets or lengths that do not ascend or
+ * leave their tensors. The status
  * is ONE word per device, shared by all streams; a non-zero value is returned
  * once and reset by the call that returns it. rmn_table_info returns the same
  * status (and resets it) when the table itself is fine, so a host that builds

@@ -371,9 +371,12 @@ __global__ void __launch_bounds__(BwdShape<DP>::THREADS, BwdShape<DP>::BLOCKS)
             tma_load_3d(ring + s * C::TILE + c * (STEP * 128), which ? &map_g : &map_q, &tail->full[s], c * 64, h, g.q0 + q0);
         }
       }
-      __syncwarp();
       const int b = step % kStats;
-      if (!wait(&tail->st_empty[b], (((uint32_t)step / kStats) & 1u) ^ 1u)) break;
+      wait(&tail->st_empty[b], (((uint32_t)step / kStats) & 1u) ^ 1u);
+      if (__any_sync(0xffffffffu, timed_out)) {  // the warp leaves together
+        timed_out = true;
+        break;
+      }
 #pragma unroll
       for (int k = 0; k < N; ++k) {
         tail->lse[b][k * 32 + lane] = x[k];
