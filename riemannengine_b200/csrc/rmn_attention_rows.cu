@@ -7,7 +7,9 @@
 // a time as the rows of warp-wide matrix products (their rate does not bound here: 16 rows cost one product for 8 keys). Bulk copies bring a tile's keys and values into a ring in shared memory, some 100 KB in
 // flight for a block, across the borders of pieces; each of four warps (in fp32 eight, four a tile) takes 16 of the 64 keys and has a
 // running maximum and sum of its own. The warps are joined in shared memory, and the pieces of a sample that several blocks
-// share by a second kernel, in a fixed order.
+// share by a second kernel, in a fixed order. 16 samples of 509 ... 30011 keys, 16 query and 4 key heads of 128 (336 MB in bf16):
+// 62 us, 5.4 TB/s, and 8 us for the second kernel; in fp32 150 us for both, where the three products of every operand take longer
+// than its bytes.
 //
 // Keys and values go from shared memory to registers as 16-byte loads that are product operands as they stand: which of a row's
 // channels is which k of a product is free as long as q has the same order, and which channel is which column of the output is free
