@@ -648,7 +648,7 @@ RowsSizes rows_sizes(uint32_t rows_k, int heads, int kv_heads, int dim, int dtyp
   const uint64_t pairs = ((uint64_t)rows_k / kTileKeys + 1) / 2, fit = 148 * (dtype == RMN_F32 ? 1 : 2) / kv_heads;
   z.blocks = (int)std::max<uint64_t>(1, std::min(pairs, fit));
   z.most_queries = std::max(1, kMostRows / (heads / kv_heads));
-  const size_t parts = (size_t)z.blocks * 2 * heads * z.most_queries;
+  const size_t parts = z.blocks > 1 ? (size_t)z.blocks * 2 * heads * z.most_queries : 0;  // (one block: whole samples)
   auto up = [](size_t v) { return (v + 255) / 256 * 256; };
   z.sums_at = up((size_t)z.blocks * 3 * sizeof(int32_t));
   z.parts_at = up(z.sums_at + parts * 2 * sizeof(float));

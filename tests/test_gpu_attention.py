@@ -442,6 +442,49 @@ def test_uneven_new_rows_against_long_keys(dtype, h, hk, d):
                 P.check(_host(host)(q, k, v, offsets, kv_offsets, lengths, causal), want, f"{used[:4]} {causal} {host}")
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_hundreds_of_heads(dtype):
+    """More key heads than the GPU has places for blocks of one each."""
+    q, k, v, grad = _inputs(70, 70, 320, 320, 16, TYPES[dtype])
+    _check("cpp", q, k, v, grad, _offsets([20, 50]), causal=True)
+    one = torch.arange(3, dtype=torch.int32, device=DEV)
+    want = P.attention(q[:2], k, v, one, _offsets([20, 50]), None, True)["out"]
+    P.check(_host("cpp")(q[:2], k, v, one, _offsets([20, 50]), None, True), want)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("causal", [False, True])
+def test_lengths_without_offsets_of_their_own(dtype, causal):
+    lens, used = [40, 200, 1, 130, 9], [40, 33, 0, 129, 1]
+    q, k, v, grad = _inputs(sum(lens), sum(lens), 4, 2, 64, TYPES[dtype])
+    lengths = torch.tensor(used, dtype=torch.int32, device=DEV)
+    for host in ("python", "cpp"):
+        _check(host, q, k, v, grad, _offsets(lens), None, lengths, causal)
+
+
+@pytest.mark.parametrize("dtype,d", [("bf16", 64), ("f32", 32), ("f32", 30)])
+def test_a_cache_of_more_than_2_31_elements(dtype, d):
+    """The samples at the very end of it: prompts with their gradients, and new rows."""
+    lens = [300, 77]
+    rows = (1 << 31) // d + 5000
+    cache = torch.zeros(rows, 1, d, dtype=TYPES[dtype], device=DEV)
+    q, k, _, grad = _inputs(sum(lens), sum(lens), 2, 1, d, TYPES[dtype])
+    cache[-sum(lens):] = k
+    offsets, kv_offsets = _offsets(lens), _offsets(lens, rows - sum(lens))
+    want = P.attention(q, k, k, offsets, causal=True, grad=grad)
+    leaves = [q.requires_grad_(True), cache.requires_grad_(True)]
+    out = _host("cpp")(q, cache, cache.detach(), offsets, kv_offsets, None, True)
+    dq, dk = torch.autograd.grad(out, leaves, grad)
+    for name, got in (("out", out), ("dq", dq), ("dk", dk[-sum(lens):])):
+        P.check(got, want[name], name)
+    assert not dk[:5000].any() and not dk[rows - sum(lens) - 5000:rows - sum(lens)].any()
+    del dq, dk, out
+    one = torch.arange(3, dtype=torch.int32, device=DEV)
+    with torch.no_grad():
+        got = _host("cpp")(q[:2], cache, cache, one, kv_offsets, None, True)
+    P.check(got, P.attention(q[:2].detach(), k, k, one, offsets, None, True)["out"])
+
+
 def test_offsets_that_give_rows_to_many_samples():
     """2^17 samples that each claim all rows: more tiles than 32 bits count. The call reports it and touches only its tensors."""
     from riemannengine_b200 import capi

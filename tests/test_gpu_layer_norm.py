@@ -206,6 +206,19 @@ def test_sizes_that_do_not_fit_are_refused(host):
         _host(host)(torch.zeros(1, 8, device=DEV).expand(2**32 + 1, 8), None, None, 1e-5)
 
 
+def test_more_than_2_31_elements():
+    """The last rows of a tensor of 4 GB, forward and backward; the others are zero."""
+    n, c, last = (1 << 31) // 64 + 1000, 64, 500
+    x, w, b, dy = _inputs(last, c, torch.bfloat16)
+    many, grad = (torch.zeros(n, c, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    many[-last:], grad[-last:] = x, dy
+    want = P.layer_norm(x, w, b, 1e-5, dy)
+    y, (dx, dw, db) = _run("cpp", many, w, b, grad)
+    for name, got in (("y", y[-last:]), ("dx", dx[-last:]), ("dw", dw), ("db", db)):
+        P.check(got, want[name], name)
+    assert torch.equal(y[:1000], b.expand(1000, c)) and not dx[:1000].any()
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("n,c", [(5, 3), (1000, 64), (300, 1024), (7, 5000)])
 def test_in_place(dtype, n, c):
