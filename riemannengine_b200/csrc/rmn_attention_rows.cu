@@ -21,6 +21,7 @@
 #include <math_constants.h>
 
 #include <algorithm>
+#include <cmath>
 
 namespace rmn {
 namespace {
@@ -572,8 +573,8 @@ __global__ void __launch_bounds__(RowsShape<T, DP>::THREADS, RowsShape<T, DP>::B
   if (timed_out) atomicExch(a.status, (uint32_t)RMN_ERR_TIMEOUT);
 }
 
-// Sums the pieces of the sample that the run of block b begins inside of, for one head, each of eight warps every eighth
-// piece; the first of several blocks that begin inside of one sample does it.
+// Sums the pieces of the sample that the run of block b begins inside of, for one head and every gridDim.y-th row, each of eight
+// warps every eighth piece; the first of several blocks that begin inside of one sample does it.
 template <typename T>
 __global__ void __launch_bounds__(kSumThreads) k_attention_rows_sum(const AttnArgs a, const RowsWork w) {
   __shared__ float s_m[kSumWarps], s_l[kSumWarps], s_o[kSumWarps][128];
@@ -593,7 +594,7 @@ __global__ void __launch_bounds__(kSumThreads) k_attention_rows_sum(const AttnAr
   const int64_t past = ((int64_t)end * w.blocks + all - 1) / all;
   const int pieces = (int)min(past, (int64_t)w.blocks) - first;
   auto has_none = [&](int k) { return all < w.blocks && first_of(w, all, k) == first_of(w, all, k + 1); };  // more blocks than tiles
-  for (int i = 0; i < g.n_q; ++i) {
+  for (int i = blockIdx.y; i < g.n_q; i += gridDim.y) {
     const size_t at = ((size_t)(g.q0 + i) * a.heads + h) * a.dim;
     const int r = i * group + h % group;
     float top = -CUDART_INF_F, sum = 0.f;
@@ -642,10 +643,11 @@ struct RowsSizes {
   int blocks, most_queries;
   size_t sums_at, parts_at, total;
 };
-// As many blocks as fit the SMs at once, but two tiles for each at least.
-RowsSizes rows_sizes(uint32_t rows_k, int heads, int kv_heads, int dim, int dtype) {
+// As many blocks as fit the SMs at once, but two tiles for each at least (of as many tiles as there may be: 512 samples of 4 keys,
+// 8 / 2 heads of 64, 154 us by the tiles of their rows together).
+RowsSizes rows_sizes(uint32_t rows_k, uint32_t sequences, int heads, int kv_heads, int dim, int dtype) {
   RowsSizes z;
-  const uint64_t pairs = ((uint64_t)rows_k / kTileKeys + 1) / 2, fit = 148 * (dtype == RMN_F32 ? 1 : 2) / kv_heads;
+  const uint64_t pairs = ((uint64_t)rows_k / kTileKeys + sequences + 1) / 2, fit = 148 * (dtype == RMN_F32 ? 1 : 2) / kv_heads;
   z.blocks = (int)std::max<uint64_t>(1, std::min(pairs, fit));
   z.most_queries = std::max(1, kMostRows / (heads / kv_heads));
   const size_t parts = z.blocks > 1 ? (size_t)z.blocks * 2 * heads * z.most_queries : 0;  // (one block: whole samples)
@@ -664,20 +666,39 @@ int launch_rows(const CUtensorMap& k, const CUtensorMap& v, const AttnArgs& a, c
   RMN_CUDA_TRY(launch_overlapped(k_attention_rows<T, DP>, dim3((uint32_t)(w.blocks * a.kv_heads)), dim3(RowsShape<T, DP>::THREADS), smem, stream, k, v, a, w));
   RMN_LAUNCH_CHECK();
   if (w.blocks == 1) return RMN_OK;  // every sample is one piece
-  RMN_CUDA_TRY(launch_overlapped(k_attention_rows_sum<T>, dim3((uint32_t)(w.blocks - 1) * (uint32_t)a.heads), dim3(kSumThreads), 0,
-                                 stream, a, w));
+  const uint32_t rows = (a.rows_q + a.sequences - 1) / a.sequences;  // of a sample, on average
+  RMN_CUDA_TRY(launch_overlapped(k_attention_rows_sum<T>, dim3((uint32_t)(w.blocks - 1) * (uint32_t)a.heads, rows),
+                                 dim3(kSumThreads), 0, stream, a, w));
   RMN_LAUNCH_CHECK();
   return RMN_OK;
 }
 
 }  // namespace
 
+namespace {
+// Whether this form takes less time than whole tiles of 128 queries a head (bf16), both estimated in us from averages over the
+// samples: here sixteen rows of a sample and key head pass over its keys at a time, 64 keys a step, all SMs taking their share; there
+// every query head passes once, 128 keys a step, and the longest sample's chain is not cut. Measured (here, there): 16 samples of one
+// row and 509 ... 30011 keys, 16 / 4 heads of 128, 71 and 503 us; 16 samples of 5 rows and 8000 keys (16 x 5 / 8000), 8 heads of 64, 59 and 102; 512 x 4 / 4, 8 / 2 heads of 64, 32 and
+// 85; 512 x 16 / 16, 8 heads of 64, 81 and 88; but 64 x 20 / 1024 94 and 38, 256 x 32 / 32 84 and 46, 4 x 8 / 60 7.5 and 6.1.
+bool rows_take_less(uint32_t rows_q, uint32_t rows_k, uint32_t sequences, int heads, int kv_heads, int dim) {
+  const double n = sequences, rows = std::ceil(rows_q / n) * (heads / kv_heads), keys = rows_k / n;
+  const bool wide = dim > 64;
+  const double places = 148 * 2, pieces = std::max(1.0, n * kv_heads / places);
+  const double tiles = std::max(1.0, n * kv_heads * std::max(1.0, keys / kTileKeys) / places);  // a block
+  const double here = 4 + std::ceil(rows / 16) * (pieces * (1.5 + 0.22 * std::min(16.0, rows)) + tiles * (wide ? 1.8 : 1.2));
+  const double there = std::max(1.0, n * heads / places) * (5.5 + std::max(1.0, keys / 128) * (wide ? 1.9 : 1.1));
+  return here < there;
+}
+}  // namespace
+
 size_t attention_rows_workspace(uint32_t rows_q, uint32_t rows_k, uint32_t sequences, int heads, int kv_heads, int dim, int dtype) {
   if (!rows_q || !rows_k || !sequences || dim > 128 || dim % (dtype == RMN_F32 ? 4 : 8)) return 0;
   const uint64_t rows = ((uint64_t)rows_q + sequences - 1) / sequences * (heads / kv_heads);
   if (rows > kMostRows) return 0;
+  if (dtype == RMN_BF16 && !rows_take_less(rows_q, rows_k, sequences, heads, kv_heads, dim)) return 0;
   if ((uint64_t)rows_q * heads > 0x7fffffffull) return 0;
-  return rows_sizes(rows_k, heads, kv_heads, dim, dtype).total;
+  return rows_sizes(rows_k, sequences, heads, kv_heads, dim, dtype).total;
 }
 
 int attention_rows_forward(const AttnArgs& a, int dtype, void* workspace, cudaStream_t stream) {
@@ -687,7 +708,7 @@ int attention_rows_forward(const AttnArgs& a, int dtype, void* workspace, cudaSt
   if (!make_head_map(&k, a.k, a.rows_k, a.kv_heads, a.dim, a.k_row, a.k_head, kTileKeys, elem) ||
       !make_head_map(&v, a.v, a.rows_k, a.kv_heads, a.dim, a.v_row, a.v_head, kTileKeys, elem))
     return RMN_ERR_UNSUPPORTED;
-  const RowsSizes z = rows_sizes(a.rows_k, a.heads, a.kv_heads, a.dim, dtype);
+  const RowsSizes z = rows_sizes(a.rows_k, a.sequences, a.heads, a.kv_heads, a.dim, dtype);
   char* base = static_cast<char*>(workspace);
   const RowsWork w = {z.blocks, z.most_queries, reinterpret_cast<int32_t*>(base), reinterpret_cast<float*>(base + z.sums_at),
                       reinterpret_cast<float*>(base + z.parts_at)};
