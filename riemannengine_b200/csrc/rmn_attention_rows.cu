@@ -676,18 +676,22 @@ int launch_rows(const CUtensorMap& k, const CUtensorMap& v, const AttnArgs& a, c
 }  // namespace
 
 namespace {
-// Whether this form takes less time than whole tiles of 128 queries a head (bf16), both estimated in us from averages over the
-// samples: here sixteen rows of a sample and key head pass over its keys at a time, 64 keys a step, all SMs taking their share; there
-// every query head passes once, 128 keys a step, and the longest sample's chain is not cut. Measured (here, there): 16 samples of one
-// row and 509 ... 30011 keys, 16 / 4 heads of 128, 71 and 503 us; 16 samples of 5 rows and 8000 keys (16 x 5 / 8000), 8 heads of 64, 59 and 102; 512 x 4 / 4, 8 / 2 heads of 64, 32 and
-// 85; 512 x 16 / 16, 8 heads of 64, 81 and 88; but 64 x 20 / 1024 94 and 38, 256 x 32 / 32 84 and 46, 4 x 8 / 60 7.5 and 6.1.
-bool rows_take_less(uint32_t rows_q, uint32_t rows_k, uint32_t sequences, int heads, int kv_heads, int dim) {
-  const double n = sequences, rows = std::ceil(rows_q / n) * (heads / kv_heads), keys = rows_k / n;
-  const bool wide = dim > 64;
-  const double places = 148 * 2, pieces = std::max(1.0, n * kv_heads / places);
+// Whether this form takes less time than whole tiles of a head's queries (bf16 128 of them on the tensor cores, fp32 64), both
+// estimated in us from averages over the samples: here sixteen rows of a sample and key head pass over its keys at a time, 64 keys a
+// step, all SMs taking their share; there every query head passes once, and the longest sample's chain is not cut. Measured in bf16
+// (here, there): 16 samples of one row and 509 ... 30011 keys, 16 / 4 heads of 128, 71 and 503 us; 16 samples of 5 rows and 8000 keys
+// (16 x 5 / 8000), 8 heads of 64, 59 and 102; 512 x 4 / 4, 8 / 2 heads of 64, 32 and 85; 512 x 16 / 16, 8 heads of 64, 81 and 88; but
+// 64 x 20 / 1024 94 and 38, 256 x 32 / 32 84 and 46, 4 x 8 / 60 7.5 and 6.1. In fp32, 8 heads of 64: 64 x 20 / 1024 178 and 318,
+// 256 x 1 / 200 123 and 489, but 256 x 32 / 32 183 and 70, 512 x 1 / 4 136 and 106.
+bool rows_take_less(uint32_t rows_q, uint32_t rows_k, uint32_t sequences, int heads, int kv_heads, int dim, int dtype) {
+  const double n = sequences, rows = std::ceil(rows_q / n) * (heads / kv_heads), keys = rows_k / n, pass_rows = std::min(16.0, rows);
+  const bool wide = dim > 64, f32 = dtype == RMN_F32;
+  const double places = f32 ? 148 : 2 * 148, pieces = std::max(1.0, n * kv_heads / places);
   const double tiles = std::max(1.0, n * kv_heads * std::max(1.0, keys / kTileKeys) / places);  // a block
-  const double here = 4 + std::ceil(rows / 16) * (pieces * (1.5 + 0.22 * std::min(16.0, rows)) + tiles * (wide ? 1.8 : 1.2));
-  const double there = std::max(1.0, n * heads / places) * (5.5 + std::max(1.0, keys / 128) * (wide ? 1.9 : 1.1));
+  const double piece = f32 ? (wide ? 6.0 : 4.0) + 0.15 * pass_rows : 1.5 + 0.22 * pass_rows;
+  const double here = 4 + std::ceil(rows / 16) * (pieces * piece + tiles * (wide ? 1.8 : 1.2));
+  const double there = f32 ? std::max(1.0, n * heads / (wide ? 148 : 2 * 148)) * (std::max(1.0, keys / 64) * (wide ? 14 : 10.5) - 2)
+                           : std::max(1.0, n * heads / (2 * 148)) * (5.5 + std::max(1.0, keys / 128) * (wide ? 1.9 : 1.1));
   return here < there;
 }
 }  // namespace
@@ -696,7 +700,7 @@ size_t attention_rows_workspace(uint32_t rows_q, uint32_t rows_k, uint32_t seque
   if (!rows_q || !rows_k || !sequences || dim > 128 || dim % (dtype == RMN_F32 ? 4 : 8)) return 0;
   const uint64_t rows = ((uint64_t)rows_q + sequences - 1) / sequences * (heads / kv_heads);
   if (rows > kMostRows) return 0;
-  if (dtype == RMN_BF16 && !rows_take_less(rows_q, rows_k, sequences, heads, kv_heads, dim)) return 0;
+  if (!rows_take_less(rows_q, rows_k, sequences, heads, kv_heads, dim, dtype)) return 0;
   if ((uint64_t)rows_q * heads > 0x7fffffffull) return 0;
   return rows_sizes(rows_k, sequences, heads, kv_heads, dim, dtype).total;
 }

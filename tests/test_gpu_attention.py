@@ -485,6 +485,16 @@ def test_a_cache_of_more_than_2_31_elements(dtype, d):
     P.check(got, P.attention(q[:2].detach(), k, k, one, offsets, None, True)["out"])
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("h,hk,d", [(4, 4, 32), (4, 2, 128), (3, 3, 80)])
+def test_uneven_new_rows_against_a_thousand_keys(dtype, h, hk, d):
+    nq, nk = [60, 0, 7, 20] + [1] * 12, [3000, 700, 2500, 1000] + [900, 1000, 30] * 4
+    q, k, v, _ = _inputs(sum(nq), sum(nk), h, hk, d, TYPES[dtype], seed=5)
+    for causal in (False, True):
+        want = P.attention(q, k, v, _offsets(nq), _offsets(nk), None, causal)["out"]
+        P.check(_host("cpp")(q, k, v, _offsets(nq), _offsets(nk), None, causal), want)
+
+
 def test_offsets_that_give_rows_to_many_samples():
     """2^17 samples that each claim all rows: more tiles than 32 bits count. The call reports it and touches only its tensors."""
     from riemannengine_b200 import capi
