@@ -1043,6 +1043,30 @@ class RiemannBatchNorm(torch.nn.Module):
 RiemannSyncBatchNorm = RiemannBatchNorm  # the reference's alias (engine/nn/normalization.hpp:36-37)
 
 
+class _Once(torch.autograd.Function):
+    """Hands on the first ``n`` of ``tensors``, gradients, as functions of all of them whose derivative is an error: without it a
+    gradient's gradient would be zero, as kernels leave no graph. (torch's once_differentiable leaves the graph out where the output's
+    gradient needs none, as that of a sum.)"""
+
+    @staticmethod
+    def forward(ctx, what: str, n: int, *tensors):
+        ctx.what = what
+        return tuple(t.detach() for t in tensors[:n])
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError(f"{ctx.what} is differentiable once only")
+
+
+def _once(what: str, grads, of):
+    """``grads`` as they are handed back by the backward pass of ``what``, made from ``of``."""
+    if not torch.is_grad_enabled():
+        return grads
+    made = [g for g in grads if g is not None]
+    out = iter(_Once.apply(what, len(made), *made, *(t for t in of if t is not None)))
+    return tuple(None if g is None else next(out) for g in grads)
+
+
 class _LayerNormFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps: float):
@@ -1053,16 +1077,17 @@ class _LayerNormFunction(torch.autograd.Function):
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad_out):
         x, weight, mean, inv = ctx.saved_tensors
         need = ctx.needs_input_grad
-        return (*ops.layer_norm_backward(grad_out, x, weight, mean, inv, need[0], need[1], need[2], ctx.bias_dtype), None)
+        with torch.no_grad():
+            grads = ops.layer_norm_backward(grad_out, x, weight, mean, inv, need[0], need[1], need[2], ctx.bias_dtype)
+        return (*_once("layer norm", grads, (x, weight, grad_out)), None)
 
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
                eps: float = 1e-5) -> torch.Tensor:
-    """Layer norm over the channels of a feature matrix [N, C], differentiable in all three."""
+    """Layer norm over the channels of a feature matrix [N, C], differentiable (once) in all three."""
     return _LayerNormFunction.apply(x, weight, bias, eps)
 
 
@@ -1091,17 +1116,17 @@ class _PackedAttentionFunction(torch.autograd.Function):
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad_out):
         q, k, v, out, low, lse, offsets, kv_offsets, kv_lengths = ctx.saved_tensors
-        return (*ops.attention_backward(grad_out, q, k, v, out, low, lse, offsets, kv_offsets, kv_lengths, ctx.causal, ctx.scale),
-                None, None, None, None, None)
+        with torch.no_grad():
+            grads = ops.attention_backward(grad_out, q, k, v, out, low, lse, offsets, kv_offsets, kv_lengths, ctx.causal, ctx.scale)
+        return (*_once("packed_attention", grads, (q, k, v, grad_out)), None, None, None, None, None)
 
 
 def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: torch.Tensor,
                      kv_offsets: Optional[torch.Tensor] = None, kv_lengths: Optional[torch.Tensor] = None,
                      causal: bool = False, scale: Optional[float] = None) -> torch.Tensor:
-    """softmax(scale q k^T) v within packed samples, differentiable in q, k and v. ``q`` [rows, heads, channels], ``k`` and
+    """softmax(scale q k^T) v within packed samples, differentiable (once) in q, k and v. ``q`` [rows, heads, channels], ``k`` and
     ``v`` [key rows, key heads, channels] (heads a multiple of key heads); ``offsets`` int32 [samples + 1]: first row of
     every sample and the end of the last. ``kv_offsets`` where the keys' rows are others than the queries', ``kv_lengths``
     [samples] where only the first rows of a sample's keys are in use (a cache). ``causal`` is aligned at the end of the keys.

@@ -1826,8 +1826,34 @@ bool fits_int32(const at::Tensor& t) {
     if (n > std::numeric_limits<int32_t>::max()) return false;
   return true;
 }
-void check_once(const at::Tensor& grad, const char* what) {
-  TORCH_CHECK(!(at::GradMode::is_enabled() && grad.requires_grad()), what, " is differentiable once only");
+// Hands on the first `n` of the tensors, gradients, as functions of all of them whose derivative is an error: without it a
+// gradient's gradient would be zero, as kernels leave no graph.
+class Once : public torch::autograd::Function<Once> {
+public:
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, at::TensorList tensors, int64_t n,
+                                                std::string what) {
+    ctx->saved_data["what"] = std::move(what);
+    torch::autograd::variable_list out;
+    for (int64_t i = 0; i < n; ++i) out.push_back(tensors[i].detach());
+    return out;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list) {
+    TORCH_CHECK(false, ctx->saved_data["what"].toStringRef(), " is differentiable once only");
+  }
+};
+// The gradients (undefined where not wanted) as the backward pass of `what` hands them back, made from `of`.
+void once(std::initializer_list<at::Tensor*> grads, std::initializer_list<at::Tensor> of, const char* what) {
+  if (!at::GradMode::is_enabled()) return;
+  std::vector<at::Tensor> tensors;
+  for (auto* g : grads)
+    if (g->defined()) tensors.push_back(*g);
+  const int64_t n = static_cast<int64_t>(tensors.size());
+  for (auto const& t : of)
+    if (t.defined()) tensors.push_back(t);
+  auto out = Once::apply(at::TensorList(tensors), n, std::string(what));
+  size_t at = 0;
+  for (auto* g : grads)
+    if (g->defined()) *g = out[at++];
 }
 
 // rows of x and their distance; a copy where its channels are not adjacent
@@ -1867,7 +1893,6 @@ public:
     auto saved = ctx->get_saved_variables();
     const auto &x = saved[0], &stats = saved[2];
     auto weight = saved[1].contiguous();
-    check_once(grad_outputs[0], "layer norm");
     c10::cuda::CUDAGuard guard(x.device());
     auto [rows, ld_x] = norm_rows(x);
     auto [dy, ld_dy] = norm_rows(grad_outputs[0]);
@@ -1885,6 +1910,7 @@ public:
                                   ptr(weight), bf16 ? RMN_BF16 : RMN_F32, mean, mean ? mean + n : nullptr, ptr(dx), ptr(dw),
                                   ptr(db), dtype_code(x), ptr(ws), ws_bytes, current_stream()),
           "rmn_layer_norm_backward");
+    once({&dx, &dw, &db}, {x, saved[1], grad_outputs[0]}, "layer norm");
     return {dx, dw, db, at::Tensor()};
   }
 };
@@ -1949,7 +1975,6 @@ public:
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                  torch::autograd::variable_list grad_outputs) {
     auto saved = ctx->get_saved_variables();
-    check_once(grad_outputs[0], "packed_attention");
     const AttentionInputs in{saved[0], saved[1], saved[2], saved[3], saved[4], saved[5], ctx->saved_data["causal"].toBool(),
                              ctx->saved_data["scale"].toDouble()};
     c10::cuda::CUDAGuard guard(in.q.device());
@@ -1962,6 +1987,7 @@ public:
     check(rmn_attention_backward(&p, ptr(saved[6]), ptr(saved[7]), static_cast<const float*>(ptr(saved[8])), ptr(grad),
                                  grad.stride(0), grad.stride(1), ptr(dq), ptr(dk), ptr(dv), ptr(ws), ws_bytes, current_stream()),
           "rmn_attention_backward");
+    once({&dq, &dk, &dv}, {in.q, in.k, in.v, grad_outputs[0]}, "packed_attention");
     return {dq, dk, dv, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
   }
 };

@@ -580,3 +580,22 @@ def test_layers_on_sparse_tensors(host):
         attend(mixed)
     with pytest.raises(RuntimeError, match="channel count"):
         attend(H.SparseTensor(x[:, :32], coords))
+
+
+@pytest.mark.parametrize("host", ["python", "cpp"])
+def test_second_derivatives_are_refused_where_the_first_is_of_a_sum(host):
+    """As one of several terms, too, whose derivative would lack it without an error."""
+    q, k, v, _ = _inputs(20, 20, 2, 1, 32, torch.float32)
+    offsets = _offsets([8, 12])
+    for wanted in ((0,), (1,), (2,), (0, 1, 2)):
+        leaves = [t.clone().requires_grad_(i in wanted) for i, t in enumerate((q, k, v))]
+        some = [leaves[i] for i in wanted]
+        loss = _host(host)(*leaves, offsets).sum()
+        grads = torch.autograd.grad(loss, some, create_graph=True)
+        want = P.attention(q, k, v, offsets, grad=torch.ones_like(q))
+        for i, g in zip(wanted, grads):
+            P.check(g, want[("dq", "dk", "dv")[i]])
+        for grad in (lambda: (loss + grads[0].square().sum()).backward(retain_graph=True),
+                     lambda: torch.autograd.grad(loss + grads[0].square().sum(), some, retain_graph=True)):
+            with pytest.raises(RuntimeError, match="packed_attention is differentiable once only"):
+                grad()

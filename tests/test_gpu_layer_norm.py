@@ -260,3 +260,20 @@ def test_refusals(host):
     with pytest.raises(RuntimeError, match="once|differentiate twice"):
         (g,) = torch.autograd.grad(f(a, w, w, 1e-5), a, dy, create_graph=True)
         g.sum().backward()
+
+
+@pytest.mark.parametrize("host", ["python", "cpp"])
+def test_second_derivatives_are_refused_where_the_first_is_of_a_sum(host):
+    x, w, b, _ = _inputs(9, 32, torch.float32)
+    for wanted in ((0,), (1,), (0, 1, 2)):
+        leaves = [t.clone().requires_grad_(i in wanted) for i, t in enumerate((x, w, b))]
+        some = [leaves[i] for i in wanted]
+        loss = _host(host)(*leaves, 1e-5).sum()
+        grads = torch.autograd.grad(loss, some, create_graph=True)
+        want = P.layer_norm(x, w, b, 1e-5, torch.ones_like(x))
+        for i, g in zip(wanted, grads):
+            P.check(g, want[("dx", "dw", "db")[i]])
+        for grad in (lambda: (loss + grads[0].square().sum()).backward(retain_graph=True),
+                     lambda: torch.autograd.grad(loss + grads[0].square().sum(), some, retain_graph=True)):
+            with pytest.raises(RuntimeError, match="layer norm is differentiable once only"):
+                grad()

@@ -99,3 +99,43 @@ def test_hosts_refuse_cpu_tensors_and_bad_layers():
             host.RiemannSelfAttention(32, 4, 3)
         layer = host.RiemannSelfAttention(32, 4, 2)
         assert tuple(dict(layer.named_parameters())["qkv.weight"].shape) == (64, 32)
+
+
+def _layer_norm_on_the_cpu(monkeypatch):
+    """engine.layer_norm with torch's arithmetic in the place of the kernels (which leave no graph either)."""
+    def forward(x, weight=None, bias=None, eps=1e-5, want_stats=False):
+        with torch.no_grad():
+            out, mean, inv = torch.native_layer_norm(x, x.shape[1:], weight, bias, eps)
+        return (out, mean, inv) if want_stats else (out, None, None)
+
+    def backward(grad_out, x, weight, mean, inv, want_input=True, want_weight=True, want_bias=True, param_dtype=None):
+        bias = torch.zeros(x.size(1))
+        with torch.no_grad():
+            return torch.ops.aten.native_layer_norm_backward(grad_out.contiguous(), x, x.shape[1:], mean, inv, weight, bias,
+                                                             [want_input, want_weight, want_bias])
+
+    monkeypatch.setattr(engine.ops, "layer_norm_forward", forward)
+    monkeypatch.setattr(engine.ops, "layer_norm_backward", backward)
+
+
+def test_second_derivatives_are_refused_where_the_first_is_of_a_sum(monkeypatch):
+    """The gradient of a sum comes in without a graph; what is made of the layer's own gradient has to be refused all the same, also
+    as one of several terms, whose derivative would lack it otherwise."""
+    _layer_norm_on_the_cpu(monkeypatch)
+    x, w, b = torch.randn(5, 8), torch.randn(8), torch.randn(8)
+    for wanted in ((0,), (1,), (0, 1, 2)):
+        leaves = [t.clone().requires_grad_(i in wanted) for i, t in enumerate((x, w, b))]
+        some = [leaves[i] for i in wanted]
+        loss = engine.layer_norm(*leaves).sum()
+        grads = torch.autograd.grad(loss, some, create_graph=True)
+        for grad in (lambda: (loss + grads[0].square().sum()).backward(retain_graph=True),
+                     lambda: torch.autograd.grad(loss + grads[0].square().sum(), some, retain_graph=True)):
+            with pytest.raises(RuntimeError, match="layer norm is differentiable once only"):
+                grad()
+    # a gradient kept with its graph is a tensor like others
+    x = x.clone().requires_grad_(True)
+    engine.layer_norm(x, w, b).square().sum().backward(create_graph=True)
+    want = torch.autograd.grad(torch.nn.functional.layer_norm(x, (8,), w, b).square().sum(), x)[0]
+    assert torch.allclose(x.grad, want, atol=1e-5)
+    torch.optim.SGD([x], lr=0.1).zero_grad(set_to_none=False)
+    assert not x.grad.any() and not x.grad.requires_grad
