@@ -5,10 +5,10 @@
 // neighbouring blocks take the same tiles of neighbouring key heads (whose rows are neighbours in memory). A block walks through its
 // run of tiles, which is a piece of one sample or of several, with all query rows and heads that go with them, up to 16 of them at
 // a time as the rows of warp-wide matrix products (their rate does not bound here: 16 rows cost one product for 8 keys). Bulk copies bring a tile's keys and values into a ring in shared memory, some 100 KB in
-// flight for a block, across the borders of pieces; each of four warps (in fp32 eight, four a tile) takes 16 of the 64 keys and has a
+// flight for a block, across the borders of pieces; each of four warps takes 16 of the 64 keys and has a
 // running maximum and sum of its own. The warps are joined in shared memory, and the pieces of a sample that several blocks
 // share by a second kernel, in a fixed order. 16 samples of 509 ... 30011 keys, 16 query and 4 key heads of 128 (336 MB in bf16):
-// 62 us, 5.4 TB/s, and 8 us for the second kernel; in fp32 150 us for both, where the three products of every operand take longer
+// 62 us, 5.4 TB/s, and 8 us for the second kernel; in fp32 163 us for both, where the three products of every operand take longer
 // than its bytes.
 //
 // Keys and values go from shared memory to registers as 16-byte loads that are product operands as they stand: which of a row's
@@ -64,7 +64,9 @@ __device__ __forceinline__ uint4 load16(const void* p, bool ok) {
 // The ring: a slot is 64 rows of keys and 64 of values, each as columns of 128-byte swizzled lines.
 template <typename T, int DP>
 struct RowsShape {
-  static constexpr int WARPS = sizeof(T) == 4 ? 8 : 4;              // with keys of their own, four to a tile
+  // with keys of their own, 16 of every tile: a warp waits for all phases of a slot's barrier. (Two fours of warps that took turns at the
+  // tiles of a ring of three slots waited for every second phase of each; the parity of the one before lets such a wait pass early.)
+  static constexpr int WARPS = 4;
   static constexpr int THREADS = WARPS * 32 + 32;                   // and one warp for the copies
   static constexpr int BLOCKS = sizeof(T) == 4 ? 1 : 2;             // an SM
   static constexpr int LINES = DP * (int)sizeof(T) / 128;           // of a row
@@ -219,7 +221,7 @@ __global__ void __launch_bounds__(RowsShape<T, DP>::THREADS, RowsShape<T, DP>::B
     s_timed_out = 0;
     for (int i = 0; i < C::SLOTS; ++i) {
       mbar_init(&full[i], 1);
-      mbar_init(&empty[i], 4);
+      mbar_init(&empty[i], WARPS);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_proxy_async();
@@ -298,7 +300,7 @@ __global__ void __launch_bounds__(RowsShape<T, DP>::THREADS, RowsShape<T, DP>::B
   }
 
   auto sync_warps = [] { asm volatile("bar.sync 1, %0;" ::"n"(WARPS * 32) : "memory"); };  // those that compute
-  const int mine16 = (warp & 3) * 16;                                                      // this warp's keys of a tile
+  const int mine16 = warp * 16;                                                            // this warp's keys of a tile
   auto next_piece = [&] {
     __syncwarp();
     bool more = false;
@@ -358,7 +360,7 @@ __global__ void __launch_bounds__(RowsShape<T, DP>::THREADS, RowsShape<T, DP>::B
         for (int e = 0; e < 4; ++e) o[j][e] = 0.f;
       float m[2] = {-CUDART_INF_F, -CUDART_INF_F}, l[2] = {0.f, 0.f};
 
-      for (int t64 = first_tile + warp / 4; t64 < last_tile; t64 += WARPS / 4) {
+      for (int t64 = first_tile; t64 < last_tile; ++t64) {
         const uint32_t load = it + (uint32_t)(t64 - first_tile), slot = load % C::SLOTS;
         const bool here = mbar_wait(&full[slot], (load / C::SLOTS) & 1u);
         if (!__all_sync(0xffffffffu, here)) {

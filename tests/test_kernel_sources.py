@@ -37,3 +37,45 @@ def test_register_splits_are_executed_by_whole_warpgroups(file, kernel, text):
         branch = text[text.rindex("if (", 0, m.start()):m.start()]
         limit = re.match(r"if \(warp < (\w+)\) \{", branch)
         assert limit and int(constants[limit.group(1)]) % 4 == 0, (file, kernel, branch)
+
+
+def _passes_early(slots, groups, loads=24):
+    """Whether some order of events lets a wait by parity pass before its load has landed: `groups` of warps take the loads of a ring in
+    turn, each load goes into its slot once the one before there has been released, and lands late. Every slot's barrier counts the
+    landings; a wait for its n-th passes when the count is n + 1, or any other number of that parity."""
+    done = [0] * groups  # loads that a group is through with
+
+    def landed_first(late):  # all that may land without `late` does, then every group goes as far as it can
+        landed, released = set(), set()
+        for _ in range(loads * 2):
+            for i in range(loads):
+                if i != late and (i < slots or i - slots in released):
+                    landed.add(i)
+            for g in range(groups):
+                i = g + done[g] * groups
+                if i >= loads:
+                    continue
+                count = sum(1 for j in landed if j % slots == i % slots and j <= i)
+                if (count - (i // slots + 1)) % 2 == 0:  # the wait passes
+                    if i not in landed:
+                        return True
+                    released.add(i)
+                    done[g] += 1
+        return False
+
+    for late in range(loads):
+        done[:] = [0] * groups
+        if landed_first(late):
+            return True
+    return False
+
+
+def test_rings_are_waited_for_phase_by_phase():
+    """Warps that take a ring's slots in turn skip phases of its barriers unless the turns divide the slots; a wait by parity then passes
+    for a load that has not landed. The kernel of few query rows has one group of warps that waits for every load."""
+    assert _passes_early(3, 2) and not any(_passes_early(n, 1) for n in (2, 3, 6)) and not _passes_early(4, 2)
+    with open(os.path.join(CSRC, "rmn_attention_rows.cu")) as f:
+        text = f.read()
+    loops = re.findall(r"for \(int t64 = ([^;]*); t64 < last_tile; ([^)]*)\)", text)
+    assert loops and all(loop == ("first_tile", "++t64") for loop in loops)
+    assert "mbar_init(&empty[i], WARPS)" in text
