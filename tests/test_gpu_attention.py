@@ -599,3 +599,52 @@ def test_second_derivatives_are_refused_where_the_first_is_of_a_sum(host):
                      lambda: torch.autograd.grad(loss + grads[0].square().sum(), some, retain_graph=True)):
             with pytest.raises(RuntimeError, match="packed_attention is differentiable once only"):
                 grad()
+
+
+def _unaligned(x):
+    """The same values one element off 16 bytes: only the multiply-add kernels of whole tiles take them."""
+    y = torch.empty(x.numel() + 1, dtype=x.dtype, device=x.device)[1:].view(x.shape)
+    return y.copy_(x)
+
+
+@pytest.mark.parametrize("sign", ["either", "one"])
+@pytest.mark.parametrize("keys", [500, 30_000])
+@pytest.mark.parametrize("rows,h,hk,d", [(1, 4, 4, 32), (1, 8, 2, 64), (1, 16, 2, 128), (5, 4, 2, 64), (12, 1, 1, 128)])
+def test_few_rows_in_fp32_are_as_exact_as_whole_tiles(rows, h, hk, d, keys, sign):
+    """What a batch's averages decide is the time, not how exact fp32 is: the error (root of the mean square) against 64 bits is not above
+    that of the kernel of whole tiles but for the last rounding of every output, half a step of its size."""
+    nk = [keys, keys // 3 + 1]
+    q, k, v, _ = _inputs(2 * rows, sum(nk), h, hk, d, torch.float32, seed=keys)
+    if sign == "one":
+        q, k, v = q.abs() * 0.2, k.abs(), v.abs()
+    offsets, kv_offsets = _offsets([rows, rows]), _offsets(nk)
+    want = P.attention(q, k, v, offsets, kv_offsets, None, True)["out"][0]
+    rms = lambda t: t.square().mean().sqrt().item()  # noqa: E731
+    for host in ("python", "cpp"):
+        few = rms(_host(host)(q, k, v, offsets, kv_offsets, None, True).double() - want)
+        whole = rms(_host(host)(_unaligned(q), k, v, offsets, kv_offsets, None, True).double() - want)
+        assert few <= whole + P.U32 * rms(want), (few, whole, rms(want))
+
+
+@pytest.mark.parametrize("rows,h,hk,d", [(1, 4, 4, 32), (1, 8, 2, 64), (1, 16, 2, 128), (12, 1, 1, 64)])
+def test_infinite_and_largest_values_with_few_rows_in_fp32(rows, h, hk, d):
+    """Keys that are infinitely or as far off as numbers go have no weight; an infinite value with a weight makes the output infinite,
+    a largest one does not, as in the kernel of whole tiles."""
+    n, lowest = 700, torch.finfo(torch.float32).min
+    q, k, v, _ = _inputs(rows, n, h, hk, d, torch.float32)
+    q[..., 0] = q[..., 0].abs() + 0.1
+    offsets, kv_offsets = _offsets([rows]), _offsets([n])
+    keep = torch.ones(n, dtype=torch.bool, device=DEV)
+    k[100, :, 0], k[300, :, 0], k[650, :, 0] = float("-inf"), lowest, lowest
+    keep[[100, 300, 650]] = False
+    want = P.attention(q, k[keep], v[keep], offsets, _offsets([n - 3]))["out"]
+    f = _host("cpp")
+    for x in (q, _unaligned(q)):
+        P.check(f(x, k, v, offsets, kv_offsets), want)
+    # (a weight of a few thousandths of what is largest: no sum leaves the numbers)
+    v[7, :, 3], v[8, :, 5], v[9, :, 6] = float("inf"), float("-inf"), torch.finfo(torch.float32).max
+    for x in (q, _unaligned(q)):
+        out = f(x, k, v, offsets, kv_offsets)
+        assert (out[..., 3] == float("inf")).all() and (out[..., 5] == float("-inf")).all() and torch.isfinite(out[..., 6]).all()
+        rest = [c for c in range(d) if c not in (3, 5, 6)]
+        P.check(out[..., rest], tuple(t[..., rest] for t in want))
