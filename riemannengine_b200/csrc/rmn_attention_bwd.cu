@@ -139,8 +139,12 @@ __global__ void __launch_bounds__(BwdShape<DP>::THREADS, BwdShape<DP>::BLOCKS)
   const int rows = min(128, g.n_q - first);
   const int steps = exists ? (visible_keys(g, first + rows - 1, a.causal) + STEP - 1) / STEP : 0;
 
-  auto wait = [&](uint64_t* bar, uint32_t parity) {
+  auto lane_wait = [&](uint64_t* bar, uint32_t parity) {
     if (!timed_out && !mbar_wait(bar, parity)) timed_out = true;
+    return !timed_out;
+  };
+  auto wait = [&](uint64_t* bar, uint32_t parity) {  // of a whole warp
+    if (!timed_out && !warp_wait(bar, parity)) timed_out = true;
     return !timed_out;
   };
   if (!exists) {
@@ -158,7 +162,7 @@ __global__ void __launch_bounds__(BwdShape<DP>::THREADS, BwdShape<DP>::BLOCKS)
       uint32_t i = 0;
       for (; i < 2u * (uint32_t)steps; ++i) {
         const uint32_t s = i % SLOTS;
-        if (!wait(&tail->empty[s], ((i / SLOTS) & 1u) ^ 1u)) break;
+        if (!lane_wait(&tail->empty[s], ((i / SLOTS) & 1u) ^ 1u)) break;
         mbar_arrive_expect_tx(&tail->full[s], C::TILE);
         const CUtensorMap* map = (i & 1u) ? &map_v : &map_k;
 #pragma unroll
@@ -333,8 +337,12 @@ __global__ void __launch_bounds__(BwdShape<DP>::THREADS, BwdShape<DP>::BLOCKS)
   const int tiles = exists && first < g.n_k ? max(0, (g.n_q + STEP - 1) / STEP - from) : 0;
   const int steps = tiles * group;
 
-  auto wait = [&](uint64_t* bar, uint32_t parity) {
+  auto lane_wait = [&](uint64_t* bar, uint32_t parity) {
     if (!timed_out && !mbar_wait(bar, parity)) timed_out = true;
+    return !timed_out;
+  };
+  auto wait = [&](uint64_t* bar, uint32_t parity) {  // of a whole warp
+    if (!timed_out && !warp_wait(bar, parity)) timed_out = true;
     return !timed_out;
   };
   if (!exists) {
@@ -365,7 +373,7 @@ __global__ void __launch_bounds__(BwdShape<DP>::THREADS, BwdShape<DP>::BLOCKS)
       if (lane == 0) {
         for (int which = 0; which < 2; ++which, ++i) {
           const uint32_t s = i % SLOTS;
-          if (!wait(&tail->empty[s], ((i / SLOTS) & 1u) ^ 1u)) break;
+          if (!lane_wait(&tail->empty[s], ((i / SLOTS) & 1u) ^ 1u)) break;
           mbar_arrive_expect_tx(&tail->full[s], C::TILE);
 #pragma unroll
           for (int c = 0; c < C::ATOMS; ++c)
@@ -373,7 +381,7 @@ __global__ void __launch_bounds__(BwdShape<DP>::THREADS, BwdShape<DP>::BLOCKS)
         }
       }
       const int b = step % kStats;
-      wait(&tail->st_empty[b], (((uint32_t)step / kStats) & 1u) ^ 1u);
+      lane_wait(&tail->st_empty[b], (((uint32_t)step / kStats) & 1u) ^ 1u);
       if (__any_sync(0xffffffffu, timed_out)) {  // the warp leaves together
         timed_out = true;
         break;

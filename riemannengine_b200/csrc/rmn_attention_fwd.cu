@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(FwdShape<DP, NQ>::THREADS, NQ == 2 ? 1 : 2)
     const int n_tiles = NQ == 1 ? key_tiles[0] : (t == 0 ? key_tiles[0] : key_tiles[NQ - 1]);
     for (int j = 0; j < n_tiles; ++j) {
       const uint32_t ph = (uint32_t)j & 1u;
-      if (!mbar_wait(&s_full[t], ph)) { timed_out = true; break; }
+      if (!warp_wait(&s_full[t], ph)) { timed_out = true; break; }
       tc_fence_after();
       uint32_t r[128];
       tc_ld32_at<0>(s_t, r);
@@ -176,7 +176,7 @@ __global__ void __launch_bounds__(FwdShape<DP, NQ>::THREADS, NQ == 2 ? 1 : 2)
       if (j > 0) {
         // P and O of the tile before are free (kAlias: these scores were made behind that)
         if constexpr (!C::kAlias) {
-          if (!mbar_wait(&o_done[t], ph ^ 1u)) { timed_out = true; break; }
+          if (!warp_wait(&o_done[t], ph ^ 1u)) { timed_out = true; break; }
           tc_fence_after();
         }
         if (__any_sync(0xffffffffu, rise)) {
@@ -199,7 +199,7 @@ __global__ void __launch_bounds__(FwdShape<DP, NQ>::THREADS, NQ == 2 ? 1 : 2)
     }
     // ------------------------------ output ---------------------------------------------
     if (!timed_out && n_tiles > 0) {
-      if (!mbar_wait(&o_done[t], (uint32_t)(n_tiles - 1) & 1u)) timed_out = true;
+      if (!warp_wait(&o_done[t], (uint32_t)(n_tiles - 1) & 1u)) timed_out = true;
       tc_fence_after();
     }
     if (!timed_out) {
@@ -270,7 +270,7 @@ __global__ void __launch_bounds__(FwdShape<DP, NQ>::THREADS, NQ == 2 ? 1 : 2)
       const uint32_t idesc_s = instr_desc(128, 128, false);
       const uint32_t idesc_o = instr_desc(128, 0, true) | ((uint32_t)(steps * 2) << 17);
       auto ready = [&](uint32_t i) {  // load i has arrived
-        if (!mbar_wait(&full[i % SLOTS], (i / SLOTS) & 1u)) timed_out = true;
+        if (!warp_wait(&full[i % SLOTS], (i / SLOTS) & 1u)) timed_out = true;
         return !timed_out;
       };
       auto scores = [&](int t, int j) {
@@ -282,7 +282,7 @@ __global__ void __launch_bounds__(FwdShape<DP, NQ>::THREADS, NQ == 2 ? 1 : 2)
 #pragma unroll
         for (int t = 0; t < NQ; ++t) {
           if (key_tiles[t] == 0 || timed_out) continue;
-          if (!mbar_wait(&q_full[t], 0)) { timed_out = true; break; }
+          if (!warp_wait(&q_full[t], 0)) { timed_out = true; break; }
           scores(t, 0);
         }
         if (!timed_out) tc_commit_elect(&empty[0]);
@@ -298,7 +298,7 @@ __global__ void __launch_bounds__(FwdShape<DP, NQ>::THREADS, NQ == 2 ? 1 : 2)
             v_here = true;
             if (g.n_k - j * 128 < 128) zero_rows(v_s, g.n_k - j * 128, C::ATOMS);
           }
-          if (!mbar_wait(&p_full[t], ph)) { timed_out = true; return; }
+          if (!warp_wait(&p_full[t], ph)) { timed_out = true; return; }
           tc_fence_after();
           mma_columns(tmem + C::O0 + t * DP, tmem + C::P0 + t * C::P_STEP, v_s, idesc_o, j > 0);
           tc_commit_elect(&o_done[t]);
@@ -310,14 +310,14 @@ __global__ void __launch_bounds__(FwdShape<DP, NQ>::THREADS, NQ == 2 ? 1 : 2)
             if (j >= key_tiles[t] || timed_out) continue;
             output(t);
             if (timed_out || j + 1 >= key_tiles[t]) continue;
-            if (!mbar_wait(&o_done[t], ph)) { timed_out = true; break; }  // P has been read
+            if (!warp_wait(&o_done[t], ph)) { timed_out = true; break; }  // P has been read
             scores(t, j + 1);
           }
         } else {
 #pragma unroll
           for (int t = 0; t < NQ; ++t) {
             if (j + 1 >= key_tiles[t] || timed_out) continue;
-            if (!mbar_wait(&s_free[t], ph)) { timed_out = true; break; }
+            if (!warp_wait(&s_free[t], ph)) { timed_out = true; break; }
             scores(t, j + 1);
           }
 #pragma unroll

@@ -71,6 +71,19 @@ __device__ __forceinline__ void tc_ld32_at(uint32_t taddr, uint32_t (&r)[N]) {
       : "memory");
 }
 
+// A wait of a whole warp, left by all lanes together: what follows is executed by whole warps (tcgen05, elect), also when it ran out.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
+  const uint32_t addr = smem_u32(bar);
+  if (__all_sync(0xffffffffu, mbar_try_wait(addr, parity))) return true;
+  const unsigned long long t0 = global_ns();
+  for (;;) {
+#pragma unroll 1
+    for (int i = 0; i < 256; ++i)
+      if (__all_sync(0xffffffffu, mbar_try_wait(addr, parity))) return true;
+    if (__any_sync(0xffffffffu, global_ns() - t0 > 2000000000ull)) return false;
+  }
+}
+
 // The address field of a shared-memory descriptor. In a block of a cluster other than its first, addresses have bits above the
 // block's own window, which would run into the next field.
 __device__ __forceinline__ uint64_t desc_address(uint32_t addr) { return (addr >> 4) & 0x3FFFu; }

@@ -39,6 +39,34 @@ def test_register_splits_are_executed_by_whole_warpgroups(file, kernel, text):
         assert limit and int(constants[limit.group(1)]) % 4 == 0, (file, kernel, branch)
 
 
+def _blocks_around(text, at):
+    """What stands in front of every brace that is open at a place of a text, the innermost last."""
+    heads, last = [], 0
+    for m in re.finditer(r"[{};]", text[:at]):
+        if m.group() == "{":
+            heads.append(text[last:m.start()])
+        elif m.group() == "}" and heads:
+            heads.pop()
+        last = m.end()
+    return heads
+
+
+@pytest.mark.parametrize("file", ["rmn_attention_fwd.cu", "rmn_attention_bwd.cu", "rmn_attention_rows.cu"])
+def test_warps_leave_the_waits_of_attention_together(file):
+    """A wait that runs out ends lane by lane. Behind it stand instructions of whole warps (tcgen05, elect, barriers), so either one lane
+    alone waits, or the lanes vote: in warp_wait, or right behind the wait."""
+    with open(os.path.join(CSRC, file)) as f:
+        text = re.sub(r"//[^\n]*", "", f.read())
+    calls = list(re.finditer(r"\b(mbar_wait|lane_wait)\(", text))
+    assert calls
+    for m in calls:
+        around = _blocks_around(text, m.start())
+        one_lane = any(re.search(r"if \(lane == 0\b", head) for head in around)
+        own = any("auto lane_wait = " in head for head in around)
+        voted = re.search(r"__(all|any)_sync\(0xffffffffu, (here|timed_out)\)", text[m.start():m.start() + 200])
+        assert one_lane or own or voted, text[m.start():m.start() + 80]
+
+
 def _passes_early(slots, groups, loads=24):
     """Whether some order of events lets a wait by parity pass before its load has landed: `groups` of warps take the loads of a ring in
     turn, each load goes into its slot once the one before there has been released, and lands late. Every slot's barrier counts the
