@@ -667,7 +667,8 @@ int rmn_sample_offsets(const int32_t *d_coords, uint32_t n_rows, int W, uint32_t
  * given, only its first kv_lengths[s] key rows are in use (a cache with room behind what it holds) and the others are never
  * read as keys. causal: aligned at the end, query i of n sees keys 0 ... i + m - n of m. scale multiplies the scores.
  * Offsets or lengths that do not ascend or leave the tensors are clamped to them and reported as RMN_ERR_BAD_ARG by
- * rmn_device_status; outputs are of no use then, and need not be written. dim <= 256 (RMN_ERR_UNSUPPORTED beyond).
+ * rmn_device_status; the outputs are of no use then (with few query rows a sample they are zeros, elsewhere rows of no sample may
+ * stay as they were). dim <= 256 (RMN_ERR_UNSUPPORTED beyond).
  */
 typedef struct {
   const void *q, *k, *v;

@@ -407,7 +407,14 @@ __global__ void __launch_bounds__(RowsShape<T, DP>::THREADS, RowsShape<T, DP>::B
   bool in_order;
   find_begin<C::THREADS>(a, w, block, &found, warp_sums, &in_order);
   if (kv == 0 && threadIdx.x == 0) w.starts[3 * block + 2] = found.all;
-  if (!in_order) return;  // (rows of several samples: no bound on the work)
+  if (!in_order) {  // rows of several samples: no bound on the work. The call is reported; its outputs are those of rows without keys
+    const uint64_t rows = (uint64_t)a.rows_q * a.heads, first = (uint64_t)blockIdx.x * C::THREADS + threadIdx.x;
+    const uint64_t all = (uint64_t)gridDim.x * C::THREADS;
+    for (uint64_t i = first; i < rows * a.dim; i += all) store_row<T>(a, i, 0, 0.f);
+    if (a.lse)
+      for (uint64_t i = first; i < rows; i += all) a.lse[i] = -CUDART_INF_F;
+    return;
+  }
   // rows of segments without keys become zeros, while the first copies are on their way: a warp looks at 32 segments at a time
   const uint32_t looked_at = warp < WARPS ? a.sequences + 2 : 0;
   for (uint32_t s0 = (uint32_t)(block * WARPS + warp) * 32; s0 < looked_at; s0 += (uint32_t)w.blocks * WARPS * 32) {

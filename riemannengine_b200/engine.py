@@ -1130,7 +1130,9 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     ``v`` [key rows, key heads, channels] (heads a multiple of key heads); ``offsets`` int32 [samples + 1]: first row of
     every sample and the end of the last. ``kv_offsets`` where the keys' rows are others than the queries', ``kv_lengths``
     [samples] where only the first rows of a sample's keys are in use (a cache). ``causal`` is aligned at the end of the keys.
-    ``scale``: channels ** -0.5 unless given. Rows of no sample, and rows that see no key, are zero."""
+    ``scale``: channels ** -0.5 unless given. Rows of no sample, and rows that see no key, are zero. Offsets and lengths are looked
+    at on the device: where they descend or leave the tensors nothing outside is touched, the outputs are of no use, and
+    rmn_device_status (or the next map that is built, which reads the same word) reports a bad argument."""
     return _PackedAttentionFunction.apply(q, k, v, offsets, kv_offsets, kv_lengths, bool(causal), scale)
 
 

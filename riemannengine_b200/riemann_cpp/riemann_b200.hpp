@@ -462,7 +462,9 @@ TORCH_MODULE(RiemannLayerNorm);
 // [key rows, key heads, channels] with any row and head strides, heads a multiple of key heads; offsets int32 [samples + 1]: first
 // row of every sample and the end of the last. kv_offsets where the keys' rows are others than the queries', kv_lengths [samples]
 // where only the first rows of a sample's keys are in use (a cache). causal is aligned at the end of the keys. scale: channels ^ -1/2
-// unless given. Rows of no sample, and rows that see no key, are zero.
+// unless given. Rows of no sample, and rows that see no key, are zero. Offsets and lengths are looked at on the device: where they
+// descend or leave the tensors nothing outside is touched, the outputs are of no use, and rmn_device_status (or the next map
+// that is built, which reads the same word) reports a bad argument.
 at::Tensor packed_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& offsets,
                             const at::Tensor& kv_offsets = {}, const at::Tensor& kv_lengths = {}, bool causal = false,
                             c10::optional<double> scale = c10::nullopt);

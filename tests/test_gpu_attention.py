@@ -648,3 +648,25 @@ def test_infinite_and_largest_values_with_few_rows_in_fp32(rows, h, hk, d):
         assert (out[..., 3] == float("inf")).all() and (out[..., 5] == float("-inf")).all() and torch.isfinite(out[..., 6]).all()
         rest = [c for c in range(d) if c not in (3, 5, 6)]
         P.check(out[..., rest], tuple(t[..., rest] for t in want))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("h,hk,d", [(2, 1, 64), (16, 4, 128), (4, 4, 40)])
+def test_few_rows_with_descending_offsets_are_zero(dtype, h, hk, d):
+    """The call is reported, and what was in the outputs' memory does not come back as a result."""
+    from riemannengine_b200 import capi, ops
+    lib, p = capi.lib(), lambda t: ctypes.c_void_p(t.data_ptr())  # noqa: E731
+    stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    q, k, v, _ = _inputs(3, 900, h, hk, d, TYPES[dtype])
+    offsets = _offsets([1, 1, 1])
+    for bad in ([0, 500, 200, 900], [300, 0, 400, 900], [0, 901, 1, 900]):
+        kv_offsets = torch.tensor(bad, dtype=torch.int32, device=DEV)  # (the problem holds its address only)
+        problem = ops._attention(q, k, v, offsets, kv_offsets, None, True, None)
+        nbytes = lib.rmn_attention_forward_workspace_bytes(ctypes.byref(problem))
+        assert nbytes > 0  # few query rows
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=DEV)
+        out, low, lse = torch.full_like(q, 7), torch.full_like(q, 7), torch.full((h, 3), 7.0, device=DEV)
+        assert lib.rmn_attention_forward(ctypes.byref(problem), p(out), p(low), p(lse), p(ws), nbytes, stream) == capi.OK
+        assert lib.rmn_device_status(stream) == capi.ERR_BAD_ARG, bad
+        assert not out.any() and (lse == float("-inf")).all()
+        assert not low.any() if dtype == "bf16" else (low == 7).all()
