@@ -1069,8 +1069,8 @@ def _once(what: str, grads, of):
 
 class _LayerNormFunction(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, eps: float):
-        train = builtins.any(ctx.needs_input_grad)
+    def forward(ctx, x, weight, bias, eps: float, grad_mode: bool):
+        train = grad_mode and builtins.any(ctx.needs_input_grad)  # (needs_input_grad does not look at the mode)
         out, mean, inv = ops.layer_norm_forward(x, weight, bias, eps, want_stats=train)
         ctx.save_for_backward(x, weight, mean, inv)
         ctx.bias_dtype = bias.dtype if bias is not None else None
@@ -1082,13 +1082,13 @@ class _LayerNormFunction(torch.autograd.Function):
         need = ctx.needs_input_grad
         with torch.no_grad():
             grads = ops.layer_norm_backward(grad_out, x, weight, mean, inv, need[0], need[1], need[2], ctx.bias_dtype)
-        return (*_once("layer norm", grads, (x, weight, grad_out)), None)
+        return (*_once("layer norm", grads, (x, weight, grad_out)), None, None)
 
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
                eps: float = 1e-5) -> torch.Tensor:
     """Layer norm over the channels of a feature matrix [N, C], differentiable (once) in all three."""
-    return _LayerNormFunction.apply(x, weight, bias, eps)
+    return _LayerNormFunction.apply(x, weight, bias, eps, torch.is_grad_enabled())
 
 
 class RiemannLayerNorm(torch.nn.Module):
@@ -1108,8 +1108,8 @@ class RiemannLayerNorm(torch.nn.Module):
 
 class _PackedAttentionFunction(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, offsets, kv_offsets, kv_lengths, causal: bool, scale):
-        train = builtins.any(ctx.needs_input_grad)
+    def forward(ctx, q, k, v, offsets, kv_offsets, kv_lengths, causal: bool, scale, grad_mode: bool):
+        train = grad_mode and builtins.any(ctx.needs_input_grad)
         out, low, lse = ops.attention_forward(q, k, v, offsets, kv_offsets, kv_lengths, causal, scale, want_stats=train)
         ctx.save_for_backward(q, k, v, out, low, lse, offsets, kv_offsets, kv_lengths)
         ctx.causal, ctx.scale = causal, scale
@@ -1120,7 +1120,7 @@ class _PackedAttentionFunction(torch.autograd.Function):
         q, k, v, out, low, lse, offsets, kv_offsets, kv_lengths = ctx.saved_tensors
         with torch.no_grad():
             grads = ops.attention_backward(grad_out, q, k, v, out, low, lse, offsets, kv_offsets, kv_lengths, ctx.causal, ctx.scale)
-        return (*_once("packed_attention", grads, (q, k, v, grad_out)), None, None, None, None, None)
+        return (*_once("packed_attention", grads, (q, k, v, grad_out)), None, None, None, None, None, None)
 
 
 def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: torch.Tensor,
@@ -1133,7 +1133,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     ``scale``: channels ** -0.5 unless given. Rows of no sample, and rows that see no key, are zero. Offsets and lengths are looked
     at on the device: where they descend or leave the tensors nothing outside is touched, the outputs are of no use, and
     rmn_device_status (or the next map that is built, which reads the same word) reports a bad argument."""
-    return _PackedAttentionFunction.apply(q, k, v, offsets, kv_offsets, kv_lengths, bool(causal), scale)
+    return _PackedAttentionFunction.apply(q, k, v, offsets, kv_offsets, kv_lengths, bool(causal), scale, torch.is_grad_enabled())
 
 
 class RiemannSelfAttention(torch.nn.Module):

@@ -139,3 +139,30 @@ def test_second_derivatives_are_refused_where_the_first_is_of_a_sum(monkeypatch)
     assert torch.allclose(x.grad, want, atol=1e-5)
     torch.optim.SGD([x], lr=0.1).zero_grad(set_to_none=False)
     assert not x.grad.any() and not x.grad.requires_grad
+
+
+def test_without_gradients_nothing_is_kept_for_them(monkeypatch):
+    """Parameters and features that require gradients, under no_grad: the kernels are not asked for what a backward pass needs."""
+    asked = []
+
+    def norm(x, weight=None, bias=None, eps=1e-5, want_stats=False):
+        asked.append(want_stats)
+        return x.detach().clone(), (x.new_zeros(x.size(0)) if want_stats else None), (x.new_zeros(x.size(0)) if want_stats else None)
+
+    def attention(q, k, v, offsets, kv_offsets=None, kv_lengths=None, causal=False, scale=None, want_stats=False):
+        asked.append(want_stats)
+        return q.detach().clone(), None, (q.new_zeros(q.size(1), q.size(0)) if want_stats else None)
+
+    monkeypatch.setattr(engine.ops, "layer_norm_forward", norm)
+    monkeypatch.setattr(engine.ops, "attention_forward", attention)
+    x, w = torch.zeros(4, 8, requires_grad=True), torch.ones(8, requires_grad=True)
+    q, o = torch.zeros(4, 2, 8, requires_grad=True), torch.tensor([0, 4], dtype=torch.int32)
+    calls = (lambda: engine.layer_norm(x, w), lambda: engine.layer_norm(x.detach(), w), lambda: engine.packed_attention(q, q, q, o),
+             lambda: engine.packed_attention(q.detach(), q, q.detach(), o))
+    for call in calls:
+        assert call().requires_grad
+    with torch.no_grad():
+        for call in calls:
+            assert not call().requires_grad
+    assert not engine.layer_norm(x.detach(), w.detach()).requires_grad
+    assert asked == [True] * 4 + [False] * 5
