@@ -23,6 +23,8 @@
 
 #include <math_constants.h>
 
+#include <algorithm>
+
 namespace rmn {
 namespace tc {
 namespace {
@@ -604,12 +606,14 @@ int launch_bwd(const AttnArgs& a, cudaStream_t stream) {
   constexpr int STEPS = C::STEP == 128 ? 0 : 1;
   const uint64_t q_blocks = most_tiles(a.rows_q, a.sequences, 128) * a.heads;
   const uint64_t k_blocks = most_tiles(a.rows_k, a.sequences, 128) * a.kv_heads;
-  // With fewer than two blocks for each that fits the GPU: clusters of as many blocks, up to eight (the portable size), as the query
-  // heads of a key head divide into. Backward of 8 samples of 151 ... 5003 rows, 8 / 2 heads of 64, 238 tiles for 296 places:
-  // 560 us without, 340 with; of two samples of 3989 and 4600 rows, 16 / 8 heads of 128, 536 tiles for 148 places: 548 and 604.
+  // With fewer than two tiles of keys for each block that fits the GPU (a sample has a tile at least): clusters of as many blocks, up to
+  // eight (the portable size), as the query heads of a key head divide into. Backward of 8 samples of 151 ... 5003 rows, 8 / 2 heads of
+  // 64, 238 tiles for 296 places: 560 us without, 340 with; of two samples of 3989 and 4600 rows, 16 / 8 heads of 128, 536 tiles for 148
+  // places: 548 and 604; of 4096 samples of 4 rows, 8 / 1 heads of 64: 990 and 2121.
   const int group = a.heads / a.kv_heads;
   int cluster = 1;
-  if ((uint64_t)a.rows_k / 128 * a.kv_heads < 2 * 148 * C::BLOCKS) {
+  const uint64_t samples = std::max<uint64_t>(1, a.sequences), tiles = samples * ((a.rows_k / samples + 127) / 128);
+  if (tiles * a.kv_heads < 2 * 148 * C::BLOCKS) {
     for (int n = 2; n <= 8; ++n)
       if (group % n == 0) cluster = n;
   }

@@ -670,3 +670,48 @@ def test_few_rows_with_descending_offsets_are_zero(dtype, h, hk, d):
         assert lib.rmn_device_status(stream) == capi.ERR_BAD_ARG, bad
         assert not out.any() and (lse == float("-inf")).all()
         assert not low.any() if dtype == "bf16" else (low == 7).all()
+
+
+def _grids(call):
+    """Blocks of every kernel that `call` launches on the current stream, in order: from the nodes of a captured graph."""
+    class Params(ctypes.Structure):  # CUDA_KERNEL_NODE_PARAMS_v2 of the driver's interface
+        _fields_ = ([("func", ctypes.c_void_p)] + [(f"{what}{axis}", ctypes.c_uint) for what in ("grid", "block") for axis in "xyz"]
+                    + [("smem", ctypes.c_uint), ("args", ctypes.c_void_p), ("extra", ctypes.c_void_p), ("kern", ctypes.c_void_p),
+                       ("ctx", ctypes.c_void_p)])
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(graph):
+        call()
+    cu, raw, n = ctypes.CDLL("libcuda.so.1"), ctypes.c_void_p(graph.raw_cuda_graph()), ctypes.c_size_t()
+    assert cu.cuGraphGetNodes(raw, None, ctypes.byref(n)) == 0
+    nodes = (ctypes.c_void_p * n.value)()
+    assert cu.cuGraphGetNodes(raw, nodes, ctypes.byref(n)) == 0
+    grids = []
+    for node in nodes:
+        kind, p = ctypes.c_int(), Params()
+        assert cu.cuGraphNodeGetType(ctypes.c_void_p(node), ctypes.byref(kind)) == 0
+        if kind.value == 0:
+            assert cu.cuGraphKernelNodeGetParams_v2(ctypes.c_void_p(node), ctypes.byref(p)) == 0
+            grids.append(p.gridx * p.gridy * p.gridz)
+    return grids
+
+
+@pytest.mark.parametrize("samples,rows,h,hk,d,clusters", [(4096, 4, 8, 1, 64, False), (700, 60, 8, 2, 128, False), (64, 130, 8, 1, 64, True),
+                                                          (2, 700, 8, 2, 128, True)])
+def test_key_heads_are_shared_by_clusters_where_there_are_few_tiles(samples, rows, h, hk, d, clusters):
+    """Every sample has a tile of its own at least: many short ones fill the GPU without clusters."""
+    from riemannengine_b200 import ops
+    n = samples * rows
+    q, k, v, grad = _inputs(n, n, h, hk, d, torch.bfloat16)
+    offsets = _offsets([rows] * samples)
+    out, low, lse = ops.attention_forward(q, k, v, offsets, want_stats=True)
+    grids = _grids(lambda: ops.attention_backward(grad, q, k, v, out, low, lse, offsets))
+    blocks = (n // 128 + samples + 2) * hk  # one for every tile of keys that there may be, and key head
+    assert len(grids) == 2 and grids[1] == blocks * (h // hk if clusters else 1), (grids, blocks)
+    got = ops.attention_backward(grad, q, k, v, out, low, lse, offsets)
+    few = slice(0, 3 * rows)
+    want = P.attention(q[few], k[few], v[few], offsets[:4] if samples > 2 else offsets, grad=grad[few]) if samples > 2 else \
+        P.attention(q, k, v, offsets, grad=grad)
+    for name, t in zip(("dq", "dk", "dv"), got):
+        P.check(t[few] if samples > 2 else t, want[name], name)
