@@ -661,6 +661,16 @@ def _heads(t: torch.Tensor) -> torch.Tensor:
     return t if t.dim() != 3 or t.size(2) == 1 or t.stride(2) == 1 else t.contiguous()
 
 
+def _gradient_heads(t: torch.Tensor) -> torch.Tensor:
+    """``_heads`` of an output's gradient; in bfloat16 a copy, too, where rows or heads are broadcast (as behind a sum over them) or do not
+    begin on 16 bytes, which the tensor-core kernels cannot read: one pass over it against a backward pass by multiply-adds."""
+    t = _heads(t)
+    if t.dim() != 3 or t.dtype != torch.bfloat16 or t.size(2) % 8 or t.size(2) > 128 or not t.numel():
+        return t
+    whole = t.data_ptr() % 16 == 0 and all(t.size(i) == 1 or (t.stride(i) > 0 and t.stride(i) % 8 == 0) for i in (0, 1))
+    return t if whole else t.clone(memory_format=torch.contiguous_format)
+
+
 def _attention(q, k, v, offsets, kv_offsets, kv_lengths, causal, scale) -> capi.Attention:
     """The checked problem; q, k and v have adjacent channels (``_heads``)."""
     for name, t in (("q", q), ("k", k), ("v", v)):
@@ -727,7 +737,7 @@ def attention_backward(grad_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor,
                        low: Optional[torch.Tensor], lse: torch.Tensor, offsets: torch.Tensor, kv_offsets: Optional[torch.Tensor] = None,
                        kv_lengths: Optional[torch.Tensor] = None, causal: bool = False, scale: Optional[float] = None):
     """(dq, dk, dv) of attention_forward (rmn_attention_backward)."""
-    q, k, v, grad_out = _heads(q), _heads(k), _heads(v), _heads(grad_out)
+    q, k, v, grad_out = _heads(q), _heads(k), _heads(v), _gradient_heads(grad_out)
     p = _attention(q, k, v, offsets, kv_offsets, kv_lengths, causal, scale)
     if grad_out.shape != q.shape or grad_out.dtype != q.dtype or grad_out.device != q.device:
         raise RuntimeError("the output gradient must have q's shape, dtype and device")

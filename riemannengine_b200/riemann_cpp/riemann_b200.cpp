@@ -1918,6 +1918,16 @@ public:
 // q, k or v [rows, heads, channels] with adjacent channels; a copy where they are not
 at::Tensor head_rows(const at::Tensor& t) { return t.size(2) > 1 && t.stride(2) != 1 ? t.contiguous() : t; }
 
+// the same of an output's gradient; in bf16 a copy, too, where rows or heads are broadcast (as behind a sum over them) or do not begin
+// on 16 bytes, which the tensor-core kernels cannot read: one pass over it against a backward pass by multiply-adds
+at::Tensor gradient_rows(const at::Tensor& grad) {
+  auto t = head_rows(grad);
+  if (t.scalar_type() != at::kBFloat16 || t.size(2) % 8 != 0 || t.size(2) > 128 || t.numel() == 0) return t;
+  bool whole = reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  for (int i : {0, 1}) whole = whole && (t.size(i) == 1 || (t.stride(i) > 0 && t.stride(i) % 8 == 0));
+  return whole ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
 struct AttentionInputs {
   at::Tensor q, k, v, offsets, kv_offsets, kv_lengths;  // an absent one of the last two: undefined or empty
   bool causal;
@@ -1978,7 +1988,7 @@ public:
     const AttentionInputs in{saved[0], saved[1], saved[2], saved[3], saved[4], saved[5], ctx->saved_data["causal"].toBool(),
                              ctx->saved_data["scale"].toDouble()};
     c10::cuda::CUDAGuard guard(in.q.device());
-    auto grad = head_rows(grad_outputs[0]);
+    auto grad = gradient_rows(grad_outputs[0]);
     const rmn_attention p = in.problem();
     auto dq = at::empty(in.q.sizes(), in.q.options()), dk = at::empty(in.k.sizes(), in.k.options());
     auto dv = at::empty(in.v.sizes(), in.v.options());

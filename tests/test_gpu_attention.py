@@ -715,3 +715,28 @@ def test_key_heads_are_shared_by_clusters_where_there_are_few_tiles(samples, row
         P.attention(q, k, v, offsets, grad=grad)
     for name, t in zip(("dq", "dk", "dv"), got):
         P.check(t[few] if samples > 2 else t, want[name], name)
+
+
+@pytest.mark.parametrize("host", ["python", "cpp"])
+@pytest.mark.parametrize("d", [32, 128])
+def test_broadcast_and_unaligned_gradients_stay_on_the_tensor_cores(host, d):
+    from riemannengine_b200 import capi
+    h, hk, lens = 4, 2, [150, 3, 200]
+    n = sum(lens)
+    q, k, v, grad = _inputs(n, n, h, hk, d, torch.bfloat16)
+    offsets = _offsets(lens)
+    gradients = {"a mean over rows": grad[:1].expand(n, h, d), "a mean over heads": grad[:, :1].expand(n, h, d), "unaligned": _unaligned(grad),
+                 "rows apart": torch.zeros(n, h * d + 4, dtype=grad.dtype, device=DEV)[:, 4:].unflatten(1, (h, d)).copy_(grad)}
+    for what, g in gradients.items():
+        leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+        out = _host(host)(*leaves, offsets)
+        before = capi.lib().rmn_tensor_core_launch_count()
+        grads = torch.autograd.grad(out, leaves, g)
+        assert capi.lib().rmn_tensor_core_launch_count() == before + 2, what
+        want = P.attention(q, k, v, offsets, grad=g)
+        for name, t in zip(("dq", "dk", "dv"), grads):
+            P.check(t, want[name], f"{name} {what}")
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    before = capi.lib().rmn_tensor_core_launch_count()
+    _host(host)(*leaves, offsets).mean(0).square().sum().backward()
+    assert capi.lib().rmn_tensor_core_launch_count() == before + 3
