@@ -740,3 +740,56 @@ def test_broadcast_and_unaligned_gradients_stay_on_the_tensor_cores(host, d):
     before = capi.lib().rmn_tensor_core_launch_count()
     _host(host)(*leaves, offsets).mean(0).square().sum().backward()
     assert capi.lib().rmn_tensor_core_launch_count() == before + 3
+
+
+def _check_statistics(q, k, v, offsets, kv_offsets=None, kv_lengths=None, causal=False):
+    """lse, and what is stored of the output with what rounding took from it: it differs from the value by the roundings of the weights and
+    of fp32, no more by the output's own."""
+    from riemannengine_b200 import ops
+    out, low, lse = ops.attention_forward(q, k, v, offsets, kv_offsets, kv_lengths, causal, want_stats=True)
+    want = P.attention(q, k, v, offsets, kv_offsets, kv_lengths, causal)
+    assert lse.dtype == torch.float32 and lse.shape == want["lse"][0].shape
+    P.check(lse, want["lse"], "lse")
+    P.check(out, want["out"], "out")
+    if q.dtype == torch.float32:
+        assert low is None
+    else:
+        u = P.half_step(q.dtype)
+        value, bound = want["out"]
+        # (low is rounded, too: u of what is at most u of the output)
+        P.check(out.double() + low.double(), (value, bound - u * value.abs() + 2 * u * u * value.abs()), "out and low")
+    return want["lse"][0]
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("h,hk,d", [(4, 2, 32), (4, 1, 64), (3, 3, 128), (2, 2, 20), (2, 1, 192)])
+def test_statistics_of_packed_samples(dtype, h, hk, d, causal):
+    """Rows before the first sample and behind the last, samples of no rows, more queries than keys: -infinity where nothing is seen."""
+    t, lens = TYPES[dtype], [70, 0, 140, 1, 300]
+    q, k, v, _ = _inputs(sum(lens) + 14, sum(lens) + 14, h, hk, d, t)
+    lse = _check_statistics(q, k, v, _offsets(lens, 9), causal=causal)
+    assert (lse[:, :9] == float("-inf")).all() and (lse[:, -5:] == float("-inf")).all() and torch.isfinite(lse[:, 9:-5]).all()
+    nk = [30, 12, 150, 0, 300]
+    k, v = _inputs(sum(nk), sum(nk), h, hk, d, t)[1:3]
+    lse = _check_statistics(q, k, v, _offsets(lens, 9), _offsets(nk), causal=causal)
+    assert (lse[:, 9 + 210] == float("-inf")).all()  # no key at all
+    assert torch.equal(lse[:, 9:9 + 40] == float("-inf"), torch.full_like(lse[:, 9:9 + 40], float(causal)) > 0)
+
+
+FEW_ROWS = {"single": ([1] * 7, [1, 700, 33, 2500, 64, 0, 129]), "several": ([1, 3, 0, 4, 1, 2, 5], [1, 700, 33, 2500, 64, 0, 129]),
+            "uneven": ([60, 0, 7, 20] + [1] * 12, [3000, 700, 2500, 1000] + [900, 1000, 30] * 4), "one": ([1], [20_000]), "two": ([2], [5000])}
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("which", FEW_ROWS)
+@pytest.mark.parametrize("h,hk,d", [(4, 4, 32), (8, 1, 64), (16, 4, 128), (6, 2, 40)])
+def test_statistics_and_gradients_of_few_rows(which, dtype, h, hk, d):
+    """The form for few query rows leaves what a backward pass needs, also where several blocks have pieces of a sample."""
+    nq, nk = FEW_ROWS[which]
+    slots = [n + 3 for n in nk]
+    q, k, v, grad = _inputs(sum(nq), sum(slots), h, hk, d, TYPES[dtype], seed=len(nq))
+    kv_lengths = torch.tensor(nk, dtype=torch.int32, device=DEV)
+    for causal in (False, True):
+        _check_statistics(q, k, v, _offsets(nq), _offsets(slots), kv_lengths, causal)
+        _check("cpp", q, k, v, grad, _offsets(nq), _offsets(slots), kv_lengths, causal)
