@@ -564,9 +564,12 @@ _INT32_MAX = (1 << 31) - 1  # (the C ABI would take what is left of a larger siz
 
 
 def _rows(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
-    """``t`` [N, C] with adjacent channels and the distance of its rows; a copy where its strides are others."""
+    """``t`` [N, C] with adjacent channels and the distance of its rows; a copy where its strides are others, and where rows too wide to be
+    read one channel at a time do not begin on 16 bytes."""
     if (t.size(1) > 1 and t.stride(1) != 1) or t.stride(0) < 0:
         t = t.contiguous()
+    if t.size(1) > 4096 and (t.data_ptr() % 16 or (t.size(0) > 1 and t.stride(0) * t.element_size() % 16)):
+        t = t.clone(memory_format=torch.contiguous_format)
     return t, int(t.stride(0)) if t.size(0) > 1 else int(t.size(1))
 
 

@@ -1856,9 +1856,12 @@ void once(std::initializer_list<at::Tensor*> grads, std::initializer_list<at::Te
     if (g->defined()) *g = out[at++];
 }
 
-// rows of x and their distance; a copy where its channels are not adjacent
+// rows of x and their distance; a copy where its channels are not adjacent, and where rows too wide to be read one channel at a time do
+// not begin on 16 bytes
 std::pair<at::Tensor, int64_t> norm_rows(const at::Tensor& x) {
   auto y = x.size(1) > 1 && x.stride(1) != 1 ? x.contiguous() : x;
+  if (y.size(1) > 4096 && (reinterpret_cast<uintptr_t>(ptr(y)) % 16 || (y.size(0) > 1 && y.stride(0) * y.element_size() % 16)))
+    y = y.clone(at::MemoryFormat::Contiguous);
   return {y, y.size(0) > 1 ? y.stride(0) : y.size(1)};
 }
 

@@ -277,3 +277,24 @@ def test_second_derivatives_are_refused_where_the_first_is_of_a_sum(host):
                      lambda: torch.autograd.grad(loss + grads[0].square().sum(), some, retain_graph=True)):
             with pytest.raises(RuntimeError, match="layer norm is differentiable once only"):
                 grad()
+
+
+@pytest.mark.parametrize("host", ["python", "cpp"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_wide_rows_at_any_alignment(host, dtype):
+    """Rows beyond what is read one channel at a time: features and gradients that are parts of wider matrices (as behind a concatenation)."""
+    t, c = TYPES[dtype], 5000
+    x, w, b, dy = _inputs(5, c, t)
+    want = P.layer_norm(x, w, b, 1e-5, dy)
+    for first, room in ((1, 1), (8, 11), (0, 1)):
+        whole, grads = (torch.zeros(5, first + c + room, dtype=t, device=DEV) for _ in range(2))
+        view, dview = whole[:, first:first + c], grads[:, first:first + c]
+        view.copy_(x)
+        dview.copy_(dy)
+        leaf, ww, bb = view.detach().requires_grad_(True), w.clone().requires_grad_(True), b.clone().requires_grad_(True)
+        y = _host(host)(leaf, ww, bb, 1e-5)
+        got = (y, *torch.autograd.grad(y, (leaf, ww, bb), dview))
+        for name, value in zip(("y", "dx", "dw", "db"), got):
+            P.check(value, want[name], f"{name} {first} {room}")
+    one = _host(host)(view[2:3], w, b, 1e-5)
+    P.check(one, tuple(v[2:3] for v in want["y"]))
