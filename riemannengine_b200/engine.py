@@ -1087,7 +1087,11 @@ class _LayerNormFunction(torch.autograd.Function):
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
                eps: float = 1e-5) -> torch.Tensor:
-    """Layer norm over the channels of a feature matrix [N, C], differentiable (once) in all three."""
+    """Layer norm over the channels of a feature matrix [N, C], differentiable (once) in all three. C up to 4096, up to 16384 where it is
+    a multiple of 4 (float32), up to 32768 where it is one of 8 (bfloat16; with gradients of weight or bias 25600)."""
+    if torch.is_grad_enabled() and x.dim() == 2 and x.size(1) > 25600 and builtins.any(
+            p is not None and p.requires_grad for p in (weight, bias)):
+        raise RuntimeError("layer norm has gradients of weight and bias up to 25600 channels")
     return _LayerNormFunction.apply(x, weight, bias, eps, torch.is_grad_enabled())
 
 

@@ -2020,6 +2020,7 @@ at::Tensor layer_norm(const at::Tensor& x, const at::Tensor& weight, const at::T
   }
   TORCH_CHECK(!weight.defined() || !bias.defined() || weight.scalar_type() == bias.scalar_type(),
               "layer norm weight and bias must have the same dtype");
+  TORCH_CHECK(x.size(1) <= 25600 || !wants_gradient({weight, bias}), "layer norm has gradients of weight and bias up to 25600 channels");
   if (!wants_gradient({x, weight, bias})) return layer_norm_forward(x, weight, bias, eps, nullptr);
   auto none = at::empty({0}, x.options());
   return LayerNormAutograd::apply(x, weight.defined() ? weight : none, bias.defined() ? bias : none, eps);

@@ -442,7 +442,9 @@ TORCH_MODULE(RiemannBatchNorm);
 using RiemannSyncBatchNormImpl = RiemannBatchNormImpl;  // as in the reference (normalization.hpp:36-37)
 using RiemannSyncBatchNorm = RiemannBatchNorm;
 
-// Layer norm over the channels of a feature matrix [N, C], differentiable (once) in all three; weight and bias may be undefined.
+// Layer norm over the channels of a feature matrix [N, C], differentiable (once) in all three; weight and bias may be undefined. C up to
+// 4096, up to 16384 where it is a multiple of 4 (float32), up to 32768 where it is one of 8 (bfloat16; with gradients of weight or bias
+// 25600).
 at::Tensor layer_norm(const at::Tensor& x, const at::Tensor& weight = {}, const at::Tensor& bias = {}, double eps = 1e-5);
 
 // Layer norm over the channels of every row. `normalization` is the torch layer that holds the parameters, as in

@@ -298,3 +298,19 @@ def test_wide_rows_at_any_alignment(host, dtype):
             P.check(value, want[name], f"{name} {first} {room}")
     one = _host(host)(view[2:3], w, b, 1e-5)
     P.check(one, tuple(v[2:3] for v in want["y"]))
+
+
+@pytest.mark.parametrize("host", ["python", "cpp"])
+def test_the_widest_rows_with_parameter_gradients_are_refused_by_the_forward_pass(host):
+    x, w, b, dy = _inputs(2, 32768, torch.bfloat16)
+    f = _host(host)
+    for leaves in ((x, w.clone().requires_grad_(True), b), (x, None, b.clone().requires_grad_(True))):
+        with pytest.raises(RuntimeError, match="25600"):
+            f(*leaves, 1e-5)
+        with torch.no_grad():
+            f(*leaves, 1e-5)
+    leaf = x.clone().requires_grad_(True)  # without them the widest rows have a backward pass
+    y = f(leaf, w, b, 1e-5)
+    want = P.layer_norm(x, w, b, 1e-5, dy)
+    P.check(y, want["y"])
+    P.check(torch.autograd.grad(y, leaf, dy)[0], want["dx"])
