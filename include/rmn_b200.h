@@ -668,7 +668,8 @@ int rmn_sample_offsets(const int32_t *d_coords, uint32_t n_rows, int W, uint32_t
  * read as keys. causal: aligned at the end, query i of n sees keys 0 ... i + m - n of m. scale multiplies the scores.
  * Offsets or lengths that do not ascend or leave the tensors are clamped to them and reported as RMN_ERR_BAD_ARG by
  * rmn_device_status; the outputs are of no use then (with few query rows a sample they are zeros, elsewhere rows of no sample may
- * stay as they were). dim <= 256 (RMN_ERR_UNSUPPORTED beyond).
+ * stay as they were). dim <= 256 (RMN_ERR_UNSUPPORTED beyond). bf16 runs on the tensor cores where dim is a multiple of 8 up to 128,
+ * scale > 0, pointers are 16-byte aligned and strides are positive multiples of 8; elsewhere, and in fp32, by multiply-adds.
  */
 typedef struct {
   const void *q, *k, *v;

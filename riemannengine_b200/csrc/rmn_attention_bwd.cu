@@ -14,8 +14,10 @@
 // A step is 128 rows of the other side at head sizes above 64, and eight warps do the arithmetic between the products, each thread with
 // 64 columns of one row. Up to 64 a step is 64 rows and four warps: half the tensor memory, so that two blocks share an SM and one's
 // arithmetic runs beside the other's products and waits (8192 rows x 16 heads of 64 1155 us, with 128-row steps and one
-// block 1333). 16 heads of 128: 1650 us, 833 TFLOP/s by the five products of the formula, causal 877 us; the tensor pipe is active
-// 42 and 49 % of the two kernels' time, the rest is the chain from a product over the arithmetic to the next. P and dS of the second kernel take the places of S and dP, which are made anew once they have been used.
+// block 1333; 1264 now, with clocks of a longer run and waits that are votes). 16 heads of 128: 1790 us, 768 TFLOP/s by the five products
+// of the formula, causal 892 us; the tensor pipe is active 43 and 50 % of the two kernels' time, the rest is the chain from a product
+// over the arithmetic to the next. P and dS of the second kernel take the places of S and dP, which are made anew once they have been
+// used.
 // One warp makes the bulk copies (and fetches the queries' statistics), one issues the products.
 // Where the key tiles alone would leave the GPU waiting for the longest sample's first ones, the query heads that share a key head
 // are dealt out to the blocks of a cluster, whose sums of dK and dV are added up through shared memory in the order of the blocks.

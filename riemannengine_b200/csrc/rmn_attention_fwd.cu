@@ -13,7 +13,7 @@
 // Head sizes up to 64: one query tile and two blocks an SM, P has columns of its own, and the next scores are made while the
 // exponentials of these run (8192 rows, 16 heads of 64: 414 us; two tiles and one block 433: their softmax groups fall into step).
 // Above, tensor memory has no room for it: P takes the place of S, and the next scores wait until P has been used (a softmax
-// thread waits about half of the time then, while the other tile's works: 8192 rows, 16 heads of 128: 514 us, 1070 TFLOP/s).
+// thread waits about half of the time then, while the other tile's works: 8192 rows, 16 heads of 128: 522 us, 1053 TFLOP/s).
 #include "rmn_attention_tc.cuh"
 
 #include <math_constants.h>
@@ -395,7 +395,8 @@ int attention_tc_forward(const AttnArgs& a, cudaStream_t stream) {
     return RMN_ERR_UNSUPPORTED;
   if (a.dim <= 64) return launch_fwd<64, 1>(q, k, v, a, stream);
   // two query tiles a block read the keys half as often, one leaves two blocks an SM: 16 heads of 128, one causal sample of 8192
-  // rows 249 us with two and 260 with one; 100 samples of 256 rows, 8 heads, 76 and 66.5; 12 of 2048 the same
+  // rows 249 us with two and 260 with one (262 with two since the waits are votes); 100 samples of 256 rows, 8 heads, 76 and 66.5; 12 of
+  // 2048 the same
   const bool two = a.rows_q / 2048 >= a.sequences;
   return two ? launch_fwd<128, 2>(q, k, v, a, stream) : launch_fwd<128, 1>(q, k, v, a, stream);
 }

@@ -8,15 +8,15 @@
 // of pieces; each of four warps takes 16 of the 64 keys (in fp32 each of eight takes 8) and has a running maximum and sum of its own. The
 // warps are joined in shared memory, and the pieces of a sample that several blocks share by a second kernel, in a fixed order.
 // 16 samples of 509 ... 30011 keys, 16 query and 4 key heads of 128 (336 MB in bf16): 62 us, 5.4 TB/s, and 8 us for the second kernel;
-// in fp32 128 us for both, 5.0 TB/s.
+// in fp32 123 us, 5.5 TB/s, and 8.
 //
 // In bf16 the rows are those of warp-wide matrix products (their rate does not bound here: 16 rows cost one product for 8 keys). Keys
 // and values go from shared memory to registers as 16-byte loads that are product operands as they stand: which of a row's
 // channels is which k of a product is free as long as q has the same order, and which channel is which column of the output is free
 // as long as the store undoes it. A thread's 8 adjacent channels of a key are its operands of two products; of the values
 // it has 8 channels of the four keys whose weights it holds, paired by a byte permutation.
-// In fp32 they are multiplied and added in fp32 (Rows32): of up to 4 rows that takes less time than the bytes, of 16 rows it bounds (the
-// same samples and one key head: 93 us for 160 MB).
+// In fp32 they are multiplied and added in fp32 (Rows32): of up to 4 rows that takes less time than the bytes, of 16 rows it bounds (such
+// samples with one key head: 93 us for 160 MB).
 #include "rmn_attention_tc.cuh"
 
 #include <math_constants.h>
