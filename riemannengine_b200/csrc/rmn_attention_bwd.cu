@@ -614,7 +614,8 @@ int launch_bwd(const AttnArgs& a, cudaStream_t stream) {
   // places: 548 and 604; of 4096 samples of 4 rows, 8 / 1 heads of 64: 990 and 2121.
   const int group = a.heads / a.kv_heads;
   int cluster = 1;
-  const uint64_t samples = std::max<uint64_t>(1, a.sequences), tiles = samples * ((a.rows_k / samples + 127) / 128);
+  const uint64_t samples = std::max<uint64_t>(1, std::min(a.sequences, a.rows_k));  // (that can have a row)
+  const uint64_t tiles = samples * ((a.rows_k / samples + 127) / 128);
   if (tiles * a.kv_heads < 2 * 148 * C::BLOCKS) {
     for (int n = 2; n <= 8; ++n)
       if (group % n == 0) cluster = n;

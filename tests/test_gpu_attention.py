@@ -793,3 +793,19 @@ def test_statistics_and_gradients_of_few_rows(which, dtype, h, hk, d):
     for causal in (False, True):
         _check_statistics(q, k, v, _offsets(nq), _offsets(slots), kv_lengths, causal)
         _check("cpp", q, k, v, grad, _offsets(nq), _offsets(slots), kv_lengths, causal)
+
+
+def test_samples_without_rows_among_thousands_of_one_row():
+    """More samples than rows: the tiles there may be are those of the rows."""
+    from riemannengine_b200 import ops
+    lens, h, d = [i % 2 for i in range(4096)], 8, 64
+    n = sum(lens)
+    q, k, v, grad = _inputs(n, n, h, 1, d, torch.bfloat16)
+    offsets = _offsets(lens)
+    out, low, lse = ops.attention_forward(q, k, v, offsets, want_stats=True)
+    grids = _grids(lambda: ops.attention_backward(grad, q, k, v, out, low, lse, offsets))
+    assert grids[1] == n // 128 + 4096 + 2, grids
+    got = ops.attention_backward(grad, q, k, v, out, low, lse, offsets)
+    want = P.attention(q[:20], k[:20], v[:20], offsets[:41], grad=grad[:20])
+    for name, t in zip(("dq", "dk", "dv"), got):
+        P.check(t[:20], want[name], name)
