@@ -707,6 +707,54 @@ int rmn_attention_backward(const rmn_attention *problem, const void *d_out, cons
                            const void *d_grad_out, int64_t grad_row, int64_t grad_head, void *d_dq, void *d_dk, void *d_dv,
                            void *d_workspace, size_t workspace_bytes, void *stream);
 
+/* ------------------- rotary positions, and norms of queries and keys -------------------
+ * Where a row lies (the integer coordinates of a sparse tensor, the places of a clip's or a text's tokens), turned into its queries and
+ * keys before they are multiplied; alone, or behind a norm of every head. No counterpart in the reference. */
+
+/*
+ * One problem. q is [rows, heads, dim], k [rows, kv_heads, dim] (kv_heads 0: there is no k); channels are adjacent, rows and heads lie
+ * *_row and *_head elements apart (>= 0; 0 broadcasts). dim is even. positions are int32 [rows, axes], rows and axes position_row and
+ * position_axis elements apart, so that the columns behind the first of a coordinate matrix serve as they lie. Pair i of a head belongs to
+ * the axis whose section it is in: sections[0] pairs (a HOST array of `axes` numbers, read during the call) belong to axis 0, the next
+ * sections[1] to axis 1 ...; frequencies (device, float64, one per pair) are the radians that a unit of position turns a pair by.
+ * Pair i is channels i and i + the number of pairs, or, where interleaved, 2 i and 2 i + 1; channels behind the pairs stay as they
+ * are. norm: every head is first divided by the root of the mean of its squares plus eps, and multiplied by q_weight or k_weight
+ * ([dim], weight_dtype; NULL: ones). Without axes or pairs nothing turns, and positions and frequencies are not looked at. dim <= 256
+ * (RMN_ERR_UNSUPPORTED beyond), up to 8 axes.
+ */
+typedef struct {
+  const void *q, *k;
+  int64_t q_row, q_head, k_row, k_head;
+  uint32_t rows;
+  int heads, kv_heads, dim;
+  const int32_t *positions;
+  int64_t position_row, position_axis;
+  const double *frequencies;
+  const int *sections;
+  int axes, interleaved, norm;
+  const void *q_weight, *k_weight;
+  int weight_dtype;
+  float eps;
+  int dtype;
+} rmn_rotary;
+
+/*
+ * q_out [rows, heads, dim] and k_out [rows, kv_heads, dim] without gaps, each value rounded once. Angles are exact to 2^-32 of a turn (and
+ * what 64 bits lose of frequency / 2 pi) at any position; sums in fp32. In place (q_out == q) where rows and heads lie without gaps.
+ */
+int rmn_rotary_forward(const rmn_rotary *problem, void *d_q_out, void *d_k_out, void *stream);
+/* Scratch bytes of rmn_rotary_backward (0 without a norm). */
+size_t rmn_rotary_backward_workspace_bytes(const rmn_rotary *problem);
+/*
+ * Gradients of rmn_rotary_forward: dq [rows, heads, dim] and dk without gaps, and of the weights ([dim], weight_dtype; summed in fp32 and
+ * 64 bits, rounded once; each may be NULL, and has to be without a norm). The output's gradients have rows and heads grad_*_row and
+ * grad_*_head elements apart. Without a norm q and k are not looked at. No atomics: the same bits every time. d_workspace: 16-byte
+ * aligned, needed for the weights' gradients alone; it may be shared by calls on one stream.
+ */
+int rmn_rotary_backward(const rmn_rotary *problem, const void *d_grad_q, int64_t grad_q_row, int64_t grad_q_head, const void *d_grad_k,
+                        int64_t grad_k_row, int64_t grad_k_head, void *d_dq, void *d_dk, void *d_dq_weight, void *d_dk_weight,
+                        void *d_workspace, size_t workspace_bytes, void *stream);
+
 /* ------------------- weight-gradient all-reduce (data-parallel training) -------------------
  * Batches shard by sample: every rank hashes, maps and convolves its own samples, and the one
  * collective of a training step is the sum of the fp32 weight gradients over the ranks (NCCL over

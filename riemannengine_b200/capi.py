@@ -121,6 +121,10 @@ SIGNATURES = {
     "rmn_attention_backward_workspace_bytes": (c_size_t, [c_void_p]),
     "rmn_attention_backward": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p,
                                        c_void_p, c_void_p, c_size_t, c_void_p]),
+    "rmn_rotary_forward": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p]),
+    "rmn_rotary_backward_workspace_bytes": (c_size_t, [c_void_p]),
+    "rmn_rotary_backward": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p,
+                                    c_void_p, c_void_p, c_size_t, c_void_p]),
     "rmn_comm_unique_id": (c_int, [c_void_p]),
     "rmn_comm_init": (c_int, [c_void_p, c_int, c_int, c_void_p]),
     "rmn_comm_destroy": (c_int, [c_void_p]),
@@ -152,6 +156,17 @@ class Attention(ctypes.Structure):
                 + [(name, c_int) for name in ("heads", "kv_heads", "dim")]
                 + [(name, c_void_p) for name in ("offsets", "kv_offsets", "kv_lengths")]
                 + [("causal", c_int), ("dtype", c_int), ("scale", ctypes.c_float)])
+
+
+class Rotary(ctypes.Structure):
+    """rmn_rotary of the header."""
+    _fields_ = ([(name, c_void_p) for name in ("q", "k")]
+                + [(name, c_int64) for name in ("q_row", "q_head", "k_row", "k_head")]
+                + [("rows", c_uint32)] + [(name, c_int) for name in ("heads", "kv_heads", "dim")]
+                + [("positions", c_void_p), ("position_row", c_int64), ("position_axis", c_int64), ("frequencies", c_void_p),
+                   ("sections", ctypes.POINTER(c_int))]
+                + [(name, c_int) for name in ("axes", "interleaved", "norm")]
+                + [("q_weight", c_void_p), ("k_weight", c_void_p), ("weight_dtype", c_int), ("eps", ctypes.c_float), ("dtype", c_int)])
 
 
 _lib = None

@@ -1142,6 +1142,83 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     return _PackedAttentionFunction.apply(q, k, v, offsets, kv_offsets, kv_lengths, bool(causal), scale, torch.is_grad_enabled())
 
 
+def rotary_sections(channels: int, axes: int) -> List[int]:
+    """All pairs of a head of ``channels``, dealt out evenly to the axes (the first ones take what is left over)."""
+    if channels < 2 or channels % 2 or not 1 <= axes <= 8:
+        raise RuntimeError("rotary positions take an even number of channels and 1 to 8 axes")
+    pairs = channels // 2
+    return [pairs // axes + (1 if a < pairs % axes else 0) for a in range(axes)]
+
+
+def rotary_frequencies(sections: Sequence[int], base: float = 10000.0, whole: bool = False) -> torch.Tensor:
+    """float64 [pairs], on the CPU: the radians that a unit of position turns every pair by, base ** (-i / n) with i counting the n pairs of
+    each axis, or, ``whole``, those of all axes together."""
+    n = [int(s) for s in sections]
+    total = builtins.sum(n)
+    if builtins.any(s < 0 for s in n) or not base > 0:
+        raise RuntimeError("rotary frequencies take sections that are not negative and a positive base")
+    out, start = [], 0
+    for s in n:
+        out += [base ** -((start + i) / total if whole else i / s) for i in range(s)]
+        start += s
+    return torch.tensor(out, dtype=torch.float64)
+
+
+class _RotaryFunction(torch.autograd.Function):
+    """A rotation, or (``back``) the one the other way, which is its derivative: differentiable any number of times."""
+
+    @staticmethod
+    def forward(ctx, x, positions, frequencies, sections, interleaved: bool, back: bool):
+        ctx.save_for_backward(positions, frequencies)
+        ctx.sections, ctx.interleaved, ctx.back = sections, interleaved, back
+        if back:
+            return ops.rotary_backward(x, None, x, None, positions, frequencies, sections, interleaved)[0]
+        return ops.rotary_forward(x, None, positions, frequencies, sections, interleaved)[0]
+
+    @staticmethod
+    def backward(ctx, grad_out):
+        dx = _RotaryFunction.apply(grad_out, *ctx.saved_tensors, ctx.sections, ctx.interleaved, not ctx.back)
+        return dx, None, None, None, None, None
+
+
+def rotary_positions(x: torch.Tensor, positions: torch.Tensor, frequencies: torch.Tensor, sections: Sequence[int],
+                     interleaved: bool = False) -> torch.Tensor:
+    """``x`` [rows, heads, channels] with pairs of channels turned by where their row lies, differentiable in ``x``. ``positions`` int32
+    [rows, axes] (or [rows]) with any strides, such as ``coordinates[:, 1:]``; ``sections``: how many pairs belong to each axis;
+    ``frequencies`` float64 [pairs]: radians that a unit of position turns a pair by (see rotary_frequencies). Pair i is channels i and i +
+    the number of pairs, or, ``interleaved``, 2 i and 2 i + 1; channels behind the pairs stay as they are. Up to 256 channels and 8 axes;
+    any position is as exact as a near one. float32 and bfloat16, each value rounded once."""
+    return _RotaryFunction.apply(x, positions, frequencies, [int(n) for n in sections], bool(interleaved), False)
+
+
+class _QKNormRotaryFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, q_weight, k_weight, positions, frequencies, sections, eps: float, interleaved: bool):
+        out = ops.rotary_forward(q, k, positions, frequencies, sections, interleaved, True, q_weight, k_weight, eps)
+        ctx.save_for_backward(q, k, q_weight, k_weight, positions, frequencies)
+        ctx.sections, ctx.eps, ctx.interleaved = sections, eps, interleaved
+        return out
+
+    @staticmethod
+    def backward(ctx, grad_q, grad_k):
+        q, k, q_weight, k_weight, positions, frequencies = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        with torch.no_grad():
+            grads = ops.rotary_backward(grad_q, grad_k, q, k, positions, frequencies, ctx.sections, ctx.interleaved, True, q_weight,
+                                        k_weight, ctx.eps, (need[2], need[3]))
+        return (*_once("qk_norm_rotary", grads, (q, k, q_weight, k_weight, grad_q, grad_k)), None, None, None, None, None)
+
+
+def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None,
+                   positions: Optional[torch.Tensor] = None, frequencies: Optional[torch.Tensor] = None, sections: Sequence[int] = (),
+                   eps: float = 1e-6, interleaved: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Queries [rows, heads, channels] and keys [rows, key heads, channels], every head divided by the root of the mean of its squares plus
+    ``eps``, times ``q_weight`` or ``k_weight`` [channels] (None: ones), then turned as by rotary_positions (without positions: not at
+    all), in one pass. Differentiable (once) in q, k and the weights. Sums in fp32, each value rounded once."""
+    return _QKNormRotaryFunction.apply(q, k, q_weight, k_weight, positions, frequencies, [int(n) for n in sections], float(eps),
+                                       bool(interleaved))
+
+
 class RiemannSelfAttention(torch.nn.Module):
     """Self-attention of the rows of a SparseTensor within their sample: ``qkv`` projects the features to queries, keys and
     values, packed_attention runs on the row ranges of CoordinateManager.sample_offsets, ``projection`` mixes the heads. The

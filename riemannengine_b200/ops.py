@@ -755,3 +755,106 @@ def attention_backward(grad_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor,
                                               int(grad_out.stride(0)), int(grad_out.stride(1)), _ptr(dq), _ptr(dk), _ptr(dv),
                                               _ptr(ws), wbytes, _stream()), "rmn_attention_backward")
     return dq, dk, dv
+
+
+def _rotary(q, k, q_weight, k_weight, positions, frequencies, sections, eps, interleaved, norm) -> capi.Rotary:
+    """The checked problem; q and k (which may be None) have adjacent channels (``_heads``)."""
+    for name, t in (("q", q), ("k", k)):
+        if t is None:
+            continue
+        _require_cuda(t, name)
+        if t.dim() != 3 or t.size(1) < 1 or t.size(2) < 2 or t.size(2) % 2:
+            raise RuntimeError(f"{name} must be [rows, heads, channels] with an even number of channels")
+        if t.dtype != q.dtype or t.device != q.device:
+            raise RuntimeError("q and k must have the same dtype and device")
+        if t.size(0) != q.size(0) or t.size(2) != q.size(2):
+            raise RuntimeError("q and k must have the same rows and channels")
+        if max(t.shape) > _INT32_MAX:
+            raise RuntimeError(f"{name} must have fewer than 2^31 rows, heads and channels")
+    sections = [int(n) for n in sections]
+    pairs = sum(sections)
+    if any(n < 0 for n in sections) or 2 * pairs > q.size(2) or len(sections) > 8:
+        raise RuntimeError("sections must be the pairs of up to 8 axes, no more than half of the channels together")
+    if positions is not None:
+        _require_cuda(positions, "positions")
+        if positions.dim() == 1:
+            positions = positions[:, None]
+        if positions.dim() != 2 or positions.dtype != torch.int32 or positions.device != q.device or positions.size(0) != q.size(0):
+            raise RuntimeError("positions must be int32 [rows, axes] on q's device")
+        if positions.size(1) != len(sections):
+            raise RuntimeError("sections must have one entry per axis of the positions")
+    if frequencies is not None:
+        _require_cuda(frequencies, "frequencies")
+        if frequencies.dim() != 1 or frequencies.dtype != torch.float64 or not frequencies.is_contiguous() or frequencies.device != q.device:
+            raise RuntimeError("frequencies must be a contiguous 1-D float64 tensor on q's device")
+        if frequencies.numel() != pairs:
+            raise RuntimeError("frequencies must have one entry per pair")
+    if pairs and (positions is None or frequencies is None):
+        raise RuntimeError("pairs need positions and frequencies")
+    code = None
+    for name, t in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if t is None:
+            continue
+        _require_cuda(t, name)
+        if t.dim() != 1 or t.size(0) != q.size(2) or t.device != q.device or not t.is_contiguous():
+            raise RuntimeError(f"{name} must be contiguous, with one entry per channel of a head, on q's device")
+        if code is not None and _dtype_code(t) != code:
+            raise RuntimeError("q_weight and k_weight must have the same dtype")
+        code = _dtype_code(t)
+    if not eps >= 0:
+        raise RuntimeError("eps must not be negative")
+    p = capi.Rotary()
+    p.q, p.q_row, p.q_head = (q.data_ptr() if q.numel() else None), int(q.stride(0)), int(q.stride(1))
+    p.rows, p.heads, p.dim = int(q.size(0)), int(q.size(1)), int(q.size(2))
+    if k is not None:
+        p.k, p.k_row, p.k_head = (k.data_ptr() if k.numel() else None), int(k.stride(0)), int(k.stride(1))
+        p.kv_heads = int(k.size(1))
+    if pairs:
+        p.positions = positions.data_ptr() if positions.numel() else None
+        p.position_row, p.position_axis = int(positions.stride(0)), int(positions.stride(1))
+        p.frequencies = frequencies.data_ptr()
+        p.axes, p.sections = len(sections), (ctypes.c_int * len(sections))(*sections)
+    p.interleaved, p.norm, p.eps, p.dtype = int(bool(interleaved)), int(norm), float(eps), _dtype_code(q)
+    p.q_weight = q_weight.data_ptr() if q_weight is not None else None
+    p.k_weight = k_weight.data_ptr() if k_weight is not None else None
+    p.weight_dtype = capi.F32 if code is None else code
+    return p
+
+
+def rotary_forward(q: torch.Tensor, k: Optional[torch.Tensor], positions: Optional[torch.Tensor], frequencies: Optional[torch.Tensor],
+                   sections: Sequence[int], interleaved: bool = False, norm: bool = False, q_weight: Optional[torch.Tensor] = None,
+                   k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6):
+    """(q, k) turned by their rows' positions, with ``norm`` behind a norm of every head (rmn_rotary_forward)."""
+    q, k = _heads(q), None if k is None else _heads(k)
+    p = _rotary(q, k, q_weight, k_weight, positions, frequencies, sections, eps, interleaved, norm)
+    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    k_out = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    with torch.cuda.device(q.device):
+        capi.check(capi.lib().rmn_rotary_forward(ctypes.byref(p), _ptr(q_out), _ptr(k_out), _stream()), "rmn_rotary_forward")
+    return q_out, k_out
+
+
+def rotary_backward(grad_q: torch.Tensor, grad_k: Optional[torch.Tensor], q: torch.Tensor, k: Optional[torch.Tensor],
+                    positions: Optional[torch.Tensor], frequencies: Optional[torch.Tensor], sections: Sequence[int],
+                    interleaved: bool = False, norm: bool = False, q_weight: Optional[torch.Tensor] = None,
+                    k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6, want_weights: Tuple[bool, bool] = (False, False)):
+    """(dq, dk, dq_weight, dk_weight) of rotary_forward (rmn_rotary_backward), the last two None where not wanted. Without ``norm`` q and k
+    may be any tensors of the gradients' shapes (they are not read)."""
+    q, k = _heads(q), None if k is None else _heads(k)
+    grad_q, grad_k = _heads(grad_q), None if grad_k is None else _heads(grad_k)
+    p = _rotary(q, k, q_weight, k_weight, positions, frequencies, sections, eps, interleaved, norm)
+    for g, t in ((grad_q, q), (grad_k, k)):
+        if (g is None) != (t is None) or (g is not None and (g.shape != t.shape or g.dtype != t.dtype or g.device != t.device)):
+            raise RuntimeError("the output gradients must have the shapes, dtype and device of q and k")
+    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    dk = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    dw = [torch.empty_like(w) if want and w is not None else None for want, w in zip(want_weights, (q_weight, k_weight))]
+    lib = capi.lib()
+    wbytes = lib.rmn_rotary_backward_workspace_bytes(ctypes.byref(p)) if dw[0] is not None or dw[1] is not None else 0
+    ws = torch.empty(wbytes, dtype=torch.uint8, device=q.device) if wbytes else None
+    strides = [int(s) for g in (grad_q, grad_k) for s in ((g.stride(0), g.stride(1)) if g is not None else (0, 0))]
+    with torch.cuda.device(q.device):
+        capi.check(lib.rmn_rotary_backward(ctypes.byref(p), _ptr(grad_q), strides[0], strides[1], _ptr(grad_k), strides[2], strides[3],
+                                           _ptr(dq), _ptr(dk), _ptr(dw[0]), _ptr(dw[1]), _ptr(ws), wbytes, _stream()),
+                   "rmn_rotary_backward")
+    return dq, dk, dw[0], dw[1]

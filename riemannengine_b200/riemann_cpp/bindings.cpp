@@ -323,6 +323,27 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
       py::arg("q"), py::arg("k"), py::arg("v"), py::arg("offsets"), py::arg("kv_offsets") = py::none(),
       py::arg("kv_lengths") = py::none(), py::arg("causal") = false, py::arg("scale") = py::none(),
       py::call_guard<py::gil_scoped_release>());
+  m.def("rotary_sections", &rotary_sections, py::arg("channels"), py::arg("axes"));
+  m.def("rotary_frequencies", &rotary_frequencies, py::arg("sections"), py::arg("base") = 10000.0, py::arg("whole") = false);
+  m.def(
+      "rotary_positions",
+      [](const at::Tensor& x, const c10::optional<at::Tensor>& positions, const c10::optional<at::Tensor>& frequencies,
+         const std::vector<int64_t>& sections, bool interleaved) {
+        return rotary_positions(x, positions.value_or(at::Tensor()), frequencies.value_or(at::Tensor()), sections, interleaved);
+      },
+      py::arg("x"), py::arg("positions"), py::arg("frequencies"), py::arg("sections"), py::arg("interleaved") = false,
+      py::call_guard<py::gil_scoped_release>());
+  m.def(
+      "qk_norm_rotary",
+      [](const at::Tensor& q, const at::Tensor& k, const c10::optional<at::Tensor>& q_weight, const c10::optional<at::Tensor>& k_weight,
+         const c10::optional<at::Tensor>& positions, const c10::optional<at::Tensor>& frequencies, const std::vector<int64_t>& sections,
+         double eps, bool interleaved) {
+        return qk_norm_rotary(q, k, q_weight.value_or(at::Tensor()), k_weight.value_or(at::Tensor()), positions.value_or(at::Tensor()),
+                              frequencies.value_or(at::Tensor()), sections, eps, interleaved);
+      },
+      py::arg("q"), py::arg("k"), py::arg("q_weight") = py::none(), py::arg("k_weight") = py::none(), py::arg("positions") = py::none(),
+      py::arg("frequencies") = py::none(), py::arg("sections") = std::vector<int64_t>(), py::arg("eps") = 1e-6,
+      py::arg("interleaved") = false, py::call_guard<py::gil_scoped_release>());
   {
     using LN = RiemannLayerNormImpl;
     auto cls = bind_layer<LN>(m, "RiemannLayerNorm");

@@ -2072,6 +2072,235 @@ at::Tensor packed_attention(const at::Tensor& q, const at::Tensor& k, const at::
                                         kv_lengths.defined() ? kv_lengths : none, causal, by);
 }
 
+// ---------------------------------------------------------------------------------------------
+// Rotary positions, and norms of queries and keys
+// ---------------------------------------------------------------------------------------------
+namespace {
+struct RotaryInputs {
+  at::Tensor q, k, q_weight, k_weight, positions, frequencies;  // an absent one (all but q): undefined or empty
+  std::vector<int64_t> sections;
+  double eps;
+  bool interleaved, norm;
+  // `sections_of` holds what the problem points to
+  rmn_rotary problem(std::vector<int>& sections_of) const {
+    rmn_rotary p = {};
+    p.q = ptr(q);
+    p.q_row = q.stride(0);
+    p.q_head = q.stride(1);
+    p.rows = static_cast<uint32_t>(q.size(0));
+    p.heads = static_cast<int>(q.size(1));
+    p.dim = static_cast<int>(q.size(2));
+    if (keys()) {
+      p.k = ptr(k);
+      p.k_row = k.stride(0);
+      p.k_head = k.stride(1);
+      p.kv_heads = static_cast<int>(k.size(1));
+    }
+    sections_of.assign(sections.begin(), sections.end());
+    if (frequencies.defined() && frequencies.numel()) {
+      p.positions = static_cast<const int32_t*>(ptr(positions));
+      p.position_row = positions.stride(0);
+      p.position_axis = positions.stride(1);
+      p.frequencies = static_cast<const double*>(ptr(frequencies));
+      p.axes = static_cast<int>(sections_of.size());
+      p.sections = sections_of.data();
+    }
+    p.interleaved = interleaved ? 1 : 0;
+    p.norm = norm ? 1 : 0;
+    p.q_weight = ptr(q_weight);
+    p.k_weight = ptr(k_weight);
+    p.weight_dtype = q_weight.defined() && q_weight.numel() ? dtype_code(q_weight)
+                     : k_weight.defined() && k_weight.numel() ? dtype_code(k_weight)
+                                                              : RMN_F32;
+    p.eps = static_cast<float>(eps);
+    p.dtype = dtype_code(q);
+    return p;
+  }
+  bool keys() const { return k.defined() && k.dim() == 3; }
+};
+
+void check_rotary(RotaryInputs& in) {
+  check_plain(in.q, "q");
+  const auto& q = in.q;
+  for (auto const& [t, name] : {std::pair<const at::Tensor&, const char*>{in.q, "q"}, {in.k, "k"}}) {
+    if (!t.defined()) continue;
+    check_plain(t, name);
+    TORCH_CHECK(t.dim() == 3 && t.size(1) >= 1 && t.size(2) >= 2 && t.size(2) % 2 == 0, name,
+                " must be [rows, heads, channels] with an even number of channels");
+    TORCH_CHECK(t.scalar_type() == q.scalar_type() && t.device() == q.device(), "q and k must have the same dtype and device");
+    TORCH_CHECK(t.size(0) == q.size(0) && t.size(2) == q.size(2), "q and k must have the same rows and channels");
+    TORCH_CHECK(fits_int32(t), name, " must have fewer than 2^31 rows, heads and channels");
+  }
+  dtype_code(q);
+  int64_t pairs = 0;
+  bool fits = in.sections.size() <= 8;
+  for (int64_t n : in.sections) {
+    fits = fits && n >= 0 && n <= q.size(2);
+    pairs += fits ? n : 0;
+  }
+  TORCH_CHECK(fits && 2 * pairs <= q.size(2),
+              "sections must be the pairs of up to 8 axes, no more than half of the channels together");
+  if (in.positions.defined()) {
+    auto& p = in.positions;
+    check_plain(p, "positions");
+    if (p.dim() == 1) p = p.unsqueeze(1);
+    TORCH_CHECK(p.dim() == 2 && p.scalar_type() == at::kInt && p.device() == q.device() && p.size(0) == q.size(0),
+                "positions must be int32 [rows, axes] on q's device");
+    TORCH_CHECK(p.size(1) == static_cast<int64_t>(in.sections.size()), "sections must have one entry per axis of the positions");
+  }
+  if (in.frequencies.defined()) {
+    auto const& f = in.frequencies;
+    check_plain(f, "frequencies");
+    TORCH_CHECK(f.dim() == 1 && f.scalar_type() == at::kDouble && f.is_contiguous() && f.device() == q.device(),
+                "frequencies must be a contiguous 1-D float64 tensor on q's device");
+    TORCH_CHECK(f.numel() == pairs, "frequencies must have one entry per pair");
+  }
+  TORCH_CHECK(!pairs || (in.positions.defined() && in.frequencies.defined()), "pairs need positions and frequencies");
+  for (auto const& [w, name] : {std::pair<const at::Tensor&, const char*>{in.q_weight, "q_weight"}, {in.k_weight, "k_weight"}}) {
+    if (!w.defined()) continue;
+    check_plain(w, name);
+    TORCH_CHECK(w.dim() == 1 && w.size(0) == q.size(2) && w.device() == q.device() && w.is_contiguous(), name,
+                " must be contiguous, with one entry per channel of a head, on q's device");
+    dtype_code(w);
+  }
+  TORCH_CHECK(!in.q_weight.defined() || !in.k_weight.defined() || in.q_weight.scalar_type() == in.k_weight.scalar_type(),
+              "q_weight and k_weight must have the same dtype");
+  TORCH_CHECK(in.eps >= 0, "eps must not be negative");
+  in.q = head_rows(in.q);
+  if (in.k.defined()) in.k = head_rows(in.k);
+}
+
+std::pair<at::Tensor, at::Tensor> rotary_forward(const RotaryInputs& in) {
+  c10::cuda::CUDAGuard guard(in.q.device());
+  std::vector<int> sections;
+  const rmn_rotary p = in.problem(sections);
+  auto q = at::empty(in.q.sizes(), in.q.options());
+  at::Tensor k;
+  if (in.keys()) k = at::empty(in.k.sizes(), in.k.options());
+  check(rmn_rotary_forward(&p, ptr(q), ptr(k), current_stream()), "rmn_rotary_forward");
+  return {q, k};
+}
+
+// in's q and k: what the norm was of (without one: the gradients)
+void rotary_backward(const RotaryInputs& in, const at::Tensor& grad_q, const at::Tensor& grad_k, at::Tensor& dq, at::Tensor& dk,
+                     at::Tensor* dq_weight, at::Tensor* dk_weight) {
+  c10::cuda::CUDAGuard guard(in.q.device());
+  std::vector<int> sections;
+  const rmn_rotary p = in.problem(sections);
+  dq = at::empty(in.q.sizes(), in.q.options());
+  if (in.keys()) dk = at::empty(in.k.sizes(), in.k.options());
+  if (dq_weight) *dq_weight = at::empty(in.q_weight.sizes(), in.q_weight.options());
+  if (dk_weight) *dk_weight = at::empty(in.k_weight.sizes(), in.k_weight.options());
+  const size_t ws_bytes = dq_weight || dk_weight ? rmn_rotary_backward_workspace_bytes(&p) : 0;
+  at::Tensor ws;
+  if (ws_bytes) ws = at::empty({static_cast<int64_t>(ws_bytes)}, in.q.options().dtype(at::kByte));
+  auto gq = head_rows(grad_q);
+  auto gk = in.keys() ? head_rows(grad_k) : at::Tensor();
+  check(rmn_rotary_backward(&p, ptr(gq), gq.stride(0), gq.stride(1), ptr(gk), gk.defined() ? gk.stride(0) : 0,
+                            gk.defined() ? gk.stride(1) : 0, ptr(dq), ptr(dk), dq_weight ? ptr(*dq_weight) : nullptr,
+                            dk_weight ? ptr(*dk_weight) : nullptr, ptr(ws), ws_bytes, current_stream()),
+        "rmn_rotary_backward");
+}
+
+// A rotation, or (back) the one the other way, which is its derivative: differentiable any number of times.
+class RotaryAutograd : public torch::autograd::Function<RotaryAutograd> {
+public:
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, at::Tensor x, at::Tensor positions, at::Tensor frequencies,
+                            std::vector<int64_t> sections, bool interleaved, bool back) {
+    const RotaryInputs in{head_rows(x), {}, {}, {}, positions, frequencies, sections, 0.0, interleaved, false};
+    at::Tensor out, none;
+    if (back) rotary_backward(in, in.q, {}, out, none, nullptr, nullptr);
+    else out = rotary_forward(in).first;
+    ctx->save_for_backward({positions, frequencies});
+    ctx->saved_data["sections"] = sections;
+    ctx->saved_data["interleaved"] = interleaved;
+    ctx->saved_data["back"] = back;
+    return out;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grad_outputs) {
+    auto saved = ctx->get_saved_variables();
+    auto dx = apply(grad_outputs[0], saved[0], saved[1], ctx->saved_data["sections"].toIntVector(),
+                    ctx->saved_data["interleaved"].toBool(), !ctx->saved_data["back"].toBool());
+    return {dx, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+  }
+};
+
+class QKNormRotaryAutograd : public torch::autograd::Function<QKNormRotaryAutograd> {
+public:
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, at::Tensor q, at::Tensor k, at::Tensor q_weight,
+                                                at::Tensor k_weight, at::Tensor positions, at::Tensor frequencies,
+                                                std::vector<int64_t> sections, double eps, bool interleaved) {
+    auto [qo, ko] = rotary_forward({q, k, q_weight, k_weight, positions, frequencies, sections, eps, interleaved, true});
+    ctx->save_for_backward({q, k, q_weight, k_weight, positions, frequencies});
+    ctx->saved_data["sections"] = sections;
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["interleaved"] = interleaved;
+    return {qo, ko};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grad_outputs) {
+    auto saved = ctx->get_saved_variables();
+    const RotaryInputs in{saved[0], saved[1], saved[2], saved[3], saved[4], saved[5], ctx->saved_data["sections"].toIntVector(),
+                          ctx->saved_data["eps"].toDouble(), ctx->saved_data["interleaved"].toBool(), true};
+    at::Tensor dq, dk, dwq, dwk;
+    const bool want_q = ctx->needs_input_grad(2), want_k = ctx->needs_input_grad(3);
+    rotary_backward(in, grad_outputs[0], grad_outputs[1], dq, dk, want_q ? &dwq : nullptr, want_k ? &dwk : nullptr);
+    once({&dq, &dk, &dwq, &dwk}, {saved[0], saved[1], saved[2], saved[3], grad_outputs[0], grad_outputs[1]}, "qk_norm_rotary");
+    return {dq, dk, dwq, dwk, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+  }
+};
+}  // namespace
+
+std::vector<int64_t> rotary_sections(int64_t channels, int64_t axes) {
+  TORCH_CHECK(channels >= 2 && channels % 2 == 0 && axes >= 1 && axes <= 8,
+              "rotary positions take an even number of channels and 1 to 8 axes");
+  std::vector<int64_t> out;
+  for (int64_t a = 0; a < axes; ++a) out.push_back(channels / 2 / axes + (a < channels / 2 % axes ? 1 : 0));
+  return out;
+}
+
+at::Tensor rotary_frequencies(const std::vector<int64_t>& sections, double base, bool whole) {
+  int64_t total = 0, start = 0;
+  for (int64_t n : sections) {
+    TORCH_CHECK(n >= 0, "rotary frequencies take sections that are not negative and a positive base");
+    total += n;
+  }
+  TORCH_CHECK(base > 0, "rotary frequencies take sections that are not negative and a positive base");
+  auto out = at::empty({total}, at::TensorOptions().dtype(at::kDouble));
+  double* f = out.data_ptr<double>();
+  for (int64_t n : sections) {
+    for (int64_t i = 0; i < n; ++i)
+      f[start + i] = std::pow(base, -(whole ? static_cast<double>(start + i) / total : static_cast<double>(i) / n));
+    start += n;
+  }
+  return out;
+}
+
+at::Tensor rotary_positions(const at::Tensor& x, const at::Tensor& positions, const at::Tensor& frequencies,
+                            const std::vector<int64_t>& sections, bool interleaved) {
+  RotaryInputs in{x, {}, {}, {}, positions, frequencies, sections, 0.0, interleaved, false};
+  check_rotary(in);
+  if (!wants_gradient({x})) return rotary_forward(in).first;
+  auto none = at::empty({0}, x.options());
+  return RotaryAutograd::apply(in.q, in.positions.defined() ? in.positions : none, frequencies.defined() ? frequencies : none, sections,
+                               interleaved, false);
+}
+
+std::pair<at::Tensor, at::Tensor> qk_norm_rotary(const at::Tensor& q, const at::Tensor& k, const at::Tensor& q_weight,
+                                                 const at::Tensor& k_weight, const at::Tensor& positions, const at::Tensor& frequencies,
+                                                 const std::vector<int64_t>& sections, double eps, bool interleaved) {
+  TORCH_CHECK(k.defined(), "k must be a tensor");
+  RotaryInputs in{q, k, q_weight, k_weight, positions, frequencies, sections, eps, interleaved, true};
+  check_rotary(in);
+  if (!wants_gradient({q, k, q_weight, k_weight})) return rotary_forward(in);
+  auto none = at::empty({0}, q.options());
+  auto or_none = [&](const at::Tensor& t) { return t.defined() ? t : none; };
+  auto out = QKNormRotaryAutograd::apply(in.q, in.k, or_none(q_weight), or_none(k_weight), or_none(in.positions), or_none(frequencies),
+                                         sections, eps, interleaved);
+  return {out[0], out[1]};
+}
+
 RiemannSelfAttentionImpl::RiemannSelfAttentionImpl(int64_t channels, int64_t num_heads, int64_t num_kv_heads, bool causal,
                                                    bool bias)
     : channels_(channels), heads_(num_heads), kv_heads_(num_kv_heads ? num_kv_heads : num_heads), causal_(causal) {

@@ -473,6 +473,28 @@ at::Tensor packed_attention(const at::Tensor& q, const at::Tensor& k, const at::
                             const at::Tensor& kv_offsets = {}, const at::Tensor& kv_lengths = {}, bool causal = false,
                             c10::optional<double> scale = c10::nullopt);
 
+// All pairs of a head of `channels`, dealt out evenly to the axes (the first ones take what is left over).
+std::vector<int64_t> rotary_sections(int64_t channels, int64_t axes);
+// float64 [pairs], on the CPU: the radians that a unit of position turns every pair by, base ^ (-i / n) with i counting the n pairs of each
+// axis, or, `whole`, those of all axes together.
+at::Tensor rotary_frequencies(const std::vector<int64_t>& sections, double base = 10000.0, bool whole = false);
+
+// x [rows, heads, channels] with pairs of channels turned by where their row lies, differentiable in x. positions int32
+// [rows, axes] (or [rows]) with any strides, such as the coordinates' columns behind the first; sections: how many pairs belong to each
+// axis; frequencies float64 [pairs]: radians that a unit of position turns a pair by. Pair i is channels i and i + the number of pairs,
+// or, interleaved, 2 i and 2 i + 1; channels behind the pairs stay as they are. Up to 256 channels and 8 axes; any position is as exact as
+// a near one. float32 and bfloat16, each value rounded once.
+at::Tensor rotary_positions(const at::Tensor& x, const at::Tensor& positions, const at::Tensor& frequencies,
+                            const std::vector<int64_t>& sections, bool interleaved = false);
+
+// Queries [rows, heads, channels] and keys [rows, key heads, channels], every head divided by the root of the mean of its squares plus
+// eps, times q_weight or k_weight [channels] (undefined: ones), then turned as by rotary_positions (without positions: not at all), in one
+// pass. Differentiable (once) in q, k and the weights. Sums in fp32, each value rounded once.
+std::pair<at::Tensor, at::Tensor> qk_norm_rotary(const at::Tensor& q, const at::Tensor& k, const at::Tensor& q_weight = {},
+                                                 const at::Tensor& k_weight = {}, const at::Tensor& positions = {},
+                                                 const at::Tensor& frequencies = {}, const std::vector<int64_t>& sections = {},
+                                                 double eps = 1e-6, bool interleaved = false);
+
 // Self-attention of the rows of a SparseTensor within their sample: `qkv` projects the features to queries, keys and values,
 // packed_attention runs on CoordinateManager::sample_offsets, `projection` mixes the heads. num_kv_heads 0: as many as heads.
 class RiemannSelfAttentionImpl : public torch::nn::Module {
