@@ -707,6 +707,20 @@ int rmn_attention_backward(const rmn_attention *problem, const void *d_out, cons
                            const void *d_grad_out, int64_t grad_row, int64_t grad_head, void *d_dq, void *d_dk, void *d_dv,
                            void *d_workspace, size_t workspace_bytes, void *stream);
 
+/*
+ * The same with a sliding window and sinks: query i of n stands at place p = i + m - n of its sample's m keys and sees key j where
+ * |p - j| < window or j < sinks; causal: those of them with j <= p. window >= 1, 0 <= sinks < 2^30 (RMN_ERR_BAD_ARG otherwise). Arguments,
+ * types, outputs and workspaces are those of the entry points without a window (the sizes of workspaces are others); key rows that no query
+ * sees have gradients of zero. The work grows with the keys that are seen, not with all.
+ */
+size_t rmn_window_attention_forward_workspace_bytes(const rmn_attention *problem, int32_t window, int32_t sinks);
+int rmn_window_attention_forward(const rmn_attention *problem, int32_t window, int32_t sinks, void *d_out, void *d_low, float *d_lse,
+                                 void *d_workspace, size_t workspace_bytes, void *stream);
+size_t rmn_window_attention_backward_workspace_bytes(const rmn_attention *problem, int32_t window, int32_t sinks);
+int rmn_window_attention_backward(const rmn_attention *problem, int32_t window, int32_t sinks, const void *d_out, const void *d_low,
+                                  const float *d_lse, const void *d_grad_out, int64_t grad_row, int64_t grad_head, void *d_dq,
+                                  void *d_dk, void *d_dv, void *d_workspace, size_t workspace_bytes, void *stream);
+
 /* ------------------- rotary positions, and norms of queries and keys -------------------
  * Where a row lies (the integer coordinates of a sparse tensor, the places of a clip's or a text's tokens), turned into its queries and
  * keys before they are multiplied; alone, or behind a norm of every head. No counterpart in the reference. */

@@ -8,7 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import c_char_p, c_int, c_int64, c_size_t, c_uint32, c_uint64, c_void_p
+from ctypes import c_char_p, c_int, c_int32, c_int64, c_size_t, c_uint32, c_uint64, c_void_p
 
 from . import _build
 
@@ -121,6 +121,11 @@ SIGNATURES = {
     "rmn_attention_backward_workspace_bytes": (c_size_t, [c_void_p]),
     "rmn_attention_backward": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p,
                                        c_void_p, c_void_p, c_size_t, c_void_p]),
+    "rmn_window_attention_forward_workspace_bytes": (c_size_t, [c_void_p, c_int32, c_int32]),
+    "rmn_window_attention_forward": (c_int, [c_void_p, c_int32, c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "rmn_window_attention_backward_workspace_bytes": (c_size_t, [c_void_p, c_int32, c_int32]),
+    "rmn_window_attention_backward": (c_int, [c_void_p, c_int32, c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64,
+                                              c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
     "rmn_rotary_forward": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p]),
     "rmn_rotary_backward_workspace_bytes": (c_size_t, [c_void_p]),
     "rmn_rotary_backward": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p,

@@ -136,23 +136,28 @@ extern "C" int rmn_sample_offsets(const int32_t* d_coords, uint32_t n_rows, int 
   return RMN_OK;
 }
 
-extern "C" size_t rmn_attention_forward_workspace_bytes(const rmn_attention* p) {
-  if (!p || p->heads < 1 || p->kv_heads < 1 || p->heads % p->kv_heads || p->dim < 1) return 0;
+namespace {
+constexpr int32_t kMostSinks = 1 << 30;
+bool window_ok(int32_t window, int32_t sinks) { return window >= 1 && sinks >= 0 && sinks < kMostSinks; }
+
+// window 0: none
+size_t forward_workspace(const rmn_attention* p, int32_t window, int32_t) {
+  if (!p || p->heads < 1 || p->kv_heads < 1 || p->heads % p->kv_heads || p->dim < 1 || window) return 0;
   return attention_rows_workspace(p->rows_q, p->rows_k, p->sequences, p->heads, p->kv_heads, p->dim, p->dtype);
 }
-
-extern "C" int rmn_attention_forward(const rmn_attention* problem, void* d_out, void* d_low, float* d_lse, void* d_workspace,
-                                     size_t workspace_bytes, void* stream_) {
-  cudaStream_t stream = (cudaStream_t)stream_;
+int forward(const rmn_attention* problem, int32_t window, int32_t sinks, void* d_out, void* d_low, float* d_lse, void* d_workspace,
+            size_t workspace_bytes, cudaStream_t stream) {
   AttnArgs a;
   const int st = arguments(problem, &a);
   if (st != RMN_OK) return st;
   if (a.rows_q == 0) return RMN_OK;
-  const size_t need = rmn_attention_forward_workspace_bytes(problem);
+  const size_t need = forward_workspace(problem, window, sinks);
   if (!d_out || (need && (!d_workspace || ((uintptr_t)d_workspace & 15)))) return RMN_ERR_BAD_ARG;
   if (workspace_bytes < need) return RMN_ERR_ALLOC;
   const int found = find_status(&a);
   if (found != RMN_OK) return found;
+  a.window = window;
+  a.sinks = sinks;
   a.out = d_out;
   a.low = problem->dtype == RMN_BF16 ? d_low : nullptr;
   a.lse = d_lse;
@@ -167,14 +172,12 @@ extern "C" int rmn_attention_forward(const rmn_attention* problem, void* d_out, 
   return attention_simt_forward(a, problem->dtype, stream);
 }
 
-extern "C" size_t rmn_attention_backward_workspace_bytes(const rmn_attention* problem) {
+size_t backward_workspace(const rmn_attention* problem, int32_t, int32_t) {
   return problem && problem->heads > 0 ? (size_t)problem->heads * problem->rows_q * sizeof(float) : 0;
 }
-
-extern "C" int rmn_attention_backward(const rmn_attention* problem, const void* d_out, const void* d_low, const float* d_lse,
-                                      const void* d_grad_out, int64_t grad_row, int64_t grad_head, void* d_dq, void* d_dk,
-                                      void* d_dv, void* d_workspace, size_t workspace_bytes, void* stream_) {
-  cudaStream_t stream = (cudaStream_t)stream_;
+int backward(const rmn_attention* problem, int32_t window, int32_t sinks, const void* d_out, const void* d_low, const float* d_lse,
+             const void* d_grad_out, int64_t grad_row, int64_t grad_head, void* d_dq, void* d_dk, void* d_dv, void* d_workspace,
+             size_t workspace_bytes, cudaStream_t stream) {
   AttnArgs a;
   const int st = arguments(problem, &a);
   if (st != RMN_OK) return st;
@@ -190,9 +193,11 @@ extern "C" int rmn_attention_backward(const rmn_attention* problem, const void* 
     return RMN_OK;
   }
   if (!d_out || !d_lse || !d_grad_out || !d_workspace || ((uintptr_t)d_workspace & 15)) return RMN_ERR_BAD_ARG;
-  if (workspace_bytes < rmn_attention_backward_workspace_bytes(problem)) return RMN_ERR_ALLOC;
+  if (workspace_bytes < backward_workspace(problem, window, sinks)) return RMN_ERR_ALLOC;
   const int found = find_status(&a);
   if (found != RMN_OK) return found;
+  a.window = window;
+  a.sinks = sinks;
   a.fwd_out = d_out;
   a.low = problem->dtype == RMN_BF16 ? const_cast<void*>(d_low) : nullptr;
   a.lse = const_cast<float*>(d_lse);
@@ -206,4 +211,44 @@ extern "C" int rmn_attention_backward(const rmn_attention* problem, const void* 
     if (tc != RMN_ERR_UNSUPPORTED) return tc;
   }
   return attention_simt_backward(a, problem->dtype, stream);
+}
+}  // namespace
+
+extern "C" size_t rmn_attention_forward_workspace_bytes(const rmn_attention* problem) { return forward_workspace(problem, 0, 0); }
+
+extern "C" int rmn_attention_forward(const rmn_attention* problem, void* d_out, void* d_low, float* d_lse, void* d_workspace,
+                                     size_t workspace_bytes, void* stream) {
+  return forward(problem, 0, 0, d_out, d_low, d_lse, d_workspace, workspace_bytes, (cudaStream_t)stream);
+}
+
+extern "C" size_t rmn_attention_backward_workspace_bytes(const rmn_attention* problem) { return backward_workspace(problem, 0, 0); }
+
+extern "C" int rmn_attention_backward(const rmn_attention* problem, const void* d_out, const void* d_low, const float* d_lse,
+                                      const void* d_grad_out, int64_t grad_row, int64_t grad_head, void* d_dq, void* d_dk,
+                                      void* d_dv, void* d_workspace, size_t workspace_bytes, void* stream) {
+  return backward(problem, 0, 0, d_out, d_low, d_lse, d_grad_out, grad_row, grad_head, d_dq, d_dk, d_dv, d_workspace, workspace_bytes,
+                  (cudaStream_t)stream);
+}
+
+extern "C" size_t rmn_window_attention_forward_workspace_bytes(const rmn_attention* problem, int32_t window, int32_t sinks) {
+  return window_ok(window, sinks) ? forward_workspace(problem, window, sinks) : 0;
+}
+
+extern "C" int rmn_window_attention_forward(const rmn_attention* problem, int32_t window, int32_t sinks, void* d_out, void* d_low,
+                                            float* d_lse, void* d_workspace, size_t workspace_bytes, void* stream) {
+  if (!window_ok(window, sinks)) return RMN_ERR_BAD_ARG;
+  return forward(problem, window, sinks, d_out, d_low, d_lse, d_workspace, workspace_bytes, (cudaStream_t)stream);
+}
+
+extern "C" size_t rmn_window_attention_backward_workspace_bytes(const rmn_attention* problem, int32_t window, int32_t sinks) {
+  return window_ok(window, sinks) ? backward_workspace(problem, window, sinks) : 0;
+}
+
+extern "C" int rmn_window_attention_backward(const rmn_attention* problem, int32_t window, int32_t sinks, const void* d_out,
+                                             const void* d_low, const float* d_lse, const void* d_grad_out, int64_t grad_row,
+                                             int64_t grad_head, void* d_dq, void* d_dk, void* d_dv, void* d_workspace,
+                                             size_t workspace_bytes, void* stream) {
+  if (!window_ok(window, sinks)) return RMN_ERR_BAD_ARG;
+  return backward(problem, window, sinks, d_out, d_low, d_lse, d_grad_out, grad_row, grad_head, d_dq, d_dk, d_dv, d_workspace,
+                  workspace_bytes, (cudaStream_t)stream);
 }

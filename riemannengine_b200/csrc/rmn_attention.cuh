@@ -16,6 +16,7 @@ struct AttnArgs {
   int heads, kv_heads, dim;
   const int32_t *offsets, *kv_offsets, *kv_lengths;     // kv_offsets never NULL here
   int causal;
+  int32_t window, sinks;                                // window 0: all keys; sinks: first keys of a sample that stay visible
   float scale;                                          // of the scores
   uint32_t* status;                                     // device status word
   void* out;                                            // [rows_q, heads, dim]
@@ -85,6 +86,79 @@ __device__ __forceinline__ int32_t first_query(const Segment& g, int32_t j, int 
 
 __device__ __forceinline__ int32_t tiles_of(int32_t rows, int tile_rows) {
   return (int32_t)(((uint32_t)rows + (uint32_t)tile_rows - 1) / (uint32_t)tile_rows);
+}
+
+// Windows. Query row i of a segment stands at place i + n_k - n_q of its keys. It sees the keys whose distance from there is less than the
+// window (causal: those up to its own place), and the sinks, the first keys of the sample (causal: of those up to its own place).
+__device__ __forceinline__ int32_t clamp_to(int64_t v, int32_t most) { return (int32_t)max((int64_t)0, min(v, (int64_t)most)); }
+struct RowWindow {
+  int32_t low, end, sinks;  // keys of the window, and those of the sinks: 0 ... sinks - 1. Nothing is checked for sense: low may pass end
+};
+__device__ __forceinline__ RowWindow row_window(const AttnArgs& a, const Segment& g, int32_t i) {
+  const int64_t place = (int64_t)i + g.n_k - g.n_q;
+  const int32_t most = a.causal ? clamp_to(place + 1, g.n_k) : g.n_k;
+  return {clamp_to(place - a.window + 1, g.n_k), a.causal ? most : clamp_to(place + a.window, g.n_k), min(a.sinks, most)};
+}
+// The keys that one query row sees: those below `sinks`, and those from `low` to `end` - 1 (all of them together where they meet).
+struct RowKeys {
+  int32_t low, end, sinks;
+};
+template <bool kWindow>
+__device__ __forceinline__ RowKeys row_keys(const AttnArgs& a, const Segment& g, int32_t i) {
+  if constexpr (!kWindow) return {0, visible_keys(g, i, a.causal), 0};
+  const RowWindow w = row_window(a, g, i);
+  if (w.low >= w.end || w.low <= w.sinks) return {0, w.low >= w.end ? w.sinks : max(w.end, w.sinks), 0};
+  return {w.low, w.end, w.sinks};
+}
+// Whether a row sees column c of a tile that begins at key k0.
+template <bool kWindow>
+__device__ __forceinline__ bool sees(const RowKeys& r, int32_t k0, int32_t c) {
+  if constexpr (!kWindow) return c < r.end - k0;
+  return c < r.sinks - k0 || (c >= r.low - k0 && c < r.end - k0);
+}
+// The tiles of kTile keys that some of the query rows first ... last of a segment see: those of the sinks, from key 0 on, and behind them
+// those of the window, from its first key on; one run from key 0 on where the two would share a tile.
+template <bool kWindow, int kTile>
+struct KeyWalk {
+  int32_t tiles, end;                  // of all; behind the last key
+  int32_t sink_tiles, sink_end, from;  // (kWindow)
+  __device__ __forceinline__ KeyWalk(const AttnArgs& a, const Segment& g, int32_t first, int32_t last) {
+    sink_tiles = sink_end = from = 0;
+    if constexpr (!kWindow) {
+      end = visible_keys(g, last, a.causal);
+    } else {
+      const RowWindow lo = row_window(a, g, first), hi = row_window(a, g, last);
+      end = max(hi.end, hi.sinks);
+      if (lo.low >= hi.end) {
+        end = hi.sinks;
+      } else if (lo.low > tiles_of(hi.sinks, kTile) * kTile) {
+        from = lo.low;
+        sink_tiles = tiles_of(hi.sinks, kTile);
+        sink_end = hi.sinks;
+      }
+    }
+    tiles = sink_tiles + tiles_of(end - from, kTile);
+  }
+  // the first key of a tile, and how many of its keys may be seen
+  __device__ __forceinline__ int32_t key(int32_t t) const {
+    if constexpr (!kWindow) return t * kTile;
+    return t < sink_tiles ? t * kTile : from + (t - sink_tiles) * kTile;
+  }
+  __device__ __forceinline__ int32_t keys(int32_t t) const {
+    if constexpr (!kWindow) return min(kTile, end - t * kTile);
+    return min(kTile, (t < sink_tiles ? sink_end : end) - key(t));
+  }
+};
+// The queries that see key j: rows lo ... end - 1.
+struct KeyRows {
+  int32_t lo, end;
+};
+template <bool kWindow>
+__device__ __forceinline__ KeyRows key_rows(const AttnArgs& a, const Segment& g, int32_t j) {
+  if constexpr (!kWindow) return {first_query(g, j, a.causal), g.n_q};
+  const int64_t row = (int64_t)j - g.n_k + g.n_q;  // the query at the key's place
+  if (j < a.sinks) return {a.causal ? clamp_to(row, g.n_q) : 0, g.n_q};
+  return {clamp_to(a.causal ? row : row - a.window + 1, g.n_q), clamp_to(row + a.window, g.n_q)};
 }
 
 // The tile of `tile_rows` rows that a block works on: of query rows, or of key rows (whole slots, in use or not).

@@ -640,7 +640,7 @@ int launch_bwd(const AttnArgs& a, cudaStream_t stream) {
 
 int attention_tc_backward(const AttnArgs& a, cudaStream_t stream) {
   using namespace tc;
-  if (a.dim > 128 || !(a.scale > 0.f)) return RMN_ERR_UNSUPPORTED;
+  if (a.window || a.dim > 128 || !(a.scale > 0.f)) return RMN_ERR_UNSUPPORTED;
   for (const void* p : {a.fwd_out, (const void*)a.low, (const void*)a.dq, (const void*)a.dk, (const void*)a.dv})
     if ((uintptr_t)p & 15) return RMN_ERR_UNSUPPORTED;
   return a.dim <= 64 ? launch_bwd<64>(a, stream) : launch_bwd<128>(a, stream);

@@ -386,7 +386,7 @@ int launch_fwd(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
 
 int attention_tc_forward(const AttnArgs& a, cudaStream_t stream) {
   using namespace tc;
-  if (a.dim > 128 || !(a.scale > 0.f) || a.rows_k == 0 || ((uintptr_t)a.out & 15) || ((uintptr_t)a.low & 15))
+  if (a.window || a.dim > 128 || !(a.scale > 0.f) || a.rows_k == 0 || ((uintptr_t)a.out & 15) || ((uintptr_t)a.low & 15))
     return RMN_ERR_UNSUPPORTED;
   CUtensorMap q, k, v;
   if (!make_head_map(&q, a.q, a.rows_q, a.heads, a.dim, a.q_row, a.q_head) ||

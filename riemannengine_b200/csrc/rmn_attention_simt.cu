@@ -18,6 +18,7 @@
 
 #include <math_constants.h>
 
+#include <algorithm>
 #include <type_traits>
 
 namespace rmn {
@@ -232,7 +233,7 @@ __device__ __forceinline__ void store_tile(T* to, int64_t row, int n, int dim, i
   }
 }
 
-template <typename T, int DP, int BM>
+template <typename T, int DP, int BM, bool kWindow>
 __global__ void __launch_bounds__(kSimtThreads, kBlocksPerSM<DP>) k_attention_simt(const AttnArgs a) {
   using S = SimtShape<DP, BM>;
   constexpr int R = S::R, NC = S::NC, CW = S::CW;
@@ -256,20 +257,20 @@ __global__ void __launch_bounds__(kSimtThreads, kBlocksPerSM<DP>) k_attention_si
   Pair o[R][NC][CW / 2];
   clear(o);
   float m[R], l[R];
-  int seen[R];
+  RowKeys seen[R];
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     m[i] = -CUDART_INF_F;
     l[i] = 0.f;
-    seen[i] = ty + 16 * i < rows ? visible_keys(g, first + ty + 16 * i, a.causal) : 0;
+    seen[i] = ty + 16 * i < rows ? row_keys<kWindow>(a, g, first + ty + 16 * i) : RowKeys{0, 0, 0};
   }
-  const int keys = visible_keys(g, first + rows - 1, a.causal);  // of the last row: the most
+  const KeyWalk<kWindow, BM> walk(a, g, first, first + rows - 1);
   const T* k0 = static_cast<const T*>(a.k) + (int64_t)g.k0 * a.k_row + kv * a.k_head;
   const T* v0 = static_cast<const T*>(a.v) + (int64_t)g.k0 * a.v_row + kv * a.v_head;
   Share<T, DP, BM> share;
-  share.fetch(k0 + (int64_t)rank * BM * a.k_row, a.k_row, min(BM, keys - rank * BM), a.dim);
-  for (int j0 = rank * BM; j0 < keys; j0 += blocks * BM) {
-    const int n = min(BM, keys - j0);
+  share.fetch(k0 + (int64_t)walk.key(rank) * a.k_row, a.k_row, rank < walk.tiles ? walk.keys(rank) : 0, a.dim);
+  for (int t = rank; t < walk.tiles; t += blocks) {
+    const int j0 = walk.key(t), n = walk.keys(t);
     __syncthreads();  // the products with the tile before are done
     share.put(s_kv, 1.f);
     share.fetch(v0 + (int64_t)j0 * a.v_row, a.v_row, n, a.dim);
@@ -281,7 +282,7 @@ __global__ void __launch_bounds__(kSimtThreads, kBlocksPerSM<DP>) k_attention_si
       float top = -CUDART_INF_F;
 #pragma unroll
       for (int j = 0; j < R; ++j) {
-        if (j0 + tx + 16 * j >= seen[i]) s[i][j] = -CUDART_INF_F;
+        if (!sees<kWindow>(seen[i], j0, tx + 16 * j)) s[i][j] = -CUDART_INF_F;
         top = fmaxf(top, s[i][j]);
       }
 #pragma unroll
@@ -307,7 +308,7 @@ __global__ void __launch_bounds__(kSimtThreads, kBlocksPerSM<DP>) k_attention_si
     }
     __syncthreads();  // the keys have been read
     share.put(s_kv, 1.f);
-    share.fetch(k0 + (int64_t)(j0 + blocks * BM) * a.k_row, a.k_row, min(BM, keys - j0 - blocks * BM), a.dim);
+    share.fetch(k0 + (int64_t)walk.key(t + blocks) * a.k_row, a.k_row, t + blocks < walk.tiles ? walk.keys(t + blocks) : 0, a.dim);
     __syncthreads();
     product_columns<DP, BM>(s_p, s_kv, n, tx, ty, o);
   }
@@ -372,7 +373,7 @@ __global__ void __launch_bounds__(kSimtThreads, kBlocksPerSM<DP>) k_attention_si
 }
 
 // dq of a query tile, and delta of its rows for the kernel of the key tiles
-template <typename T, int DP, int BM>
+template <typename T, int DP, int BM, bool kWindow>
 __global__ void __launch_bounds__(kSimtThreads, kBlocksPerSM<DP>) k_attention_simt_dq(const AttnArgs a) {
   using S = SimtShape<DP, BM>;
   constexpr int R = S::R, NC = S::NC, CW = S::CW;
@@ -407,7 +408,7 @@ __global__ void __launch_bounds__(kSimtThreads, kBlocksPerSM<DP>) k_attention_si
   Pair o[R][NC][CW / 2];
   clear(o);
   float delta[R], lse[R];
-  int seen[R];
+  RowKeys seen[R];
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     const int r = ty + 16 * i;
@@ -417,26 +418,27 @@ __global__ void __launch_bounds__(kSimtThreads, kBlocksPerSM<DP>) k_attention_si
 #pragma unroll
     for (int w = 8; w > 0; w >>= 1) d += __shfl_xor_sync(0xffffffffu, d, w, 16);
     delta[i] = d;
-    seen[i] = r < rows ? visible_keys(g, first + r, a.causal) : 0;
+    seen[i] = r < rows ? row_keys<kWindow>(a, g, first + r) : RowKeys{0, 0, 0};
     const size_t at = (size_t)head * a.rows_q + g.q0 + first + r;
     lse[i] = r < rows ? __ldg(a.lse + at) : 0.f;
     if (r < rows && tx == 0 && rank == 0) a.delta[at] = d;
   }
-  const int keys = visible_keys(g, first + rows - 1, a.causal);
+  const KeyWalk<kWindow, BM> walk(a, g, first, first + rows - 1);
   const T* k0 = static_cast<const T*>(a.k) + (int64_t)g.k0 * a.k_row + kv * a.k_head;
   const T* v0 = static_cast<const T*>(a.v) + (int64_t)g.k0 * a.v_row + kv * a.v_head;
   Share<T, DP, BM> next_k, next_v;
-  auto fetch = [&](int j) {
-    next_k.fetch(k0 + (int64_t)j * a.k_row, a.k_row, min(BM, keys - j), a.dim);
-    next_v.fetch(v0 + (int64_t)j * a.v_row, a.v_row, min(BM, keys - j), a.dim);
+  auto fetch = [&](int t) {
+    const int j = walk.key(t), n = t < walk.tiles ? walk.keys(t) : 0;
+    next_k.fetch(k0 + (int64_t)j * a.k_row, a.k_row, n, a.dim);
+    next_v.fetch(v0 + (int64_t)j * a.v_row, a.v_row, n, a.dim);
   };
-  fetch(rank * BM);
-  for (int j0 = rank * BM; j0 < keys; j0 += blocks * BM) {
-    const int n = min(BM, keys - j0);
+  fetch(rank);
+  for (int t = rank; t < walk.tiles; t += blocks) {
+    const int j0 = walk.key(t), n = walk.keys(t);
     __syncthreads();
     next_k.put(s_k, 1.f);
     next_v.put(s_v, 1.f);
-    fetch(j0 + blocks * BM);
+    fetch(t + blocks);
     __syncthreads();
     float s[R][R], dp[R][R];
     product_rows<DP, BM>(s_q, s_k, tx, ty, s);
@@ -445,7 +447,7 @@ __global__ void __launch_bounds__(kSimtThreads, kBlocksPerSM<DP>) k_attention_si
     for (int i = 0; i < R; ++i)
 #pragma unroll
       for (int j = 0; j < R; ++j) {
-        const bool see = j0 + tx + 16 * j < seen[i];
+        const bool see = sees<kWindow>(seen[i], j0, tx + 16 * j);
         s_p[(ty + 16 * i) * S::LP + tx + 16 * j] = see ? expf(s[i][j] - lse[i]) * (dp[i][j] - delta[i]) : 0.f;
       }
     __syncthreads();
@@ -467,7 +469,7 @@ __global__ void __launch_bounds__(kSimtThreads, kBlocksPerSM<DP>) k_attention_si
 }
 
 // dk and dv of a key tile: the queries of all heads that share its head
-template <typename T, int DP, int BM>
+template <typename T, int DP, int BM, bool kWindow>
 __global__ void __launch_bounds__(kSimtThreads, kBlocksPerSM<DP>) k_attention_simt_dkv(const AttnArgs a) {
   using S = SimtShape<DP, BM>;
   constexpr int R = S::R, NC = S::NC, CW = S::CW;
@@ -496,8 +498,10 @@ __global__ void __launch_bounds__(kSimtThreads, kBlocksPerSM<DP>) k_attention_si
   clear(dk);
   clear(dv);
   // tiles of queries that see any of these keys, over all heads: every block of the cluster takes its own
-  const int from = first_query(g, first, a.causal) / BM * BM;
-  const int tiles = used > 0 ? max(0, (g.n_q - from + BM - 1) / BM) : 0;
+  // (the first key's queries begin first; the last one's end last, unless there are sinks, which are seen to the end)
+  const KeyRows lo = key_rows<kWindow>(a, g, first), hi = key_rows<kWindow>(a, g, first + max(used, 1) - 1);
+  const int from = kWindow ? lo.lo : lo.lo / BM * BM;
+  const int tiles = used > 0 ? max(0, (max(lo.end, hi.end) - from + BM - 1) / BM) : 0;
   Share<T, DP, BM> next_q, next_g;
   auto fetch = [&](int turn) {
     const int h = kv * group + turn / max(tiles, 1), i = from + turn % max(tiles, 1) * BM;
@@ -522,10 +526,10 @@ __global__ void __launch_bounds__(kSimtThreads, kBlocksPerSM<DP>) k_attention_si
       const int qi = tx + 16 * j;
       const size_t at = (size_t)h * a.rows_q + g.q0 + i0 + qi;
       const float lse = qi < n ? __ldg(a.lse + at) : 0.f, delta = qi < n ? __ldg(a.delta + at) : 0.f;
-      const int seen = qi < n ? visible_keys(g, i0 + qi, a.causal) : 0;
+      const RowKeys seen = qi < n ? row_keys<kWindow>(a, g, i0 + qi) : RowKeys{0, 0, 0};
 #pragma unroll
       for (int i = 0; i < R; ++i) {
-        const float p = first + ty + 16 * i < seen ? expf(s[i][j] - lse) : 0.f;
+        const float p = sees<kWindow>(seen, first, ty + 16 * i) ? expf(s[i][j] - lse) : 0.f;
         s[i][j] = p;
         dp[i][j] = p == 0.f ? 0.f : p * (dp[i][j] - delta);
         s_p[(ty + 16 * i) * S::LP + qi] = p;
@@ -589,24 +593,39 @@ int launch_simt(Kernel kern, SmemOptIn& opt_in, const AttnArgs& a, uint64_t tile
   return RMN_OK;
 }
 
-template <typename T, int DP, int BM>
-int forward(const AttnArgs& a, cudaStream_t stream) {
+// The rows of the other side that a tile may see of `rows`: all, or those of the window (and the sinks).
+uint64_t rows_seen(const AttnArgs& a, uint64_t rows, int BM, uint64_t sinks) {
+  return a.window ? std::min<uint64_t>(rows, (uint64_t)a.window * (a.causal ? 1 : 2) + BM + sinks) : rows;
+}
+template <typename T, int DP, int BM, bool kWindow>
+int forward_as(const AttnArgs& a, cudaStream_t stream) {
   using S = SimtShape<DP, BM>;
   static SmemOptIn opt_in;
   const uint64_t samples = a.sequences ? a.sequences : 1;
-  return launch_simt(k_attention_simt<T, DP, BM>, opt_in, a, most_tiles(a.rows_q, a.sequences, BM) * a.heads,
-                     blocks_a_tile(a.rows_q, a.heads, a.rows_k / samples, BM, 4), 2 * S::tile + S::square, stream);
+  return launch_simt(k_attention_simt<T, DP, BM, kWindow>, opt_in, a, most_tiles(a.rows_q, a.sequences, BM) * a.heads,
+                     blocks_a_tile(a.rows_q, a.heads, rows_seen(a, a.rows_k / samples, BM, (uint64_t)a.sinks), BM, 4),
+                     2 * S::tile + S::square, stream);
 }
-template <typename T, int DP, int BM>
-int backward(const AttnArgs& a, cudaStream_t stream) {
+template <typename T, int DP, int BM, bool kWindow>
+int backward_as(const AttnArgs& a, cudaStream_t stream) {
   using S = SimtShape<DP, BM>;
   static SmemOptIn opt_q, opt_kv;
   const uint64_t samples = a.sequences ? a.sequences : 1, group = a.heads / a.kv_heads;
-  const int st = launch_simt(k_attention_simt_dq<T, DP, BM>, opt_q, a, most_tiles(a.rows_q, a.sequences, BM) * a.heads,
-                             blocks_a_tile(a.rows_q, a.heads, a.rows_k / samples, BM, 2), 4 * S::tile + S::square, stream);
+  const int st = launch_simt(k_attention_simt_dq<T, DP, BM, kWindow>, opt_q, a, most_tiles(a.rows_q, a.sequences, BM) * a.heads,
+                             blocks_a_tile(a.rows_q, a.heads, rows_seen(a, a.rows_k / samples, BM, (uint64_t)a.sinks), BM, 2),
+                             4 * S::tile + S::square, stream);
   if (st != RMN_OK) return st;
-  return launch_simt(k_attention_simt_dkv<T, DP, BM>, opt_kv, a, most_tiles(a.rows_k, a.sequences, BM) * a.kv_heads,
-                     blocks_a_tile(a.rows_k, a.kv_heads, a.rows_q / samples * group, BM, 2), 4 * S::tile + S::square, stream);
+  return launch_simt(k_attention_simt_dkv<T, DP, BM, kWindow>, opt_kv, a, most_tiles(a.rows_k, a.sequences, BM) * a.kv_heads,
+                     blocks_a_tile(a.rows_k, a.kv_heads, rows_seen(a, a.rows_q / samples, BM, 0) * group, BM, 2),
+                     4 * S::tile + S::square, stream);
+}
+template <typename T, int DP, int BM>
+int forward(const AttnArgs& a, cudaStream_t stream) {
+  return a.window ? forward_as<T, DP, BM, true>(a, stream) : forward_as<T, DP, BM, false>(a, stream);
+}
+template <typename T, int DP, int BM>
+int backward(const AttnArgs& a, cudaStream_t stream) {
+  return a.window ? backward_as<T, DP, BM, true>(a, stream) : backward_as<T, DP, BM, false>(a, stream);
 }
 
 }  // namespace

@@ -1112,34 +1112,39 @@ class RiemannLayerNorm(torch.nn.Module):
 
 class _PackedAttentionFunction(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, offsets, kv_offsets, kv_lengths, causal: bool, scale, grad_mode: bool):
+    def forward(ctx, q, k, v, offsets, kv_offsets, kv_lengths, causal: bool, scale, grad_mode: bool, window):
+        """``window``: {} or the arguments of one."""
         train = grad_mode and builtins.any(ctx.needs_input_grad)
-        out, low, lse = ops.attention_forward(q, k, v, offsets, kv_offsets, kv_lengths, causal, scale, want_stats=train)
+        out, low, lse = ops.attention_forward(q, k, v, offsets, kv_offsets, kv_lengths, causal, scale, want_stats=train, **window)
         ctx.save_for_backward(q, k, v, out, low, lse, offsets, kv_offsets, kv_lengths)
-        ctx.causal, ctx.scale = causal, scale
+        ctx.causal, ctx.scale, ctx.window = causal, scale, window
         return out
 
     @staticmethod
     def backward(ctx, grad_out):
         q, k, v, out, low, lse, offsets, kv_offsets, kv_lengths = ctx.saved_tensors
         with torch.no_grad():
-            grads = ops.attention_backward(grad_out, q, k, v, out, low, lse, offsets, kv_offsets, kv_lengths, ctx.causal, ctx.scale)
-        return (*_once("packed_attention", grads, (q, k, v, grad_out)), None, None, None, None, None, None)
+            grads = ops.attention_backward(grad_out, q, k, v, out, low, lse, offsets, kv_offsets, kv_lengths, ctx.causal, ctx.scale,
+                                           **ctx.window)
+        return (*_once("packed_attention", grads, (q, k, v, grad_out)), None, None, None, None, None, None, None)
 
 
 def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: torch.Tensor,
                      kv_offsets: Optional[torch.Tensor] = None, kv_lengths: Optional[torch.Tensor] = None,
-                     causal: bool = False, scale: Optional[float] = None) -> torch.Tensor:
+                     causal: bool = False, scale: Optional[float] = None, window: Optional[int] = None, sinks: int = 0) -> torch.Tensor:
     """softmax(scale q k^T) v within packed samples, differentiable (once) in q, k and v. ``q`` [rows, heads, channels], ``k`` and
     ``v`` [key rows, key heads, channels] (heads a multiple of key heads); ``offsets`` int32 [samples + 1]: first row of
     every sample and the end of the last. ``kv_offsets`` where the keys' rows are others than the queries', ``kv_lengths``
     [samples] where only the first rows of a sample's keys are in use (a cache). ``causal`` is aligned at the end of the keys.
-    ``scale``: channels ** -0.5 unless given. Rows of no sample, and rows that see no key, are zero. Offsets and lengths are looked
+    ``scale``: channels ** -0.5 unless given. ``window``: query i of n stands at place p = i + m - n of its sample's m keys and sees key j
+    only where |p - j| < window, or j < ``sinks`` (and j <= p where ``causal``); the work is that of the keys that are seen.
+    Rows of no sample, and rows that see no key, are zero. Offsets and lengths are looked
     at on the device: where they descend or leave the tensors nothing outside is touched, the outputs are of no use, and
     rmn_device_status (or the next map that is built, which reads the same word) reports a bad argument. bfloat16 runs on the
     tensor cores where channels are a multiple of 8 up to 128, the scale is positive, and rows and heads begin on 16 bytes and are not
     broadcast; elsewhere by multiply-adds, 10 to 30 times slower."""
-    return _PackedAttentionFunction.apply(q, k, v, offsets, kv_offsets, kv_lengths, bool(causal), scale, torch.is_grad_enabled())
+    args = {"window": window, "sinks": sinks} if window is not None or sinks else {}
+    return _PackedAttentionFunction.apply(q, k, v, offsets, kv_offsets, kv_lengths, bool(causal), scale, torch.is_grad_enabled(), args)
 
 
 def rotary_sections(channels: int, axes: int) -> List[int]:

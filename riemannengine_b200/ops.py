@@ -716,32 +716,52 @@ def _attention(q, k, v, offsets, kv_offsets, kv_lengths, causal, scale) -> capi.
     return p
 
 
+def _window(window, sinks) -> Tuple[int, int]:
+    if window is None:
+        if sinks:
+            raise RuntimeError("sinks need a window")
+        return 0, 0
+    if not 1 <= window <= _INT32_MAX or not 0 <= sinks < 1 << 30:
+        raise RuntimeError("window must be from 1 to 2^31 - 1, sinks from 0 to 2^30 - 1")
+    return int(window), int(sinks)
+
+
 def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: torch.Tensor,
                       kv_offsets: Optional[torch.Tensor] = None, kv_lengths: Optional[torch.Tensor] = None,
-                      causal: bool = False, scale: Optional[float] = None, want_stats: bool = False):
-    """Attention within packed samples (rmn_attention_forward): ``q`` [rows, heads, channels], ``k`` and ``v``
-    [key rows, key heads, channels], any row and head strides; returns (out, low, lse). Unless ``want_stats`` the last two are
+                      causal: bool = False, scale: Optional[float] = None, want_stats: bool = False, window: Optional[int] = None,
+                      sinks: int = 0):
+    """Attention within packed samples (rmn_attention_forward, rmn_window_attention_forward): ``q`` [rows, heads, channels], ``k`` and
+    ``v`` [key rows, key heads, channels], any row and head strides; returns (out, low, lse). Unless ``want_stats`` the last two are
     None; else what the backward pass needs: lse float32 [heads, rows], and for bfloat16 low, what rounding took from out."""
     q, k, v = _heads(q), _heads(k), _heads(v)
     p = _attention(q, k, v, offsets, kv_offsets, kv_lengths, causal, scale)
+    window, sinks = _window(window, sinks)
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     lse = torch.empty((p.heads, p.rows_q), dtype=torch.float32, device=q.device) if want_stats else None
     low = torch.empty_like(out) if want_stats and out.dtype == torch.bfloat16 else None
     lib = capi.lib()
     with torch.cuda.device(q.device):
-        wbytes = lib.rmn_attention_forward_workspace_bytes(ctypes.byref(p))
+        if window:
+            wbytes = lib.rmn_window_attention_forward_workspace_bytes(ctypes.byref(p), window, sinks)
+        else:
+            wbytes = lib.rmn_attention_forward_workspace_bytes(ctypes.byref(p))
         ws = torch.empty(wbytes, dtype=torch.uint8, device=q.device) if wbytes else None
-        capi.check(lib.rmn_attention_forward(ctypes.byref(p), _ptr(out), _ptr(low), _ptr(lse), _ptr(ws), wbytes, _stream()),
-                   "rmn_attention_forward")
+        args = (_ptr(out), _ptr(low), _ptr(lse), _ptr(ws), wbytes, _stream())
+        if window:
+            capi.check(lib.rmn_window_attention_forward(ctypes.byref(p), window, sinks, *args), "rmn_window_attention_forward")
+        else:
+            capi.check(lib.rmn_attention_forward(ctypes.byref(p), *args), "rmn_attention_forward")
     return out, low, lse
 
 
 def attention_backward(grad_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor,
                        low: Optional[torch.Tensor], lse: torch.Tensor, offsets: torch.Tensor, kv_offsets: Optional[torch.Tensor] = None,
-                       kv_lengths: Optional[torch.Tensor] = None, causal: bool = False, scale: Optional[float] = None):
-    """(dq, dk, dv) of attention_forward (rmn_attention_backward)."""
+                       kv_lengths: Optional[torch.Tensor] = None, causal: bool = False, scale: Optional[float] = None,
+                       window: Optional[int] = None, sinks: int = 0):
+    """(dq, dk, dv) of attention_forward (rmn_attention_backward, rmn_window_attention_backward)."""
     q, k, v, grad_out = _heads(q), _heads(k), _heads(v), _gradient_heads(grad_out)
     p = _attention(q, k, v, offsets, kv_offsets, kv_lengths, causal, scale)
+    window, sinks = _window(window, sinks)
     if grad_out.shape != q.shape or grad_out.dtype != q.dtype or grad_out.device != q.device:
         raise RuntimeError("the output gradient must have q's shape, dtype and device")
     dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
@@ -749,11 +769,17 @@ def attention_backward(grad_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor,
     dv = torch.empty(v.shape, dtype=v.dtype, device=q.device)
     lib = capi.lib()
     with torch.cuda.device(q.device):
-        wbytes = lib.rmn_attention_backward_workspace_bytes(ctypes.byref(p))
+        if window:
+            wbytes = lib.rmn_window_attention_backward_workspace_bytes(ctypes.byref(p), window, sinks)
+        else:
+            wbytes = lib.rmn_attention_backward_workspace_bytes(ctypes.byref(p))
         ws = torch.empty(wbytes, dtype=torch.uint8, device=q.device)
-        capi.check(lib.rmn_attention_backward(ctypes.byref(p), _ptr(out), _ptr(low), _ptr(lse), _ptr(grad_out),
-                                              int(grad_out.stride(0)), int(grad_out.stride(1)), _ptr(dq), _ptr(dk), _ptr(dv),
-                                              _ptr(ws), wbytes, _stream()), "rmn_attention_backward")
+        args = (_ptr(out), _ptr(low), _ptr(lse), _ptr(grad_out), int(grad_out.stride(0)), int(grad_out.stride(1)), _ptr(dq), _ptr(dk),
+                _ptr(dv), _ptr(ws), wbytes, _stream())
+        if window:
+            capi.check(lib.rmn_window_attention_backward(ctypes.byref(p), window, sinks, *args), "rmn_window_attention_backward")
+        else:
+            capi.check(lib.rmn_attention_backward(ctypes.byref(p), *args), "rmn_attention_backward")
     return dq, dk, dv
 
 

@@ -316,12 +316,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
       "packed_attention",
       [](const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& offsets,
          const c10::optional<at::Tensor>& kv_offsets, const c10::optional<at::Tensor>& kv_lengths, bool causal,
-         c10::optional<double> scale) {
+         c10::optional<double> scale, c10::optional<int64_t> window, int64_t sinks) {
         return packed_attention(q, k, v, offsets, kv_offsets.value_or(at::Tensor()), kv_lengths.value_or(at::Tensor()), causal,
-                                scale);
+                                scale, window, sinks);
       },
       py::arg("q"), py::arg("k"), py::arg("v"), py::arg("offsets"), py::arg("kv_offsets") = py::none(),
-      py::arg("kv_lengths") = py::none(), py::arg("causal") = false, py::arg("scale") = py::none(),
+      py::arg("kv_lengths") = py::none(), py::arg("causal") = false, py::arg("scale") = py::none(), py::arg("window") = py::none(),
+      py::arg("sinks") = 0,
       py::call_guard<py::gil_scoped_release>());
   m.def("rotary_sections", &rotary_sections, py::arg("channels"), py::arg("axes"));
   m.def("rotary_frequencies", &rotary_frequencies, py::arg("sections"), py::arg("base") = 10000.0, py::arg("whole") = false);

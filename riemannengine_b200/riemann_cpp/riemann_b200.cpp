@@ -1935,6 +1935,7 @@ struct AttentionInputs {
   at::Tensor q, k, v, offsets, kv_offsets, kv_lengths;  // an absent one of the last two: undefined or empty
   bool causal;
   double scale;
+  int32_t window, sinks;  // window 0: none
   rmn_attention problem() const {
     rmn_attention p = {};
     p.q = ptr(q); p.k = ptr(k); p.v = ptr(v);
@@ -1965,43 +1966,60 @@ at::Tensor attention_forward(const AttentionInputs& in, at::Tensor* low, at::Ten
   auto out = at::empty(in.q.sizes(), in.q.options());
   if (lse) *lse = at::empty({in.q.size(1), in.q.size(0)}, in.q.options().dtype(at::kFloat));
   if (low) *low = at::empty(in.q.scalar_type() == at::kBFloat16 ? in.q.sizes() : at::IntArrayRef({0}), in.q.options());
-  const size_t ws_bytes = rmn_attention_forward_workspace_bytes(&p);
+  const size_t ws_bytes = in.window ? rmn_window_attention_forward_workspace_bytes(&p, in.window, in.sinks)
+                                    : rmn_attention_forward_workspace_bytes(&p);
   at::Tensor ws;
   if (ws_bytes) ws = at::empty({static_cast<int64_t>(ws_bytes)}, in.q.options().dtype(at::kByte));
-  check(rmn_attention_forward(&p, ptr(out), low ? ptr(*low) : nullptr, lse ? static_cast<float*>(ptr(*lse)) : nullptr, ptr(ws),
-                              ws_bytes, current_stream()),
-        "rmn_attention_forward");
+  void* low_out = low ? ptr(*low) : nullptr;
+  float* lse_out = lse ? static_cast<float*>(ptr(*lse)) : nullptr;
+  if (in.window)
+    check(rmn_window_attention_forward(&p, in.window, in.sinks, ptr(out), low_out, lse_out, ptr(ws), ws_bytes, current_stream()),
+          "rmn_window_attention_forward");
+  else
+    check(rmn_attention_forward(&p, ptr(out), low_out, lse_out, ptr(ws), ws_bytes, current_stream()), "rmn_attention_forward");
   return out;
 }
 
 class PackedAttentionAutograd : public torch::autograd::Function<PackedAttentionAutograd> {
 public:
   static at::Tensor forward(torch::autograd::AutogradContext* ctx, at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor offsets,
-                            at::Tensor kv_offsets, at::Tensor kv_lengths, bool causal, double scale) {
+                            at::Tensor kv_offsets, at::Tensor kv_lengths, bool causal, double scale, int64_t window, int64_t sinks) {
     at::Tensor low, lse;
-    auto out = attention_forward({q, k, v, offsets, kv_offsets, kv_lengths, causal, scale}, &low, &lse);
+    auto out = attention_forward({q, k, v, offsets, kv_offsets, kv_lengths, causal, scale, static_cast<int32_t>(window),
+                                  static_cast<int32_t>(sinks)},
+                                 &low, &lse);
     ctx->save_for_backward({q, k, v, offsets, kv_offsets, kv_lengths, out, low, lse});
     ctx->saved_data["causal"] = causal;
     ctx->saved_data["scale"] = scale;
+    ctx->saved_data["window"] = window;
+    ctx->saved_data["sinks"] = sinks;
     return out;
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                  torch::autograd::variable_list grad_outputs) {
     auto saved = ctx->get_saved_variables();
     const AttentionInputs in{saved[0], saved[1], saved[2], saved[3], saved[4], saved[5], ctx->saved_data["causal"].toBool(),
-                             ctx->saved_data["scale"].toDouble()};
+                             ctx->saved_data["scale"].toDouble(), static_cast<int32_t>(ctx->saved_data["window"].toInt()),
+                             static_cast<int32_t>(ctx->saved_data["sinks"].toInt())};
     c10::cuda::CUDAGuard guard(in.q.device());
     auto grad = gradient_rows(grad_outputs[0]);
     const rmn_attention p = in.problem();
     auto dq = at::empty(in.q.sizes(), in.q.options()), dk = at::empty(in.k.sizes(), in.k.options());
     auto dv = at::empty(in.v.sizes(), in.v.options());
-    const size_t ws_bytes = rmn_attention_backward_workspace_bytes(&p);
+    const size_t ws_bytes = in.window ? rmn_window_attention_backward_workspace_bytes(&p, in.window, in.sinks)
+                                      : rmn_attention_backward_workspace_bytes(&p);
     auto ws = at::empty({static_cast<int64_t>(ws_bytes)}, in.q.options().dtype(at::kByte));
-    check(rmn_attention_backward(&p, ptr(saved[6]), ptr(saved[7]), static_cast<const float*>(ptr(saved[8])), ptr(grad),
-                                 grad.stride(0), grad.stride(1), ptr(dq), ptr(dk), ptr(dv), ptr(ws), ws_bytes, current_stream()),
-          "rmn_attention_backward");
+    const float* lse = static_cast<const float*>(ptr(saved[8]));
+    if (in.window)
+      check(rmn_window_attention_backward(&p, in.window, in.sinks, ptr(saved[6]), ptr(saved[7]), lse, ptr(grad), grad.stride(0),
+                                          grad.stride(1), ptr(dq), ptr(dk), ptr(dv), ptr(ws), ws_bytes, current_stream()),
+            "rmn_window_attention_backward");
+    else
+      check(rmn_attention_backward(&p, ptr(saved[6]), ptr(saved[7]), lse, ptr(grad), grad.stride(0), grad.stride(1), ptr(dq), ptr(dk),
+                                   ptr(dv), ptr(ws), ws_bytes, current_stream()),
+            "rmn_attention_backward");
     once({&dq, &dk, &dv}, {in.q, in.k, in.v, grad_outputs[0]}, "packed_attention");
-    return {dq, dk, dv, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+    return {dq, dk, dv, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
   }
 };
 }  // namespace
@@ -2040,7 +2058,7 @@ SparseTensor RiemannLayerNormImpl::forward(const SparseTensor& input) {
 
 at::Tensor packed_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& offsets,
                             const at::Tensor& kv_offsets, const at::Tensor& kv_lengths, bool causal,
-                            c10::optional<double> scale) {
+                            c10::optional<double> scale, c10::optional<int64_t> window, int64_t sinks) {
   for (auto const& [t, name] : {std::pair<const at::Tensor&, const char*>{q, "q"}, {k, "k"}, {v, "v"}}) {
     check_plain(t, name);
     TORCH_CHECK(t.dim() == 3 && t.size(2) >= 1, name, " must be [rows, heads, channels]");
@@ -2064,12 +2082,17 @@ at::Tensor packed_attention(const at::Tensor& q, const at::Tensor& k, const at::
   TORCH_CHECK(!kv_lengths.defined() || kv_lengths.numel() == n, "kv_lengths must have one entry per sample");
   TORCH_CHECK(kv_offsets.defined() || k.size(0) == q.size(0), "q and k must have the same rows unless kv_offsets are given");
   const double by = scale.value_or(1.0 / std::sqrt(static_cast<double>(q.size(2))));
+  TORCH_CHECK(window.has_value() || !sinks, "sinks need a window");
+  TORCH_CHECK(!window.has_value() || (*window >= 1 && *window <= std::numeric_limits<int32_t>::max() && sinks >= 0 && sinks < (1 << 30)),
+              "window must be from 1 to 2^31 - 1, sinks from 0 to 2^30 - 1");
+  const int64_t width = window.value_or(0);
   if (!wants_gradient({q, k, v}))
-    return attention_forward({head_rows(q), head_rows(k), head_rows(v), offsets, kv_offsets, kv_lengths, causal, by}, nullptr,
-                             nullptr);
+    return attention_forward({head_rows(q), head_rows(k), head_rows(v), offsets, kv_offsets, kv_lengths, causal, by,
+                              static_cast<int32_t>(width), static_cast<int32_t>(sinks)},
+                             nullptr, nullptr);
   auto none = at::empty({0}, offsets.options());
   return PackedAttentionAutograd::apply(head_rows(q), head_rows(k), head_rows(v), offsets, kv_offsets.defined() ? kv_offsets : none,
-                                        kv_lengths.defined() ? kv_lengths : none, causal, by);
+                                        kv_lengths.defined() ? kv_lengths : none, causal, by, width, sinks);
 }
 
 // ---------------------------------------------------------------------------------------------

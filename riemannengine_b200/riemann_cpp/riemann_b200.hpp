@@ -464,14 +464,17 @@ TORCH_MODULE(RiemannLayerNorm);
 // [key rows, key heads, channels] with any row and head strides, heads a multiple of key heads; offsets int32 [samples + 1]: first
 // row of every sample and the end of the last. kv_offsets where the keys' rows are others than the queries', kv_lengths [samples]
 // where only the first rows of a sample's keys are in use (a cache). causal is aligned at the end of the keys. scale: channels ^ -1/2
-// unless given. Rows of no sample, and rows that see no key, are zero. Offsets and lengths are looked at on the device: where they
+// unless given. window: query i of n stands at place p = i + m - n of its sample's m keys and sees key j only where |p - j| < window, or
+// j < sinks (and j <= p where causal); the work is that of the keys that are seen.
+// Rows of no sample, and rows that see no key, are zero. Offsets and lengths are looked at on the device: where they
 // descend or leave the tensors nothing outside is touched, the outputs are of no use, and rmn_device_status (or the next map
 // that is built, which reads the same word) reports a bad argument. bf16 runs on the tensor cores where channels are a multiple of 8 up to
 // 128, the scale is positive, and rows and heads begin on 16 bytes and are not broadcast; elsewhere by multiply-adds, 10 to 30 times
 // slower.
 at::Tensor packed_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& offsets,
                             const at::Tensor& kv_offsets = {}, const at::Tensor& kv_lengths = {}, bool causal = false,
-                            c10::optional<double> scale = c10::nullopt);
+                            c10::optional<double> scale = c10::nullopt, c10::optional<int64_t> window = c10::nullopt,
+                            int64_t sinks = 0);
 
 // All pairs of a head of `channels`, dealt out evenly to the axes (the first ones take what is left over).
 std::vector<int64_t> rotary_sections(int64_t channels, int64_t axes);
