@@ -116,6 +116,16 @@ __device__ __forceinline__ bool sees(const RowKeys& r, int32_t k0, int32_t c) {
   if constexpr (!kWindow) return c < r.end - k0;
   return c < r.sinks - k0 || (c >= r.low - k0 && c < r.end - k0);
 }
+// Columns 32 k ... 32 k + 31 of such a tile that a row sees, as bits.
+__device__ __forceinline__ uint32_t bits_below(int32_t n) {
+  uint32_t m;
+  asm("shl.b32 %0, %1, %2;" : "=r"(m) : "r"(0xffffffffu), "r"(max(n, 0)));  // (by 32 or more: 0)
+  return ~m;
+}
+__device__ __forceinline__ uint32_t seen_bits(const RowKeys& r, int32_t k0, int k) {
+  const int32_t at = k0 + 32 * k;
+  return bits_below(r.sinks - at) | (bits_below(r.end - at) & ~bits_below(r.low - at));
+}
 // The tiles of kTile keys that some of the query rows first ... last of a segment see: those of the sinks, from key 0 on, and behind them
 // those of the window, from its first key on; one run from key 0 on where the two would share a tile.
 template <bool kWindow, int kTile>

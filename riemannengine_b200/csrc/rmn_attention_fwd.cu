@@ -45,11 +45,12 @@ constexpr float kRescale = 8.f;  // log2 of how far a row's maximum may rise bef
 constexpr int kOneTile = 4;      // softmax warps
 constexpr int kTwoTiles = 8;
 
-template <int DP, int NQ>
+template <int DP, int NQ, bool kWindow>
 __global__ void __launch_bounds__(FwdShape<DP, NQ>::THREADS, NQ == 2 ? 1 : 2)
     k_attention_fwd(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                     const __grid_constant__ CUtensorMap map_v, const AttnArgs a) {
   using C = FwdShape<DP, NQ>;
+  static_assert(!kWindow || NQ == 1, "the query tiles of a block walk over the same keys");
   constexpr int SLOTS = C::SLOTS;
   extern __shared__ uint8_t smem_raw[];
   __shared__ FoundTile found;
@@ -106,11 +107,12 @@ __global__ void __launch_bounds__(FwdShape<DP, NQ>::THREADS, NQ == 2 ? 1 : 2)
   const Segment g = found.g;
   const int first = (found.tiles - 1 - found.tile) * 128 * NQ;  // the tiles that see the most keys first
   // key tiles of each query tile
+  const KeyWalk<kWindow, 128> walk(a, g, first, min(first + 128, g.n_q) - 1);
   int key_tiles[NQ], most = 0;
 #pragma unroll
   for (int t = 0; t < NQ; ++t) {
     const int rows = min(128, g.n_q - first - t * 128);
-    key_tiles[t] = exists && rows > 0 ? (visible_keys(g, first + t * 128 + rows - 1, a.causal) + 127) / 128 : 0;
+    key_tiles[t] = !exists || rows <= 0 ? 0 : kWindow ? walk.tiles : (visible_keys(g, first + t * 128 + rows - 1, a.causal) + 127) / 128;
     most = max(most, key_tiles[t]);
   }
 
@@ -122,7 +124,7 @@ __global__ void __launch_bounds__(FwdShape<DP, NQ>::THREADS, NQ == 2 ? 1 : 2)
                    o_t = tmem + lanes + C::O0 + t * DP;
     const int row = first + t * 128 + (warp & 3) * 32 + lane;
     const bool mine = row < g.n_q;
-    const int see = visible_keys(g, row, a.causal);
+    const RowKeys seen = row_keys<kWindow>(a, g, row);
     const float scale = a.scale * kLog2e;  // (> 0)
     float m = -CUDART_INF_F, l = 0.f;      // maximum in use (times scale, log 2), sum
     const int n_tiles = NQ == 1 ? key_tiles[0] : (t == 0 ? key_tiles[0] : key_tiles[NQ - 1]);
@@ -140,8 +142,18 @@ __global__ void __launch_bounds__(FwdShape<DP, NQ>::THREADS, NQ == 2 ? 1 : 2)
         tc_fence_before();
         mbar_arrive(&s_free[t]);
       }
-      const int left = see - j * 128;  // columns that this row sees
-      if (left < 128) {
+      const int k0 = walk.key(j), left = seen.end - k0;  // columns that this row sees (with a window: if it sees them from the first on)
+      if constexpr (kWindow) {
+        if (left < 128 || seen.low > k0) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t bits = seen_bits(seen, k0, k);
+#pragma unroll
+            for (int c = 0; c < 32; ++c)
+              if (!(bits >> c & 1u)) r[k * 32 + c] = 0xff800000u;
+          }
+        }
+      } else if (left < 128) {
 #pragma unroll
         for (int c = 0; c < 128; ++c)
           if (c >= left) r[c] = 0xff800000u;
@@ -256,7 +268,7 @@ __global__ void __launch_bounds__(FwdShape<DP, NQ>::THREADS, NQ == 2 ? 1 : 2)
           const CUtensorMap* map = (i & 1u) ? &map_v : &map_k;
 #pragma unroll
           for (int c = 0; c < C::ATOMS; ++c)
-            tma_load_3d(slots + s * C::TILE + c * kAtomBytes, map, &full[s], c * 64, kv, g.k0 + (int)(i >> 1) * 128);
+            tma_load_3d(slots + s * C::TILE + c * kAtomBytes, map, &full[s], c * 64, kv, g.k0 + walk.key((int)(i >> 1)));
         }
         if (timed_out) {  // no copy may be in flight when the block ends
           for (uint32_t k = i > SLOTS ? i - SLOTS : 0; k < i; ++k) mbar_wait(&full[k % SLOTS], (k / SLOTS) & 1u);
@@ -296,7 +308,7 @@ __global__ void __launch_bounds__(FwdShape<DP, NQ>::THREADS, NQ == 2 ? 1 : 2)
           if (!v_here) {
             if (!ready(2u * j + 1u)) return;
             v_here = true;
-            if (g.n_k - j * 128 < 128) zero_rows(v_s, g.n_k - j * 128, C::ATOMS);
+            if (g.n_k - walk.key(j) < 128) zero_rows(v_s, g.n_k - walk.key(j), C::ATOMS);
           }
           if (!warp_wait(&p_full[t], ph)) { timed_out = true; return; }
           tc_fence_after();
@@ -359,11 +371,11 @@ __global__ void __launch_bounds__(FwdShape<DP, NQ>::THREADS, NQ == 2 ? 1 : 2)
   }
 }
 
-template <int DP, int NQ>
+template <int DP, int NQ, bool kWindow>
 int launch_fwd(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const AttnArgs& a, cudaStream_t stream) {
   using C = FwdShape<DP, NQ>;
   static SmemOptIn opt_in;
-  auto kern = k_attention_fwd<DP, NQ>;
+  auto kern = k_attention_fwd<DP, NQ, kWindow>;
   const uint64_t blocks = most_tiles(a.rows_q, a.sequences, 128 * NQ) * a.heads;
   if (blocks > 0x7fffffffull) return RMN_ERR_UNSUPPORTED;
   // the registers dealt out have to be there: asked for once
@@ -386,19 +398,20 @@ int launch_fwd(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
 
 int attention_tc_forward(const AttnArgs& a, cudaStream_t stream) {
   using namespace tc;
-  if (a.window || a.dim > 128 || !(a.scale > 0.f) || a.rows_k == 0 || ((uintptr_t)a.out & 15) || ((uintptr_t)a.low & 15))
+  if (a.dim > 128 || !(a.scale > 0.f) || a.rows_k == 0 || ((uintptr_t)a.out & 15) || ((uintptr_t)a.low & 15))
     return RMN_ERR_UNSUPPORTED;
   CUtensorMap q, k, v;
   if (!make_head_map(&q, a.q, a.rows_q, a.heads, a.dim, a.q_row, a.q_head) ||
       !make_head_map(&k, a.k, a.rows_k, a.kv_heads, a.dim, a.k_row, a.k_head) ||
       !make_head_map(&v, a.v, a.rows_k, a.kv_heads, a.dim, a.v_row, a.v_head))
     return RMN_ERR_UNSUPPORTED;
-  if (a.dim <= 64) return launch_fwd<64, 1>(q, k, v, a, stream);
+  if (a.window) return a.dim <= 64 ? launch_fwd<64, 1, true>(q, k, v, a, stream) : launch_fwd<128, 1, true>(q, k, v, a, stream);
+  if (a.dim <= 64) return launch_fwd<64, 1, false>(q, k, v, a, stream);
   // two query tiles a block read the keys half as often, one leaves two blocks an SM: 16 heads of 128, one causal sample of 8192
   // rows 249 us with two and 260 with one (262 with two since the waits are votes); 100 samples of 256 rows, 8 heads, 76 and 66.5; 12 of
   // 2048 the same
   const bool two = a.rows_q / 2048 >= a.sequences;
-  return two ? launch_fwd<128, 2>(q, k, v, a, stream) : launch_fwd<128, 1>(q, k, v, a, stream);
+  return two ? launch_fwd<128, 2, false>(q, k, v, a, stream) : launch_fwd<128, 1, false>(q, k, v, a, stream);
 }
 
 }  // namespace rmn
