@@ -2,6 +2,8 @@
 // the samples of a coordinate map.
 #include "rmn_attention.cuh"
 
+#include <algorithm>
+
 namespace rmn {
 
 const uint32_t* tc_status_device_address();  // defined in rmn_conv_tc.cu
@@ -113,7 +115,44 @@ int find_status(AttnArgs* a) {
   return a->status ? RMN_OK : RMN_ERR_CUDA;
 }
 
+
+// dK and dV of the sinks of the samples that are cut: the sums of their chunks' parts, in order.
+constexpr int kSumThreads = 256;
+template <typename T>
+__global__ void __launch_bounds__(kSumThreads) k_attention_sinks_sum(const AttnArgs a) {
+  __shared__ FoundTile found;
+  __shared__ int32_t warp_sums[kSumThreads / 32];
+  after_previous_kernel();
+  const int kv = blockIdx.x % a.kv_heads;
+  if (!find_tile<kSumThreads, TilesOf::kLongQueries>(a, blockIdx.x / a.kv_heads, a.sink_chunk, &found, warp_sums)) return;
+  const Segment g = found.g;
+  // each of a sample's chunks has a block, which sums a share of its sinks' channels
+  const int64_t sinks = min(a.sinks, g.n_k), n = 2 * sinks * a.dim;
+  for (int64_t i = (int64_t)found.tile * kSumThreads + threadIdx.x; i < n; i += (int64_t)found.tiles * kSumThreads) {
+    const int which = i >= sinks * a.dim;
+    const int64_t at = i - which * sinks * a.dim;  // of the sinks' channels
+    float sum = 0.f;
+#pragma unroll 4
+    for (int c = 0; c < found.tiles; ++c) sum += __ldg(a.sink_parts + sink_part(a, g.q0, c, kv) + (int64_t)which * a.sink_most * a.dim + at);
+    const int64_t key = at / a.dim, to = ((g.k0 + key) * a.kv_heads + kv) * a.dim + at % a.dim;
+    if (!which) sum *= a.scale;
+    void* out = which ? a.dv : a.dk;
+    if constexpr (sizeof(T) == 4) static_cast<float*>(out)[to] = sum;
+    else static_cast<__nv_bfloat16*>(out)[to] = __float2bfloat16_rn(sum);
+  }
+}
+
 }  // namespace
+
+int attention_sinks_sum(const AttnArgs& a, int dtype, cudaStream_t stream) {
+  const uint64_t blocks = (uint64_t)a.sink_chunks * a.kv_heads;
+  if (blocks > 0x7fffffffull) return RMN_ERR_UNSUPPORTED;
+  RMN_CUDA_TRY(launch_overlapped(dtype == RMN_F32 ? k_attention_sinks_sum<float> : k_attention_sinks_sum<__nv_bfloat16>, dim3((uint32_t)blocks),
+                                 dim3(kSumThreads), 0, stream, a));
+  RMN_LAUNCH_CHECK();
+  return RMN_OK;
+}
+
 }  // namespace rmn
 
 using namespace rmn;
@@ -172,8 +211,17 @@ int forward(const rmn_attention* problem, int32_t window, int32_t sinks, void* d
   return attention_simt_forward(a, problem->dtype, stream);
 }
 
-size_t backward_workspace(const rmn_attention* problem, int32_t, int32_t) {
-  return problem && problem->heads > 0 ? (size_t)problem->heads * problem->rows_q * sizeof(float) : 0;
+// delta, and behind it the sinks' parts
+size_t delta_bytes(const rmn_attention* p) { return (size_t)p->heads * p->rows_q * sizeof(float); }
+size_t parts_at(const rmn_attention* p) { return (delta_bytes(p) + 255) / 256 * 256; }
+SinkPlan sinks_of(const rmn_attention* p, int32_t window, int32_t sinks) {
+  return sink_plan(p->rows_q, p->rows_k, p->sequences, p->kv_heads, p->dim, p->causal, window, sinks);
+}
+size_t backward_workspace(const rmn_attention* p, int32_t window, int32_t sinks) {
+  if (!p || p->heads < 1) return 0;
+  if (!window || p->kv_heads < 1 || p->dim < 1) return delta_bytes(p);
+  const SinkPlan plan = sinks_of(p, window, sinks);
+  return plan.parts ? parts_at(p) + plan.parts * sizeof(float) : delta_bytes(p);
 }
 int backward(const rmn_attention* problem, int32_t window, int32_t sinks, const void* d_out, const void* d_low, const float* d_lse,
              const void* d_grad_out, int64_t grad_row, int64_t grad_head, void* d_dq, void* d_dk, void* d_dv, void* d_workspace,
@@ -205,12 +253,15 @@ int backward(const rmn_attention* problem, int32_t window, int32_t sinks, const 
   a.grad_row = grad_row;
   a.grad_head = grad_head;
   a.delta = static_cast<float*>(d_workspace);
+  const SinkPlan plan = sinks_of(problem, window, sinks);
+  a.sink_chunk = plan.chunk;
+  a.sink_most = plan.most;
+  a.sink_chunks = (int32_t)std::min<int64_t>(plan.chunks, 0x7fffffff);
+  a.sink_parts = plan.parts ? reinterpret_cast<float*>(static_cast<char*>(d_workspace) + parts_at(problem)) : nullptr;
   a.dq = d_dq; a.dk = d_dk; a.dv = d_dv;
-  if (problem->dtype == RMN_BF16) {
-    const int tc = attention_tc_backward(a, stream);
-    if (tc != RMN_ERR_UNSUPPORTED) return tc;
-  }
-  return attention_simt_backward(a, problem->dtype, stream);
+  int done = problem->dtype == RMN_BF16 ? attention_tc_backward(a, stream) : RMN_ERR_UNSUPPORTED;
+  if (done == RMN_ERR_UNSUPPORTED) done = attention_simt_backward(a, problem->dtype, stream);
+  return done == RMN_OK && a.sink_chunk ? attention_sinks_sum(a, problem->dtype, stream) : done;
 }
 }  // namespace
 

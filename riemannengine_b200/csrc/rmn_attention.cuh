@@ -28,7 +28,44 @@ struct AttnArgs {
   const void* fwd_out;
   float* delta;                                         // [heads, rows_q]: sum over the channels of grad * out
   void *dq, *dk, *dv;                                   // contiguous
+  // backward with sinks (see SinkPlan)
+  int32_t sink_chunk, sink_most, sink_chunks;           // chunk 0: no sample is cut
+  float* sink_parts;
 };
+
+// The sinks' gradients are sums over all queries, those of other keys over a window of them. So the sinks of samples longer than
+// `chunk` queries are left to blocks of their own: each takes a tile of the sinks and a chunk of the queries, and stores its part of dK
+// and dV in fp32; a last kernel adds the parts in order. Parts are [slot][key head][dk, dv][sink][channel]. Beyond kCountedSamples samples,
+// where blocks cannot count such chunks, no sample is cut.
+struct SinkPlan {
+  int32_t chunk = 0, most = 0;  // queries of a chunk; sinks of a sample
+  int64_t chunks = 0;           // of all samples, at most: of a sample that is cut, fewer than twice as many as its rows fill
+  size_t parts = 0;             // floats
+};
+constexpr uint32_t kCountedSamples = 384;  // (see find_tile)
+// Chunks of about the queries that another key sees, so that blocks of both kinds take the same time, and of eight times the sinks, so that
+// the parts are no larger than the gradients.
+inline SinkPlan sink_plan(uint32_t rows_q, uint32_t rows_k, uint32_t sequences, int kv_heads, int dim, int causal, int32_t window,
+                          int32_t sinks) {
+  SinkPlan p;
+  if (!window || !sinks || !rows_k || sequences > kCountedSamples) return p;
+  const uint64_t most = (uint32_t)sinks < rows_k ? (uint32_t)sinks : rows_k, span = (uint64_t)window * (causal ? 1 : 2) + 128;
+  uint64_t chunk = span > 512 ? span : 512;
+  if (chunk < 8 * most) chunk = 8 * most;
+  chunk = (chunk + 127) / 128 * 128;
+  if (chunk >= rows_q) return p;
+  p.chunk = (int32_t)chunk;
+  p.most = (int32_t)most;
+  p.chunks = 2 * (int64_t)(rows_q / chunk);
+  p.parts = (size_t)2 * (rows_q / chunk + 1) * kv_heads * 2 * most * dim;
+  return p;
+}
+// Where the parts of a chunk of a sample that is cut begin, of key head kv: of chunks that begin in the same stretch of `chunk` rows one at
+// most is the first of its sample, and one at most is not.
+__device__ __forceinline__ size_t sink_part(const AttnArgs& a, int32_t q0, int32_t chunk, int kv) {
+  const uint32_t slot = 2 * (uint32_t)(((int64_t)q0 + (int64_t)chunk * a.sink_chunk) / a.sink_chunk) + (chunk > 0 ? 1u : 0u);
+  return ((size_t)slot * a.kv_heads + kv) * 2 * a.sink_most * a.dim;
+}
 
 // Row ranges of one sample. Every row of the tensors belongs to exactly one segment: segments 0 ... S - 1 are the samples,
 // segment S the rows behind the last sample and S + 1 those before the first; the last two have no keys to attend to, so that
@@ -170,15 +207,56 @@ __device__ __forceinline__ KeyRows key_rows(const AttnArgs& a, const Segment& g,
   if (j < a.sinks) return {a.causal ? clamp_to(row, g.n_q) : 0, g.n_q};
   return {clamp_to(a.causal ? row : row - a.window + 1, g.n_q), clamp_to(row + a.window, g.n_q)};
 }
+// A tile of keys of one sample and the queries that it is multiplied with.
+struct KeyTile {
+  int32_t first;      // key
+  int32_t lo, end;    // keys of the tile that are summed here (of those in use)
+  int32_t from, to;   // queries that see any of them
+  int32_t least;      // rows from here on are stored
+  int32_t chunk;      // of the queries, where the sinks of a sample that is cut are summed; else -1
+  bool used;
+};
+template <bool kWindow, int kTile>
+__device__ __forceinline__ KeyTile key_tile(const AttnArgs& a, const Segment& g, int32_t tile, int32_t chunk) {
+  KeyTile t;
+  t.first = tile * kTile;
+  t.lo = t.first;
+  t.end = min(t.first + kTile, g.n_k);
+  t.least = 0;
+  t.chunk = kWindow ? chunk : -1;
+  if constexpr (kWindow) {
+    const int32_t sinks = min(a.sinks, g.n_k);
+    if (chunk >= 0) {
+      t.end = min(t.end, sinks);
+    } else if (a.sink_chunk && g.n_q > a.sink_chunk) {
+      t.lo = max(t.lo, sinks);
+      t.least = sinks;
+    }
+  }
+  t.from = t.to = 0;
+  if (t.lo < t.end) {
+    const KeyRows lo = key_rows<kWindow>(a, g, t.lo), hi = key_rows<kWindow>(a, g, t.end - 1);
+    t.from = lo.lo;
+    t.to = max(lo.end, hi.end);  // (the first key's queries begin first, and end last where it is a sink)
+    if (kWindow && chunk >= 0) {
+      t.from = max(t.from, chunk * a.sink_chunk);
+      t.to = (int32_t)min((int64_t)t.to, ((int64_t)chunk + 1) * a.sink_chunk);
+    }
+  }
+  t.used = t.from < t.to;
+  return t;
+}
 
-// The tile of `tile_rows` rows that a block works on: of query rows, or of key rows (whole slots, in use or not).
-enum class TilesOf { kQueries, kSlots };
+// The tile of `tile_rows` rows that a block works on: of query rows, of key rows (whole slots, in use or not), or of the query rows of
+// samples that have more than one (of up to kCountedSamples samples).
+enum class TilesOf { kQueries, kSlots, kLongQueries };
 struct FoundTile {
   Segment g;
   int32_t tile, tiles;  // number of the tile in its segment, and the segment's tiles
 };
 template <TilesOf kOf>
 __device__ __forceinline__ int32_t segment_tiles(const Segment& g, int tile_rows) {
+  if (kOf == TilesOf::kLongQueries) return g.n_q > tile_rows && g.n_k > 0 ? tiles_of(g.n_q, tile_rows) : 0;
   return tiles_of(kOf == TilesOf::kQueries ? g.n_q : g.k_slot, tile_rows);
 }
 // Sums stop at the largest number: offsets that descend may give a row to many samples.
@@ -205,14 +283,13 @@ __device__ __forceinline__ void scan_block(int32_t mine, int32_t* warp_sums, int
   }
 }
 
-// Up to kCountedSamples samples: every thread counts the tiles of a run of segments, a scan over the block places them, and the
+// Up to kCountedSamples (384) samples: every thread counts the tiles of a run of segments, a scan over the block places them, and the
 // numbers behind the last tile are of no tile. Beyond, counting would cost the square of the samples: segment j in the order of the
 // rows (those before the first sample, the samples, those behind) begins at row b(j) and has the numbers from b(j) / tile_rows + j
 // on, as many as it has tiles or one more, which is of no tile; every warp searches for its number, 32 places at a time. Numbers
 // without a tile cost a block each, and the search leaves them among the others. 8 heads of 64, backward, with counts and with the
 // search: 128 samples of 96 rows 81 and 94 us; 256, 512, 1024, 4096 samples of 64 rows 115 and 122, 240 and 238, 523 and 476,
 // 3650 and 1885.
-constexpr uint32_t kCountedSamples = 384;
 template <int kThreads, TilesOf kOf>
 __device__ __forceinline__ bool find_tile(const AttnArgs& a, uint32_t want, int tile_rows, FoundTile* found, int32_t* warp_sums) {
   const uint32_t n = a.sequences + 2;
@@ -305,6 +382,7 @@ int attention_simt_forward(const AttnArgs& a, int dtype, cudaStream_t stream);
 int attention_simt_backward(const AttnArgs& a, int dtype, cudaStream_t stream);
 int attention_tc_forward(const AttnArgs& a, cudaStream_t stream);  // bf16
 int attention_tc_backward(const AttnArgs& a, cudaStream_t stream);
+int attention_sinks_sum(const AttnArgs& a, int dtype, cudaStream_t stream);  // behind a backward pass that has cut samples
 // few query rows a sample: chunks of the keys, then their sum. Scratch bytes, 0 where this form is not meant for the sizes
 size_t attention_rows_workspace(uint32_t rows_q, uint32_t rows_k, uint32_t sequences, int heads, int kv_heads, int dim, int dtype);
 int attention_rows_forward(const AttnArgs& a, int dtype, void* workspace, cudaStream_t stream);

@@ -105,7 +105,7 @@ __device__ __forceinline__ void init_barriers(BwdTail* tail) {
 }
 
 // map_q and map_g (the output's gradient) in boxes of 128 rows, map_k and map_v of a step's
-template <int DP>
+template <int DP, bool kWindow>
 __global__ void __launch_bounds__(BwdShape<DP>::THREADS, BwdShape<DP>::BLOCKS)
     k_attention_dq(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_g,
                    const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const AttnArgs a) {
@@ -141,7 +141,8 @@ __global__ void __launch_bounds__(BwdShape<DP>::THREADS, BwdShape<DP>::BLOCKS)
   const Segment g = tail->found.g;
   const int first = (tail->found.tiles - 1 - tail->found.tile) * 128;  // the tiles that see the most keys first
   const int rows = min(128, g.n_q - first);
-  const int steps = exists ? (visible_keys(g, first + rows - 1, a.causal) + STEP - 1) / STEP : 0;
+  const KeyWalk<kWindow, STEP> walk(a, g, first, first + rows - 1);
+  const int steps = exists ? walk.tiles : 0;
 
   auto lane_wait = [&](uint64_t* bar, uint32_t parity) {
     if (!timed_out && !mbar_wait(bar, parity)) timed_out = true;
@@ -171,7 +172,7 @@ __global__ void __launch_bounds__(BwdShape<DP>::THREADS, BwdShape<DP>::BLOCKS)
         const CUtensorMap* map = (i & 1u) ? &map_v : &map_k;
 #pragma unroll
         for (int c = 0; c < C::ATOMS; ++c)
-          tma_load_3d(ring + s * C::TILE + c * (STEP * 128), map, &tail->full[s], c * 64, kv, g.k0 + (int)(i >> 1) * STEP);
+          tma_load_3d(ring + s * C::TILE + c * (STEP * 128), map, &tail->full[s], c * 64, kv, g.k0 + walk.key((int)(i >> 1)));
       }
       if (timed_out) {  // no copy may be in flight when the block ends
         for (uint32_t k = i > SLOTS ? i - SLOTS : 0; k < i; ++k) mbar_wait(&tail->full[k % SLOTS], (k / SLOTS) & 1u);
@@ -188,7 +189,8 @@ __global__ void __launch_bounds__(BwdShape<DP>::THREADS, BwdShape<DP>::BLOCKS)
     // S and dP of step j
     auto first_products = [&](int j) {
       if (!ready(2u * j)) return;
-      if (g.n_k - j * STEP < STEP) zero_rows<STEP>(slot(2u * j), g.n_k - j * STEP, C::ATOMS);  // dS is zero there, K has to be finite
+      const int left = g.n_k - walk.key(j);
+      if (left < STEP) zero_rows<STEP>(slot(2u * j), left, C::ATOMS);  // dS is zero there, K has to be finite
       if (j > 0 && !wait(&tail->s_free, (uint32_t)(j - 1) & 1u)) return;
       tc_fence_after();
       mma_rows<STEP>(tmem + T_S, smem_base, slot(2u * j), idesc_s, ksteps);
@@ -214,7 +216,7 @@ __global__ void __launch_bounds__(BwdShape<DP>::THREADS, BwdShape<DP>::BLOCKS)
     const uint32_t lanes = ((uint32_t)(warp & 3) * 32u) << 16;
     const int r = (warp & 3) * 32 + lane, row = first + r;
     const bool mine = row < g.n_q;
-    const int see = mine ? visible_keys(g, row, a.causal) : 0;
+    const RowKeys seen = mine ? row_keys<kWindow>(a, g, row) : RowKeys{0, 0, 0};
     float lse = 0.f, delta = 0.f;
     const size_t at = ((size_t)(g.q0 + row) * a.heads + head) * a.dim;
     if (mine) {
@@ -258,7 +260,7 @@ __global__ void __launch_bounds__(BwdShape<DP>::THREADS, BwdShape<DP>::BLOCKS)
       tc_fence_before();
       mbar_arrive(&tail->s_free);
       uint32_t w[32];
-      const int left = see - j * STEP - half * 64;  // columns that this row sees
+      const int k0 = walk.key(j) + half * 64, left = seen.end - k0;  // columns that this row sees (with a window: from seen.low on)
 #pragma unroll
       for (int c = 0; c < 64; c += 2) {
         float x, y;
@@ -267,7 +269,17 @@ __global__ void __launch_bounds__(BwdShape<DP>::THREADS, BwdShape<DP>::BLOCKS)
         parts(mul(p, add(pair_of(dp[c], dp[c + 1]), minus_delta)), x, y);
         w[c / 2] = pack_bf16(x, y);
       }
-      if (left < 64) {
+      if constexpr (kWindow) {
+        if (left < 64 || seen.low > k0) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const uint32_t bits = seen_bits(seen, k0, k);
+#pragma unroll
+            for (int c = 0; c < 16; ++c)
+              w[k * 16 + c] &= (bits >> (2 * c) & 1u ? 0xffffu : 0u) | (bits >> (2 * c + 1) & 1u ? 0xffff0000u : 0u);
+          }
+        }
+      } else if (left < 64) {
 #pragma unroll
         for (int c = 0; c < 32; ++c) w[c] = 2 * c >= left ? 0u : 2 * c + 1 >= left ? w[c] & 0xffffu : w[c];
       }
@@ -299,7 +311,7 @@ __global__ void __launch_bounds__(BwdShape<DP>::THREADS, BwdShape<DP>::BLOCKS)
 }
 
 // map_k and map_v in boxes of 128 rows, map_q and map_g of a step's
-template <int DP>
+template <int DP, bool kWindow>
 __global__ void __launch_bounds__(BwdShape<DP>::THREADS, BwdShape<DP>::BLOCKS)
     k_attention_dkv(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                     const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_g, const AttnArgs a) {
@@ -332,13 +344,28 @@ __global__ void __launch_bounds__(BwdShape<DP>::THREADS, BwdShape<DP>::BLOCKS)
 
   const int blocks = (int)cluster_size(), rank = (int)cluster_rank(), group = a.heads / a.kv_heads / blocks;  // heads of this block
   const int kv = blockIdx.x / blocks % a.kv_heads, head0 = (kv * blocks + rank) * group;
-  const bool exists =
-      find_tile<C::THREADS, TilesOf::kSlots>(a, blockIdx.x / blocks / a.kv_heads, 128, &tail->found, tail->warp_sums);
+  int number = blockIdx.x / blocks / a.kv_heads, chunk = -1, at_tile = 0;
+  bool exists = true;
+  if constexpr (kWindow) {  // first the chunks' tiles of the sinks
+    const int sink_tiles = tiles_of(a.sink_most, 128), of_sinks = a.sink_chunks * sink_tiles;
+    if (number < of_sinks) {
+      exists = find_tile<C::THREADS, TilesOf::kLongQueries>(a, number / sink_tiles, a.sink_chunk, &tail->found, tail->warp_sums);
+      chunk = tail->found.tile;
+      at_tile = number % sink_tiles;
+    }
+    number -= of_sinks;
+  }
+  if (!kWindow || number >= 0) {
+    exists = find_tile<C::THREADS, TilesOf::kSlots>(a, number, 128, &tail->found, tail->warp_sums);
+    at_tile = tail->found.tile;
+    chunk = -1;
+  }
   const Segment g = tail->found.g;
-  const int first = tail->found.tile * 128;  // the first keys are seen by the most queries
+  const KeyTile keys = key_tile<kWindow, 128>(a, g, at_tile, chunk);
+  const int first = keys.first;  // the first keys are seen by the most queries
   // steps of each head that see any of these keys
-  const int from = first_query(g, first, a.causal) / STEP;
-  const int tiles = exists && first < g.n_k ? max(0, (g.n_q + STEP - 1) / STEP - from) : 0;
+  const int from = kWindow ? keys.from : keys.from / STEP * STEP;
+  const int tiles = exists && keys.used ? (keys.to - from + STEP - 1) / STEP : 0;
   const int steps = tiles * group;
 
   auto lane_wait = [&](uint64_t* bar, uint32_t parity) {
@@ -362,7 +389,7 @@ __global__ void __launch_bounds__(BwdShape<DP>::THREADS, BwdShape<DP>::BLOCKS)
       }
     }
     uint32_t i = 0;  // tiles asked for
-    int h = head0, q0 = from * STEP;
+    int h = head0, q0 = from;
     for (int step = 0; step < steps; ++step) {
       // the statistics first: their loads run while the slots are waited for
       constexpr int N = STEP / 32;
@@ -397,8 +424,8 @@ __global__ void __launch_bounds__(BwdShape<DP>::THREADS, BwdShape<DP>::BLOCKS)
       }
       mbar_arrive(&tail->st_full[b]);
       q0 += STEP;
-      if (q0 >= g.n_q) {
-        q0 = from * STEP;
+      if (q0 >= keys.to) {
+        q0 = from;
         ++h;
       }
     }
@@ -415,7 +442,7 @@ __global__ void __launch_bounds__(BwdShape<DP>::THREADS, BwdShape<DP>::BLOCKS)
     // tile i of the ring has arrived; rows behind the sample's last query become zeros, as P and dS are there
     auto ready = [&](uint32_t i) {
       if (!wait(&tail->full[i % SLOTS], (i / SLOTS) & 1u)) return false;
-      const int q = (from + (int)(i >> 1) % tiles) * STEP;
+      const int q = from + (int)(i >> 1) % tiles * STEP;
       if (g.n_q - q < STEP) zero_rows<STEP>(slot(i), g.n_q - q, C::ATOMS);
       tc_fence_after();
       return true;
@@ -455,14 +482,15 @@ __global__ void __launch_bounds__(BwdShape<DP>::THREADS, BwdShape<DP>::BLOCKS)
     const int half = warp >> 2;
     const uint32_t lanes = ((uint32_t)(warp & 3) * 32u) << 16;
     const int row = first + (warp & 3) * 32 + lane;  // key
-    const int sees = first_query(g, row, a.causal);  // its first query
+    const KeyRows seen = !kWindow || (row >= keys.lo && row < keys.end) ? key_rows<kWindow>(a, g, row) : KeyRows{0, 0};
+    const int last = min(seen.end, keys.to);
     const Pair scale = make_pair(a.scale * kLog2e, a.scale * kLog2e);
-    int q0 = from * STEP;
+    int q0 = from;
     for (int i = 0; i < steps; ++i) {
       const uint32_t ph = (uint32_t)i & 1u;
       const int b = i % kStats;
-      const int lo = sees - q0 - half * 64, hi = g.n_q - q0 - half * 64;  // columns of the queries that see this key
-      q0 = q0 + STEP >= g.n_q ? from * STEP : q0 + STEP;
+      const int lo = seen.lo - q0 - half * 64, hi = last - q0 - half * 64;  // columns of the queries that see this key
+      q0 = q0 + STEP >= keys.to ? from : q0 + STEP;
       const ulonglong2* lse = reinterpret_cast<const ulonglong2*>(&tail->lse[b][half * 64]);
       const ulonglong2* delta = reinterpret_cast<const ulonglong2*>(&tail->delta[b][half * 64]);
       uint32_t s[64], w[32];
@@ -523,12 +551,28 @@ __global__ void __launch_bounds__(BwdShape<DP>::THREADS, BwdShape<DP>::BLOCKS)
     tc_fence_after();
     if (!timed_out) {
       const size_t at = ((size_t)(g.k0 + row) * a.kv_heads + kv) * a.dim;
-      const bool mine = row < g.k_slot;
+      const bool mine = chunk >= 0 ? row < keys.end : row < g.k_slot && row >= keys.least;
 #pragma unroll
       for (int which = 0; which < 2; ++which) {  // dv, dk; where there are two halves of the warps, one each
         if (C::HALVES == 2 && which != half) continue;
         const uint32_t from_t = tmem + lanes + (which ? T_DK : T_DV);
-        if (blocks == 1) {
+        if (kWindow && blocks == 1 && chunk >= 0) {  // the part as it is
+          float* to = a.sink_parts + sink_part(a, g.q0, chunk, kv) + ((which ? 0 : (int64_t)a.sink_most) + row) * a.dim;
+#pragma unroll
+          for (int c = 0; c < DP; c += 32) {
+            uint32_t o[32];
+            if (steps > 0) {
+              tc_ld32(from_t + c, o);
+              tc_wait_ld();
+            }
+#pragma unroll
+            for (int k = 0; k < 32; k += 4)
+              if (mine && c + k < a.dim)
+                *reinterpret_cast<float4*>(to + c + k) =
+                    steps == 0 ? make_float4(0.f, 0.f, 0.f, 0.f)
+                               : make_float4(__uint_as_float(o[k]), __uint_as_float(o[k + 1]), __uint_as_float(o[k + 2]), __uint_as_float(o[k + 3]));
+          }
+        } else if (blocks == 1) {
           __nv_bfloat16* to = static_cast<__nv_bfloat16*>(which ? a.dk : a.dv) + at;
           const float by = row >= g.n_k ? 0.f : which ? a.scale : 1.f;
 #pragma unroll
@@ -570,7 +614,15 @@ __global__ void __launch_bounds__(BwdShape<DP>::THREADS, BwdShape<DP>::BLOCKS)
           x.x += u.x; x.y += u.y; x.z += u.z; x.w += u.w;
           y.x += v.x; y.y += v.y; y.z += v.z; y.w += v.w;
         }
-        if (row >= g.k_slot) continue;
+        if (kWindow && chunk >= 0) {  // the part as it is
+          float4* part = reinterpret_cast<float4*>(a.sink_parts + sink_part(a, g.q0, chunk, kv) + ((which ? 0 : (int64_t)a.sink_most) + row) * a.dim + c);
+          if (row < keys.end) {
+            part[0] = x;
+            part[1] = y;
+          }
+          continue;
+        }
+        if (row >= g.k_slot || row < keys.least) continue;
         const float by = which ? a.scale : 1.f;
         __nv_bfloat16* to = static_cast<__nv_bfloat16*>(which ? a.dk : a.dv) + at + c;
         *reinterpret_cast<uint4*>(to) =
@@ -591,7 +643,7 @@ __global__ void __launch_bounds__(BwdShape<DP>::THREADS, BwdShape<DP>::BLOCKS)
   }
 }
 
-template <int DP>
+template <int DP, bool kWindow>
 int launch_bwd(const AttnArgs& a, cudaStream_t stream) {
   using C = BwdShape<DP>;
   static SmemOptIn opt_q, opt_kv;
@@ -607,7 +659,8 @@ int launch_bwd(const AttnArgs& a, cudaStream_t stream) {
   }
   constexpr int STEPS = C::STEP == 128 ? 0 : 1;
   const uint64_t q_blocks = most_tiles(a.rows_q, a.sequences, 128) * a.heads;
-  const uint64_t k_blocks = most_tiles(a.rows_k, a.sequences, 128) * a.kv_heads;
+  const uint64_t of_sinks = (uint64_t)a.sink_chunks * ((a.sink_most + 127) / 128);
+  const uint64_t k_blocks = (of_sinks + most_tiles(a.rows_k, a.sequences, 128)) * a.kv_heads;
   // With fewer than two tiles of keys for each block that fits the GPU (a sample has a tile at least): clusters of as many blocks, up to
   // eight (the portable size), as the query heads of a key head divide into. Backward of 8 samples of 151 ... 5003 rows, 8 / 2 heads of
   // 64, 238 tiles for 296 places: 560 us without, 340 with; of two samples of 3989 and 4600 rows, 16 / 8 heads of 128, 536 tiles for 148
@@ -622,13 +675,13 @@ int launch_bwd(const AttnArgs& a, cudaStream_t stream) {
   }
   if (k_blocks * cluster > 0x7fffffffull) return RMN_ERR_UNSUPPORTED;
   if (q_blocks > 0x7fffffffull || k_blocks > 0x7fffffffull) return RMN_ERR_UNSUPPORTED;
-  RMN_CUDA_TRY(opt_q.apply(reinterpret_cast<const void*>(k_attention_dq<DP>), C::SMEM));
-  RMN_CUDA_TRY(opt_kv.apply(reinterpret_cast<const void*>(k_attention_dkv<DP>), C::SMEM));
-  RMN_CUDA_TRY(launch_overlapped(k_attention_dq<DP>, dim3((uint32_t)q_blocks), dim3(C::THREADS), C::SMEM, stream, q[0], g[0],
+  RMN_CUDA_TRY(opt_q.apply(reinterpret_cast<const void*>(k_attention_dq<DP, kWindow>), C::SMEM));
+  RMN_CUDA_TRY(opt_kv.apply(reinterpret_cast<const void*>(k_attention_dkv<DP, kWindow>), C::SMEM));
+  RMN_CUDA_TRY(launch_overlapped(k_attention_dq<DP, kWindow>, dim3((uint32_t)q_blocks), dim3(C::THREADS), C::SMEM, stream, q[0], g[0],
                                  k[STEPS], v[STEPS], a));
   RMN_LAUNCH_CHECK();
   count_tc_launch();
-  RMN_CUDA_TRY(launch_overlapped_clusters(k_attention_dkv<DP>, (uint32_t)cluster, dim3((uint32_t)(k_blocks * cluster)),
+  RMN_CUDA_TRY(launch_overlapped_clusters(k_attention_dkv<DP, kWindow>, (uint32_t)cluster, dim3((uint32_t)(k_blocks * cluster)),
                                           dim3(C::THREADS), C::SMEM, stream, k[0], v[0], q[STEPS], g[STEPS], a));
   RMN_LAUNCH_CHECK();
   count_tc_launch();
@@ -640,10 +693,11 @@ int launch_bwd(const AttnArgs& a, cudaStream_t stream) {
 
 int attention_tc_backward(const AttnArgs& a, cudaStream_t stream) {
   using namespace tc;
-  if (a.window || a.dim > 128 || !(a.scale > 0.f)) return RMN_ERR_UNSUPPORTED;
+  if (a.dim > 128 || !(a.scale > 0.f)) return RMN_ERR_UNSUPPORTED;
   for (const void* p : {a.fwd_out, (const void*)a.low, (const void*)a.dq, (const void*)a.dk, (const void*)a.dv})
     if ((uintptr_t)p & 15) return RMN_ERR_UNSUPPORTED;
-  return a.dim <= 64 ? launch_bwd<64>(a, stream) : launch_bwd<128>(a, stream);
+  if (a.window) return a.dim <= 64 ? launch_bwd<64, true>(a, stream) : launch_bwd<128, true>(a, stream);
+  return a.dim <= 64 ? launch_bwd<64, false>(a, stream) : launch_bwd<128, false>(a, stream);
 }
 
 }  // namespace rmn

@@ -216,13 +216,13 @@ __device__ __forceinline__ void sum_parts(const float* part, int tx, int ty, int
   }
 }
 
-// o times `by` into rows [0, n) of `to`, `row` elements apart: those of this block of the cluster
+// o times `by` into rows [skip, n) of `to`, `row` elements apart: those of this block of the cluster
 template <typename T, int DP, int BM, int R = SimtShape<DP, BM>::R, int NC = SimtShape<DP, BM>::NC, int CW = SimtShape<DP, BM>::CW>
 __device__ __forceinline__ void store_tile(T* to, int64_t row, int n, int dim, int tx, int ty, int rank, int blocks,
-                                           const float (&o)[R][NC][CW], const float (&by)[R]) {
+                                           const float (&o)[R][NC][CW], const float (&by)[R], int skip = 0) {
 #pragma unroll
   for (int i = 0; i < R; ++i) {
-    if (ty + 16 * i >= n || i % blocks != rank) continue;
+    if (ty + 16 * i >= n || ty + 16 * i < skip || i % blocks != rank) continue;
 #pragma unroll
     for (int g = 0; g < NC; ++g)
 #pragma unroll
@@ -484,9 +484,23 @@ __global__ void __launch_bounds__(kSimtThreads, kBlocksPerSM<DP>) k_attention_si
   after_previous_kernel();
   const int blocks = (int)cluster_size(), rank = (int)cluster_rank(), tile = blockIdx.x / blocks;
   const int kv = tile % a.kv_heads;
-  if (!find_tile<kSimtThreads, TilesOf::kSlots>(a, tile / a.kv_heads, BM, &found, warp_sums)) return;
+  int number = tile / a.kv_heads, chunk = -1, at_tile = 0;
+  if constexpr (kWindow) {  // first the chunks' tiles of the sinks
+    const int sink_tiles = tiles_of(a.sink_most, BM), of_sinks = a.sink_chunks * sink_tiles;
+    if (number < of_sinks) {
+      if (!find_tile<kSimtThreads, TilesOf::kLongQueries>(a, number / sink_tiles, a.sink_chunk, &found, warp_sums)) return;
+      chunk = found.tile;
+      at_tile = number % sink_tiles;
+    }
+    number -= of_sinks;
+  }
+  if (chunk < 0) {
+    if (!find_tile<kSimtThreads, TilesOf::kSlots>(a, number, BM, &found, warp_sums)) return;
+    at_tile = found.tile;
+  }
   const Segment g = found.g;
-  const int first = found.tile * BM;  // the first keys are seen by the most queries
+  const KeyTile keys = key_tile<kWindow, BM>(a, g, at_tile, chunk);
+  const int first = keys.first;  // the first keys are seen by the most queries
   const int rows = min(BM, g.k_slot - first), used = max(0, min(BM, g.n_k - first));
   const int group = a.heads / a.kv_heads;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
@@ -498,21 +512,19 @@ __global__ void __launch_bounds__(kSimtThreads, kBlocksPerSM<DP>) k_attention_si
   clear(dk);
   clear(dv);
   // tiles of queries that see any of these keys, over all heads: every block of the cluster takes its own
-  // (the first key's queries begin first; the last one's end last, unless there are sinks, which are seen to the end)
-  const KeyRows lo = key_rows<kWindow>(a, g, first), hi = key_rows<kWindow>(a, g, first + max(used, 1) - 1);
-  const int from = kWindow ? lo.lo : lo.lo / BM * BM;
-  const int tiles = used > 0 ? max(0, (max(lo.end, hi.end) - from + BM - 1) / BM) : 0;
+  const int from = kWindow ? keys.from : keys.from / BM * BM;
+  const int tiles = keys.used ? (keys.to - from + BM - 1) / BM : 0;
   Share<T, DP, BM> next_q, next_g;
   auto fetch = [&](int turn) {
     const int h = kv * group + turn / max(tiles, 1), i = from + turn % max(tiles, 1) * BM;
-    const int n = turn < tiles * group ? min(BM, g.n_q - i) : 0;
+    const int n = turn < tiles * group ? min(BM, keys.to - i) : 0;
     next_q.fetch(static_cast<const T*>(a.q) + (int64_t)(g.q0 + i) * a.q_row + (int64_t)h * a.q_head, a.q_row, n, a.dim);
     next_g.fetch(static_cast<const T*>(a.grad) + (int64_t)(g.q0 + i) * a.grad_row + (int64_t)h * a.grad_head, a.grad_row, n, a.dim);
   };
   fetch(rank);
   for (int turn = rank; turn < tiles * group; turn += blocks) {
     const int h = kv * group + turn / tiles, i0 = from + turn % tiles * BM;
-    const int n = min(BM, g.n_q - i0);
+    const int n = min(BM, keys.to - i0);
     __syncthreads();
     next_q.put(s_q, 1.f);
     next_g.put(s_g, 1.f);
@@ -529,7 +541,8 @@ __global__ void __launch_bounds__(kSimtThreads, kBlocksPerSM<DP>) k_attention_si
       const RowKeys seen = qi < n ? row_keys<kWindow>(a, g, i0 + qi) : RowKeys{0, 0, 0};
 #pragma unroll
       for (int i = 0; i < R; ++i) {
-        const float p = sees<kWindow>(seen, first, ty + 16 * i) ? expf(s[i][j] - lse) : 0.f;
+        const bool here = !kWindow || (first + ty + 16 * i >= keys.lo && first + ty + 16 * i < keys.end);
+        const float p = here && sees<kWindow>(seen, first, ty + 16 * i) ? expf(s[i][j] - lse) : 0.f;
         s[i][j] = p;
         dp[i][j] = p == 0.f ? 0.f : p * (dp[i][j] - delta);
         s_p[(ty + 16 * i) * S::LP + qi] = p;
@@ -561,9 +574,18 @@ __global__ void __launch_bounds__(kSimtThreads, kBlocksPerSM<DP>) k_attention_si
     by_k[i] = a.scale;
     by_v[i] = 1.f;
   }
-  const int64_t kv_row = (int64_t)a.kv_heads * a.dim, at = (int64_t)(g.k0 + first) * kv_row + (int64_t)kv * a.dim;
-  store_tile<T, DP, BM>(static_cast<T*>(a.dk) + at, kv_row, rows, a.dim, tx, ty, rank, blocks, x, by_k);
-  store_tile<T, DP, BM>(static_cast<T*>(a.dv) + at, kv_row, rows, a.dim, tx, ty, rank, blocks, y, by_v);
+  if (kWindow && chunk >= 0) {  // the parts as they are
+    float* part = a.sink_parts + sink_part(a, g.q0, chunk, kv) + (int64_t)first * a.dim;
+#pragma unroll
+    for (int i = 0; i < R; ++i) by_k[i] = 1.f;
+    store_tile<float, DP, BM>(part, a.dim, keys.end - first, a.dim, tx, ty, rank, blocks, x, by_k);
+    store_tile<float, DP, BM>(part + (int64_t)a.sink_most * a.dim, a.dim, keys.end - first, a.dim, tx, ty, rank, blocks, y, by_v);
+  } else {
+    const int64_t kv_row = (int64_t)a.kv_heads * a.dim, at = (int64_t)(g.k0 + first) * kv_row + (int64_t)kv * a.dim;
+    const int skip = max(0, keys.least - first);
+    store_tile<T, DP, BM>(static_cast<T*>(a.dk) + at, kv_row, rows, a.dim, tx, ty, rank, blocks, x, by_k, skip);
+    store_tile<T, DP, BM>(static_cast<T*>(a.dv) + at, kv_row, rows, a.dim, tx, ty, rank, blocks, y, by_v, skip);
+  }
   if (blocks > 1) cluster_sync();  // no block leaves while another reads its part
 }
 
@@ -615,7 +637,8 @@ int backward_as(const AttnArgs& a, cudaStream_t stream) {
                              blocks_a_tile(a.rows_q, a.heads, rows_seen(a, a.rows_k / samples, BM, (uint64_t)a.sinks), BM, 2),
                              4 * S::tile + S::square, stream);
   if (st != RMN_OK) return st;
-  return launch_simt(k_attention_simt_dkv<T, DP, BM, kWindow>, opt_kv, a, most_tiles(a.rows_k, a.sequences, BM) * a.kv_heads,
+  const uint64_t of_sinks = (uint64_t)a.sink_chunks * ((a.sink_most + BM - 1) / BM);
+  return launch_simt(k_attention_simt_dkv<T, DP, BM, kWindow>, opt_kv, a, (of_sinks + most_tiles(a.rows_k, a.sequences, BM)) * a.kv_heads,
                      blocks_a_tile(a.rows_k, a.kv_heads, rows_seen(a, a.rows_q / samples, BM, 0) * group, BM, 2),
                      4 * S::tile + S::square, stream);
 }
