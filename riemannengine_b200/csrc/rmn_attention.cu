@@ -180,9 +180,9 @@ constexpr int32_t kMostSinks = 1 << 30;
 bool window_ok(int32_t window, int32_t sinks) { return window >= 1 && sinks >= 0 && sinks < kMostSinks; }
 
 // window 0: none
-size_t forward_workspace(const rmn_attention* p, int32_t window, int32_t) {
-  if (!p || p->heads < 1 || p->kv_heads < 1 || p->heads % p->kv_heads || p->dim < 1 || window) return 0;
-  return attention_rows_workspace(p->rows_q, p->rows_k, p->sequences, p->heads, p->kv_heads, p->dim, p->dtype);
+size_t forward_workspace(const rmn_attention* p, int32_t window, int32_t sinks) {
+  if (!p || p->heads < 1 || p->kv_heads < 1 || p->heads % p->kv_heads || p->dim < 1) return 0;
+  return attention_rows_workspace(p->rows_q, p->rows_k, p->sequences, p->heads, p->kv_heads, p->dim, p->dtype, p->causal, window, sinks);
 }
 int forward(const rmn_attention* problem, int32_t window, int32_t sinks, void* d_out, void* d_low, float* d_lse, void* d_workspace,
             size_t workspace_bytes, cudaStream_t stream) {

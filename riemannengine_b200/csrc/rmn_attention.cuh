@@ -384,7 +384,8 @@ int attention_tc_forward(const AttnArgs& a, cudaStream_t stream);  // bf16
 int attention_tc_backward(const AttnArgs& a, cudaStream_t stream);
 int attention_sinks_sum(const AttnArgs& a, int dtype, cudaStream_t stream);  // behind a backward pass that has cut samples
 // few query rows a sample: chunks of the keys, then their sum. Scratch bytes, 0 where this form is not meant for the sizes
-size_t attention_rows_workspace(uint32_t rows_q, uint32_t rows_k, uint32_t sequences, int heads, int kv_heads, int dim, int dtype);
+size_t attention_rows_workspace(uint32_t rows_q, uint32_t rows_k, uint32_t sequences, int heads, int kv_heads, int dim, int dtype,
+                                int causal, int32_t window, int32_t sinks);
 int attention_rows_forward(const AttnArgs& a, int dtype, void* workspace, cudaStream_t stream);
 
 }  // namespace rmn

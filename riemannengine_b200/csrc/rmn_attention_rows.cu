@@ -79,6 +79,14 @@ struct RowsWork {  // scratch, and how the keys are cut
 };
 // Of `tiles` tiles, block b of a head takes those from first_of(b) to first_of(b + 1).
 __device__ __forceinline__ int64_t first_of(const RowsWork& w, int64_t tiles, int64_t block) { return tiles * block / w.blocks; }
+// The tiles of a sample: those of its keys, or with a window those that one of its queries sees.
+template <bool kWindow>
+using RowsWalk = KeyWalk<kWindow, kTileKeys>;
+template <bool kWindow>
+__device__ __forceinline__ int32_t key_tiles(const AttnArgs& a, const Segment& g) {
+  if constexpr (!kWindow) return tiles_of(g.n_k, kTileKeys);
+  return g.n_q > 0 ? RowsWalk<kWindow>(a, g, 0, g.n_q - 1).tiles : 0;
+}
 // The tile that a block begins with, by counts over all samples.
 struct Begin {
   int32_t all;          // tiles; 0 where the samples' rows are out of order
@@ -87,7 +95,7 @@ struct Begin {
   int32_t tile, tiles;
 };
 // All threads of the block count: each a run of samples, a scan over the block places them.
-template <int kThreads>
+template <int kThreads, bool kWindow>
 __device__ __forceinline__ void find_begin(const AttnArgs& a, const RowsWork& w, int block, Begin* found, int32_t* warp_sums, bool* in_order) {
   const uint32_t per = (a.sequences + kThreads - 1) / kThreads;
   const uint32_t lo = min(threadIdx.x * per, a.sequences), hi = min(lo + per, a.sequences);
@@ -96,7 +104,7 @@ __device__ __forceinline__ void find_begin(const AttnArgs& a, const RowsWork& w,
   bool descends = false;
   for (uint32_t s = lo; s < hi; ++s) {
     g = segment(a, s, &descends);
-    mine = add_tiles(mine, tiles_of(g.n_k, kTileKeys));
+    mine = add_tiles(mine, key_tiles<kWindow>(a, g));
   }
   int32_t first, all;
   scan_block<kThreads>(mine, warp_sums, first, all, descends);
@@ -105,7 +113,7 @@ __device__ __forceinline__ void find_begin(const AttnArgs& a, const RowsWork& w,
   if (*in_order && want >= first && want - first < mine) {
     for (uint32_t s = lo; s < hi; ++s) {
       if (hi - lo > 1) g = segment(a, s);
-      const int32_t tiles = tiles_of(g.n_k, kTileKeys);
+      const int32_t tiles = key_tiles<kWindow>(a, g);
       if (want - first < tiles) {
         *found = {all, g, s, want - first, tiles};
         break;
@@ -127,6 +135,7 @@ __device__ __forceinline__ size_t part_at(const AttnArgs& a, const RowsWork& w, 
 }
 
 // A run of tiles as pieces of samples: the same walk by the warp that copies and those that compute.
+template <bool kWindow>
 struct Piece {
   Segment g;
   uint32_t s;
@@ -168,7 +177,7 @@ struct Piece {
     do {
       if (++s >= a.sequences) return false;
       g = segment(a, s);
-      tiles = tiles_of(g.n_k, kTileKeys);
+      tiles = key_tiles<kWindow>(a, g);
     } while (tiles == 0);
     tile = 0;
     first = false;
@@ -195,13 +204,13 @@ __device__ __forceinline__ void store_row(const AttnArgs& a, size_t at, int c, f
 // behind which lane i has the score of key i / R and row i % R. What is where makes every exchange one shuffle without a choice: lane i
 // has the rows (and goes through the keys) in an order of its own, number r being row r ^ (i % R), number k key k ^ (i / R); so the number
 // that it gives at distance n is the one that lane i ^ n keeps, and the weight that it needs for number (k, r) is in lane i ^ (k R + r).
-template <int DP, int R, int K>
+template <int DP, int R, int K, bool kWindow>
 struct Rows32 {
   static constexpr int W = DP == 32 ? 2 : 4, DL = DP / W, KG = 32 / DL;
   static constexpr int KEYS = K / KG, KB = DL / R, NB = KEYS / KB;  // keys of a lane's half, of a batch of scores; batches
   Pair q[R / 2][W], o[R / 2][W];                                    // of two rows each
   float m, l;                                                       // of row lane % R; l: the lane's part
-  int see;
+  RowKeys see;
 
   static __device__ __forceinline__ int ch() { return (threadIdx.x & 31) % DL; }
   static __device__ __forceinline__ int half() { return (threadIdx.x & 31) / DL; }
@@ -249,7 +258,7 @@ struct Rows32 {
       }
     }
     const int mine = r0 + ch() % R;
-    see = mine < rows ? visible_keys(g, mine / group, a.causal) : 0;
+    see = mine < rows ? row_keys<kWindow>(a, g, mine / group) : RowKeys{0, 0, 0};
     m = -CUDART_INF_F;
     l = 0.f;
   }
@@ -287,10 +296,10 @@ struct Rows32 {
       s[b] = x + from(y, 1);
     }
     float top = -CUDART_INF_F;
-    const int left = min(see, hi) - k0 - half() * KEYS - key_of(0);  // keys that the row sees from the lane's first one on
+    const int at = k0 + half() * KEYS + key_of(0);  // the lane's first key
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-      if (b * KB >= left) s[b] = -CUDART_INF_F;
+      if (!sees<kWindow>(see, at, b * KB)) s[b] = -CUDART_INF_F;
       top = fmaxf(top, s[b]);
     }
 #pragma unroll
@@ -370,7 +379,7 @@ struct Rows32 {
   }
 };
 
-template <typename T, int DP>
+template <typename T, int DP, bool kWindow>
 __global__ void __launch_bounds__(RowsShape<T, DP>::THREADS, RowsShape<T, DP>::BLOCKS)
     k_attention_rows(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const AttnArgs a,
                      const RowsWork w) {
@@ -383,7 +392,7 @@ __global__ void __launch_bounds__(RowsShape<T, DP>::THREADS, RowsShape<T, DP>::B
   constexpr int LD = DP + 4, WARPS = C::WARPS;
   __shared__ int s_timed_out;
   __shared__ Begin found;
-  __shared__ Piece s_piece[WARPS + 1];
+  __shared__ Piece<kWindow> s_piece[WARPS + 1];
   __shared__ int32_t warp_sums[WARPS + 1];
   __shared__ float s_m[WARPS][16], s_l[WARPS][16];
   extern __shared__ uint8_t smem_raw[];
@@ -405,7 +414,7 @@ __global__ void __launch_bounds__(RowsShape<T, DP>::THREADS, RowsShape<T, DP>::B
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gr = lane >> 2, c = lane & 3;
   const int group = a.heads / a.kv_heads;
   bool in_order;
-  find_begin<C::THREADS>(a, w, block, &found, warp_sums, &in_order);
+  find_begin<C::THREADS, kWindow>(a, w, block, &found, warp_sums, &in_order);
   if (kv == 0 && threadIdx.x == 0) w.starts[3 * block + 2] = found.all;
   if (!in_order) {  // rows of several samples: no bound on the work. The call is reported; its outputs are those of rows without keys
     const uint64_t rows = (uint64_t)a.rows_q * a.heads, first = (uint64_t)blockIdx.x * C::THREADS + threadIdx.x;
@@ -437,7 +446,7 @@ __global__ void __launch_bounds__(RowsShape<T, DP>::THREADS, RowsShape<T, DP>::B
   }
   if (want == end) return;
   // in shared memory, a copy for every warp: registers are short
-  Piece& piece = s_piece[warp];
+  Piece<kWindow>& piece = s_piece[warp];
   if (lane == 0) {
     piece.g = found.g;
     piece.s = found.s;
@@ -459,6 +468,7 @@ __global__ void __launch_bounds__(RowsShape<T, DP>::THREADS, RowsShape<T, DP>::B
     if (lane == 0) {
       for (bool more = true; more && !timed_out; more = piece.next(a, w, found.all, block)) {
         if (piece.skip) continue;
+        const RowsWalk<kWindow> keys(a, piece.g, 0, piece.g.n_q - 1);
         for (uint32_t r = piece.row; r < (uint32_t)(group * piece.g.n_q) && !timed_out; r += piece.step) {
           for (int t = piece.from; t < piece.to; ++t, ++it) {
             const uint32_t s = it % C::SLOTS;
@@ -467,8 +477,8 @@ __global__ void __launch_bounds__(RowsShape<T, DP>::THREADS, RowsShape<T, DP>::B
 #pragma unroll
             for (int b = 0; b < C::LINES; ++b) {
               const uint32_t at = ring + s * C::SLOT + b * C::LINE;
-              tma_load_3d(at, &map_k, &full[s], b * 8 * E, kv, piece.g.k0 + t * kTileKeys);
-              tma_load_3d(at + C::HALF, &map_v, &full[s], b * 8 * E, kv, piece.g.k0 + t * kTileKeys);
+              tma_load_3d(at, &map_k, &full[s], b * 8 * E, kv, piece.g.k0 + keys.key(t));
+              tma_load_3d(at + C::HALF, &map_v, &full[s], b * 8 * E, kv, piece.g.k0 + keys.key(t));
             }
           }
         }
@@ -494,6 +504,7 @@ __global__ void __launch_bounds__(RowsShape<T, DP>::THREADS, RowsShape<T, DP>::B
     const Segment& g = piece.g;
     const int hi = g.n_k, first_tile = piece.from, last_tile = piece.to;
     const int rows = group * g.n_q;
+    const RowsWalk<kWindow> keys(a, g, 0, g.n_q - 1);
     for (uint32_t from = piece.row; from < (uint32_t)rows && !timed_out; from += piece.step) {
       const int r0 = (int)from;
       // the tiles of this piece, as f(keys and values of the tile, its first key, what releases its place)
@@ -505,7 +516,7 @@ __global__ void __launch_bounds__(RowsShape<T, DP>::THREADS, RowsShape<T, DP>::B
             timed_out = true;
             break;
           }
-          f(smem + slot * C::SLOT, t64 * kTileKeys, [&] {
+          f(smem + slot * C::SLOT, keys.key(t64), [&] {
             __syncwarp();
             if (lane == 0) mbar_arrive(&empty[slot]);
           });
@@ -532,7 +543,7 @@ __global__ void __launch_bounds__(RowsShape<T, DP>::THREADS, RowsShape<T, DP>::B
         auto fp32 = [&](auto rows_at_once, auto keys_at_once) {
           constexpr int R = decltype(rows_at_once)::value, K = decltype(keys_at_once)::value;
           constexpr int SHARE = kTileKeys / K, ROWS = R * WARPS / SHARE;  // warps that have a row; rows of all
-          using Rows = Rows32<DP, R, K>;
+          using Rows = Rows32<DP, R, K, kWindow>;
           const int mine0 = warp / SHARE * R, part = warp % SHARE;
           Rows x;
           x.begin(a, g, kv, group, r0 + mine0, rows);
@@ -564,13 +575,13 @@ __global__ void __launch_bounds__(RowsShape<T, DP>::THREADS, RowsShape<T, DP>::B
       } else {
         // q of rows gr and gr + 8 as operands
         uint32_t q[2 * KC][4];
-        int see[2];
+        RowKeys see[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int r = r0 + gr + 8 * e;
           const bool ok = r < rows;
           const int i = ok ? r / group : 0, h = kv * group + (ok ? r % group : 0);
-          see[e] = ok ? visible_keys(g, i, a.causal) : 0;
+          see[e] = ok ? row_keys<kWindow>(a, g, i) : RowKeys{0, 0, 0};
           const T* from = static_cast<const T*>(a.q) + (int64_t)(g.q0 + i) * a.q_row + (int64_t)h * a.q_head;
 #pragma unroll
           for (int b = 0; b < KC; ++b) {
@@ -629,7 +640,7 @@ __global__ void __launch_bounds__(RowsShape<T, DP>::THREADS, RowsShape<T, DP>::B
 #pragma unroll
               for (int k = 0; k < 2; ++k) {
                 float& x = s[t][2 * e + k];
-                x = k0 + t * 8 + 2 * c + k < min(see[e], hi) ? x * scale : -CUDART_INF_F;
+                x = sees<kWindow>(see[e], k0, t * 8 + 2 * c + k) ? x * scale : -CUDART_INF_F;
                 top = fmaxf(top, x);
               }
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
@@ -753,7 +764,7 @@ __global__ void __launch_bounds__(RowsShape<T, DP>::THREADS, RowsShape<T, DP>::B
 
 // Sums the pieces of the sample that the run of block b begins inside of, for one head and every gridDim.y-th row, each of eight
 // warps every eighth piece; the first of several blocks that begin inside of one sample does it.
-template <typename T>
+template <typename T, bool kWindow>
 __global__ void __launch_bounds__(kSumThreads) k_attention_rows_sum(const AttnArgs a, const RowsWork w) {
   __shared__ float s_m[kSumWarps], s_l[kSumWarps], s_o[kSumWarps][128];
   after_previous_kernel();
@@ -764,7 +775,7 @@ __global__ void __launch_bounds__(kSumThreads) k_attention_rows_sum(const AttnAr
   if (all <= 0 || first_of(w, all, block) == at0 || first_of(w, all, block - 1) > at0) return;
   const Segment g = segment(a, s);
   if (g.n_q > w.most_queries) return;  // stored by the first kernel
-  const int32_t end = at0 + tiles_of(g.n_k, kTileKeys);
+  const int32_t end = at0 + key_tiles<kWindow>(a, g);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int first = block - 1;
   const bool whole = first_of(w, all, first) == at0;  // its run begins with this sample
@@ -836,19 +847,24 @@ RowsSizes rows_sizes(uint32_t rows_k, uint32_t sequences, int heads, int kv_head
   return z;
 }
 
-template <typename T, int DP>
-int launch_rows(const CUtensorMap& k, const CUtensorMap& v, const AttnArgs& a, const RowsWork& w, cudaStream_t stream) {
+template <typename T, int DP, bool kWindow>
+int launch_rows_as(const CUtensorMap& k, const CUtensorMap& v, const AttnArgs& a, const RowsWork& w, cudaStream_t stream) {
   constexpr size_t smem = RowsShape<T, DP>::SMEM;
   static SmemOptIn opt_in;
-  RMN_CUDA_TRY(opt_in.apply(reinterpret_cast<const void*>(k_attention_rows<T, DP>), smem));
-  RMN_CUDA_TRY(launch_overlapped(k_attention_rows<T, DP>, dim3((uint32_t)(w.blocks * a.kv_heads)), dim3(RowsShape<T, DP>::THREADS), smem, stream, k, v, a, w));
+  RMN_CUDA_TRY(opt_in.apply(reinterpret_cast<const void*>(k_attention_rows<T, DP, kWindow>), smem));
+  RMN_CUDA_TRY(launch_overlapped(k_attention_rows<T, DP, kWindow>, dim3((uint32_t)(w.blocks * a.kv_heads)), dim3(RowsShape<T, DP>::THREADS), smem, stream, k, v, a, w));
   RMN_LAUNCH_CHECK();
   if (w.blocks == 1) return RMN_OK;  // every sample is one piece
   const uint32_t rows = (a.rows_q + a.sequences - 1) / a.sequences;  // of a sample, on average
-  RMN_CUDA_TRY(launch_overlapped(k_attention_rows_sum<T>, dim3((uint32_t)(w.blocks - 1) * (uint32_t)a.heads, rows),
+  RMN_CUDA_TRY(launch_overlapped(k_attention_rows_sum<T, kWindow>, dim3((uint32_t)(w.blocks - 1) * (uint32_t)a.heads, rows),
                                  dim3(kSumThreads), 0, stream, a, w));
   RMN_LAUNCH_CHECK();
   return RMN_OK;
+}
+
+template <typename T, int DP>
+int launch_rows(const CUtensorMap& k, const CUtensorMap& v, const AttnArgs& a, const RowsWork& w, cudaStream_t stream) {
+  return a.window ? launch_rows_as<T, DP, true>(k, v, a, w, stream) : launch_rows_as<T, DP, false>(k, v, a, w, stream);
 }
 
 }  // namespace
@@ -874,13 +890,23 @@ bool rows_take_less(uint32_t rows_q, uint32_t rows_k, uint32_t sequences, int he
 }
 }  // namespace
 
-size_t attention_rows_workspace(uint32_t rows_q, uint32_t rows_k, uint32_t sequences, int heads, int kv_heads, int dim, int dtype) {
+namespace {
+// Keys that the queries of all samples see together, at most, where a sample has `rows` of them.
+uint32_t keys_seen(uint32_t rows_k, uint32_t sequences, uint64_t rows, int causal, int32_t window, int32_t sinks) {
+  if (!window) return rows_k;
+  return (uint32_t)std::min<uint64_t>(rows_k, ((uint64_t)window * (causal ? 1 : 2) + rows + (uint64_t)sinks) * sequences);
+}
+}  // namespace
+
+size_t attention_rows_workspace(uint32_t rows_q, uint32_t rows_k, uint32_t sequences, int heads, int kv_heads, int dim, int dtype,
+                                int causal, int32_t window, int32_t sinks) {
   if (!rows_q || !rows_k || !sequences || dim > 128 || dim % (dtype == RMN_F32 ? 4 : 8)) return 0;
-  const uint64_t rows = ((uint64_t)rows_q + sequences - 1) / sequences * (heads / kv_heads);
+  const uint64_t queries = ((uint64_t)rows_q + sequences - 1) / sequences, rows = queries * (heads / kv_heads);
   if (rows > kMostRows) return 0;
-  if (!rows_take_less(rows_q, rows_k, sequences, heads, kv_heads, dim, dtype)) return 0;
+  const uint32_t keys = keys_seen(rows_k, sequences, queries, causal, window, sinks);
+  if (!rows_take_less(rows_q, keys, sequences, heads, kv_heads, dim, dtype)) return 0;
   if ((uint64_t)rows_q * heads > 0x7fffffffull) return 0;
-  return rows_sizes(rows_k, sequences, heads, kv_heads, dim, dtype).total;
+  return rows_sizes(keys, sequences, heads, kv_heads, dim, dtype).total;
 }
 
 int attention_rows_forward(const AttnArgs& a, int dtype, void* workspace, cudaStream_t stream) {
@@ -890,7 +916,8 @@ int attention_rows_forward(const AttnArgs& a, int dtype, void* workspace, cudaSt
   if (!make_head_map(&k, a.k, a.rows_k, a.kv_heads, a.dim, a.k_row, a.k_head, kTileKeys, elem) ||
       !make_head_map(&v, a.v, a.rows_k, a.kv_heads, a.dim, a.v_row, a.v_head, kTileKeys, elem))
     return RMN_ERR_UNSUPPORTED;
-  const RowsSizes z = rows_sizes(a.rows_k, a.sequences, a.heads, a.kv_heads, a.dim, dtype);
+  const uint32_t keys = keys_seen(a.rows_k, a.sequences, ((uint64_t)a.rows_q + a.sequences - 1) / a.sequences, a.causal, a.window, a.sinks);
+  const RowsSizes z = rows_sizes(keys, a.sequences, a.heads, a.kv_heads, a.dim, dtype);
   char* base = static_cast<char*>(workspace);
   const RowsWork w = {z.blocks, z.most_queries, reinterpret_cast<int32_t*>(base), reinterpret_cast<float*>(base + z.sums_at),
                       reinterpret_cast<float*>(base + z.parts_at)};
