@@ -10,23 +10,27 @@
 // where a turn is full. No bits are lost however far the position is, and no range has to be reduced. What is left of a turn is cut into
 // quarters; sine and cosine of up to an eighth either way are their Taylor polynomials (off by less than 2e-9).
 //
-// Bound by memory: every value is read once and written once. A head's channels lie over L lanes (a power of two), each with units of V
-// pairs, 16 bytes a load where sizes and alignment allow. Such a group takes a row's heads one after the other, U of them in flight,
-// so that the angles of a row are made once; few rows are dealt out to several groups a row, each with every second, fourth ... head. The
-// norm's sums go over the L lanes. dw is summed in registers over the rows that a thread visits, over the block in a fixed order and over
-// the blocks by a second kernel: no atomics, the same bits every time.
+// Bound by memory: every value is read once and written once. A block works on queries or on keys. A head's channels lie over L lanes (a
+// power of two), each with units of V pairs, 16 bytes a load where sizes and alignment allow; the L lanes are a group. A warp has one or
+// several rows, each with one or several groups that take the row's heads in turn, U at a time; the next ones are asked for before these
+// are worked on, across rows. The warp makes the angles of its rows once, every lane a share of them, and hands them on through shared
+// memory. The norm's sums go over the L lanes. dw is summed in registers over the rows that a thread visits, over the block in a
+// fixed order and over the blocks by a second kernel: no atomics, the same bits every time.
 #include "rmn_common.cuh"
+#include "rmn_pair.cuh"
 
 #include <cuda_bf16.h>
 
 #include <algorithm>
+#include <type_traits>
 
 namespace rmn {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr uint32_t kMostBackwardBlocks = 148 * 4;
 constexpr int kMostAxes = 8;
+constexpr int kMostDim = 256;
 
 struct Heads {  // [rows, heads, dim]
   const void* x;
@@ -36,18 +40,21 @@ struct Heads {  // [rows, heads, dim]
   const void* weight;  // NULL: ones
   void* out;           // no gaps; backward: the gradient of x
   int heads;
+  // layout: groups of a row within a warp (a power of two), warps of a row, blocks
+  int groups, warps;
+  uint32_t blocks;
 };
 struct RotaryArgs {
   Heads part[2];  // queries, keys (0 heads: none)
   uint32_t rows;
-  int dim, pairs, lanes, per_row;  // lanes of a head, groups of lanes of a row
+  int dim, pairs, lanes;  // lanes of a head
   const int32_t* positions;
   int64_t position_row, position_axis;
   const double* frequencies;
   int ends[kMostAxes];  // the pair behind the last one of an axis
   int weight_bf16, back;  // back: turned the other way (without a norm the gradient is nothing else)
   float eps;
-  float* sums;  // backward: [block][2][dim]
+  float* sums;  // backward: [block][dim], those of the queries first
 };
 
 template <typename T, int V>
@@ -103,319 +110,482 @@ __device__ __forceinline__ void turn_of(int32_t position, uint64_t fraction, flo
   s = quarter & 2u ? -b : b;
 }
 
-// A unit: V pairs of a lane, as 2 V numbers in two loads of V channels. Halves: the first numbers of the pairs, then the second ones.
-template <int V, bool kNext>  // kNext: a pair's numbers are neighbours
+// The arithmetic is on pairs of fp32 numbers, of two neighbouring pairs of channels; units of one pair use plain floats in their place.
+__device__ __forceinline__ float add(float a, float b) { return a + b; }
+__device__ __forceinline__ float mul(float a, float b) { return a * b; }
+__device__ __forceinline__ float fma(float a, float b, float c) { return fmaf(a, b, c); }
+__device__ __forceinline__ float total(float a) { return a; }
+template <int V>
+using Number = std::conditional_t<V == 1, float, Pair>;
+template <int V>
+constexpr int kNumbers = V == 1 ? 1 : V / 2;
+template <int V>
+__device__ __forceinline__ Number<V> splat(float x) {
+  if constexpr (V == 1) return x;
+  else return make_pair(x, x);
+}
+
+// A unit: V pairs of channels, as numbers a (the first of every pair) and b (the second), from two loads of V channels: the first and the
+// second ones, or (kNext: a pair's channels are neighbours) the pairs themselves.
+template <int V>
 struct Unit {
-  int lo, hi;  // channels of the two loads
-  __device__ __forceinline__ Unit(int u, int pairs, int dim) {
-    if (kNext) {
-      lo = 2 * u * V;
-      hi = lo + V;
-    } else if (u * V < pairs) {
-      lo = u * V;
-      hi = lo + pairs;
-    } else {  // what stays as it is
-      lo = u * V + pairs;
-      hi = lo + dim / 2 - pairs;
+  Number<V> a[kNumbers<V>], b[kNumbers<V>];
+};
+template <typename T, int V, bool kNext>
+__device__ __forceinline__ Unit<V> unit_of(const Pack<T, V> (&p)[2]) {
+  Unit<V> u;
+  if constexpr (V == 1) {
+    u.a[0] = number(p[0].v[0]);
+    u.b[0] = number(p[1].v[0]);
+  } else {
+    auto at = [&](int i) { return number(p[i / V].v[i % V]); };
+#pragma unroll
+    for (int k = 0; k < V / 2; ++k) {
+      u.a[k] = kNext ? make_pair(at(4 * k), at(4 * k + 2)) : make_pair(at(2 * k), at(2 * k + 1));
+      u.b[k] = kNext ? make_pair(at(4 * k + 1), at(4 * k + 3)) : make_pair(at(V + 2 * k), at(V + 2 * k + 1));
     }
   }
-  static constexpr int first(int j) { return kNext ? 2 * j : j; }
-  static constexpr int second(int j) { return kNext ? 2 * j + 1 : V + j; }
-};
-
-template <int V, bool kNext>
-__device__ __forceinline__ void rotate(const float (&x)[2 * V], const float (&c)[V], const float (&s)[V], int turned, float (&y)[2 * V]) {
+  return u;
+}
+template <typename T, int V, bool kNext>
+__device__ __forceinline__ void store_unit(T* lo, T* hi, const Unit<V>& u) {
+  Pack<T, V> p[2];
+  if constexpr (V == 1) {
+    p[0].v[0] = rounded<T>(u.a[0]);
+    p[1].v[0] = rounded<T>(u.b[0]);
+  } else {
+    auto put = [&](int i, float x, float y) {  // channels i and i + 1 of the two loads
+      if constexpr (sizeof(T) == 4) {
+        p[i / V].v[i % V] = x;
+        p[i / V].v[i % V + 1] = y;
+      } else {
+        reinterpret_cast<__nv_bfloat162*>(&p[i / V])[i % V / 2] = __floats2bfloat162_rn(x, y);
+      }
+    };
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    constexpr auto first = Unit<V, kNext>::first;
-    constexpr auto second = Unit<V, kNext>::second;
-    const float a = x[first(j)], b = x[second(j)];
-    y[first(j)] = j < turned ? fmaf(a, c[j], -(b * s[j])) : a;
-    y[second(j)] = j < turned ? fmaf(b, c[j], a * s[j]) : b;
+    for (int k = 0; k < V / 2; ++k) {
+      float a0, a1, b0, b1;
+      parts(u.a[k], a0, a1);
+      parts(u.b[k], b0, b1);
+      put(kNext ? 4 * k : 2 * k, a0, kNext ? b0 : a1);
+      put(kNext ? 4 * k + 2 : V + 2 * k, kNext ? a1 : b0, b1);
+    }
   }
+  *reinterpret_cast<Pack<T, V>*>(lo) = p[0];
+  *reinterpret_cast<Pack<T, V>*>(hi) = p[1];
 }
 
-// The angles of a lane's pairs.
+// What a lane does: its units' channels, its rows and heads.
+template <int V, int NU, bool kNext>
+struct Lane {
+  int at, group, row_of_warp;  // lane of its head, group of its row, row of the warp
+  int lo[NU], hi[NU];          // channels of the two loads
+  int turned[NU];              // pairs of the unit that turn
+  bool has[NU];
+  __device__ __forceinline__ Lane(const RotaryArgs& a, const Heads& p) {
+    const int lane = threadIdx.x & 31;
+    at = lane & (a.lanes - 1);
+    group = lane / a.lanes & (p.groups - 1);
+    row_of_warp = lane / (a.lanes * p.groups);
+#pragma unroll
+    for (int i = 0; i < NU; ++i) {
+      const int u = at + i * a.lanes, first = u * V;
+      has[i] = first < a.dim / 2;
+      turned[i] = min(max(a.pairs - first, 0), V);
+      if (kNext) {
+        lo[i] = 2 * first;
+        hi[i] = lo[i] + V;
+      } else if (first < a.pairs) {
+        lo[i] = first;
+        hi[i] = first + a.pairs;
+      } else {  // what stays as it is
+        lo[i] = first + a.pairs;
+        hi[i] = first + a.dim / 2;
+      }
+    }
+  }
+};
+
+// The tables of a block, [lane's number of four (or fewer) pairs][unit][pair], so that the lanes of a head read neighbouring words:
+// w of the first and of the second channels, and for each warp cosines and sines of its rows.
 template <int V, int NU>
-struct Angles {
-  uint64_t fraction[NU][V];
-  int axis[NU][V];
-  int turned[NU];  // pairs of the unit that turn
-  __device__ __forceinline__ void begin(const RotaryArgs& a, int lane) {
+struct alignas(16) Tables {
+  static constexpr int W = V < 4 ? V : 4, PAIRS = 32 * NU * V;  // words of a read; pairs of a warp's rows at most
+  float w[2][kMostDim / 2];
+  uint64_t fraction[kMostDim / 2];
+  int axis[kMostDim / 2];  // -1: does not turn
+  float turns[kWarps][2][PAIRS];
+  // where pair p is, of `units` units
+  static __device__ __forceinline__ int place(int p, int units) { return (p % V / W * units + p / V) * W + p % W; }
+  static __device__ __forceinline__ void read(const float* from, int units, int u, Number<V> (&out)[kNumbers<V>]) {
 #pragma unroll
-    for (int i = 0; i < NU; ++i) {
-      const int p0 = (lane + i * a.lanes) * V;
-      turned[i] = min(max(a.pairs - p0, 0), V);
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        fraction[i][j] = p0 + j < a.pairs ? fraction_of_turn(__ldg(a.frequencies + p0 + j)) : 0;
-        axis[i][j] = 0;
-#pragma unroll
-        for (int k = 0; k < kMostAxes - 1; ++k) axis[i][j] += p0 + j >= a.ends[k] && p0 + j < a.pairs ? 1 : 0;
+    for (int k = 0; k < V / W; ++k) {
+      const float* p = from + (k * units + u) * W;
+      if constexpr (W == 4) {
+        const float4 v = *reinterpret_cast<const float4*>(p);
+        out[2 * k] = make_pair(v.x, v.y);
+        out[2 * k + 1] = make_pair(v.z, v.w);
+      } else if constexpr (W == 2) {
+        const float2 v = *reinterpret_cast<const float2*>(p);
+        out[k] = make_pair(v.x, v.y);
+      } else {
+        out[k] = *p;
       }
     }
   }
-  __device__ __forceinline__ void of_row(const RotaryArgs& a, uint64_t row, float (&c)[NU][V], float (&s)[NU][V]) const {
-    const int32_t* at = a.positions + (int64_t)row * a.position_row;
-#pragma unroll
-    for (int i = 0; i < NU; ++i) {
-      int32_t place = 0;
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        if (j < turned[i] && (j == 0 || axis[i][j] != axis[i][j - 1])) place = __ldg(at + (int64_t)axis[i][j] * a.position_axis);
-        turn_of(place, fraction[i][j], c[i][j], s[i][j]);
-        if (a.back) s[i][j] = -s[i][j];
+  __device__ __forceinline__ void begin(const RotaryArgs& a, const void* weight, bool next, bool norm) {
+    const int units = a.lanes * NU;
+    for (int p = threadIdx.x; p < units * V; p += kThreads) {
+      if (norm) {
+        int lo = next ? 2 * p : p < a.pairs ? p : p + a.pairs;
+        int hi = next ? 2 * p + 1 : p < a.pairs ? p + a.pairs : p + a.dim / 2;
+        const bool here = weight && p < a.dim / 2;
+        auto of = [&](int c) {
+          return !here ? 1.f : a.weight_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(weight)[c]) : static_cast<const float*>(weight)[c];
+        };
+        w[0][place(p, units)] = of(lo);
+        w[1][place(p, units)] = of(hi);
       }
-    }
-  }
-};
-
-// w of a lane's channels
-template <int V, bool kNext, int NU>
-__device__ __forceinline__ void weights(const RotaryArgs& a, const void* w, int lane, float (&out)[NU][2 * V]) {
-#pragma unroll
-  for (int i = 0; i < NU; ++i) {
-    const int u = lane + i * a.lanes;
-    const Unit<V, kNext> unit(u, a.pairs, a.dim);
-#pragma unroll
-    for (int j = 0; j < 2 * V; ++j) {
-      const int ch = j < V ? unit.lo + j : unit.hi + j - V;
-      out[i][j] = !w || u * V >= a.dim / 2 ? 1.f
-                  : a.weight_bf16          ? __bfloat162float(static_cast<const __nv_bfloat16*>(w)[ch])
-                                           : static_cast<const float*>(w)[ch];
-    }
-  }
-}
-// the sum over the lanes of a head; every one gets it
-__device__ __forceinline__ float over_lanes(float v, int lanes, uint32_t mask) {
-  for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(mask, v, o);
-  return v;
-}
-
-template <typename T, int V, int NU>
-__device__ __forceinline__ void load_units(const T* from, const int (&lo)[NU], const int (&hi)[NU], bool here, const bool (&has)[NU],
-                                           Pack<T, V> (&x)[NU][2]) {
-#pragma unroll
-  for (int i = 0; i < NU; ++i)
-    if (here && has[i]) {
-      x[i][0] = load_pack<T, V>(from + lo[i]);
-      x[i][1] = load_pack<T, V>(from + hi[i]);
-    }
-}
-
-template <typename T, int V, int NU, bool kNext, bool kNorm>
-__global__ void __launch_bounds__(kThreads) k_rotary(const __grid_constant__ RotaryArgs a) {
-  constexpr int U = NU == 1 ? 4 : 2;  // heads in flight
-  after_previous_kernel();
-  const int lane = threadIdx.x & (a.lanes - 1);
-  const uint64_t group = ((uint64_t)blockIdx.x * kThreads + threadIdx.x) / a.lanes, groups = (uint64_t)gridDim.x * (kThreads / a.lanes);
-  const uint32_t mask = a.lanes == 32 ? 0xffffffffu : ((1u << a.lanes) - 1u) << (threadIdx.x & 31 & ~(a.lanes - 1));
-  const int head0 = (int)(group % a.per_row);
-  const float inv_dim = 1.f / (float)a.dim;
-  Angles<V, NU> angles;
-  angles.begin(a, lane);
-  int lo[NU], hi[NU];
-  bool has[NU];
-#pragma unroll
-  for (int i = 0; i < NU; ++i) {
-    const Unit<V, kNext> unit(lane + i * a.lanes, a.pairs, a.dim);
-    lo[i] = unit.lo;
-    hi[i] = unit.hi;
-    has[i] = (lane + i * a.lanes) * V < a.dim / 2;
-  }
-  float w[2][NU][2 * V];
-  if constexpr (kNorm) {
-    weights<V, kNext, NU>(a, a.part[0].weight, lane, w[0]);
-    weights<V, kNext, NU>(a, a.part[1].weight, lane, w[1]);
-  }
-  for (uint64_t row = group / a.per_row; row < a.rows; row += groups / a.per_row) {
-    float c[NU][V], s[NU][V];
-    angles.of_row(a, row, c, s);
-#pragma unroll
-    for (int which = 0; which < 2; ++which) {
-      const Heads& p = a.part[which];
-      const T* from = static_cast<const T*>(p.x) + (int64_t)row * p.row;
-      T* to = static_cast<T*>(p.out) + row * (uint64_t)p.heads * a.dim;
-      for (int h0 = head0; h0 < p.heads; h0 += U * a.per_row) {
-        Pack<T, V> raw[U][NU][2];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int h = h0 + u * a.per_row;
-          load_units<T, V, NU>(from + (int64_t)h * p.head, lo, hi, h < p.heads, has, raw[u]);
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int h = h0 + u * a.per_row;
-          if (h >= p.heads) break;
-          float x[NU][2 * V];
-          float sum = 0.f;
-#pragma unroll
-          for (int i = 0; i < NU; ++i)
-#pragma unroll
-            for (int j = 0; j < 2 * V; ++j) {
-              x[i][j] = has[i] ? number(raw[u][i][j / V].v[j % V]) : 0.f;
-              if constexpr (kNorm) sum = fmaf(x[i][j], x[i][j], sum);
-            }
-          if constexpr (kNorm) {
-            const float inv = 1.f / sqrtf(over_lanes(sum, a.lanes, mask) * inv_dim + a.eps);
-#pragma unroll
-            for (int i = 0; i < NU; ++i)
-#pragma unroll
-              for (int j = 0; j < 2 * V; ++j) x[i][j] = x[i][j] * inv * w[which][i][j];
-          }
-#pragma unroll
-          for (int i = 0; i < NU; ++i) {
-            if (!has[i]) continue;
-            float y[2 * V];
-            rotate<V, kNext>(x[i], c[i], s[i], angles.turned[i], y);
-            Pack<T, V> o[2];
-#pragma unroll
-            for (int j = 0; j < 2 * V; ++j) o[j / V].v[j % V] = rounded<T>(y[j]);
-            *reinterpret_cast<Pack<T, V>*>(to + (int64_t)h * a.dim + lo[i]) = o[0];
-            *reinterpret_cast<Pack<T, V>*>(to + (int64_t)h * a.dim + hi[i]) = o[1];
-          }
-        }
+      int of = -1;
+      if (p < a.pairs) {
+        of = 0;
+        for (int k = 0; k < kMostAxes - 1; ++k) of += p >= a.ends[k] ? 1 : 0;
+        fraction[p] = fraction_of_turn(__ldg(a.frequencies + p));
       }
-    }
-  }
-}
-
-// dx of the norm and the rotation (a.back is set: gradients are turned back), and a block's part of dw of both.
-template <typename T, int V, int NU, bool kNext>
-__global__ void __launch_bounds__(kThreads) k_rotary_backward(const __grid_constant__ RotaryArgs a) {
-  constexpr int U = NU == 1 ? 2 : 1;
-  __shared__ float block_sums[2 * 256];
-  after_previous_kernel();
-  const int lane = threadIdx.x & (a.lanes - 1);
-  const uint64_t group = ((uint64_t)blockIdx.x * kThreads + threadIdx.x) / a.lanes, groups = (uint64_t)gridDim.x * (kThreads / a.lanes);
-  const uint32_t mask = a.lanes == 32 ? 0xffffffffu : ((1u << a.lanes) - 1u) << (threadIdx.x & 31 & ~(a.lanes - 1));
-  const int head0 = (int)(group % a.per_row);
-  const float inv_dim = 1.f / (float)a.dim;
-  Angles<V, NU> angles;
-  angles.begin(a, lane);
-  int lo[NU], hi[NU];
-  bool has[NU];
-#pragma unroll
-  for (int i = 0; i < NU; ++i) {
-    const Unit<V, kNext> unit(lane + i * a.lanes, a.pairs, a.dim);
-    lo[i] = unit.lo;
-    hi[i] = unit.hi;
-    has[i] = (lane + i * a.lanes) * V < a.dim / 2;
-  }
-  float w[2][NU][2 * V], dw[2][NU][2 * V];
-#pragma unroll
-  for (int which = 0; which < 2; ++which) {
-    weights<V, kNext, NU>(a, a.part[which].weight, lane, w[which]);
-#pragma unroll
-    for (int i = 0; i < NU; ++i)
-#pragma unroll
-      for (int j = 0; j < 2 * V; ++j) dw[which][i][j] = 0.f;
-  }
-  for (uint64_t row = group / a.per_row; row < a.rows; row += groups / a.per_row) {
-    float c[NU][V], s[NU][V];
-    angles.of_row(a, row, c, s);
-#pragma unroll
-    for (int which = 0; which < 2; ++which) {
-      const Heads& p = a.part[which];
-      const T* from = static_cast<const T*>(p.x) + (int64_t)row * p.row;
-      const T* grad = static_cast<const T*>(p.grad) + (int64_t)row * p.grad_row;
-      T* to = static_cast<T*>(p.out) + row * (uint64_t)p.heads * a.dim;
-      for (int h0 = head0; h0 < p.heads; h0 += U * a.per_row) {
-        Pack<T, V> raw[U][NU][2], dy[U][NU][2];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int h = h0 + u * a.per_row;
-          load_units<T, V, NU>(from + (int64_t)h * p.head, lo, hi, h < p.heads, has, raw[u]);
-          load_units<T, V, NU>(grad + (int64_t)h * p.grad_head, lo, hi, h < p.heads, has, dy[u]);
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int h = h0 + u * a.per_row;
-          if (h >= p.heads) break;
-          float x[NU][2 * V], g[NU][2 * V];
-          float sum = 0.f, dot = 0.f;
-#pragma unroll
-          for (int i = 0; i < NU; ++i) {
-            float y[2 * V];
-#pragma unroll
-            for (int j = 0; j < 2 * V; ++j) {
-              x[i][j] = has[i] ? number(raw[u][i][j / V].v[j % V]) : 0.f;
-              y[j] = has[i] ? number(dy[u][i][j / V].v[j % V]) : 0.f;
-              sum = fmaf(x[i][j], x[i][j], sum);
-            }
-            rotate<V, kNext>(y, c[i], s[i], angles.turned[i], g[i]);
-          }
-          const float inv = 1.f / sqrtf(over_lanes(sum, a.lanes, mask) * inv_dim + a.eps);
-#pragma unroll
-          for (int i = 0; i < NU; ++i)
-#pragma unroll
-            for (int j = 0; j < 2 * V; ++j) {
-              x[i][j] *= inv;
-              dw[which][i][j] = fmaf(g[i][j], x[i][j], dw[which][i][j]);
-              g[i][j] *= w[which][i][j];
-              dot = fmaf(g[i][j], x[i][j], dot);
-            }
-          dot = over_lanes(dot, a.lanes, mask) * inv_dim;
-#pragma unroll
-          for (int i = 0; i < NU; ++i) {
-            if (!has[i]) continue;
-            Pack<T, V> o[2];
-#pragma unroll
-            for (int j = 0; j < 2 * V; ++j) o[j / V].v[j % V] = rounded<T>(inv * fmaf(-dot, x[i][j], g[i][j]));
-            *reinterpret_cast<Pack<T, V>*>(to + (int64_t)h * a.dim + lo[i]) = o[0];
-            *reinterpret_cast<Pack<T, V>*>(to + (int64_t)h * a.dim + hi[i]) = o[1];
-          }
-        }
-      }
-    }
-  }
-  if (!a.sums) return;  // (the same for all threads)
-  // the groups of a warp hold the same channels; then the warps one after the other
-#pragma unroll
-  for (int which = 0; which < 2; ++which)
-    for (int o = a.lanes; o < 32; o <<= 1)
-#pragma unroll
-      for (int i = 0; i < NU; ++i)
-#pragma unroll
-        for (int j = 0; j < 2 * V; ++j) dw[which][i][j] += __shfl_xor_sync(0xffffffffu, dw[which][i][j], o);
-  for (int t = 0; t < kThreads / 32; ++t) {
-    if ((int)threadIdx.x / 32 == t && (int)(threadIdx.x & 31) < a.lanes) {
-#pragma unroll
-      for (int which = 0; which < 2; ++which)
-#pragma unroll
-        for (int i = 0; i < NU; ++i) {
-          if (!has[i]) continue;
-#pragma unroll
-          for (int j = 0; j < 2 * V; ++j) {
-            float* at = block_sums + which * a.dim + (j < V ? lo[i] + j : hi[i] + j - V);
-            *at = t ? *at + dw[which][i][j] : dw[which][i][j];
-          }
-        }
+      axis[p] = of;
     }
     __syncthreads();
   }
-  for (int i = threadIdx.x; i < 2 * a.dim; i += kThreads) a.sums[(size_t)blockIdx.x * 2 * a.dim + i] = block_sums[i];
+  // the angles of the warp's rows from `row` on, then each lane those of its units
+  __device__ __forceinline__ void angles(const RotaryArgs& a, const Heads& p, uint64_t row, int at, int row_of_warp,
+                                         Number<V> (&c)[NU][kNumbers<V>], Number<V> (&s)[NU][kNumbers<V>]) {
+    const int units = a.lanes * NU, lane = threadIdx.x & 31, n = 32 / p.groups * NU * V;  // of all rows; n / (units V) of them
+    const int shift = 31 - __clz(units * V);
+    float* cosines = turns[threadIdx.x >> 5][0];
+    float* sines = turns[threadIdx.x >> 5][1];
+    __syncwarp();  // the rows before have been read
+#pragma unroll 2
+    for (int i = lane; i < n; i += 32) {
+      const int of = i >> shift, pair = i & (units * V - 1), ax = axis[pair];
+      float cosine = 1.f, sine = 0.f;
+      if (ax >= 0 && row + of < a.rows) {
+        const int32_t position = __ldg(a.positions + (int64_t)(row + of) * a.position_row + (int64_t)ax * a.position_axis);
+        turn_of(position, fraction[pair], cosine, sine);
+        if (a.back) sine = -sine;
+      }
+      const int to = of * units * V + place(pair, units);
+      cosines[to] = cosine;
+      sines[to] = sine;
+    }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < NU; ++i) {
+      read(cosines + row_of_warp * units * V, units, at + i * a.lanes, c[i]);
+      read(sines + row_of_warp * units * V, units, at + i * a.lanes, s[i]);
+    }
+  }
+};
+
+// A unit turned; of a unit that turns in part (kNext) pair by pair, so that what stays is not touched.
+template <int V>
+__device__ __forceinline__ Unit<V> rotate(const Unit<V>& x, const Number<V> (&c)[kNumbers<V>], const Number<V> (&s)[kNumbers<V>], int turned) {
+  if (turned == 0) return x;
+  Unit<V> y;
+  const Number<V> minus = splat<V>(-1.f);
+#pragma unroll
+  for (int k = 0; k < kNumbers<V>; ++k) {
+    y.a[k] = fma(x.a[k], c[k], mul(mul(x.b[k], s[k]), minus));
+    y.b[k] = fma(x.b[k], c[k], mul(x.a[k], s[k]));
+  }
+  if constexpr (V > 1) {
+    if (turned < V) {
+#pragma unroll
+      for (int k = 0; k < V / 2; ++k) {
+        float a0, a1, b0, b1, x0, x1, z0, z1;
+        parts(y.a[k], a0, a1);
+        parts(y.b[k], b0, b1);
+        parts(x.a[k], x0, x1);
+        parts(x.b[k], z0, z1);
+        y.a[k] = make_pair(2 * k < turned ? a0 : x0, 2 * k + 1 < turned ? a1 : x1);
+        y.b[k] = make_pair(2 * k < turned ? b0 : z0, 2 * k + 1 < turned ? b1 : z1);
+      }
+    }
+  }
+  return y;
+}
+// the sum over the lanes of a head; every one gets it
+__device__ __forceinline__ float over_lanes(float v, int lanes) {
+  for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
 }
 
-// dw of queries and keys = the blocks' sums in a fixed order: 32 slices of them, in fp64, then the slices.
-__global__ void __launch_bounds__(1024) k_rotary_sums(const float* __restrict__ sums, uint32_t blocks, int dim, int bf16,
-                                                      void* __restrict__ dwq, void* __restrict__ dwk) {
+// The rows and heads of a warp, one batch of U heads (for each of its groups) after the other.
+template <int U>
+struct Walk {
+  uint64_t row, step;  // the warp's first row, and how far the next one is
+  int first, next, batches, batch;  // the group's first head, how far its next one is
+  __device__ __forceinline__ Walk(const RotaryArgs& a, const Heads& p, uint32_t block, int group) {
+    const uint64_t warp = (uint64_t)block * kWarps + (threadIdx.x >> 5);
+    const int rows = 32 / (a.lanes * p.groups);
+    row = warp / p.warps * rows;
+    step = (uint64_t)p.blocks * kWarps / p.warps * rows;
+    first = (int)(warp % p.warps) * p.groups + group;
+    next = p.groups * p.warps;
+    batches = (p.heads + next * U - 1) / (next * U);
+    batch = 0;
+  }
+  __device__ __forceinline__ int head(int u) const { return first + (batch * U + u) * next; }
+  __device__ __forceinline__ void forward() {
+    if (++batch == batches) {
+      batch = 0;
+      row += step;
+    }
+  }
+};
+
+// (heads in flight: twice these)
+constexpr int heads_at_once(int nu) { return nu == 1 ? 2 : 1; }
+
+template <typename T, int V, int NU, bool kNext, bool kNorm>
+__global__ void __launch_bounds__(kThreads, 2) k_rotary(const __grid_constant__ RotaryArgs a) {
+  constexpr int U = heads_at_once(NU), N = kNumbers<V>;
+  __shared__ Tables<V, NU> tables;
+  after_previous_kernel();
+  const bool keys = blockIdx.x >= a.part[0].blocks;
+  const Heads& p = a.part[keys ? 1 : 0];
+  const Lane<V, NU, kNext> lane(a, p);
+  const float inv_dim = 1.f / (float)a.dim;
+  tables.begin(a, p.weight, kNext, kNorm);
+  Walk<U> now(a, p, blockIdx.x - (keys ? a.part[0].blocks : 0), lane.group);
+  auto load = [&](const Walk<U>& w, Pack<T, V> (&x)[U][NU][2]) {
+    const uint64_t row = w.row + lane.row_of_warp;
+    const T* from = static_cast<const T*>(p.x) + (int64_t)row * p.row;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < NU; ++i)
+        if (row < a.rows && w.head(u) < p.heads && lane.has[i]) {
+          x[u][i][0] = load_pack<T, V>(from + (int64_t)w.head(u) * p.head + lane.lo[i]);
+          x[u][i][1] = load_pack<T, V>(from + (int64_t)w.head(u) * p.head + lane.hi[i]);
+        } else {
+          x[u][i][0] = x[u][i][1] = Pack<T, V>{};
+        }
+  };
+  Pack<T, V> raw[U][NU][2];
+  load(now, raw);
+  Number<V> c[NU][N], s[NU][N];
+  while (now.row < a.rows) {  // (whole warps)
+    if (now.batch == 0) tables.angles(a, p, now.row, lane.at, lane.row_of_warp, c, s);
+    Walk<U> then = now;
+    then.forward();
+    Pack<T, V> more[U][NU][2];
+    load(then, more);
+    const uint64_t row = now.row + lane.row_of_warp;
+    T* to = static_cast<T*>(p.out) + row * (uint64_t)p.heads * a.dim;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      Unit<V> x[NU];
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < NU; ++i) {
+        x[i] = unit_of<T, V, kNext>(raw[u][i]);
+        if constexpr (kNorm) {
+          Number<V> t = mul(x[i].a[0], x[i].a[0]);
+#pragma unroll
+          for (int k = 1; k < N; ++k) t = fma(x[i].a[k], x[i].a[k], t);
+#pragma unroll
+          for (int k = 0; k < N; ++k) t = fma(x[i].b[k], x[i].b[k], t);
+          sum += total(t);
+        }
+      }
+      if constexpr (kNorm) {
+        const Number<V> inv = splat<V>(rsqrtf(over_lanes(sum, a.lanes) * inv_dim + a.eps));
+#pragma unroll
+        for (int i = 0; i < NU; ++i) {
+          Number<V> w[N];
+          tables.read(tables.w[0], a.lanes * NU, lane.at + i * a.lanes, w);
+#pragma unroll
+          for (int k = 0; k < N; ++k) x[i].a[k] = mul(mul(x[i].a[k], inv), w[k]);
+          tables.read(tables.w[1], a.lanes * NU, lane.at + i * a.lanes, w);
+#pragma unroll
+          for (int k = 0; k < N; ++k) x[i].b[k] = mul(mul(x[i].b[k], inv), w[k]);
+        }
+      }
+      if (row >= a.rows || now.head(u) >= p.heads) continue;
+#pragma unroll
+      for (int i = 0; i < NU; ++i)
+        if (lane.has[i])
+          store_unit<T, V, kNext>(to + (int64_t)now.head(u) * a.dim + lane.lo[i], to + (int64_t)now.head(u) * a.dim + lane.hi[i],
+                                  rotate<V>(x[i], c[i], s[i], lane.turned[i]));
+    }
+    now = then;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < NU; ++i) {
+        raw[u][i][0] = more[u][i][0];
+        raw[u][i][1] = more[u][i][1];
+      }
+  }
+}
+
+// dx of the norm and the rotation (a.back is set: gradients are turned back), and a block's part of dw.
+template <typename T, int V, int NU, bool kNext>
+__global__ void __launch_bounds__(kThreads, 2) k_rotary_backward(const __grid_constant__ RotaryArgs a) {
+  constexpr int N = kNumbers<V>;
+  __shared__ Tables<V, NU> tables;
+  __shared__ float block_sums[kMostDim];
+  after_previous_kernel();
+  const bool keys = blockIdx.x >= a.part[0].blocks;
+  const Heads& p = a.part[keys ? 1 : 0];
+  const Lane<V, NU, kNext> lane(a, p);
+  const float inv_dim = 1.f / (float)a.dim;
+  tables.begin(a, p.weight, kNext, true);
+  Walk<1> now(a, p, blockIdx.x - (keys ? a.part[0].blocks : 0), lane.group);
+  auto load = [&](const Walk<1>& w, Pack<T, V> (&x)[NU][2], Pack<T, V> (&g)[NU][2]) {
+    const uint64_t row = w.row + lane.row_of_warp;
+    const T* from = static_cast<const T*>(p.x) + (int64_t)row * p.row + (int64_t)w.head(0) * p.head;
+    const T* grad = static_cast<const T*>(p.grad) + (int64_t)row * p.grad_row + (int64_t)w.head(0) * p.grad_head;
+#pragma unroll
+    for (int i = 0; i < NU; ++i)
+      if (row < a.rows && w.head(0) < p.heads && lane.has[i]) {
+        x[i][0] = load_pack<T, V>(from + lane.lo[i]);
+        x[i][1] = load_pack<T, V>(from + lane.hi[i]);
+        g[i][0] = load_pack<T, V>(grad + lane.lo[i]);
+        g[i][1] = load_pack<T, V>(grad + lane.hi[i]);
+      } else {
+        x[i][0] = x[i][1] = g[i][0] = g[i][1] = Pack<T, V>{};
+      }
+  };
+  Pack<T, V> raw[NU][2], dy[NU][2];
+  load(now, raw, dy);
+  Number<V> c[NU][N], s[NU][N];
+  Unit<V> dw[NU];
+#pragma unroll
+  for (int i = 0; i < NU; ++i)
+#pragma unroll
+    for (int k = 0; k < N; ++k) dw[i].a[k] = dw[i].b[k] = splat<V>(0.f);
+  while (now.row < a.rows) {  // (whole warps)
+    if (now.batch == 0) tables.angles(a, p, now.row, lane.at, lane.row_of_warp, c, s);
+    Walk<1> then = now;
+    then.forward();
+    Pack<T, V> more[NU][2], more_dy[NU][2];
+    load(then, more, more_dy);
+    Unit<V> x[NU], g[NU];
+    Number<V> square = splat<V>(0.f), dot = splat<V>(0.f);
+#pragma unroll
+    for (int i = 0; i < NU; ++i) {
+      x[i] = unit_of<T, V, kNext>(raw[i]);
+      g[i] = rotate<V>(unit_of<T, V, kNext>(dy[i]), c[i], s[i], lane.turned[i]);
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        square = fma(x[i].a[k], x[i].a[k], square);
+        square = fma(x[i].b[k], x[i].b[k], square);
+      }
+    }
+    const float inv = rsqrtf(over_lanes(total(square), a.lanes) * inv_dim + a.eps);
+    const bool here = now.row + lane.row_of_warp < a.rows && now.head(0) < p.heads;
+    // (rows and heads that are not there are zeros, but so may be eps)
+    const Number<V> by = splat<V>(here ? inv : 0.f);
+#pragma unroll
+    for (int i = 0; i < NU; ++i) {
+      Number<V> w[N];
+      tables.read(tables.w[0], a.lanes * NU, lane.at + i * a.lanes, w);
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        x[i].a[k] = mul(x[i].a[k], by);
+        dw[i].a[k] = fma(g[i].a[k], x[i].a[k], dw[i].a[k]);
+        g[i].a[k] = mul(g[i].a[k], w[k]);
+        dot = fma(g[i].a[k], x[i].a[k], dot);
+      }
+      tables.read(tables.w[1], a.lanes * NU, lane.at + i * a.lanes, w);
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        x[i].b[k] = mul(x[i].b[k], by);
+        dw[i].b[k] = fma(g[i].b[k], x[i].b[k], dw[i].b[k]);
+        g[i].b[k] = mul(g[i].b[k], w[k]);
+        dot = fma(g[i].b[k], x[i].b[k], dot);
+      }
+    }
+    const Number<V> minus = splat<V>(-over_lanes(total(dot), a.lanes) * inv_dim);
+    if (here) {
+      T* to = static_cast<T*>(p.out) + ((now.row + lane.row_of_warp) * (uint64_t)p.heads + (uint64_t)now.head(0)) * a.dim;
+#pragma unroll
+      for (int i = 0; i < NU; ++i) {
+        if (!lane.has[i]) continue;
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+          g[i].a[k] = mul(by, fma(x[i].a[k], minus, g[i].a[k]));
+          g[i].b[k] = mul(by, fma(x[i].b[k], minus, g[i].b[k]));
+        }
+        store_unit<T, V, kNext>(to + lane.lo[i], to + lane.hi[i], g[i]);
+      }
+    }
+    now = then;
+#pragma unroll
+    for (int i = 0; i < NU; ++i)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        raw[i][k] = more[i][k];
+        dy[i][k] = more_dy[i][k];
+      }
+  }
+  if (!a.sums) return;  // (the same for all threads)
+  // the groups of a warp hold the same channels; then the warps one after the other
+  float sums[NU][2 * V];
+#pragma unroll
+  for (int i = 0; i < NU; ++i) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      if constexpr (V == 1) {
+        sums[i][0] = dw[i].a[0];
+        sums[i][1] = dw[i].b[0];
+      } else {
+        parts(dw[i].a[k], sums[i][2 * k], sums[i][2 * k + 1]);
+        parts(dw[i].b[k], sums[i][V + 2 * k], sums[i][V + 2 * k + 1]);
+      }
+    }
+    for (int o = a.lanes; o < 32; o <<= 1)
+#pragma unroll
+      for (int j = 0; j < 2 * V; ++j) sums[i][j] += __shfl_xor_sync(0xffffffffu, sums[i][j], o);
+  }
+  for (int t = 0; t < kWarps; ++t) {
+    if ((int)threadIdx.x / 32 == t && (int)(threadIdx.x & 31) < a.lanes) {
+#pragma unroll
+      for (int i = 0; i < NU; ++i) {
+        if (!lane.has[i]) continue;
+#pragma unroll
+        for (int j = 0; j < 2 * V; ++j) {
+          // number j: the first channel of pair j of the unit, then the second ones
+          const int pair = j % V, second = j / V;
+          const int ch = kNext ? lane.lo[i] + 2 * pair + second : (second ? lane.hi[i] : lane.lo[i]) + pair;
+          block_sums[ch] = t ? block_sums[ch] + sums[i][j] : sums[i][j];
+        }
+      }
+    }
+    __syncthreads();
+  }
+  for (int i = threadIdx.x; i < a.dim; i += kThreads) a.sums[(size_t)blockIdx.x * a.dim + i] = block_sums[i];
+}
+
+// dw of queries and keys = their blocks' sums in a fixed order: 32 slices of them, in fp64, then the slices.
+__global__ void __launch_bounds__(1024) k_rotary_sums(const float* __restrict__ sums, uint32_t q_blocks, uint32_t k_blocks, int dim,
+                                                      int bf16, void* __restrict__ dwq, void* __restrict__ dwk) {
   __shared__ double part[32][33];
   after_previous_kernel();
   const int slice = threadIdx.x >> 5, lane = threadIdx.x & 31, i = blockIdx.x * 32 + lane;
+  const uint32_t first = blockIdx.y ? q_blocks : 0, blocks = blockIdx.y ? k_blocks : q_blocks;
   double t = 0.0;
-  if (i < 2 * dim)
+  if (i < dim)
 #pragma unroll 8
-    for (uint32_t b = slice; b < blocks; b += 32) t += (double)__ldg(sums + (size_t)b * 2 * dim + i);
+    for (uint32_t b = slice; b < blocks; b += 32) t += (double)__ldg(sums + (size_t)(first + b) * dim + i);
   part[slice][lane] = t;
   __syncthreads();
   t = part[lane][slice];  // number `slice` by the warp of that number
   for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-  const int out = blockIdx.x * 32 + slice;
-  if (lane != 0 || out >= 2 * dim) return;
-  void* to = out < dim ? dwq : dwk;
-  if (!to) return;
-  const int c = out < dim ? out : out - dim;
+  const int c = blockIdx.x * 32 + slice;
+  void* to = blockIdx.y ? dwk : dwq;
+  if (lane != 0 || c >= dim || !to) return;
   if (bf16) static_cast<__nv_bfloat16*>(to)[c] = __float2bfloat16_rn((float)t);
   else static_cast<float*>(to)[c] = (float)t;
 }
@@ -478,44 +648,46 @@ int pairs_a_load(const RotaryArgs& a, int elem, bool next) {
   return v;
 }
 
-// Lanes of a head, groups of a row: as many as the heads allow until the groups of all rows are 8 warps for every SM.
-void lay_out(RotaryArgs* a, int V, int units_a_lane) {
-  const int units = a->dim / 2 / V, heads = a->part[0].heads + a->part[1].heads;
+// Lanes of a head; groups of a row in a warp: as many as leave each two heads (whose loads run together), and as fit; further warps of a
+// row where there are few rows, until there are eight for every SM.
+void lay_out(RotaryArgs* a, int V, int units_a_lane, uint32_t most_blocks) {
+  const int units = a->dim / 2 / V;
   a->lanes = 1;
   while (a->lanes * units_a_lane < units) a->lanes *= 2;
-  a->per_row = 1;
-  while (a->per_row < heads && a->per_row * a->lanes < kThreads &&
-         (uint64_t)a->rows * a->per_row * a->lanes < (uint64_t)148 * kThreads)
-    a->per_row *= 2;
-}
-uint32_t blocks_of(const RotaryArgs& a, uint32_t most) {
-  const uint64_t threads = (uint64_t)a.rows * a.per_row * a.lanes;
-  return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>((threads + kThreads - 1) / kThreads, most));
+  const uint64_t heads = (uint64_t)a->part[0].heads + a->part[1].heads;
+  for (Heads& p : a->part) {
+    p.groups = p.warps = 1;
+    while (a->lanes * p.groups < 32 && p.groups * 4 <= p.heads) p.groups *= 2;
+    const uint64_t rows = 32 / (a->lanes * p.groups);  // of a warp
+    auto warps = [&] { return ((uint64_t)a->rows + rows - 1) / rows * p.warps; };
+    while (p.warps < kWarps && p.groups * p.warps < p.heads && warps() < 148 * 8) p.warps *= 2;
+    const uint64_t share = std::max<uint64_t>(1, most_blocks * (uint64_t)p.heads / heads);
+    p.blocks = p.heads ? (uint32_t)std::min<uint64_t>((warps() + kWarps - 1) / kWarps, share) : 0;
+  }
 }
 
 template <typename T, int V, int NU>
-int launch(RotaryArgs& a, bool next, bool norm, bool backward, cudaStream_t stream, uint32_t* blocks) {
-  lay_out(&a, V, NU);
-  *blocks = blocks_of(a, backward ? kMostBackwardBlocks : 148 * 16);
+int launch(RotaryArgs& a, bool next, bool norm, bool backward, cudaStream_t stream) {
+  lay_out(&a, V, NU, backward ? kMostBackwardBlocks : 148 * 8);
   void (*kern)(RotaryArgs);
   if (backward) kern = next ? k_rotary_backward<T, V, NU, true> : k_rotary_backward<T, V, NU, false>;
   else if (norm) kern = next ? k_rotary<T, V, NU, true, true> : k_rotary<T, V, NU, false, true>;
   else kern = next ? k_rotary<T, V, NU, true, false> : k_rotary<T, V, NU, false, false>;
-  RMN_CUDA_TRY(launch_overlapped(kern, dim3(*blocks), dim3(kThreads), 0, stream, a));
+  RMN_CUDA_TRY(launch_overlapped(kern, dim3(a.part[0].blocks + a.part[1].blocks), dim3(kThreads), 0, stream, a));
   RMN_LAUNCH_CHECK();
   return RMN_OK;
 }
-int run(RotaryArgs& a, int dtype, bool next, bool norm, bool backward, cudaStream_t stream, uint32_t* blocks) {
+int run(RotaryArgs& a, int dtype, bool next, bool norm, bool backward, cudaStream_t stream) {
   const int v = pairs_a_load(a, dtype == RMN_F32 ? 4 : 2, next);
   if (dtype == RMN_F32)
-    return v == 4   ? launch<float, 4, 1>(a, next, norm, backward, stream, blocks)
-           : v == 2 ? launch<float, 2, 2>(a, next, norm, backward, stream, blocks)
-                    : launch<float, 1, 4>(a, next, norm, backward, stream, blocks);
+    return v == 4   ? launch<float, 4, 1>(a, next, norm, backward, stream)
+           : v == 2 ? launch<float, 2, 2>(a, next, norm, backward, stream)
+                    : launch<float, 1, 4>(a, next, norm, backward, stream);
   using B = __nv_bfloat16;
-  return v == 8   ? launch<B, 8, 1>(a, next, norm, backward, stream, blocks)
-         : v == 4 ? launch<B, 4, 1>(a, next, norm, backward, stream, blocks)
-         : v == 2 ? launch<B, 2, 2>(a, next, norm, backward, stream, blocks)
-                  : launch<B, 1, 4>(a, next, norm, backward, stream, blocks);
+  return v == 8   ? launch<B, 8, 1>(a, next, norm, backward, stream)
+         : v == 4 ? launch<B, 4, 1>(a, next, norm, backward, stream)
+         : v == 2 ? launch<B, 2, 2>(a, next, norm, backward, stream)
+                  : launch<B, 1, 4>(a, next, norm, backward, stream);
 }
 
 }  // namespace
@@ -531,8 +703,7 @@ extern "C" int rmn_rotary_forward(const rmn_rotary* problem, void* d_q_out, void
   if (!d_q_out || (problem->kv_heads && !d_k_out)) return RMN_ERR_BAD_ARG;
   a.part[0].out = d_q_out;
   a.part[1].out = d_k_out;
-  uint32_t blocks;
-  return run(a, problem->dtype, problem->interleaved != 0, problem->norm != 0, false, (cudaStream_t)stream_, &blocks);
+  return run(a, problem->dtype, problem->interleaved != 0, problem->norm != 0, false, (cudaStream_t)stream_);
 }
 
 extern "C" size_t rmn_rotary_backward_workspace_bytes(const rmn_rotary* problem) {
@@ -565,18 +736,18 @@ extern "C" int rmn_rotary_backward(const rmn_rotary* problem, const void* d_grad
   a.part[0].out = d_dq;
   a.part[1].out = d_dk;
   a.back = 1;
-  uint32_t blocks = 0;
-  if (a.rows && !norm) return run(a, problem->dtype, problem->interleaved != 0, false, false, stream, &blocks);
+  if (a.rows && !norm) return run(a, problem->dtype, problem->interleaved != 0, false, false, stream);
   if (a.rows) {
     a.part[0].grad = d_grad_q; a.part[0].grad_row = grad_q_row; a.part[0].grad_head = grad_q_head;
     a.part[1].grad = d_grad_k; a.part[1].grad_row = grad_k_row; a.part[1].grad_head = grad_k_head;
     a.sums = sums ? static_cast<float*>(d_workspace) : nullptr;
-    const int launched = run(a, problem->dtype, problem->interleaved != 0, true, true, stream, &blocks);
+    const int launched = run(a, problem->dtype, problem->interleaved != 0, true, true, stream);
     if (launched != RMN_OK) return launched;
   }
   if (!sums) return RMN_OK;
-  RMN_CUDA_TRY(launch_overlapped(k_rotary_sums, dim3((uint32_t)(2 * a.dim + 31) / 32), dim3(1024), 0, stream,
-                                 static_cast<const float*>(d_workspace), blocks, a.dim, a.weight_bf16, d_dq_weight, d_dk_weight));
+  RMN_CUDA_TRY(launch_overlapped(k_rotary_sums, dim3((uint32_t)(a.dim + 31) / 32, 2), dim3(1024), 0, stream,
+                                 static_cast<const float*>(d_workspace), a.part[0].blocks, a.part[1].blocks, a.dim, a.weight_bf16,
+                                 d_dq_weight, d_dk_weight));
   RMN_LAUNCH_CHECK();
   return RMN_OK;
 }
