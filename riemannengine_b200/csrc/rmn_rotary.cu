@@ -12,10 +12,11 @@
 //
 // Bound by memory: every value is read once and written once. A block works on queries or on keys. A head's channels lie over L lanes (a
 // power of two), each with units of V pairs, 16 bytes a load where sizes and alignment allow; the L lanes are a group. A warp has one or
-// several rows, each with one or several groups that take the row's heads in turn, U at a time; the next ones are asked for before these
-// are worked on, across rows. The warp makes the angles of its rows once, every lane a share of them, and hands them on through shared
-// memory. The norm's sums go over the L lanes. dw is summed in registers over the rows that a thread visits, over the block in a
-// fixed order and over the blocks by a second kernel: no atomics, the same bits every time.
+// several rows, each with one or several groups that take the row's heads in turn, U at a time. A thread copies what it is going to
+// read into places of its own in shared memory, kStages batches ahead and across rows, so that the copies in flight take no registers and
+// need no barriers; the positions of the rows come the same way. The warp makes the angles of its rows once, every lane a share of them,
+// and hands them on through shared memory. The norm's sums go over the L lanes. dw is summed in registers over the rows that a thread
+// visits, over the block in a fixed order and over the blocks by a second kernel: no atomics, the same bits every time.
 #include "rmn_common.cuh"
 #include "rmn_pair.cuh"
 
@@ -47,7 +48,8 @@ struct Heads {  // [rows, heads, dim]
 struct RotaryArgs {
   Heads part[2];  // queries, keys (0 heads: none)
   uint32_t rows;
-  int dim, pairs, lanes;  // lanes of a head
+  int dim, pairs, lanes, axes;  // lanes of a head
+  int pair_bits;          // of the pairs that these lanes could hold (a power of two)
   const int32_t* positions;
   int64_t position_row, position_axis;
   const double* frequencies;
@@ -61,23 +63,23 @@ template <typename T, int V>
 struct alignas(sizeof(T) * V) Pack {
   T v[V];
 };
-template <typename T, int V>
-__device__ __forceinline__ Pack<T, V> load_pack(const T* p) {
-  Pack<T, V> r;
-  if constexpr (sizeof(r) == 16) {
-    const uint4 w = __ldg(reinterpret_cast<const uint4*>(p));
-    r = *reinterpret_cast<const Pack<T, V>*>(&w);
-  } else if constexpr (sizeof(r) == 8) {
-    const uint2 w = __ldg(reinterpret_cast<const uint2*>(p));
-    r = *reinterpret_cast<const Pack<T, V>*>(&w);
-  } else if constexpr (sizeof(r) == 4) {
-    const uint32_t w = __ldg(reinterpret_cast<const uint32_t*>(p));
-    r = *reinterpret_cast<const Pack<T, V>*>(&w);
+// kBytes bytes into shared memory, zeros where there is nothing (`here`). Two bytes are more than a copy can be short of: those are loaded.
+template <int kBytes>
+__device__ __forceinline__ void copy(void* to, const void* from, bool here) {
+  if constexpr (kBytes == 2) {
+    *static_cast<uint16_t*>(to) = here ? __ldg(static_cast<const uint16_t*>(from)) : (uint16_t)0;
   } else {
-    r = *reinterpret_cast<const Pack<T, V>*>(p);
+    const uint32_t at = (uint32_t)__cvta_generic_to_shared(to);
+    if constexpr (kBytes == 16)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at), "l"(from), "r"(here ? 16 : 0) : "memory");
+    else
+      asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(at), "l"(from), "r"(here ? kBytes : 0), "n"(kBytes) : "memory");
   }
-  return r;
 }
+__device__ __forceinline__ void copies_made() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kLater>  // all but the last kLater groups are there
+__device__ __forceinline__ void copies_here() { asm volatile("cp.async.wait_group %0;" ::"n"(kLater) : "memory"); }
+
 __device__ __forceinline__ float number(float v) { return v; }
 __device__ __forceinline__ float number(__nv_bfloat16 v) { return __bfloat162float(v); }
 template <typename T>
@@ -115,6 +117,8 @@ __device__ __forceinline__ float add(float a, float b) { return a + b; }
 __device__ __forceinline__ float mul(float a, float b) { return a * b; }
 __device__ __forceinline__ float fma(float a, float b, float c) { return fmaf(a, b, c); }
 __device__ __forceinline__ float total(float a) { return a; }
+__device__ __forceinline__ float negative(float a) { return -a; }
+__device__ __forceinline__ Pair negative(Pair a) { return {a.v ^ 0x8000000080000000ull}; }
 template <int V>
 using Number = std::conditional_t<V == 1, float, Pair>;
 template <int V>
@@ -175,6 +179,12 @@ __device__ __forceinline__ void store_unit(T* lo, T* hi, const Unit<V>& u) {
   *reinterpret_cast<Pack<T, V>*>(hi) = p[1];
 }
 
+// The angles of a unit's pairs.
+template <int V>
+struct Turn {
+  Number<V> c[kNumbers<V>], s[kNumbers<V>], minus[kNumbers<V>];  // cosine, sine, - sine
+};
+
 // What a lane does: its units' channels, its rows and heads.
 template <int V, int NU, bool kNext>
 struct Lane {
@@ -192,7 +202,9 @@ struct Lane {
       const int u = at + i * a.lanes, first = u * V;
       has[i] = first < a.dim / 2;
       turned[i] = min(max(a.pairs - first, 0), V);
-      if (kNext) {
+      if (!has[i]) {  // (reads what the first lane reads, and stores nothing)
+        lo[i] = hi[i] = 0;
+      } else if (kNext) {
         lo[i] = 2 * first;
         hi[i] = lo[i] + V;
       } else if (first < a.pairs) {
@@ -206,109 +218,142 @@ struct Lane {
   }
 };
 
-// The tables of a block, [lane's number of four (or fewer) pairs][unit][pair], so that the lanes of a head read neighbouring words:
-// w of the first and of the second channels, and for each warp cosines and sines of its rows.
+constexpr int kStages = 4;
+
+// The tables of a block: for every pair of a head the fraction of a turn (pairs that do not turn: none), and w of its first and of its
+// second channel; for each warp cosines and sines of its rows. Behind them for every angle of a warp's rows the place of its position
+// among theirs, for every such position where it is, from the first row's on, and which row it is of; and the ring of copies.
 template <int V, int NU>
 struct alignas(16) Tables {
-  static constexpr int W = V < 4 ? V : 4, PAIRS = 32 * NU * V;  // words of a read; pairs of a warp's rows at most
+  static constexpr int PAIRS = 32 * NU * V;  // of a warp's rows at most
   float w[2][kMostDim / 2];
-  uint64_t fraction[kMostDim / 2];
-  int axis[kMostDim / 2];  // -1: does not turn
   float turns[kWarps][2][PAIRS];
-  // where pair p is, of `units` units
-  static __device__ __forceinline__ int place(int p, int units) { return (p % V / W * units + p / V) * W + p % W; }
-  static __device__ __forceinline__ void read(const float* from, int units, int u, Number<V> (&out)[kNumbers<V>]) {
+  uint64_t fraction[kMostDim / 2];
+  int place[PAIRS];
+
+  static __device__ __forceinline__ void read(const float* p, Number<V> (&out)[kNumbers<V>]) {
+    if constexpr (V >= 4) {
 #pragma unroll
-    for (int k = 0; k < V / W; ++k) {
-      const float* p = from + (k * units + u) * W;
-      if constexpr (W == 4) {
-        const float4 v = *reinterpret_cast<const float4*>(p);
+      for (int k = 0; k < V / 4; ++k) {
+        const float4 v = *reinterpret_cast<const float4*>(p + 4 * k);
         out[2 * k] = make_pair(v.x, v.y);
         out[2 * k + 1] = make_pair(v.z, v.w);
-      } else if constexpr (W == 2) {
-        const float2 v = *reinterpret_cast<const float2*>(p);
-        out[k] = make_pair(v.x, v.y);
-      } else {
-        out[k] = *p;
       }
+    } else if constexpr (V == 2) {
+      const float2 v = *reinterpret_cast<const float2*>(p);
+      out[0] = make_pair(v.x, v.y);
+    } else {
+      out[0] = *p;
     }
   }
-  __device__ __forceinline__ void begin(const RotaryArgs& a, const void* weight, bool next, bool norm) {
-    const int units = a.lanes * NU;
-    for (int p = threadIdx.x; p < units * V; p += kThreads) {
+  // (`offset` and `row_of`: of every position)
+  __device__ __forceinline__ void begin(const RotaryArgs& a, const Heads& part, bool next, bool norm, int64_t* offset, int* row_of) {
+    const void* weight = part.weight;
+    const int rows = 32 / (a.lanes * part.groups);
+    for (int p = threadIdx.x; p < 1 << a.pair_bits; p += kThreads) {
       if (norm) {
-        int lo = next ? 2 * p : p < a.pairs ? p : p + a.pairs;
-        int hi = next ? 2 * p + 1 : p < a.pairs ? p + a.pairs : p + a.dim / 2;
+        const int lo = next ? 2 * p : p < a.pairs ? p : p + a.pairs, hi = next ? 2 * p + 1 : p < a.pairs ? p + a.pairs : p + a.dim / 2;
         const bool here = weight && p < a.dim / 2;
         auto of = [&](int c) {
           return !here ? 1.f : a.weight_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(weight)[c]) : static_cast<const float*>(weight)[c];
         };
-        w[0][place(p, units)] = of(lo);
-        w[1][place(p, units)] = of(hi);
+        w[0][p] = of(lo);
+        w[1][p] = of(hi);
       }
-      int of = -1;
-      if (p < a.pairs) {
-        of = 0;
-        for (int k = 0; k < kMostAxes - 1; ++k) of += p >= a.ends[k] ? 1 : 0;
-        fraction[p] = fraction_of_turn(__ldg(a.frequencies + p));
-      }
-      axis[p] = of;
+      int ax = 0;
+      for (int k = 0; k < kMostAxes - 1; ++k) ax += p >= a.ends[k] && p < a.pairs ? 1 : 0;
+      fraction[p] = p < a.pairs ? fraction_of_turn(__ldg(a.frequencies + p)) : 0;
+      for (int r = 0; r < rows; ++r) place[(r << a.pair_bits) + p] = r * a.axes + ax;
+    }
+    for (int i = threadIdx.x; i < rows * a.axes; i += kThreads) {
+      offset[i] = i / a.axes * a.position_row + i % a.axes * a.position_axis;
+      row_of[i] = i / a.axes;
     }
     __syncthreads();
   }
-  // the angles of the warp's rows from `row` on, then each lane those of its units
-  __device__ __forceinline__ void angles(const RotaryArgs& a, const Heads& p, uint64_t row, int at, int row_of_warp,
-                                         Number<V> (&c)[NU][kNumbers<V>], Number<V> (&s)[NU][kNumbers<V>]) {
-    const int units = a.lanes * NU, lane = threadIdx.x & 31, n = 32 / p.groups * NU * V;  // of all rows; n / (units V) of them
-    const int shift = 31 - __clz(units * V);
+  // the angles of the warp's rows from `positions`, then each lane those of its units
+  __device__ __forceinline__ void angles(const RotaryArgs& a, const Heads& p, const int32_t* positions, int at, int row_of_warp,
+                                         Turn<V> (&turn)[NU]) {
+    const int of_row = 1 << a.pair_bits, n = (32 * NU * V) / p.groups;  // (both powers of two)
     float* cosines = turns[threadIdx.x >> 5][0];
     float* sines = turns[threadIdx.x >> 5][1];
-    __syncwarp();  // the rows before have been read
-#pragma unroll 2
-    for (int i = lane; i < n; i += 32) {
-      const int of = i >> shift, pair = i & (units * V - 1), ax = axis[pair];
-      float cosine = 1.f, sine = 0.f;
-      if (ax >= 0 && row + of < a.rows) {
-        const int32_t position = __ldg(a.positions + (int64_t)(row + of) * a.position_row + (int64_t)ax * a.position_axis);
-        turn_of(position, fraction[pair], cosine, sine);
-        if (a.back) sine = -sine;
-      }
-      const int to = of * units * V + place(pair, units);
-      cosines[to] = cosine;
-      sines[to] = sine;
+    __syncwarp();  // the angles before have been read, and all lanes' copies are here
+    for (int i = threadIdx.x & 31; i < n; i += 32) {
+      float c, s;
+      turn_of(positions[place[i]], fraction[i & (of_row - 1)], c, s);
+      cosines[i] = c;
+      sines[i] = a.back ? -s : s;
     }
     __syncwarp();
 #pragma unroll
     for (int i = 0; i < NU; ++i) {
-      read(cosines + row_of_warp * units * V, units, at + i * a.lanes, c[i]);
-      read(sines + row_of_warp * units * V, units, at + i * a.lanes, s[i]);
+      const int first = row_of_warp * of_row + (at + i * a.lanes) * V;
+      read(cosines + first, turn[i].c);
+      read(sines + first, turn[i].s);
+#pragma unroll
+      for (int k = 0; k < kNumbers<V>; ++k) turn[i].minus[k] = negative(turn[i].s[k]);
     }
   }
 };
 
-// A unit turned; of a unit that turns in part (kNext) pair by pair, so that what stays is not touched.
+// A thread's places in the ring, [stage][copy][thread], and its warp's positions, [stage][warp][position]. A batch is U heads of a group;
+// kOf tensors are read.
+template <typename T, int V, int NU, int U, int kOf>
+struct Ring {
+  static constexpr int COPIES = U * kOf * NU * 2;
+  static constexpr size_t kTables = sizeof(Tables<V, NU>);
+  using Load = Pack<T, V>;
+  Load* places;
+  int32_t* positions;
+  int64_t* offset;
+  int* row_of;
+  int count;  // positions of a warp's rows
+  static size_t bytes(int positions) {
+    return kTables + (size_t)positions * (sizeof(int64_t) + kStages * kWarps * sizeof(int32_t)) + (size_t)((positions + 1) & ~1) * sizeof(int) +
+           16 + (size_t)kStages * COPIES * kThreads * sizeof(Load);
+  }
+  __device__ __forceinline__ Ring(char* smem, int positions_of_warp) {
+    count = positions_of_warp;
+    offset = reinterpret_cast<int64_t*>(smem + kTables);
+    row_of = reinterpret_cast<int*>(offset + count);
+    positions = row_of + ((count + 1) & ~1);
+    const uintptr_t end = reinterpret_cast<uintptr_t>(positions + kStages * kWarps * count);
+    places = reinterpret_cast<Load*>((end + 15) & ~(uintptr_t)15) + threadIdx.x;
+  }
+  // copy number `which` of a stage
+  __device__ __forceinline__ Load* at(int stage, int which) const { return places + (stage * COPIES + which) * kThreads; }
+  __device__ __forceinline__ int32_t* positions_of(int stage) const { return positions + (stage * kWarps + (threadIdx.x >> 5)) * count; }
+};
+
+// A unit turned. Where only a part of a head's channels turns, the others are taken as they are, so that what is not finite stays where
+// it is: by units, or (where the last pair that turns is inside one) pair by pair. The same for all threads.
+enum class Part { kAll, kUnits, kPairs };
 template <int V>
-__device__ __forceinline__ Unit<V> rotate(const Unit<V>& x, const Number<V> (&c)[kNumbers<V>], const Number<V> (&s)[kNumbers<V>], int turned) {
-  if (turned == 0) return x;
+__device__ __forceinline__ Unit<V> rotate(const Unit<V>& x, const Turn<V>& by, int turned, Part part) {
   Unit<V> y;
-  const Number<V> minus = splat<V>(-1.f);
 #pragma unroll
   for (int k = 0; k < kNumbers<V>; ++k) {
-    y.a[k] = fma(x.a[k], c[k], mul(mul(x.b[k], s[k]), minus));
-    y.b[k] = fma(x.b[k], c[k], mul(x.a[k], s[k]));
+    y.a[k] = fma(x.a[k], by.c[k], mul(x.b[k], by.minus[k]));
+    y.b[k] = fma(x.b[k], by.c[k], mul(x.a[k], by.s[k]));
   }
-  if constexpr (V > 1) {
-    if (turned < V) {
+  if (part == Part::kAll) return y;
+  if (V == 1 || part == Part::kUnits) {
+    const bool turns = turned > 0;
 #pragma unroll
-      for (int k = 0; k < V / 2; ++k) {
-        float a0, a1, b0, b1, x0, x1, z0, z1;
-        parts(y.a[k], a0, a1);
-        parts(y.b[k], b0, b1);
-        parts(x.a[k], x0, x1);
-        parts(x.b[k], z0, z1);
-        y.a[k] = make_pair(2 * k < turned ? a0 : x0, 2 * k + 1 < turned ? a1 : x1);
-        y.b[k] = make_pair(2 * k < turned ? b0 : z0, 2 * k + 1 < turned ? b1 : z1);
-      }
+    for (int k = 0; k < kNumbers<V>; ++k) {
+      y.a[k] = turns ? y.a[k] : x.a[k];
+      y.b[k] = turns ? y.b[k] : x.b[k];
+    }
+  } else if constexpr (V > 1) {
+#pragma unroll
+    for (int k = 0; k < V / 2; ++k) {
+      float a0, a1, b0, b1, x0, x1, z0, z1;
+      parts(y.a[k], a0, a1);
+      parts(y.b[k], b0, b1);
+      parts(x.a[k], x0, x1);
+      parts(x.b[k], z0, z1);
+      y.a[k] = make_pair(2 * k < turned ? a0 : x0, 2 * k + 1 < turned ? a1 : x1);
+      y.b[k] = make_pair(2 * k < turned ? b0 : z0, 2 * k + 1 < turned ? b1 : z1);
     }
   }
   return y;
@@ -319,76 +364,111 @@ __device__ __forceinline__ float over_lanes(float v, int lanes) {
   return v;
 }
 
-// The rows and heads of a warp, one batch of U heads (for each of its groups) after the other.
-template <int U>
+// The rows of a warp, and the heads of a group: rows base, base + step ...; heads first, first + next ...
 struct Walk {
-  uint64_t row, step;  // the warp's first row, and how far the next one is
-  int first, next, batches, batch;  // the group's first head, how far its next one is
+  uint64_t base, step;
+  int first, next, mine, most;  // heads of the group, of the warp's first one
+  int done;                     // heads of the group before this batch
   __device__ __forceinline__ Walk(const RotaryArgs& a, const Heads& p, uint32_t block, int group) {
-    const uint64_t warp = (uint64_t)block * kWarps + (threadIdx.x >> 5);
-    const int rows = 32 / (a.lanes * p.groups);
-    row = warp / p.warps * rows;
-    step = (uint64_t)p.blocks * kWarps / p.warps * rows;
+    const uint32_t warp = block * kWarps + (threadIdx.x >> 5), rows = 32 / (a.lanes * p.groups);
+    base = (uint64_t)(warp / p.warps) * rows;
+    step = (uint64_t)(p.blocks * kWarps / p.warps) * rows;
     first = (int)(warp % p.warps) * p.groups + group;
     next = p.groups * p.warps;
-    batches = (p.heads + next * U - 1) / (next * U);
-    batch = 0;
+    auto heads = [&](int from) { return from < p.heads ? (p.heads - from + next - 1) / next : 0; };
+    mine = heads(first);
+    most = heads(first - group);
+    done = most ? 0 : 1;
+    if (!most) base = a.rows;  // a warp without heads
   }
-  __device__ __forceinline__ int head(int u) const { return first + (batch * U + u) * next; }
-  __device__ __forceinline__ void forward() {
-    if (++batch == batches) {
-      batch = 0;
-      row += step;
-    }
+  // to the next batch of U heads; true where it is of another row
+  template <int U>
+  __device__ __forceinline__ bool forward() {
+    done += U;
+    if (done < most) return false;
+    done = 0;
+    base += step;
+    return true;
   }
 };
 
-// (heads in flight: twice these)
-constexpr int heads_at_once(int nu) { return nu == 1 ? 2 : 1; }
+// Heads that are copied together. (16 bytes a copy: 64 bytes of a thread in flight for every stage, in either pass.)
+constexpr int heads_at_once(bool backward) { return backward ? 1 : 2; }
 
 template <typename T, int V, int NU, bool kNext, bool kNorm>
 __global__ void __launch_bounds__(kThreads, 2) k_rotary(const __grid_constant__ RotaryArgs a) {
-  constexpr int U = heads_at_once(NU), N = kNumbers<V>;
-  __shared__ Tables<V, NU> tables;
+  constexpr int U = heads_at_once(false), N = kNumbers<V>;
+  extern __shared__ __align__(16) char smem[];
+  Tables<V, NU>& tables = *reinterpret_cast<Tables<V, NU>*>(smem);
   after_previous_kernel();
   const bool keys = blockIdx.x >= a.part[0].blocks;
   const Heads& p = a.part[keys ? 1 : 0];
   const Lane<V, NU, kNext> lane(a, p);
+  const Ring<T, V, NU, U, 1> ring(smem, 32 / (a.lanes * p.groups) * a.axes);
   const float inv_dim = 1.f / (float)a.dim;
-  tables.begin(a, p.weight, kNext, kNorm);
-  Walk<U> now(a, p, blockIdx.x - (keys ? a.part[0].blocks : 0), lane.group);
-  auto load = [&](const Walk<U>& w, Pack<T, V> (&x)[U][NU][2]) {
-    const uint64_t row = w.row + lane.row_of_warp;
-    const T* from = static_cast<const T*>(p.x) + (int64_t)row * p.row;
+  tables.begin(a, p, kNext, kNorm, ring.offset, ring.row_of);
+  Walk now(a, p, blockIdx.x - (keys ? a.part[0].blocks : 0), lane.group), ahead = now;
+  const int64_t in_step = p.head * now.next, out_step = (int64_t)a.dim * now.next;
+  const Part part = 2 * a.pairs == a.dim ? Part::kAll : a.pairs % V == 0 ? Part::kUnits : Part::kPairs;
+  Number<V> w[2][NU][N];
+  if constexpr (kNorm) {
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int i = 0; i < NU; ++i)
-        if (row < a.rows && w.head(u) < p.heads && lane.has[i]) {
-          x[u][i][0] = load_pack<T, V>(from + (int64_t)w.head(u) * p.head + lane.lo[i]);
-          x[u][i][1] = load_pack<T, V>(from + (int64_t)w.head(u) * p.head + lane.hi[i]);
-        } else {
-          x[u][i][0] = x[u][i][1] = Pack<T, V>{};
-        }
+    for (int i = 0; i < NU; ++i) {
+      tables.read(tables.w[0] + (lane.at + i * a.lanes) * V, w[0][i]);
+      tables.read(tables.w[1] + (lane.at + i * a.lanes) * V, w[1][i]);
+    }
+  }
+  auto row_at = [&](uint64_t base) {
+    return static_cast<const T*>(p.x) + (int64_t)(base + lane.row_of_warp) * p.row + (int64_t)now.first * p.head;
   };
-  Pack<T, V> raw[U][NU][2];
-  load(now, raw);
-  Number<V> c[NU][N], s[NU][N];
-  while (now.row < a.rows) {  // (whole warps)
-    if (now.batch == 0) tables.angles(a, p, now.row, lane.at, lane.row_of_warp, c, s);
-    Walk<U> then = now;
-    then.forward();
-    Pack<T, V> more[U][NU][2];
-    load(then, more);
-    const uint64_t row = now.row + lane.row_of_warp;
-    T* to = static_cast<T*>(p.out) + row * (uint64_t)p.heads * a.dim;
+  auto out_at = [&](uint64_t base) {
+    return static_cast<T*>(p.out) + ((base + lane.row_of_warp) * (uint64_t)p.heads + (uint64_t)now.first) * a.dim;
+  };
+  const T* from = row_at(now.base);
+  // the copies of the batch that is kStages - 1 ahead
+  auto ask = [&](int stage) {
+    if (ahead.base < a.rows) {
+      const int left = (ahead.base + lane.row_of_warp < a.rows ? ahead.mine : 0) - ahead.done;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+#pragma unroll
+        for (int i = 0; i < NU; ++i) {
+          const bool here = u < left && lane.has[i];
+          const T* at = here ? from : static_cast<const T*>(p.x);
+          copy<sizeof(Pack<T, V>)>(ring.at(stage, (u * NU + i) * 2), at + lane.lo[i], here);
+          copy<sizeof(Pack<T, V>)>(ring.at(stage, (u * NU + i) * 2 + 1), at + lane.hi[i], here);
+        }
+        from += in_step;
+      }
+      if (ahead.done == 0) {
+        const int32_t* positions = a.positions + (int64_t)ahead.base * a.position_row;
+        for (int i = threadIdx.x & 31; i < ring.count; i += 32) {
+          const bool here = ahead.base + ring.row_of[i] < a.rows;
+          copy<4>(ring.positions_of(stage) + i, positions + (here ? ring.offset[i] : 0), here);
+        }
+      }
+      if (ahead.forward<U>()) from = row_at(ahead.base);
+    }
+    copies_made();
+  };
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) ask(i);
+  T* to = out_at(now.base);
+  Turn<V> turn[NU];
+  int stage = 0;
+  while (now.base < a.rows) {  // (whole warps)
+    ask((stage + kStages - 1) % kStages);
+    copies_here<kStages - 1>();
+    if (now.done == 0 && a.pairs) tables.angles(a, p, ring.positions_of(stage), lane.at, lane.row_of_warp, turn);
+    const int left = (now.base + lane.row_of_warp < a.rows ? now.mine : 0) - now.done;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       Unit<V> x[NU];
       float sum = 0.f;
 #pragma unroll
       for (int i = 0; i < NU; ++i) {
-        x[i] = unit_of<T, V, kNext>(raw[u][i]);
+        const Pack<T, V> raw[2] = {*ring.at(stage, (u * NU + i) * 2), *ring.at(stage, (u * NU + i) * 2 + 1)};
+        x[i] = unit_of<T, V, kNext>(raw);
         if constexpr (kNorm) {
           Number<V> t = mul(x[i].a[0], x[i].a[0]);
 #pragma unroll
@@ -401,135 +481,156 @@ __global__ void __launch_bounds__(kThreads, 2) k_rotary(const __grid_constant__ 
       if constexpr (kNorm) {
         const Number<V> inv = splat<V>(rsqrtf(over_lanes(sum, a.lanes) * inv_dim + a.eps));
 #pragma unroll
-        for (int i = 0; i < NU; ++i) {
-          Number<V> w[N];
-          tables.read(tables.w[0], a.lanes * NU, lane.at + i * a.lanes, w);
+        for (int i = 0; i < NU; ++i)
 #pragma unroll
-          for (int k = 0; k < N; ++k) x[i].a[k] = mul(mul(x[i].a[k], inv), w[k]);
-          tables.read(tables.w[1], a.lanes * NU, lane.at + i * a.lanes, w);
-#pragma unroll
-          for (int k = 0; k < N; ++k) x[i].b[k] = mul(mul(x[i].b[k], inv), w[k]);
-        }
+          for (int k = 0; k < N; ++k) {
+            x[i].a[k] = mul(mul(x[i].a[k], inv), w[0][i][k]);
+            x[i].b[k] = mul(mul(x[i].b[k], inv), w[1][i][k]);
+          }
       }
-      if (row >= a.rows || now.head(u) >= p.heads) continue;
-#pragma unroll
-      for (int i = 0; i < NU; ++i)
-        if (lane.has[i])
-          store_unit<T, V, kNext>(to + (int64_t)now.head(u) * a.dim + lane.lo[i], to + (int64_t)now.head(u) * a.dim + lane.hi[i],
-                                  rotate<V>(x[i], c[i], s[i], lane.turned[i]));
-    }
-    now = then;
-#pragma unroll
-    for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int i = 0; i < NU; ++i) {
-        raw[u][i][0] = more[u][i][0];
-        raw[u][i][1] = more[u][i][1];
+        const Unit<V> y = rotate<V>(x[i], turn[i], lane.turned[i], part);
+        if (u < left && lane.has[i]) store_unit<T, V, kNext>(to + lane.lo[i], to + lane.hi[i], y);
       }
+      to += out_step;
+    }
+    if (now.forward<U>()) to = out_at(now.base);
+    stage = (stage + 1) % kStages;
   }
+  copies_here<0>();
 }
 
 // dx of the norm and the rotation (a.back is set: gradients are turned back), and a block's part of dw.
 template <typename T, int V, int NU, bool kNext>
 __global__ void __launch_bounds__(kThreads, 2) k_rotary_backward(const __grid_constant__ RotaryArgs a) {
-  constexpr int N = kNumbers<V>;
-  __shared__ Tables<V, NU> tables;
+  constexpr int U = heads_at_once(true), N = kNumbers<V>;
+  extern __shared__ __align__(16) char smem[];
+  Tables<V, NU>& tables = *reinterpret_cast<Tables<V, NU>*>(smem);
   __shared__ float block_sums[kMostDim];
   after_previous_kernel();
   const bool keys = blockIdx.x >= a.part[0].blocks;
   const Heads& p = a.part[keys ? 1 : 0];
   const Lane<V, NU, kNext> lane(a, p);
+  const Ring<T, V, NU, U, 2> ring(smem, 32 / (a.lanes * p.groups) * a.axes);
   const float inv_dim = 1.f / (float)a.dim;
-  tables.begin(a, p.weight, kNext, true);
-  Walk<1> now(a, p, blockIdx.x - (keys ? a.part[0].blocks : 0), lane.group);
-  auto load = [&](const Walk<1>& w, Pack<T, V> (&x)[NU][2], Pack<T, V> (&g)[NU][2]) {
-    const uint64_t row = w.row + lane.row_of_warp;
-    const T* from = static_cast<const T*>(p.x) + (int64_t)row * p.row + (int64_t)w.head(0) * p.head;
-    const T* grad = static_cast<const T*>(p.grad) + (int64_t)row * p.grad_row + (int64_t)w.head(0) * p.grad_head;
-#pragma unroll
-    for (int i = 0; i < NU; ++i)
-      if (row < a.rows && w.head(0) < p.heads && lane.has[i]) {
-        x[i][0] = load_pack<T, V>(from + lane.lo[i]);
-        x[i][1] = load_pack<T, V>(from + lane.hi[i]);
-        g[i][0] = load_pack<T, V>(grad + lane.lo[i]);
-        g[i][1] = load_pack<T, V>(grad + lane.hi[i]);
-      } else {
-        x[i][0] = x[i][1] = g[i][0] = g[i][1] = Pack<T, V>{};
-      }
-  };
-  Pack<T, V> raw[NU][2], dy[NU][2];
-  load(now, raw, dy);
-  Number<V> c[NU][N], s[NU][N];
+  tables.begin(a, p, kNext, true, ring.offset, ring.row_of);
+  Walk now(a, p, blockIdx.x - (keys ? a.part[0].blocks : 0), lane.group), ahead = now;
+  const int64_t x_step = p.head * now.next, g_step = p.grad_head * now.next, out_step = (int64_t)a.dim * now.next;
+  const Part part = 2 * a.pairs == a.dim ? Part::kAll : a.pairs % V == 0 ? Part::kUnits : Part::kPairs;
+  Number<V> w[2][NU][N];
   Unit<V> dw[NU];
 #pragma unroll
-  for (int i = 0; i < NU; ++i)
+  for (int i = 0; i < NU; ++i) {
+    tables.read(tables.w[0] + (lane.at + i * a.lanes) * V, w[0][i]);
+    tables.read(tables.w[1] + (lane.at + i * a.lanes) * V, w[1][i]);
 #pragma unroll
     for (int k = 0; k < N; ++k) dw[i].a[k] = dw[i].b[k] = splat<V>(0.f);
-  while (now.row < a.rows) {  // (whole warps)
-    if (now.batch == 0) tables.angles(a, p, now.row, lane.at, lane.row_of_warp, c, s);
-    Walk<1> then = now;
-    then.forward();
-    Pack<T, V> more[NU][2], more_dy[NU][2];
-    load(then, more, more_dy);
-    Unit<V> x[NU], g[NU];
-    Number<V> square = splat<V>(0.f), dot = splat<V>(0.f);
+  }
+  auto row_at = [&](uint64_t base) {
+    return static_cast<const T*>(p.x) + (int64_t)(base + lane.row_of_warp) * p.row + (int64_t)now.first * p.head;
+  };
+  auto grad_at = [&](uint64_t base) {
+    return static_cast<const T*>(p.grad) + (int64_t)(base + lane.row_of_warp) * p.grad_row + (int64_t)now.first * p.grad_head;
+  };
+  auto out_at = [&](uint64_t base) {
+    return static_cast<T*>(p.out) + ((base + lane.row_of_warp) * (uint64_t)p.heads + (uint64_t)now.first) * a.dim;
+  };
+  const T* from = row_at(now.base);
+  const T* grad = grad_at(now.base);
+  auto ask = [&](int stage) {
+    if (ahead.base < a.rows) {
+      const int left = (ahead.base + lane.row_of_warp < a.rows ? ahead.mine : 0) - ahead.done;
 #pragma unroll
-    for (int i = 0; i < NU; ++i) {
-      x[i] = unit_of<T, V, kNext>(raw[i]);
-      g[i] = rotate<V>(unit_of<T, V, kNext>(dy[i]), c[i], s[i], lane.turned[i]);
+      for (int u = 0; u < U; ++u) {
 #pragma unroll
-      for (int k = 0; k < N; ++k) {
-        square = fma(x[i].a[k], x[i].a[k], square);
-        square = fma(x[i].b[k], x[i].b[k], square);
+        for (int i = 0; i < NU; ++i) {
+          const bool here = u < left && lane.has[i];
+          const T* at = here ? from : static_cast<const T*>(p.x);
+          const T* at_grad = here ? grad : static_cast<const T*>(p.grad);
+          copy<sizeof(Pack<T, V>)>(ring.at(stage, (u * NU + i) * 4), at + lane.lo[i], here);
+          copy<sizeof(Pack<T, V>)>(ring.at(stage, (u * NU + i) * 4 + 1), at + lane.hi[i], here);
+          copy<sizeof(Pack<T, V>)>(ring.at(stage, (u * NU + i) * 4 + 2), at_grad + lane.lo[i], here);
+          copy<sizeof(Pack<T, V>)>(ring.at(stage, (u * NU + i) * 4 + 3), at_grad + lane.hi[i], here);
+        }
+        from += x_step;
+        grad += g_step;
+      }
+      if (ahead.done == 0) {
+        const int32_t* positions = a.positions + (int64_t)ahead.base * a.position_row;
+        for (int i = threadIdx.x & 31; i < ring.count; i += 32) {
+          const bool here = ahead.base + ring.row_of[i] < a.rows;
+          copy<4>(ring.positions_of(stage) + i, positions + (here ? ring.offset[i] : 0), here);
+        }
+      }
+      if (ahead.forward<U>()) {
+        from = row_at(ahead.base);
+        grad = grad_at(ahead.base);
       }
     }
-    const float inv = rsqrtf(over_lanes(total(square), a.lanes) * inv_dim + a.eps);
-    const bool here = now.row + lane.row_of_warp < a.rows && now.head(0) < p.heads;
-    // (rows and heads that are not there are zeros, but so may be eps)
-    const Number<V> by = splat<V>(here ? inv : 0.f);
+    copies_made();
+  };
 #pragma unroll
-    for (int i = 0; i < NU; ++i) {
-      Number<V> w[N];
-      tables.read(tables.w[0], a.lanes * NU, lane.at + i * a.lanes, w);
+  for (int i = 0; i < kStages - 1; ++i) ask(i);
+  T* to = out_at(now.base);
+  Turn<V> turn[NU];
+  int stage = 0;
+  while (now.base < a.rows) {  // (whole warps)
+    ask((stage + kStages - 1) % kStages);
+    copies_here<kStages - 1>();
+    if (now.done == 0 && a.pairs) tables.angles(a, p, ring.positions_of(stage), lane.at, lane.row_of_warp, turn);
+    const int left = (now.base + lane.row_of_warp < a.rows ? now.mine : 0) - now.done;
 #pragma unroll
-      for (int k = 0; k < N; ++k) {
-        x[i].a[k] = mul(x[i].a[k], by);
-        dw[i].a[k] = fma(g[i].a[k], x[i].a[k], dw[i].a[k]);
-        g[i].a[k] = mul(g[i].a[k], w[k]);
-        dot = fma(g[i].a[k], x[i].a[k], dot);
-      }
-      tables.read(tables.w[1], a.lanes * NU, lane.at + i * a.lanes, w);
-#pragma unroll
-      for (int k = 0; k < N; ++k) {
-        x[i].b[k] = mul(x[i].b[k], by);
-        dw[i].b[k] = fma(g[i].b[k], x[i].b[k], dw[i].b[k]);
-        g[i].b[k] = mul(g[i].b[k], w[k]);
-        dot = fma(g[i].b[k], x[i].b[k], dot);
-      }
-    }
-    const Number<V> minus = splat<V>(-over_lanes(total(dot), a.lanes) * inv_dim);
-    if (here) {
-      T* to = static_cast<T*>(p.out) + ((now.row + lane.row_of_warp) * (uint64_t)p.heads + (uint64_t)now.head(0)) * a.dim;
+    for (int u = 0; u < U; ++u) {
+      Unit<V> x[NU], g[NU];
+      float square = 0.f, dot = 0.f;
 #pragma unroll
       for (int i = 0; i < NU; ++i) {
-        if (!lane.has[i]) continue;
+        const int at = (u * NU + i) * 4;
+        const Pack<T, V> raw[2] = {*ring.at(stage, at), *ring.at(stage, at + 1)}, dy[2] = {*ring.at(stage, at + 2), *ring.at(stage, at + 3)};
+        x[i] = unit_of<T, V, kNext>(raw);
+        g[i] = rotate<V>(unit_of<T, V, kNext>(dy), turn[i], lane.turned[i], part);
+        Number<V> t = mul(x[i].a[0], x[i].a[0]);
+#pragma unroll
+        for (int k = 1; k < N; ++k) t = fma(x[i].a[k], x[i].a[k], t);
+#pragma unroll
+        for (int k = 0; k < N; ++k) t = fma(x[i].b[k], x[i].b[k], t);
+        square += total(t);
+      }
+      const float inv = rsqrtf(over_lanes(square, a.lanes) * inv_dim + a.eps);
+      const Number<V> by = splat<V>(u < left ? inv : 0.f);  // (heads that are not there are zeros, but so may be eps)
+#pragma unroll
+      for (int i = 0; i < NU; ++i) {
+        Number<V> t = splat<V>(0.f);
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+          x[i].a[k] = mul(x[i].a[k], by);
+          x[i].b[k] = mul(x[i].b[k], by);
+          dw[i].a[k] = fma(g[i].a[k], x[i].a[k], dw[i].a[k]);
+          dw[i].b[k] = fma(g[i].b[k], x[i].b[k], dw[i].b[k]);
+          g[i].a[k] = mul(g[i].a[k], w[0][i][k]);
+          g[i].b[k] = mul(g[i].b[k], w[1][i][k]);
+          t = fma(g[i].a[k], x[i].a[k], t);
+          t = fma(g[i].b[k], x[i].b[k], t);
+        }
+        dot += total(t);
+      }
+      const Number<V> minus = splat<V>(-over_lanes(dot, a.lanes) * inv_dim);
+#pragma unroll
+      for (int i = 0; i < NU; ++i) {
 #pragma unroll
         for (int k = 0; k < N; ++k) {
           g[i].a[k] = mul(by, fma(x[i].a[k], minus, g[i].a[k]));
           g[i].b[k] = mul(by, fma(x[i].b[k], minus, g[i].b[k]));
         }
-        store_unit<T, V, kNext>(to + lane.lo[i], to + lane.hi[i], g[i]);
+        if (u < left && lane.has[i]) store_unit<T, V, kNext>(to + lane.lo[i], to + lane.hi[i], g[i]);
       }
+      to += out_step;
     }
-    now = then;
-#pragma unroll
-    for (int i = 0; i < NU; ++i)
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        raw[i][k] = more[i][k];
-        dy[i][k] = more_dy[i][k];
-      }
+    if (now.forward<U>()) to = out_at(now.base);
+    stage = (stage + 1) % kStages;
   }
+  copies_here<0>();
   if (!a.sums) return;  // (the same for all threads)
   // the groups of a warp hold the same channels; then the warps one after the other
   float sums[NU][2 * V];
@@ -622,6 +723,7 @@ int arguments(const rmn_rotary* p, RotaryArgs* a) {
   a->rows = p->rows;
   a->dim = p->dim;
   a->pairs = pairs;
+  a->axes = pairs ? p->axes : 0;
   a->positions = p->positions;
   a->position_row = p->position_row;
   a->position_axis = p->position_axis;
@@ -631,7 +733,7 @@ int arguments(const rmn_rotary* p, RotaryArgs* a) {
   return RMN_OK;
 }
 
-// The most pairs that a load may hold: 16 bytes, or half, a quarter ... of them where sizes, strides or pointers ask for that.
+// The most pairs that a load may hold: four, or two or one where sizes, strides or pointers ask for that.
 int pairs_a_load(const RotaryArgs& a, int elem, bool next) {
   auto fits = [&](int v) {
     if (next ? a.dim / 2 % v : a.pairs % v || (a.dim / 2 - a.pairs) % v) return false;
@@ -643,7 +745,7 @@ int pairs_a_load(const RotaryArgs& a, int elem, bool next) {
     }
     return true;
   };
-  int v = 16 / elem;
+  int v = elem == 2 ? 8 : 4;
   while (v > 1 && !fits(v)) v /= 2;
   return v;
 }
@@ -654,6 +756,8 @@ void lay_out(RotaryArgs* a, int V, int units_a_lane, uint32_t most_blocks) {
   const int units = a->dim / 2 / V;
   a->lanes = 1;
   while (a->lanes * units_a_lane < units) a->lanes *= 2;
+  a->pair_bits = 0;
+  while (1 << a->pair_bits < a->lanes * units_a_lane * V) ++a->pair_bits;
   const uint64_t heads = (uint64_t)a->part[0].heads + a->part[1].heads;
   for (Heads& p : a->part) {
     p.groups = p.warps = 1;
@@ -666,16 +770,27 @@ void lay_out(RotaryArgs* a, int V, int units_a_lane, uint32_t most_blocks) {
   }
 }
 
+template <typename T, int V, int NU, bool kNext, int kPass>  // 0: a rotation, 1: behind the norm, 2: the backward pass
+int launch_as(const RotaryArgs& a, cudaStream_t stream) {
+  static SmemOptIn opt_in;
+  constexpr bool kBackward = kPass == 2;
+  using Copies = Ring<T, V, NU, heads_at_once(kBackward), kBackward ? 2 : 1>;
+  void (*kern)(RotaryArgs);
+  if constexpr (kBackward) kern = k_rotary_backward<T, V, NU, kNext>;
+  else kern = k_rotary<T, V, NU, kNext, kPass == 1>;
+  auto positions = [&](const Heads& p) { return p.blocks ? 32 / (a.lanes * p.groups) * a.axes : 0; };
+  const size_t bytes = Copies::bytes(std::max(positions(a.part[0]), positions(a.part[1])));
+  RMN_CUDA_TRY(opt_in.apply(reinterpret_cast<const void*>(kern), Copies::bytes(32 * kMostAxes)));
+  RMN_CUDA_TRY(launch_overlapped(kern, dim3(a.part[0].blocks + a.part[1].blocks), dim3(kThreads), bytes, stream, a));
+  RMN_LAUNCH_CHECK();
+  return RMN_OK;
+}
 template <typename T, int V, int NU>
 int launch(RotaryArgs& a, bool next, bool norm, bool backward, cudaStream_t stream) {
   lay_out(&a, V, NU, backward ? kMostBackwardBlocks : 148 * 8);
-  void (*kern)(RotaryArgs);
-  if (backward) kern = next ? k_rotary_backward<T, V, NU, true> : k_rotary_backward<T, V, NU, false>;
-  else if (norm) kern = next ? k_rotary<T, V, NU, true, true> : k_rotary<T, V, NU, false, true>;
-  else kern = next ? k_rotary<T, V, NU, true, false> : k_rotary<T, V, NU, false, false>;
-  RMN_CUDA_TRY(launch_overlapped(kern, dim3(a.part[0].blocks + a.part[1].blocks), dim3(kThreads), 0, stream, a));
-  RMN_LAUNCH_CHECK();
-  return RMN_OK;
+  if (backward) return next ? launch_as<T, V, NU, true, 2>(a, stream) : launch_as<T, V, NU, false, 2>(a, stream);
+  if (norm) return next ? launch_as<T, V, NU, true, 1>(a, stream) : launch_as<T, V, NU, false, 1>(a, stream);
+  return next ? launch_as<T, V, NU, true, 0>(a, stream) : launch_as<T, V, NU, false, 0>(a, stream);
 }
 int run(RotaryArgs& a, int dtype, bool next, bool norm, bool backward, cudaStream_t stream) {
   const int v = pairs_a_load(a, dtype == RMN_F32 ? 4 : 2, next);
