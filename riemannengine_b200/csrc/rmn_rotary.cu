@@ -29,7 +29,7 @@ namespace rmn {
 namespace {
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
-constexpr uint32_t kMostBackwardBlocks = 148 * 4;
+constexpr uint32_t kMostBlocks = 148 * 2;  // as many as fit the SMs at once
 constexpr int kMostAxes = 8;
 constexpr int kMostDim = 256;
 
@@ -190,6 +190,7 @@ template <int V, int NU, bool kNext>
 struct Lane {
   int at, group, row_of_warp;  // lane of its head, group of its row, row of the warp
   int lo[NU], hi[NU];          // channels of the two loads
+  int64_t to_lo[NU], to_hi[NU];  // from lo[0]
   int turned[NU];              // pairs of the unit that turn
   bool has[NU];
   __device__ __forceinline__ Lane(const RotaryArgs& a, const Heads& p) {
@@ -214,6 +215,11 @@ struct Lane {
         lo[i] = first + a.pairs;
         hi[i] = first + a.dim / 2;
       }
+    }
+#pragma unroll
+    for (int i = 0; i < NU; ++i) {
+      to_lo[i] = has[i] ? lo[i] - lo[0] : 0;
+      to_hi[i] = has[i] ? hi[i] - lo[0] : 0;
     }
   }
 };
@@ -278,11 +284,13 @@ struct alignas(16) Tables {
     float* cosines = turns[threadIdx.x >> 5][0];
     float* sines = turns[threadIdx.x >> 5][1];
     __syncwarp();  // the angles before have been read, and all lanes' copies are here
+    const float sign = a.back ? -1.f : 1.f;
+#pragma unroll 4
     for (int i = threadIdx.x & 31; i < n; i += 32) {
       float c, s;
       turn_of(positions[place[i]], fraction[i & (of_row - 1)], c, s);
       cosines[i] = c;
-      sines[i] = a.back ? -s : s;
+      sines[i] = s * sign;
     }
     __syncwarp();
 #pragma unroll
@@ -366,13 +374,13 @@ __device__ __forceinline__ float over_lanes(float v, int lanes) {
 
 // The rows of a warp, and the heads of a group: rows base, base + step ...; heads first, first + next ...
 struct Walk {
-  uint64_t base, step;
+  uint32_t base, step;  // (fewer than 2^31 rows)
   int first, next, mine, most;  // heads of the group, of the warp's first one
   int done;                     // heads of the group before this batch
   __device__ __forceinline__ Walk(const RotaryArgs& a, const Heads& p, uint32_t block, int group) {
     const uint32_t warp = block * kWarps + (threadIdx.x >> 5), rows = 32 / (a.lanes * p.groups);
-    base = (uint64_t)(warp / p.warps) * rows;
-    step = (uint64_t)(p.blocks * kWarps / p.warps) * rows;
+    base = min(warp / p.warps * rows, a.rows);
+    step = p.blocks * kWarps / p.warps * rows;
     first = (int)(warp % p.warps) * p.groups + group;
     next = p.groups * p.warps;
     auto heads = [&](int from) { return from < p.heads ? (p.heads - from + next - 1) / next : 0; };
@@ -418,11 +426,11 @@ __global__ void __launch_bounds__(kThreads, 2) k_rotary(const __grid_constant__ 
       tables.read(tables.w[1] + (lane.at + i * a.lanes) * V, w[1][i]);
     }
   }
-  auto row_at = [&](uint64_t base) {
-    return static_cast<const T*>(p.x) + (int64_t)(base + lane.row_of_warp) * p.row + (int64_t)now.first * p.head;
+  auto row_at = [&](uint32_t base) {
+    return static_cast<const T*>(p.x) + (int64_t)(base + lane.row_of_warp) * p.row + (int64_t)now.first * p.head + lane.lo[0];
   };
-  auto out_at = [&](uint64_t base) {
-    return static_cast<T*>(p.out) + ((base + lane.row_of_warp) * (uint64_t)p.heads + (uint64_t)now.first) * a.dim;
+  auto out_at = [&](uint32_t base) {
+    return static_cast<T*>(p.out) + ((uint64_t)(base + lane.row_of_warp) * (uint32_t)p.heads + (uint32_t)now.first) * (uint32_t)a.dim + lane.lo[0];
   };
   const T* from = row_at(now.base);
   // the copies of the batch that is kStages - 1 ahead
@@ -435,8 +443,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_rotary(const __grid_constant__ 
         for (int i = 0; i < NU; ++i) {
           const bool here = u < left && lane.has[i];
           const T* at = here ? from : static_cast<const T*>(p.x);
-          copy<sizeof(Pack<T, V>)>(ring.at(stage, (u * NU + i) * 2), at + lane.lo[i], here);
-          copy<sizeof(Pack<T, V>)>(ring.at(stage, (u * NU + i) * 2 + 1), at + lane.hi[i], here);
+          copy<sizeof(Pack<T, V>)>(ring.at(stage, (u * NU + i) * 2), at + lane.to_lo[i], here);
+          copy<sizeof(Pack<T, V>)>(ring.at(stage, (u * NU + i) * 2 + 1), at + lane.to_hi[i], here);
         }
         from += in_step;
       }
@@ -491,7 +499,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_rotary(const __grid_constant__ 
 #pragma unroll
       for (int i = 0; i < NU; ++i) {
         const Unit<V> y = rotate<V>(x[i], turn[i], lane.turned[i], part);
-        if (u < left && lane.has[i]) store_unit<T, V, kNext>(to + lane.lo[i], to + lane.hi[i], y);
+        if (u < left && lane.has[i]) store_unit<T, V, kNext>(to + lane.to_lo[i], to + lane.to_hi[i], y);
       }
       to += out_step;
     }
@@ -527,14 +535,14 @@ __global__ void __launch_bounds__(kThreads, 2) k_rotary_backward(const __grid_co
 #pragma unroll
     for (int k = 0; k < N; ++k) dw[i].a[k] = dw[i].b[k] = splat<V>(0.f);
   }
-  auto row_at = [&](uint64_t base) {
-    return static_cast<const T*>(p.x) + (int64_t)(base + lane.row_of_warp) * p.row + (int64_t)now.first * p.head;
+  auto row_at = [&](uint32_t base) {
+    return static_cast<const T*>(p.x) + (int64_t)(base + lane.row_of_warp) * p.row + (int64_t)now.first * p.head + lane.lo[0];
   };
-  auto grad_at = [&](uint64_t base) {
-    return static_cast<const T*>(p.grad) + (int64_t)(base + lane.row_of_warp) * p.grad_row + (int64_t)now.first * p.grad_head;
+  auto grad_at = [&](uint32_t base) {
+    return static_cast<const T*>(p.grad) + (int64_t)(base + lane.row_of_warp) * p.grad_row + (int64_t)now.first * p.grad_head + lane.lo[0];
   };
-  auto out_at = [&](uint64_t base) {
-    return static_cast<T*>(p.out) + ((base + lane.row_of_warp) * (uint64_t)p.heads + (uint64_t)now.first) * a.dim;
+  auto out_at = [&](uint32_t base) {
+    return static_cast<T*>(p.out) + ((uint64_t)(base + lane.row_of_warp) * (uint32_t)p.heads + (uint32_t)now.first) * (uint32_t)a.dim + lane.lo[0];
   };
   const T* from = row_at(now.base);
   const T* grad = grad_at(now.base);
@@ -548,10 +556,10 @@ __global__ void __launch_bounds__(kThreads, 2) k_rotary_backward(const __grid_co
           const bool here = u < left && lane.has[i];
           const T* at = here ? from : static_cast<const T*>(p.x);
           const T* at_grad = here ? grad : static_cast<const T*>(p.grad);
-          copy<sizeof(Pack<T, V>)>(ring.at(stage, (u * NU + i) * 4), at + lane.lo[i], here);
-          copy<sizeof(Pack<T, V>)>(ring.at(stage, (u * NU + i) * 4 + 1), at + lane.hi[i], here);
-          copy<sizeof(Pack<T, V>)>(ring.at(stage, (u * NU + i) * 4 + 2), at_grad + lane.lo[i], here);
-          copy<sizeof(Pack<T, V>)>(ring.at(stage, (u * NU + i) * 4 + 3), at_grad + lane.hi[i], here);
+          copy<sizeof(Pack<T, V>)>(ring.at(stage, (u * NU + i) * 4), at + lane.to_lo[i], here);
+          copy<sizeof(Pack<T, V>)>(ring.at(stage, (u * NU + i) * 4 + 1), at + lane.to_hi[i], here);
+          copy<sizeof(Pack<T, V>)>(ring.at(stage, (u * NU + i) * 4 + 2), at_grad + lane.to_lo[i], here);
+          copy<sizeof(Pack<T, V>)>(ring.at(stage, (u * NU + i) * 4 + 3), at_grad + lane.to_hi[i], here);
         }
         from += x_step;
         grad += g_step;
@@ -623,7 +631,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_rotary_backward(const __grid_co
           g[i].a[k] = mul(by, fma(x[i].a[k], minus, g[i].a[k]));
           g[i].b[k] = mul(by, fma(x[i].b[k], minus, g[i].b[k]));
         }
-        if (u < left && lane.has[i]) store_unit<T, V, kNext>(to + lane.lo[i], to + lane.hi[i], g[i]);
+        if (u < left && lane.has[i]) store_unit<T, V, kNext>(to + lane.to_lo[i], to + lane.to_hi[i], g[i]);
       }
       to += out_step;
     }
@@ -787,7 +795,7 @@ int launch_as(const RotaryArgs& a, cudaStream_t stream) {
 }
 template <typename T, int V, int NU>
 int launch(RotaryArgs& a, bool next, bool norm, bool backward, cudaStream_t stream) {
-  lay_out(&a, V, NU, backward ? kMostBackwardBlocks : 148 * 8);
+  lay_out(&a, V, NU, kMostBlocks);
   if (backward) return next ? launch_as<T, V, NU, true, 2>(a, stream) : launch_as<T, V, NU, false, 2>(a, stream);
   if (norm) return next ? launch_as<T, V, NU, true, 1>(a, stream) : launch_as<T, V, NU, false, 1>(a, stream);
   return next ? launch_as<T, V, NU, true, 0>(a, stream) : launch_as<T, V, NU, false, 0>(a, stream);
@@ -822,7 +830,7 @@ extern "C" int rmn_rotary_forward(const rmn_rotary* problem, void* d_q_out, void
 }
 
 extern "C" size_t rmn_rotary_backward_workspace_bytes(const rmn_rotary* problem) {
-  return problem && problem->norm && problem->dim > 0 ? (size_t)kMostBackwardBlocks * 2 * (size_t)problem->dim * sizeof(float) : 0;
+  return problem && problem->norm && problem->dim > 0 ? (size_t)kMostBlocks * 2 * (size_t)problem->dim * sizeof(float) : 0;
 }
 
 extern "C" int rmn_rotary_backward(const rmn_rotary* problem, const void* d_grad_q, int64_t grad_q_row, int64_t grad_q_head,

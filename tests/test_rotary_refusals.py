@@ -47,7 +47,7 @@ def test_arguments():
                    dict(strides=(-1, 32, 64, 32)), dict(strides=(128, 32, 64, -32))):
         assert backward(_problem(), **change) == capi.ERR_BAD_ARG, change
     need = lib.rmn_rotary_backward_workspace_bytes(ctypes.byref(_problem()))
-    assert need == 592 * 2 * 32 * 4 and backward(_problem(), nbytes=need - 1) == capi.ERR_ALLOC
+    assert need == 296 * 2 * 32 * 4 and backward(_problem(), nbytes=need - 1) == capi.ERR_ALLOC
     # without a norm there are no weights
     assert lib.rmn_rotary_backward_workspace_bytes(ctypes.byref(_problem(norm=0))) == 0
     assert backward(_problem(norm=0)) == capi.ERR_BAD_ARG
