@@ -128,13 +128,16 @@ __device__ __forceinline__ int32_t tiles_of(int32_t rows, int tile_rows) {
 // Windows. Query row i of a segment stands at place i + n_k - n_q of its keys. It sees the keys whose distance from there is less than the
 // window (causal: those up to its own place), and the sinks, the first keys of the sample (causal: of those up to its own place).
 __device__ __forceinline__ int32_t clamp_to(int64_t v, int32_t most) { return (int32_t)max((int64_t)0, min(v, (int64_t)most)); }
+// v - back and v + on, held to 0 ... most (back, on >= 0): in 32 bits, which no step leaves (a block waits for these numbers)
+__device__ __forceinline__ int32_t back_from(int32_t v, int32_t back, int32_t most) { return v <= back ? 0 : min(v - back, most); }
+__device__ __forceinline__ int32_t on_from(int32_t v, int32_t on, int32_t most) { return v >= most - on ? most : max(v + on, 0); }
 struct RowWindow {
   int32_t low, end, sinks;  // keys of the window, and those of the sinks: 0 ... sinks - 1. Nothing is checked for sense: low may pass end
 };
 __device__ __forceinline__ RowWindow row_window(const AttnArgs& a, const Segment& g, int32_t i) {
-  const int64_t place = (int64_t)i + g.n_k - g.n_q;
-  const int32_t most = a.causal ? clamp_to(place + 1, g.n_k) : g.n_k;
-  return {clamp_to(place - a.window + 1, g.n_k), a.causal ? most : clamp_to(place + a.window, g.n_k), min(a.sinks, most)};
+  const int32_t place = i + (g.n_k - g.n_q);  // (rows behind the last one may run over: nothing of theirs is used)
+  const int32_t most = a.causal ? max(0, min(place + 1, g.n_k)) : g.n_k;
+  return {back_from(place, a.window - 1, g.n_k), a.causal ? most : on_from(place, a.window, g.n_k), min(a.sinks, most)};
 }
 // The keys that one query row sees: those below `sinks`, and those from `low` to `end` - 1 (all of them together where they meet).
 struct RowKeys {
@@ -283,6 +286,28 @@ __device__ __forceinline__ void scan_block(int32_t mine, int32_t* warp_sums, int
   }
 }
 
+// A warp's search (see find_tile); false where the number is of no tile.
+template <TilesOf kOf>
+__device__ __forceinline__ bool search_tile(const AttnArgs& a, uint32_t want, int tile_rows, FoundTile* found) {
+  const uint32_t n = a.sequences + 2;
+  const int32_t* at = kOf == TilesOf::kQueries ? a.offsets : a.kv_offsets;
+  const uint32_t rows = kOf == TilesOf::kQueries ? a.rows_q : a.rows_k, lane = threadIdx.x & 31;
+  auto number = [&](uint32_t j) { return j == 0 ? 0u : (uint32_t)clamp_row(__ldg(at + j - 1), rows) / (uint32_t)tile_rows + j; };
+  uint32_t lo = 0, len = n;  // number(lo) <= want
+  while (len > 1) {
+    const uint32_t step = (len + 31) / 32, p = lane * step;
+    const uint32_t below = __ballot_sync(0xffffffffu, p < len && number(lo + p) <= want);
+    const uint32_t skip = (31 - __clz((int)(below | 1u))) * step;
+    lo += skip;
+    len = min(step, len - skip);
+  }
+  const Segment g = segment(a, lo == 0 ? a.sequences + 1 : lo - 1);
+  const int32_t tiles = segment_tiles<kOf>(g, tile_rows), tile = (int32_t)(want - number(lo));
+  if (tile < 0 || tile >= tiles) return false;
+  *found = {g, tile, tiles};
+  return true;
+}
+
 // Up to kCountedSamples (384) samples: every thread counts the tiles of a run of segments, a scan over the block places them, and the
 // numbers behind the last tile are of no tile. Beyond, counting would cost the square of the samples: segment j in the order of the
 // rows (those before the first sample, the samples, those behind) begins at row b(j) and has the numbers from b(j) / tile_rows + j
@@ -317,22 +342,10 @@ __device__ __forceinline__ bool find_tile(const AttnArgs& a, uint32_t want, int 
       }
     }
   } else {
-    const int32_t* at = kOf == TilesOf::kQueries ? a.offsets : a.kv_offsets;
-    const uint32_t rows = kOf == TilesOf::kQueries ? a.rows_q : a.rows_k, lane = threadIdx.x & 31;
     if (want < n && threadIdx.x == 0) segment(a, want);  // every segment is looked at: the search may step over some that are wrong
-    auto number = [&](uint32_t j) { return j == 0 ? 0u : (uint32_t)clamp_row(__ldg(at + j - 1), rows) / (uint32_t)tile_rows + j; };
-    uint32_t lo = 0, len = n;  // number(lo) <= want
-    while (len > 1) {
-      const uint32_t step = (len + 31) / 32, p = lane * step;
-      const uint32_t below = __ballot_sync(0xffffffffu, p < len && number(lo + p) <= want);
-      const uint32_t skip = (31 - __clz((int)(below | 1u))) * step;
-      lo += skip;
-      len = min(step, len - skip);
-    }
-    const Segment g = segment(a, lo == 0 ? a.sequences + 1 : lo - 1);
-    const int32_t tiles = segment_tiles<kOf>(g, tile_rows), tile = (int32_t)(want - number(lo));
-    if (tile < 0 || tile >= tiles) return false;
-    if (threadIdx.x == 0) *found = {g, tile, tiles};
+    FoundTile mine;
+    if (!search_tile<kOf>(a, want, tile_rows, &mine)) return false;
+    if (threadIdx.x == 0) *found = mine;
   }
   __syncthreads();
   return true;
@@ -382,6 +395,7 @@ int attention_simt_forward(const AttnArgs& a, int dtype, cudaStream_t stream);
 int attention_simt_backward(const AttnArgs& a, int dtype, cudaStream_t stream);
 int attention_tc_forward(const AttnArgs& a, cudaStream_t stream);  // bf16
 int attention_tc_backward(const AttnArgs& a, cudaStream_t stream);
+int attention_window_forward(const AttnArgs& a, cudaStream_t stream);  // what attention_tc_forward does with a window
 int attention_sinks_sum(const AttnArgs& a, int dtype, cudaStream_t stream);  // behind a backward pass that has cut samples
 // few query rows a sample: chunks of the keys, then their sum. Scratch bytes, 0 where this form is not meant for the sizes
 size_t attention_rows_workspace(uint32_t rows_q, uint32_t rows_k, uint32_t sequences, int heads, int kv_heads, int dim, int dtype,

@@ -400,12 +400,13 @@ int attention_tc_forward(const AttnArgs& a, cudaStream_t stream) {
   using namespace tc;
   if (a.dim > 128 || !(a.scale > 0.f) || a.rows_k == 0 || ((uintptr_t)a.out & 15) || ((uintptr_t)a.low & 15))
     return RMN_ERR_UNSUPPORTED;
+  if (a.window && a.dim <= 64) return attention_window_forward(a, stream);
   CUtensorMap q, k, v;
   if (!make_head_map(&q, a.q, a.rows_q, a.heads, a.dim, a.q_row, a.q_head) ||
       !make_head_map(&k, a.k, a.rows_k, a.kv_heads, a.dim, a.k_row, a.k_head) ||
       !make_head_map(&v, a.v, a.rows_k, a.kv_heads, a.dim, a.v_row, a.v_head))
     return RMN_ERR_UNSUPPORTED;
-  if (a.window) return a.dim <= 64 ? launch_fwd<64, 1, true>(q, k, v, a, stream) : launch_fwd<128, 1, true>(q, k, v, a, stream);
+  if (a.window) return launch_fwd<128, 1, true>(q, k, v, a, stream);
   if (a.dim <= 64) return launch_fwd<64, 1, false>(q, k, v, a, stream);
   // two query tiles a block read the keys half as often, one leaves two blocks an SM: 16 heads of 128, one causal sample of 8192
   // rows 249 us with two and 260 with one (262 with two since the waits are votes); 100 samples of 256 rows, 8 heads, 76 and 66.5; 12 of

@@ -1,0 +1,491 @@
+// Attention with a sliding window and sinks on the tensor cores, bf16, head sizes up to 128 (multiples of 8): the forward pass and dQ. The
+// mathematics and the layouts are those of rmn_attention_fwd.cu and rmn_attention_bwd.cu; the keys that a tile of 128 queries sees are
+// those of the window and the sinks (KeyWalk).
+//
+// Such a tile has few steps over keys, so that what surrounds them - to find the tile, to fetch the first rows, to store the last ones -
+// costs as much as the steps (a block a tile: 13 000 clocks for two steps, 6 000 of them around). So blocks stay and take one tile after
+// the other, `gridDim.x` apart, and the steps of all of them run as one chain: the copying warp finds the next tile and fetches its rows while
+// the steps of this one are under way, and the next tile's scores are made while this one's output is stored. Every barrier is waited
+// for phase by phase across tiles: a step's number counts from the block's first one. What a tile is goes from the copying warp to the
+// others through a ring of four places.
+#include "rmn_attention_tc.cuh"
+
+#include <math_constants.h>
+
+#include <algorithm>
+#include <atomic>
+
+namespace rmn {
+namespace tc {
+namespace {
+
+constexpr float kRescale = 8.f;  // log2 of how far a row's maximum may rise before O is scaled
+constexpr int kItems = 4;        // tiles on their way to the warps
+constexpr int kKeys = 128;       // of a step
+
+// A tile of one head, with its keys: the copying warp works ahead, the others would wait for such numbers.
+struct Item {
+  Segment g;
+  int32_t first, head, there;  // first query row; there: 0 behind the last tile
+  KeyWalk<true, kKeys> walk;
+};
+struct Items {
+  uint64_t full[kItems], empty[kItems];
+  alignas(16) unsigned char item[kItems][sizeof(Item)];
+  int32_t starts[kCountedSamples + 3];  // the first tile of every segment, and all tiles
+  int32_t warp_sums[12];
+};
+
+__device__ __forceinline__ void init_items(Items* items, int readers) {
+  for (int i = 0; i < kItems; ++i) {
+    mbar_init(&items->full[i], 1);
+    mbar_init(&items->empty[i], readers);
+  }
+}
+// All threads: where the segments' tiles of `rows` query rows begin, for up to kCountedSamples samples.
+template <int kThreads>
+__device__ __forceinline__ void count_tiles(const AttnArgs& a, Items* items) {
+  const uint32_t n = a.sequences + 2;
+  if (a.sequences > kCountedSamples) return;
+  const uint32_t per = (n + kThreads - 1) / kThreads, lo = min(threadIdx.x * per, n), hi = min(lo + per, n);
+  int32_t mine = 0, first, all;
+  for (uint32_t s = lo; s < hi; ++s) mine = add_tiles(mine, segment_tiles<TilesOf::kQueries>(segment(a, s), 128));
+  bool unused = false;
+  scan_block<kThreads>(mine, items->warp_sums, first, all, unused);
+  for (uint32_t s = lo; s < hi; ++s) {
+    items->starts[s] = first;
+    first = add_tiles(first, segment_tiles<TilesOf::kQueries>(segment(a, s), 128));
+  }
+  if (threadIdx.x == 0) items->starts[n] = all;
+  __syncthreads();
+}
+enum class Found { kTile, kNone, kEnd };
+// A warp: the tile of a number; kNone: there is none, but there may be further ones.
+__device__ __forceinline__ Found look_up(const AttnArgs& a, const Items* items, uint32_t want, FoundTile* found) {
+  const uint32_t n = a.sequences + 2, lane = threadIdx.x & 31;
+  if (a.sequences > kCountedSamples) {
+    if (want < n && lane == 0) segment(a, want);  // every segment is looked at: the search may step over some that are wrong
+    return search_tile<TilesOf::kQueries>(a, want, 128, found) ? Found::kTile : Found::kNone;
+  }
+  if (want >= (uint32_t)items->starts[n]) return Found::kEnd;
+  uint32_t lo = 0, len = n;  // starts[lo] <= want: the last such segment, which is one that has tiles
+  while (len > 1) {
+    const uint32_t step = (len + 31) / 32, p = lane * step;
+    const uint32_t below = __ballot_sync(0xffffffffu, p < len && (uint32_t)items->starts[lo + p] <= want);
+    const uint32_t skip = (31 - __clz((int)(below | 1u))) * step;
+    lo += skip;
+    len = min(step, len - skip);
+  }
+  const Segment g = segment(a, lo);
+  const int32_t tiles = segment_tiles<TilesOf::kQueries>(g, 128), tile = (int32_t)want - items->starts[lo];
+  if (tile >= tiles) return Found::kNone;  // (offsets that make no sense)
+  *found = {g, tile, tiles};
+  return Found::kTile;
+}
+__device__ __forceinline__ Item no_item(const AttnArgs& a) { return {{}, 0, 0, 0, {a, {}, 0, 0}}; }
+// A warp that reads the ring: the next tile; false behind the last one, or where a wait ran out.
+__device__ __forceinline__ bool next_item(Items* items, uint32_t& n, Item& item, bool& timed_out) {
+  const uint32_t slot = n % kItems;
+  if (!warp_wait(&items->full[slot], (n / kItems) & 1u)) {
+    timed_out = true;
+    return false;
+  }
+  item = *reinterpret_cast<const Item*>(items->item[slot]);
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(&items->empty[slot]);
+  ++n;
+  return item.there != 0;
+}
+// The copying warp: `fetch(item, steps before)` asks for a tile's rows, lane 0 alone; false where a wait ran out.
+template <class Fetch>
+__device__ __forceinline__ void hand_out(const AttnArgs& a, Items* items, uint32_t numbers, bool& timed_out, Fetch&& fetch) {
+  const int lane = threadIdx.x & 31;
+  uint32_t n = 0;
+  auto put = [&](const Item& item) {
+    const uint32_t slot = n % kItems;
+    if (!warp_wait(&items->empty[slot], ((n / kItems) & 1u) ^ 1u)) {
+      timed_out = true;
+      return;
+    }
+    if (lane == 0) {
+      *reinterpret_cast<Item*>(items->item[slot]) = item;
+      mbar_arrive(&items->full[slot]);
+    }
+    __syncwarp();
+    ++n;
+  };
+  for (uint64_t i = blockIdx.x; i < (uint64_t)numbers * a.heads && !timed_out; i += gridDim.x) {
+    FoundTile found;
+    const Found there = look_up(a, items, (uint32_t)(i / a.heads), &found);
+    if (there == Found::kEnd) break;
+    if (there == Found::kNone) continue;
+    // (the tiles that see the most keys first)
+    const int32_t first = (found.tiles - 1 - found.tile) * 128;
+    const Item item = {found.g, first, (int32_t)(i % a.heads), 1, {a, found.g, first, min(first + 128, found.g.n_q) - 1}};
+    put(item);
+    if (timed_out) break;
+    bool ok = true;
+    if (lane == 0) ok = fetch(item);
+    timed_out = __any_sync(0xffffffffu, !ok);
+  }
+  if (!timed_out) put(no_item(a));
+}
+
+// ------------------------------ forward ------------------------------------------------
+template <int DP>
+struct FwdShape {
+  static constexpr int ATOMS = DP / 64;
+  static constexpr uint32_t TILE = ATOMS * kAtomBytes;
+  static constexpr bool kAlias = DP == 128;  // P in the columns of S
+  static constexpr int SLOTS = DP == 128 ? 2 : 4;
+  static constexpr int THREADS = 256;
+  static constexpr int SOFTMAX_REGS = 200, OTHER_REGS = 56;
+  static constexpr int ALL_REGS = 128 * SOFTMAX_REGS + 128 * OTHER_REGS;
+  static constexpr uint32_t COLUMNS = 256;
+  static constexpr uint32_t S0 = 0, P0 = kAlias ? 0 : 128, O0 = kAlias ? 128 : 192;
+  static constexpr uint32_t TAIL = (1 + SLOTS) * TILE;
+  static constexpr size_t SMEM = TAIL + 4096 + 1024;  // (1024: the tiles start on a swizzle's period)
+};
+struct FwdTail {
+  uint64_t full[4], empty[4], q_full, q_empty, s_full, s_free, p_full, o_done;
+  Items items;
+  uint32_t tmem_slot;
+};
+static_assert(sizeof(FwdTail) <= 4096, "tail");
+constexpr int kSoftmaxWarps = 4;
+
+template <int DP>
+__global__ void __launch_bounds__(FwdShape<DP>::THREADS, 2)
+    k_window_fwd(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                 const __grid_constant__ CUtensorMap map_v, const AttnArgs a, const uint32_t numbers) {
+  using C = FwdShape<DP>;
+  constexpr int SLOTS = C::SLOTS;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  FwdTail* tail = reinterpret_cast<FwdTail*>(smem + C::TAIL);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  constexpr int kCopyWarp = 4, kMmaWarp = 5;
+  if (tid == 0) {
+    for (int s = 0; s < SLOTS; ++s) {
+      mbar_init(&tail->full[s], 1);
+      mbar_init(&tail->empty[s], 1);
+    }
+    uint64_t* ones[] = {&tail->q_full, &tail->q_empty, &tail->s_full, &tail->o_done};
+    for (uint64_t* b : ones) mbar_init(b, 1);
+    mbar_init(&tail->s_free, 128);
+    mbar_init(&tail->p_full, 128);
+    init_items(&tail->items, kSoftmaxWarps + 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_proxy_async();
+  }
+  if (warp == kMmaWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tail->tmem_slot)),
+                 "r"(C::COLUMNS)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  if (warp == kCopyWarp && lane == 0) {
+    tma_prefetch_map(&map_q);
+    tma_prefetch_map(&map_k);
+    tma_prefetch_map(&map_v);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  after_previous_kernel();
+  count_tiles<C::THREADS>(a, &tail->items);
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&tail->tmem_slot);
+  const uint32_t smem_base = smem_u32(smem), slots = smem_base + C::TILE;
+  bool timed_out = false;
+
+  auto softmax = [&] {
+    // ------------------------------ softmax --------------------------------------------
+    const uint32_t lanes = ((uint32_t)warp * 32u) << 16;
+    const uint32_t s_t = tmem + lanes + C::S0, p_t = tmem + lanes + C::P0, o_t = tmem + lanes + C::O0;
+    const float scale = a.scale * kLog2e;  // (> 0)
+    uint32_t n = 0, step = 0;
+    Item item = no_item(a);
+    while (next_item(&tail->items, n, item, timed_out)) {
+      const Segment& g = item.g;
+      const KeyWalk<true, kKeys>& walk = item.walk;
+      const int row = item.first + tid;
+      const RowKeys seen = row_keys<true>(a, g, row);
+      float m = -CUDART_INF_F, l = 0.f;  // maximum in use (times scale, log 2), sum
+      for (int j = 0; j < walk.tiles; ++j, ++step) {
+        const uint32_t ph = step & 1u;
+        if (!warp_wait(&tail->s_full, ph)) { timed_out = true; break; }
+        tc_fence_after();
+        uint32_t r[128];
+        tc_ld32_at<0>(s_t, r);
+        tc_ld32_at<32>(s_t + 32, r);
+        tc_ld32_at<64>(s_t + 64, r);
+        tc_ld32_at<96>(s_t + 96, r);
+        tc_wait_ld();
+        if constexpr (!C::kAlias) {
+          tc_fence_before();
+          mbar_arrive(&tail->s_free);
+        }
+        // 32 columns at a time: those that no row of the warp sees cost nothing, those that all see no masking
+        const int k0 = walk.key(j);
+        uint32_t some = 0;  // bit k: a row sees one of columns 32 k ... 32 k + 31
+        float m_new = -CUDART_INF_F;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t bits = seen_bits(seen, k0, k);
+          if (__all_sync(0xffffffffu, bits == 0u)) continue;
+          some |= 1u << k;
+          if (!__all_sync(0xffffffffu, bits == 0xffffffffu)) {
+#pragma unroll
+            for (int c = 0; c < 32; ++c)
+              if (!(bits >> c & 1u)) r[k * 32 + c] = 0xff800000u;
+          }
+          float top[2] = {-CUDART_INF_F, -CUDART_INF_F};
+#pragma unroll
+          for (int c = 0; c < 32; c += 4)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              top[e] = max3(top[e], __uint_as_float(r[k * 32 + c + 2 * e]), __uint_as_float(r[k * 32 + c + 2 * e + 1]));
+          m_new = max3(m_new, top[0], top[1]);
+        }
+        m_new = fmaxf(m, m_new * scale);
+        const bool rise = m_new > m + kRescale;  // (from -infinity: always, unless nothing is seen yet)
+        float shrink = 1.f;
+        if (rise) {
+          shrink = exp2_approx(m - m_new);
+          l *= shrink;
+          m = m_new;
+        }
+        const float base = m == -CUDART_INF_F ? 0.f : m;
+        const Pair by = make_pair(scale, scale), minus = make_pair(-base, -base);
+        Pair sum[2] = {make_pair(0.f, 0.f), make_pair(0.f, 0.f)};
+        uint32_t p[64];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if (some >> k & 1u) {
+#pragma unroll
+            for (int c = 32 * k; c < 32 * k + 32; c += 2) {
+              float x, y;
+              parts(fma(pair_of(r[c], r[c + 1]), by, minus), x, y);
+              x = exp2_approx(x);
+              y = exp2_approx(y);
+              sum[(c >> 1) & 1] = add(sum[(c >> 1) & 1], make_pair(x, y));
+              p[c / 2] = pack_bf16(x, y);
+            }
+          } else {
+#pragma unroll
+            for (int c = 0; c < 16; ++c) p[16 * k + c] = 0u;
+          }
+        }
+        l += total(add(sum[0], sum[1]));
+        if (j > 0) {
+          // P and O of the step before are free (kAlias: these scores were made behind that; j == 0: O has been stored)
+          if constexpr (!C::kAlias) {
+            if (!warp_wait(&tail->o_done, ph ^ 1u)) { timed_out = true; break; }
+            tc_fence_after();
+          }
+          if (__any_sync(0xffffffffu, rise)) {
+#pragma unroll
+            for (int c = 0; c < DP; c += 32) {
+              uint32_t o[32];
+              tc_ld32(o_t + c, o);
+              tc_wait_ld();
+#pragma unroll
+              for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * shrink);
+              tc_st32<0>(o_t + c, o);
+            }
+          }
+        }
+        tc_st32<0>(p_t, p);
+        tc_st32<32>(p_t + 32, p);
+        tc_wait_st();
+        tc_fence_before();
+        mbar_arrive(&tail->p_full);
+      }
+      if (timed_out) break;
+      // ------------------------------ output -------------------------------------------
+      if (walk.tiles > 0) {
+        if (!warp_wait(&tail->o_done, (step - 1) & 1u)) { timed_out = true; break; }
+        tc_fence_after();
+      }
+      const bool mine = row < g.n_q;
+      const float by = l == 0.f ? 0.f : 1.f / l;
+      const size_t at = ((size_t)(g.q0 + row) * a.heads + item.head) * a.dim;
+      __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + at;
+      __nv_bfloat16* low = a.low ? static_cast<__nv_bfloat16*>(a.low) + at : nullptr;
+#pragma unroll
+      for (int c = 0; c < DP; c += 32) {
+        if (c >= a.dim) break;
+        uint32_t o[32];
+        if (walk.tiles > 0) {
+          tc_ld32(o_t + c, o);
+          tc_wait_ld();
+        }
+#pragma unroll
+        for (int k = 0; k < 32; ++k) o[k] = l == 0.f ? 0u : __float_as_uint(__uint_as_float(o[k]) * by);
+#pragma unroll
+        for (int k = 0; k < 32; k += 8) {
+          if (!mine || c + k >= a.dim) continue;
+          uint32_t hi[4], lo[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float x = __uint_as_float(o[k + 2 * e]), y = __uint_as_float(o[k + 2 * e + 1]);
+            hi[e] = pack_bf16(x, y);
+            lo[e] = pack_bf16(x - __uint_as_float(hi[e] << 16), y - __uint_as_float(hi[e] & 0xffff0000u));
+          }
+          *reinterpret_cast<uint4*>(out + c + k) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+          if (low) *reinterpret_cast<uint4*>(low + c + k) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        }
+      }
+      tc_fence_before();  // (the next output takes its place behind this thread's next P)
+      if (mine && a.lse)
+        a.lse[(size_t)item.head * a.rows_q + g.q0 + row] = l == 0.f ? -CUDART_INF_F : (m + log2f(l)) * kLn2;
+    }
+  };
+  auto others = [&] {
+    if (warp == kCopyWarp) {
+      // ------------------------------ bulk copies ----------------------------------------
+      uint32_t i = 0, tiles = 0;  // keys' and values' loads: K 0, V 0, K 1, V 1, ...; tiles with keys
+      hand_out(a, &tail->items, numbers, timed_out, [&](const Item& item) {
+        const KeyWalk<true, kKeys>& walk = item.walk;
+        if (walk.tiles == 0) return true;
+        const int kv = item.head / (a.heads / a.kv_heads);
+        if (!mbar_wait(&tail->q_empty, (tiles & 1u) ^ 1u)) return false;
+        ++tiles;
+        mbar_arrive_expect_tx(&tail->q_full, C::TILE);
+#pragma unroll
+        for (int c = 0; c < C::ATOMS; ++c)
+          tma_load_3d(smem_base + c * kAtomBytes, &map_q, &tail->q_full, c * 64, item.head, item.g.q0 + item.first);
+        for (int j = 0; j < 2 * walk.tiles; ++j, ++i) {
+          const uint32_t s = i % SLOTS;
+          if (!mbar_wait(&tail->empty[s], ((i / SLOTS) & 1u) ^ 1u)) return false;
+          mbar_arrive_expect_tx(&tail->full[s], C::TILE);
+          const CUtensorMap* map = (j & 1) ? &map_v : &map_k;
+#pragma unroll
+          for (int c = 0; c < C::ATOMS; ++c)
+            tma_load_3d(slots + s * C::TILE + c * kAtomBytes, map, &tail->full[s], c * 64, kv, item.g.k0 + walk.key(j >> 1));
+        }
+        return true;
+      });
+      if (timed_out && lane == 0) {  // no copy may be in flight when the block ends
+        for (uint32_t k = i > SLOTS ? i - SLOTS : 0; k < i; ++k) mbar_wait(&tail->full[k % SLOTS], (k / SLOTS) & 1u);
+        if (tiles) mbar_wait(&tail->q_full, (tiles - 1) & 1u);
+      }
+    } else if (warp == kMmaWarp) {
+      // ------------------------------ products -------------------------------------------
+      const int steps = (a.dim + 15) / 16;
+      const uint32_t idesc_s = instr_desc(128, 128, false);
+      const uint32_t idesc_o = instr_desc(128, 0, true) | ((uint32_t)(steps * 2) << 17);
+      uint32_t n = 0, tiles = 0, made = 0;  // tiles with keys; scores made
+      Item item = no_item(a);
+      int j = 0;  // the step whose scores are made next, of the tile at hand
+      // the next step, of this tile or of the next that has keys; false behind the last
+      auto advance = [&]() -> bool {
+        if (++j < item.walk.tiles) return true;
+        do {
+          if (!next_item(&tail->items, n, item, timed_out)) return false;
+        } while (item.walk.tiles == 0);
+        j = 0;
+        return true;
+      };
+      auto wait = [&](uint64_t* bar, uint32_t parity) {
+        if (!timed_out && !warp_wait(bar, parity)) timed_out = true;
+        return !timed_out;
+      };
+      auto ready = [&](uint32_t i) { return wait(&tail->full[i % SLOTS], (i / SLOTS) & 1u); };
+      auto scores = [&] {
+        if (j == 0 && !wait(&tail->q_full, tiles++ & 1u)) return;
+        if (!ready(2u * made)) return;
+        if (!C::kAlias && made > 0 && !wait(&tail->s_free, (made - 1) & 1u)) return;
+        tc_fence_after();
+        mma_rows(tmem + C::S0, smem_base, slots + (2u * made) % SLOTS * C::TILE, idesc_s, steps);
+        tc_commit_elect(&tail->s_full);
+        tc_commit_elect(&tail->empty[(2u * made) % SLOTS]);
+        if (j == item.walk.tiles - 1) tc_commit_elect(&tail->q_empty);
+        ++made;
+      };
+      // O (+)= P V of step t; left: keys of the sample from the tile's first one on
+      auto output = [&](uint32_t t, bool accumulate, int left) {
+        const uint32_t v_s = slots + (2u * t + 1u) % SLOTS * C::TILE;
+        if (!ready(2u * t + 1u)) return;
+        if (left < 128) zero_rows(v_s, left, C::ATOMS);
+        if (!wait(&tail->p_full, t & 1u)) return;
+        tc_fence_after();
+        mma_columns(tmem + C::O0, tmem + C::P0, v_s, idesc_o, accumulate);
+        tc_commit_elect(&tail->o_done);
+        tc_commit_elect(&tail->empty[(2u * t + 1u) % SLOTS]);
+      };
+      bool more = advance();
+      if (more) scores();
+      for (uint32_t t = 0; more && !timed_out; ++t) {
+        const bool accumulate = j > 0;
+        const int left = item.g.n_k - item.walk.key(j);
+        if constexpr (C::kAlias) {
+          output(t, accumulate, left);
+          if (timed_out) break;
+          more = advance();
+          if (more && wait(&tail->o_done, t & 1u)) scores();  // P has been read
+        } else {
+          more = advance();
+          if (more) scores();
+          if (!timed_out) output(t, accumulate, left);
+        }
+      }
+    }
+  };
+  if (warp < kSoftmaxWarps) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::SOFTMAX_REGS));
+    softmax();
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::OTHER_REGS));
+    others();
+  }
+
+  if (timed_out) atomicExch(a.status, (uint32_t)RMN_ERR_TIMEOUT);
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::COLUMNS) : "memory");
+  }
+}
+
+// Blocks that stay: as many as fit the SMs at once, or as there are tiles.
+uint32_t blocks_that_stay(uint64_t items, int per_sm) { return (uint32_t)std::min<uint64_t>(items, 148ull * per_sm); }
+
+template <int DP>
+int launch_fwd(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const AttnArgs& a, cudaStream_t stream) {
+  using C = FwdShape<DP>;
+  static SmemOptIn opt_in;
+  auto kern = k_window_fwd<DP>;
+  const uint64_t numbers = most_tiles(a.rows_q, a.sequences, 128);
+  if (numbers > 0x7fffffffull) return RMN_ERR_UNSUPPORTED;
+  // the registers dealt out have to be there: asked for once
+  static std::atomic<int> enough{0};
+  if (!enough.load(std::memory_order_relaxed)) {
+    cudaFuncAttributes attr;
+    RMN_CUDA_TRY(cudaFuncGetAttributes(&attr, reinterpret_cast<const void*>(kern)));
+    enough.store(attr.numRegs * C::THREADS >= C::ALL_REGS ? 1 : 2, std::memory_order_relaxed);
+  }
+  if (enough.load(std::memory_order_relaxed) != 1) return RMN_ERR_UNSUPPORTED;
+  RMN_CUDA_TRY(opt_in.apply(reinterpret_cast<const void*>(kern), C::SMEM));
+  RMN_CUDA_TRY(launch_overlapped(kern, dim3(blocks_that_stay(numbers * a.heads, 2)), dim3(C::THREADS), C::SMEM, stream, q, k, v, a,
+                                 (uint32_t)numbers));
+  RMN_LAUNCH_CHECK();
+  count_tc_launch();
+  return RMN_OK;
+}
+
+}  // namespace
+}  // namespace tc
+
+int attention_window_forward(const AttnArgs& a, cudaStream_t stream) {
+  using namespace tc;
+  CUtensorMap q, k, v;
+  if (!make_head_map(&q, a.q, a.rows_q, a.heads, a.dim, a.q_row, a.q_head) ||
+      !make_head_map(&k, a.k, a.rows_k, a.kv_heads, a.dim, a.k_row, a.k_head) ||
+      !make_head_map(&v, a.v, a.rows_k, a.kv_heads, a.dim, a.v_row, a.v_head))
+    return RMN_ERR_UNSUPPORTED;
+  return a.dim <= 64 ? launch_fwd<64>(q, k, v, a, stream) : launch_fwd<128>(q, k, v, a, stream);
+}
+
+}  // namespace rmn

@@ -29,7 +29,8 @@ namespace rmn {
 namespace {
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
-constexpr uint32_t kMostBlocks = 148 * 2;  // as many as fit the SMs at once
+constexpr uint32_t kMostBlocks = 148 * 2;       // with a norm: as many as fit the SMs at once
+constexpr uint32_t kMostPlainBlocks = 148 * 3;  // without
 constexpr int kMostAxes = 8;
 constexpr int kMostDim = 256;
 
@@ -404,7 +405,7 @@ struct Walk {
 constexpr int heads_at_once(bool backward) { return backward ? 1 : 2; }
 
 template <typename T, int V, int NU, bool kNext, bool kNorm>
-__global__ void __launch_bounds__(kThreads, 2) k_rotary(const __grid_constant__ RotaryArgs a) {
+__global__ void __launch_bounds__(kThreads, kNorm ? 2 : 3) k_rotary(const __grid_constant__ RotaryArgs a) {
   constexpr int U = heads_at_once(false), N = kNumbers<V>;
   extern __shared__ __align__(16) char smem[];
   Tables<V, NU>& tables = *reinterpret_cast<Tables<V, NU>*>(smem);
@@ -741,8 +742,10 @@ int arguments(const rmn_rotary* p, RotaryArgs* a) {
   return RMN_OK;
 }
 
-// The most pairs that a load may hold: four, or two or one where sizes, strides or pointers ask for that.
-int pairs_a_load(const RotaryArgs& a, int elem, bool next) {
+// The most pairs that a load may hold: 16 bytes of them, fewer where sizes, strides or pointers ask for that. Four at most without a norm,
+// whose registers then leave room for a third block on an SM (1.2 M rows, 4 heads of 16 in bf16: 92 us a pass with eight and two blocks,
+// 78 so; with the norm, where three blocks would spill, 16 + 4 heads of 128 at 16411 rows 42 us with eight, 54 with four).
+int pairs_a_load(const RotaryArgs& a, int elem, bool next, bool norm) {
   auto fits = [&](int v) {
     if (next ? a.dim / 2 % v : a.pairs % v || (a.dim / 2 - a.pairs) % v) return false;
     for (const Heads& p : a.part) {
@@ -753,7 +756,7 @@ int pairs_a_load(const RotaryArgs& a, int elem, bool next) {
     }
     return true;
   };
-  int v = elem == 2 ? 8 : 4;
+  int v = elem == 2 && norm ? 8 : 4;
   while (v > 1 && !fits(v)) v /= 2;
   return v;
 }
@@ -795,13 +798,14 @@ int launch_as(const RotaryArgs& a, cudaStream_t stream) {
 }
 template <typename T, int V, int NU>
 int launch(RotaryArgs& a, bool next, bool norm, bool backward, cudaStream_t stream) {
-  lay_out(&a, V, NU, kMostBlocks);
+  lay_out(&a, V, NU, norm ? kMostBlocks : kMostPlainBlocks);
   if (backward) return next ? launch_as<T, V, NU, true, 2>(a, stream) : launch_as<T, V, NU, false, 2>(a, stream);
   if (norm) return next ? launch_as<T, V, NU, true, 1>(a, stream) : launch_as<T, V, NU, false, 1>(a, stream);
-  return next ? launch_as<T, V, NU, true, 0>(a, stream) : launch_as<T, V, NU, false, 0>(a, stream);
+  if constexpr (V <= 4) return next ? launch_as<T, V, NU, true, 0>(a, stream) : launch_as<T, V, NU, false, 0>(a, stream);
+  return RMN_ERR_UNSUPPORTED;  // (not reached: pairs_a_load)
 }
 int run(RotaryArgs& a, int dtype, bool next, bool norm, bool backward, cudaStream_t stream) {
-  const int v = pairs_a_load(a, dtype == RMN_F32 ? 4 : 2, next);
+  const int v = pairs_a_load(a, dtype == RMN_F32 ? 4 : 2, next, norm);
   if (dtype == RMN_F32)
     return v == 4   ? launch<float, 4, 1>(a, next, norm, backward, stream)
            : v == 2 ? launch<float, 2, 2>(a, next, norm, backward, stream)
