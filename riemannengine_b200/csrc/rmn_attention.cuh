@@ -127,7 +127,6 @@ __device__ __forceinline__ int32_t tiles_of(int32_t rows, int tile_rows) {
 
 // Windows. Query row i of a segment stands at place i + n_k - n_q of its keys. It sees the keys whose distance from there is less than the
 // window (causal: those up to its own place), and the sinks, the first keys of the sample (causal: of those up to its own place).
-__device__ __forceinline__ int32_t clamp_to(int64_t v, int32_t most) { return (int32_t)max((int64_t)0, min(v, (int64_t)most)); }
 // v - back and v + on, held to 0 ... most (back, on >= 0): in 32 bits, which no step leaves (a block waits for these numbers)
 __device__ __forceinline__ int32_t back_from(int32_t v, int32_t back, int32_t most) { return v <= back ? 0 : min(v - back, most); }
 __device__ __forceinline__ int32_t on_from(int32_t v, int32_t on, int32_t most) { return v >= most - on ? most : max(v + on, 0); }
@@ -206,9 +205,9 @@ struct KeyRows {
 template <bool kWindow>
 __device__ __forceinline__ KeyRows key_rows(const AttnArgs& a, const Segment& g, int32_t j) {
   if constexpr (!kWindow) return {first_query(g, j, a.causal), g.n_q};
-  const int64_t row = (int64_t)j - g.n_k + g.n_q;  // the query at the key's place
-  if (j < a.sinks) return {a.causal ? clamp_to(row, g.n_q) : 0, g.n_q};
-  return {clamp_to(a.causal ? row : row - a.window + 1, g.n_q), clamp_to(row + a.window, g.n_q)};
+  const int32_t row = j - (g.n_k - g.n_q);  // the query at the key's place
+  if (j < a.sinks) return {a.causal ? back_from(row, 0, g.n_q) : 0, g.n_q};
+  return {back_from(row, a.causal ? 0 : a.window - 1, g.n_q), on_from(row, a.window, g.n_q)};
 }
 // A tile of keys of one sample and the queries that it is multiplied with.
 struct KeyTile {

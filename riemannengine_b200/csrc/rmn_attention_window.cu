@@ -1,13 +1,16 @@
-// Attention with a sliding window and sinks on the tensor cores, bf16, head sizes up to 128 (multiples of 8): the forward pass and dQ. The
-// mathematics and the layouts are those of rmn_attention_fwd.cu and rmn_attention_bwd.cu; the keys that a tile of 128 queries sees are
-// those of the window and the sinks (KeyWalk).
+// Attention with a sliding window and sinks on the tensor cores: forward pass, bf16, head sizes up to 64 (multiples of 8). The mathematics
+// and the layout are those of k_attention_fwd (rmn_attention_fwd.cu), which also has the windows of larger heads; the keys that a tile of
+// 128 queries sees are those of the window and the sinks (KeyWalk).
 //
-// Such a tile has few steps over keys, so that what surrounds them - to find the tile, to fetch the first rows, to store the last ones -
-// costs as much as the steps (a block a tile: 13 000 clocks for two steps, 6 000 of them around). So blocks stay and take one tile after
-// the other, `gridDim.x` apart, and the steps of all of them run as one chain: the copying warp finds the next tile and fetches its rows while
-// the steps of this one are under way, and the next tile's scores are made while this one's output is stored. Every barrier is waited
-// for phase by phase across tiles: a step's number counts from the block's first one. What a tile is goes from the copying warp to the
-// others through a ring of four places.
+// Such a tile has few steps over keys, so that what surrounds them (to find it, to fetch its rows, to store its output) takes as long. So
+// blocks stay and take one tile after the other, `gridDim.x` apart, and the steps of all of them run as one chain: the copying warp finds the next tile and fetches
+// its rows while the steps of this one are under way, and the next tile's scores are made while this one's output is stored. Every barrier is
+// waited for phase by phase across tiles: a step's number counts from the block's first one. What a tile is goes from the copying warp to
+// the others through a ring of four places. Of a step's 128 columns those are left out, 32 at a time, that no row of a warp sees.
+// 8 samples of 511 ... 6007 rows, 8 heads of 32, window 65 both ways (two steps a tile): 47 us with a block a tile, 38 so; 8 samples of
+// 151 ... 4001 rows, 8 heads of 64, window 512: 62 and 59. A chain of latencies all the same: the exponentials are 1024 clocks of the 4700
+// that a step takes, and two blocks an SM, all that tensor memory holds, fill the gaps in part. Steps of 64 keys and three blocks: 47 and 103
+// us. dQ, dK and dV by blocks that stay: 67 and 91 us on the first of these samples, 63 and 85 with a block a tile.
 #include "rmn_attention_tc.cuh"
 
 #include <math_constants.h>
@@ -21,106 +24,104 @@ namespace {
 
 constexpr float kRescale = 8.f;  // log2 of how far a row's maximum may rise before O is scaled
 constexpr int kItems = 4;        // tiles on their way to the warps
-constexpr int kKeys = 128;       // of a step
 
-// A tile of one head, with its keys: the copying warp works ahead, the others would wait for such numbers.
+// A tile of 128 query rows of one head, with its keys: the copying warp works ahead, the others would wait for such numbers.
 struct Item {
   Segment g;
   int32_t first, head, there;  // first query row; there: 0 behind the last tile
-  KeyWalk<true, kKeys> walk;
+  KeyWalk<true, 128> walk;
 };
-struct Items {
-  uint64_t full[kItems], empty[kItems];
-  alignas(16) unsigned char item[kItems][sizeof(Item)];
-  int32_t starts[kCountedSamples + 3];  // the first tile of every segment, and all tiles
-  int32_t warp_sums[12];
+__device__ __forceinline__ Item no_item(const AttnArgs& a) { return {{}, 0, 0, 0, {a, {}, 0, 0}}; }
+
+// What the kernel's shared memory holds behind its tiles.
+constexpr int kSlots = 4, kThreads = 256;
+struct Tail {
+  uint64_t full[kSlots], empty[kSlots], q_full, q_empty, s_full, s_free, p_full, o_done;
+  uint64_t item_full[kItems], item_empty[kItems];
+  alignas(16) unsigned char items[kItems][sizeof(Item)];
+  int32_t starts[kCountedSamples + 3];  // the first tile of every segment, and all tiles, for up to kCountedSamples samples
+  int32_t warp_sums[kThreads / 32];
+  uint32_t tmem_slot;
 };
 
-__device__ __forceinline__ void init_items(Items* items, int readers) {
-  for (int i = 0; i < kItems; ++i) {
-    mbar_init(&items->full[i], 1);
-    mbar_init(&items->empty[i], readers);
-  }
-}
-// All threads: where the segments' tiles of `rows` query rows begin, for up to kCountedSamples samples.
-template <int kThreads>
-__device__ __forceinline__ void count_tiles(const AttnArgs& a, Items* items) {
+// All threads: where the tiles of every segment begin.
+__device__ __forceinline__ void count_tiles(const AttnArgs& a, Tail* tail) {
   const uint32_t n = a.sequences + 2;
   if (a.sequences > kCountedSamples) return;
   const uint32_t per = (n + kThreads - 1) / kThreads, lo = min(threadIdx.x * per, n), hi = min(lo + per, n);
   int32_t mine = 0, first, all;
-  for (uint32_t s = lo; s < hi; ++s) mine = add_tiles(mine, segment_tiles<TilesOf::kQueries>(segment(a, s), 128));
+  for (uint32_t s = lo; s < hi; ++s) mine = add_tiles(mine, tiles_of(segment(a, s).n_q, 128));
   bool unused = false;
-  scan_block<kThreads>(mine, items->warp_sums, first, all, unused);
+  scan_block<kThreads>(mine, tail->warp_sums, first, all, unused);
   for (uint32_t s = lo; s < hi; ++s) {
-    items->starts[s] = first;
-    first = add_tiles(first, segment_tiles<TilesOf::kQueries>(segment(a, s), 128));
+    tail->starts[s] = first;
+    first = add_tiles(first, tiles_of(segment(a, s).n_q, 128));
   }
-  if (threadIdx.x == 0) items->starts[n] = all;
+  if (threadIdx.x == 0) tail->starts[n] = all;
   __syncthreads();
 }
-enum class Found { kTile, kNone, kEnd };
 // A warp: the tile of a number; kNone: there is none, but there may be further ones.
-__device__ __forceinline__ Found look_up(const AttnArgs& a, const Items* items, uint32_t want, FoundTile* found) {
+enum class Found { kTile, kNone, kEnd };
+__device__ __forceinline__ Found look_up(const AttnArgs& a, const Tail* tail, uint32_t want, FoundTile* found) {
   const uint32_t n = a.sequences + 2, lane = threadIdx.x & 31;
   if (a.sequences > kCountedSamples) {
     if (want < n && lane == 0) segment(a, want);  // every segment is looked at: the search may step over some that are wrong
     return search_tile<TilesOf::kQueries>(a, want, 128, found) ? Found::kTile : Found::kNone;
   }
-  if (want >= (uint32_t)items->starts[n]) return Found::kEnd;
+  if (want >= (uint32_t)tail->starts[n]) return Found::kEnd;
   uint32_t lo = 0, len = n;  // starts[lo] <= want: the last such segment, which is one that has tiles
   while (len > 1) {
     const uint32_t step = (len + 31) / 32, p = lane * step;
-    const uint32_t below = __ballot_sync(0xffffffffu, p < len && (uint32_t)items->starts[lo + p] <= want);
+    const uint32_t below = __ballot_sync(0xffffffffu, p < len && (uint32_t)tail->starts[lo + p] <= want);
     const uint32_t skip = (31 - __clz((int)(below | 1u))) * step;
     lo += skip;
     len = min(step, len - skip);
   }
   const Segment g = segment(a, lo);
-  const int32_t tiles = segment_tiles<TilesOf::kQueries>(g, 128), tile = (int32_t)want - items->starts[lo];
+  const int32_t tiles = tiles_of(g.n_q, 128), tile = (int32_t)want - tail->starts[lo];
   if (tile >= tiles) return Found::kNone;  // (offsets that make no sense)
   *found = {g, tile, tiles};
   return Found::kTile;
 }
-__device__ __forceinline__ Item no_item(const AttnArgs& a) { return {{}, 0, 0, 0, {a, {}, 0, 0}}; }
+
 // A warp that reads the ring: the next tile; false behind the last one, or where a wait ran out.
-__device__ __forceinline__ bool next_item(Items* items, uint32_t& n, Item& item, bool& timed_out) {
+__device__ __forceinline__ bool next_item(Tail* tail, uint32_t& n, Item& item, bool& timed_out) {
   const uint32_t slot = n % kItems;
-  if (!warp_wait(&items->full[slot], (n / kItems) & 1u)) {
+  if (!warp_wait(&tail->item_full[slot], (n / kItems) & 1u)) {
     timed_out = true;
     return false;
   }
-  item = *reinterpret_cast<const Item*>(items->item[slot]);
+  item = *reinterpret_cast<const Item*>(tail->items[slot]);
   __syncwarp();
-  if ((threadIdx.x & 31) == 0) mbar_arrive(&items->empty[slot]);
+  if ((threadIdx.x & 31) == 0) mbar_arrive(&tail->item_empty[slot]);
   ++n;
   return item.there != 0;
 }
-// The copying warp: `fetch(item, steps before)` asks for a tile's rows, lane 0 alone; false where a wait ran out.
+// The copying warp hands out the tiles of numbers blockIdx.x, blockIdx.x + gridDim.x ... below numbers x heads; `fetch(item)` asks for a
+// tile's rows (by lane 0; false where a wait ran out).
 template <class Fetch>
-__device__ __forceinline__ void hand_out(const AttnArgs& a, Items* items, uint32_t numbers, bool& timed_out, Fetch&& fetch) {
+__device__ __forceinline__ void hand_out(const AttnArgs& a, Tail* tail, uint32_t numbers, bool& timed_out, Fetch&& fetch) {
   const int lane = threadIdx.x & 31;
   uint32_t n = 0;
   auto put = [&](const Item& item) {
     const uint32_t slot = n % kItems;
-    if (!warp_wait(&items->empty[slot], ((n / kItems) & 1u) ^ 1u)) {
+    if (!warp_wait(&tail->item_empty[slot], ((n / kItems) & 1u) ^ 1u)) {
       timed_out = true;
       return;
     }
     if (lane == 0) {
-      *reinterpret_cast<Item*>(items->item[slot]) = item;
-      mbar_arrive(&items->full[slot]);
+      *reinterpret_cast<Item*>(tail->items[slot]) = item;
+      mbar_arrive(&tail->item_full[slot]);
     }
     __syncwarp();
     ++n;
   };
   for (uint64_t i = blockIdx.x; i < (uint64_t)numbers * a.heads && !timed_out; i += gridDim.x) {
     FoundTile found;
-    const Found there = look_up(a, items, (uint32_t)(i / a.heads), &found);
+    const Found there = look_up(a, tail, (uint32_t)(i / a.heads), &found);
     if (there == Found::kEnd) break;
     if (there == Found::kNone) continue;
-    // (the tiles that see the most keys first)
-    const int32_t first = (found.tiles - 1 - found.tile) * 128;
+    const int32_t first = (found.tiles - 1 - found.tile) * 128;  // (the tiles that see the most keys first)
     const Item item = {found.g, first, (int32_t)(i % a.heads), 1, {a, found.g, first, min(first + 128, found.g.n_q) - 1}};
     put(item);
     if (timed_out) break;
@@ -131,38 +132,26 @@ __device__ __forceinline__ void hand_out(const AttnArgs& a, Items* items, uint32
   if (!timed_out) put(no_item(a));
 }
 
-// ------------------------------ forward ------------------------------------------------
-template <int DP>
-struct FwdShape {
-  static constexpr int ATOMS = DP / 64;
-  static constexpr uint32_t TILE = ATOMS * kAtomBytes;
-  static constexpr bool kAlias = DP == 128;  // P in the columns of S
-  static constexpr int SLOTS = DP == 128 ? 2 : 4;
-  static constexpr int THREADS = 256;
+// Two blocks an SM, of four warps for the softmax, one that copies and one that issues the products.
+struct Shape {
+  static constexpr uint32_t TILE = kAtomBytes;
+  // registers of a softmax thread and of the others: what the block is launched with, dealt out anew
   static constexpr int SOFTMAX_REGS = 200, OTHER_REGS = 56;
   static constexpr int ALL_REGS = 128 * SOFTMAX_REGS + 128 * OTHER_REGS;
-  static constexpr uint32_t COLUMNS = 256;
-  static constexpr uint32_t S0 = 0, P0 = kAlias ? 0 : 128, O0 = kAlias ? 128 : 192;
-  static constexpr uint32_t TAIL = (1 + SLOTS) * TILE;
-  static constexpr size_t SMEM = TAIL + 4096 + 1024;  // (1024: the tiles start on a swizzle's period)
+  static constexpr uint32_t COLUMNS = 256, S0 = 0, P0 = 128, O0 = 192;
+  static constexpr uint32_t TAIL = (1 + kSlots) * TILE;
+  static constexpr size_t SMEM = TAIL + sizeof(Tail) + 1024;  // (1024: the tiles start on a swizzle's period)
 };
-struct FwdTail {
-  uint64_t full[4], empty[4], q_full, q_empty, s_full, s_free, p_full, o_done;
-  Items items;
-  uint32_t tmem_slot;
-};
-static_assert(sizeof(FwdTail) <= 4096, "tail");
 constexpr int kSoftmaxWarps = 4;
 
-template <int DP>
-__global__ void __launch_bounds__(FwdShape<DP>::THREADS, 2)
+__global__ void __launch_bounds__(kThreads, 2)
     k_window_fwd(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                  const __grid_constant__ CUtensorMap map_v, const AttnArgs a, const uint32_t numbers) {
-  using C = FwdShape<DP>;
-  constexpr int SLOTS = C::SLOTS;
+  using C = Shape;
+  constexpr int SLOTS = kSlots;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  FwdTail* tail = reinterpret_cast<FwdTail*>(smem + C::TAIL);
+  Tail* tail = reinterpret_cast<Tail*>(smem + C::TAIL);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   constexpr int kCopyWarp = 4, kMmaWarp = 5;
   if (tid == 0) {
@@ -174,7 +163,10 @@ __global__ void __launch_bounds__(FwdShape<DP>::THREADS, 2)
     for (uint64_t* b : ones) mbar_init(b, 1);
     mbar_init(&tail->s_free, 128);
     mbar_init(&tail->p_full, 128);
-    init_items(&tail->items, kSoftmaxWarps + 1);
+    for (int i = 0; i < kItems; ++i) {
+      mbar_init(&tail->item_full[i], 1);
+      mbar_init(&tail->item_empty[i], kSoftmaxWarps + 1);
+    }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_proxy_async();
   }
@@ -193,7 +185,7 @@ __global__ void __launch_bounds__(FwdShape<DP>::THREADS, 2)
   __syncthreads();
   tc_fence_after();
   after_previous_kernel();
-  count_tiles<C::THREADS>(a, &tail->items);
+  count_tiles(a, tail);
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&tail->tmem_slot);
   const uint32_t smem_base = smem_u32(smem), slots = smem_base + C::TILE;
   bool timed_out = false;
@@ -205,9 +197,9 @@ __global__ void __launch_bounds__(FwdShape<DP>::THREADS, 2)
     const float scale = a.scale * kLog2e;  // (> 0)
     uint32_t n = 0, step = 0;
     Item item = no_item(a);
-    while (next_item(&tail->items, n, item, timed_out)) {
+    while (next_item(tail, n, item, timed_out)) {
       const Segment& g = item.g;
-      const KeyWalk<true, kKeys>& walk = item.walk;
+      const auto& walk = item.walk;
       const int row = item.first + tid;
       const RowKeys seen = row_keys<true>(a, g, row);
       float m = -CUDART_INF_F, l = 0.f;  // maximum in use (times scale, log 2), sum
@@ -221,10 +213,8 @@ __global__ void __launch_bounds__(FwdShape<DP>::THREADS, 2)
         tc_ld32_at<64>(s_t + 64, r);
         tc_ld32_at<96>(s_t + 96, r);
         tc_wait_ld();
-        if constexpr (!C::kAlias) {
-          tc_fence_before();
-          mbar_arrive(&tail->s_free);
-        }
+        tc_fence_before();
+        mbar_arrive(&tail->s_free);
         // 32 columns at a time: those that no row of the warp sees cost nothing, those that all see no masking
         const int k0 = walk.key(j);
         uint32_t some = 0;  // bit k: a row sees one of columns 32 k ... 32 k + 31
@@ -278,14 +268,12 @@ __global__ void __launch_bounds__(FwdShape<DP>::THREADS, 2)
         }
         l += total(add(sum[0], sum[1]));
         if (j > 0) {
-          // P and O of the step before are free (kAlias: these scores were made behind that; j == 0: O has been stored)
-          if constexpr (!C::kAlias) {
-            if (!warp_wait(&tail->o_done, ph ^ 1u)) { timed_out = true; break; }
-            tc_fence_after();
-          }
+          // P and O of the step before are free (j == 0: O has been stored)
+          if (!warp_wait(&tail->o_done, ph ^ 1u)) { timed_out = true; break; }
+          tc_fence_after();
           if (__any_sync(0xffffffffu, rise)) {
 #pragma unroll
-            for (int c = 0; c < DP; c += 32) {
+            for (int c = 0; c < 64; c += 32) {
               uint32_t o[32];
               tc_ld32(o_t + c, o);
               tc_wait_ld();
@@ -313,7 +301,7 @@ __global__ void __launch_bounds__(FwdShape<DP>::THREADS, 2)
       __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + at;
       __nv_bfloat16* low = a.low ? static_cast<__nv_bfloat16*>(a.low) + at : nullptr;
 #pragma unroll
-      for (int c = 0; c < DP; c += 32) {
+      for (int c = 0; c < 64; c += 32) {
         if (c >= a.dim) break;
         uint32_t o[32];
         if (walk.tiles > 0) {
@@ -345,24 +333,19 @@ __global__ void __launch_bounds__(FwdShape<DP>::THREADS, 2)
     if (warp == kCopyWarp) {
       // ------------------------------ bulk copies ----------------------------------------
       uint32_t i = 0, tiles = 0;  // keys' and values' loads: K 0, V 0, K 1, V 1, ...; tiles with keys
-      hand_out(a, &tail->items, numbers, timed_out, [&](const Item& item) {
-        const KeyWalk<true, kKeys>& walk = item.walk;
+      hand_out(a, tail, numbers, timed_out, [&](const Item& item) {
+        const auto& walk = item.walk;
         if (walk.tiles == 0) return true;
         const int kv = item.head / (a.heads / a.kv_heads);
         if (!mbar_wait(&tail->q_empty, (tiles & 1u) ^ 1u)) return false;
         ++tiles;
         mbar_arrive_expect_tx(&tail->q_full, C::TILE);
-#pragma unroll
-        for (int c = 0; c < C::ATOMS; ++c)
-          tma_load_3d(smem_base + c * kAtomBytes, &map_q, &tail->q_full, c * 64, item.head, item.g.q0 + item.first);
+        tma_load_3d(smem_base, &map_q, &tail->q_full, 0, item.head, item.g.q0 + item.first);
         for (int j = 0; j < 2 * walk.tiles; ++j, ++i) {
           const uint32_t s = i % SLOTS;
           if (!mbar_wait(&tail->empty[s], ((i / SLOTS) & 1u) ^ 1u)) return false;
           mbar_arrive_expect_tx(&tail->full[s], C::TILE);
-          const CUtensorMap* map = (j & 1) ? &map_v : &map_k;
-#pragma unroll
-          for (int c = 0; c < C::ATOMS; ++c)
-            tma_load_3d(slots + s * C::TILE + c * kAtomBytes, map, &tail->full[s], c * 64, kv, item.g.k0 + walk.key(j >> 1));
+          tma_load_3d(slots + s * C::TILE, (j & 1) ? &map_v : &map_k, &tail->full[s], 0, kv, item.g.k0 + walk.key(j >> 1));
         }
         return true;
       });
@@ -382,7 +365,7 @@ __global__ void __launch_bounds__(FwdShape<DP>::THREADS, 2)
       auto advance = [&]() -> bool {
         if (++j < item.walk.tiles) return true;
         do {
-          if (!next_item(&tail->items, n, item, timed_out)) return false;
+          if (!next_item(tail, n, item, timed_out)) return false;
         } while (item.walk.tiles == 0);
         j = 0;
         return true;
@@ -395,7 +378,7 @@ __global__ void __launch_bounds__(FwdShape<DP>::THREADS, 2)
       auto scores = [&] {
         if (j == 0 && !wait(&tail->q_full, tiles++ & 1u)) return;
         if (!ready(2u * made)) return;
-        if (!C::kAlias && made > 0 && !wait(&tail->s_free, (made - 1) & 1u)) return;
+        if (made > 0 && !wait(&tail->s_free, (made - 1) & 1u)) return;
         tc_fence_after();
         mma_rows(tmem + C::S0, smem_base, slots + (2u * made) % SLOTS * C::TILE, idesc_s, steps);
         tc_commit_elect(&tail->s_full);
@@ -407,7 +390,7 @@ __global__ void __launch_bounds__(FwdShape<DP>::THREADS, 2)
       auto output = [&](uint32_t t, bool accumulate, int left) {
         const uint32_t v_s = slots + (2u * t + 1u) % SLOTS * C::TILE;
         if (!ready(2u * t + 1u)) return;
-        if (left < 128) zero_rows(v_s, left, C::ATOMS);
+        if (left < 128) zero_rows(v_s, left, 1);
         if (!wait(&tail->p_full, t & 1u)) return;
         tc_fence_after();
         mma_columns(tmem + C::O0, tmem + C::P0, v_s, idesc_o, accumulate);
@@ -419,16 +402,9 @@ __global__ void __launch_bounds__(FwdShape<DP>::THREADS, 2)
       for (uint32_t t = 0; more && !timed_out; ++t) {
         const bool accumulate = j > 0;
         const int left = item.g.n_k - item.walk.key(j);
-        if constexpr (C::kAlias) {
-          output(t, accumulate, left);
-          if (timed_out) break;
-          more = advance();
-          if (more && wait(&tail->o_done, t & 1u)) scores();  // P has been read
-        } else {
-          more = advance();
-          if (more) scores();
-          if (!timed_out) output(t, accumulate, left);
-        }
+        more = advance();
+        if (more) scores();
+        if (!timed_out) output(t, accumulate, left);
       }
     }
   };
@@ -449,43 +425,33 @@ __global__ void __launch_bounds__(FwdShape<DP>::THREADS, 2)
   }
 }
 
-// Blocks that stay: as many as fit the SMs at once, or as there are tiles.
-uint32_t blocks_that_stay(uint64_t items, int per_sm) { return (uint32_t)std::min<uint64_t>(items, 148ull * per_sm); }
+}  // namespace
+}  // namespace tc
 
-template <int DP>
-int launch_fwd(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const AttnArgs& a, cudaStream_t stream) {
-  using C = FwdShape<DP>;
+int attention_window_forward(const AttnArgs& a, cudaStream_t stream) {
+  using namespace tc;
   static SmemOptIn opt_in;
-  auto kern = k_window_fwd<DP>;
+  CUtensorMap q, k, v;
+  if (!make_head_map(&q, a.q, a.rows_q, a.heads, a.dim, a.q_row, a.q_head) ||
+      !make_head_map(&k, a.k, a.rows_k, a.kv_heads, a.dim, a.k_row, a.k_head) ||
+      !make_head_map(&v, a.v, a.rows_k, a.kv_heads, a.dim, a.v_row, a.v_head))
+    return RMN_ERR_UNSUPPORTED;
   const uint64_t numbers = most_tiles(a.rows_q, a.sequences, 128);
   if (numbers > 0x7fffffffull) return RMN_ERR_UNSUPPORTED;
   // the registers dealt out have to be there: asked for once
   static std::atomic<int> enough{0};
   if (!enough.load(std::memory_order_relaxed)) {
     cudaFuncAttributes attr;
-    RMN_CUDA_TRY(cudaFuncGetAttributes(&attr, reinterpret_cast<const void*>(kern)));
-    enough.store(attr.numRegs * C::THREADS >= C::ALL_REGS ? 1 : 2, std::memory_order_relaxed);
+    RMN_CUDA_TRY(cudaFuncGetAttributes(&attr, reinterpret_cast<const void*>(k_window_fwd)));
+    enough.store(attr.numRegs * kThreads >= Shape::ALL_REGS ? 1 : 2, std::memory_order_relaxed);
   }
   if (enough.load(std::memory_order_relaxed) != 1) return RMN_ERR_UNSUPPORTED;
-  RMN_CUDA_TRY(opt_in.apply(reinterpret_cast<const void*>(kern), C::SMEM));
-  RMN_CUDA_TRY(launch_overlapped(kern, dim3(blocks_that_stay(numbers * a.heads, 2)), dim3(C::THREADS), C::SMEM, stream, q, k, v, a,
-                                 (uint32_t)numbers));
+  RMN_CUDA_TRY(opt_in.apply(reinterpret_cast<const void*>(k_window_fwd), Shape::SMEM));
+  const uint32_t blocks = (uint32_t)std::min<uint64_t>(numbers * a.heads, 148 * 2);  // as many as fit the SMs at once
+  RMN_CUDA_TRY(launch_overlapped(k_window_fwd, dim3(blocks), dim3(kThreads), Shape::SMEM, stream, q, k, v, a, (uint32_t)numbers));
   RMN_LAUNCH_CHECK();
   count_tc_launch();
   return RMN_OK;
-}
-
-}  // namespace
-}  // namespace tc
-
-int attention_window_forward(const AttnArgs& a, cudaStream_t stream) {
-  using namespace tc;
-  CUtensorMap q, k, v;
-  if (!make_head_map(&q, a.q, a.rows_q, a.heads, a.dim, a.q_row, a.q_head) ||
-      !make_head_map(&k, a.k, a.rows_k, a.kv_heads, a.dim, a.k_row, a.k_head) ||
-      !make_head_map(&v, a.v, a.rows_k, a.kv_heads, a.dim, a.v_row, a.v_head))
-    return RMN_ERR_UNSUPPORTED;
-  return a.dim <= 64 ? launch_fwd<64>(q, k, v, a, stream) : launch_fwd<128>(q, k, v, a, stream);
 }
 
 }  // namespace rmn
