@@ -1227,10 +1227,13 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Te
 class RiemannSelfAttention(torch.nn.Module):
     """Self-attention of the rows of a SparseTensor within their sample: ``qkv`` projects the features to queries, keys and
     values, packed_attention runs on the row ranges of CoordinateManager.sample_offsets, ``projection`` mixes the heads. The
-    key heads may be fewer than the query heads. No counterpart in the reference."""
+    key heads may be fewer than the query heads. ``rotary_base``: queries and keys are turned by their rows' coordinates
+    (rotary_positions, the pairs dealt out evenly to the axes); ``qk_norm``: behind a norm of every head with weights of its own
+    (qk_norm_rotary). ``window`` and ``sinks``: of packed_attention, over the rows in their order. No counterpart in the reference."""
 
     def __init__(self, channels: int, num_heads: int, num_kv_heads: Optional[int] = None, causal: bool = False,
-                 bias: bool = True):
+                 bias: bool = True, rotary_base: Optional[float] = None, qk_norm: bool = False, window: Optional[int] = None,
+                 sinks: int = 0):
         super().__init__()
         kv = num_heads if num_kv_heads is None else num_kv_heads
         if channels <= 0 or num_heads <= 0 or channels % num_heads:
@@ -1239,16 +1242,46 @@ class RiemannSelfAttention(torch.nn.Module):
             raise RuntimeError("the number of query heads must be a multiple of the number of key heads")
         self.channels, self.num_heads, self.num_kv_heads, self.causal = channels, num_heads, kv, causal
         self.dim = channels // num_heads
+        if (rotary_base is not None or qk_norm) and (self.dim % 2 or self.dim > 256):
+            raise RuntimeError("rotary positions and norms of heads take an even number of channels a head, up to 256")
+        if rotary_base is not None and not rotary_base > 0:
+            raise RuntimeError("the base of rotary positions must be positive")
+        ops._window(window, sinks)
+        self.rotary_base, self.qk_norm, self.window, self.sinks = rotary_base, qk_norm, window, sinks
         self.qkv = torch.nn.Linear(channels, (num_heads + 2 * kv) * self.dim, bias=bias)
         self.projection = torch.nn.Linear(channels, channels, bias=bias)
+        if qk_norm:
+            self.q_norm = torch.nn.Parameter(torch.ones(self.dim))
+            self.k_norm = torch.nn.Parameter(torch.ones(self.dim))
+        self._frequencies: Dict = {}  # by axes and device: float64 whatever the layer's type
+
+    def _rotary(self, input: "SparseTensor"):
+        """positions, frequencies and sections of the rows; nothing without a base."""
+        if self.rotary_base is None:
+            return None, None, []
+        positions = input.C[:, 1:]
+        sections = rotary_sections(self.dim, positions.size(1))
+        key = (positions.size(1), positions.device)
+        if key not in self._frequencies:
+            self._frequencies[key] = rotary_frequencies(sections, self.rotary_base).to(positions.device)
+        return positions, self._frequencies[key], sections
 
     def forward(self, input: "SparseTensor") -> "SparseTensor":
         if input.F.size(1) != self.channels:
             raise RuntimeError("Input channel count does not match attention")
         offsets = input.coordinate_manager.sample_offsets(input.coordinate_map_key)
         h, kv = self.num_heads, self.num_kv_heads
-        q, k, v = self.qkv(input.F).view(-1, h + 2 * kv, self.dim).split([h, kv, kv], 1)
-        out = packed_attention(q, k, v, offsets, causal=self.causal)
+        heads = self.qkv(input.F).view(-1, h + 2 * kv, self.dim)
+        positions, frequencies, sections = self._rotary(input)
+        if self.qk_norm:
+            q, k, v = heads.split([h, kv, kv], 1)
+            q, k = qk_norm_rotary(q, k, self.q_norm, self.k_norm, positions, frequencies, sections)
+        elif self.rotary_base is not None:
+            both, v = heads.split([h + kv, kv], 1)
+            q, k = rotary_positions(both, positions, frequencies, sections).split([h, kv], 1)
+        else:
+            q, k, v = heads.split([h, kv, kv], 1)
+        out = packed_attention(q, k, v, offsets, causal=self.causal, window=self.window, sinks=self.sinks)
         return SparseTensor(self.projection(out.reshape(-1, self.channels)), input.coordinate_map_key,
                             input.coordinate_manager)
 

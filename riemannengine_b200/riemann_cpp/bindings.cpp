@@ -355,11 +355,14 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     cls.def_property_readonly("weight", [](LN& self) { return self.normalization()->weight; });
     cls.def_property_readonly("bias", [](LN& self) { return self.normalization()->bias; });
     bind_layer<RiemannSelfAttentionImpl>(m, "RiemannSelfAttention")
-        .def(py::init([](int64_t channels, int64_t num_heads, int64_t num_kv_heads, bool causal, bool bias) {
-               return std::make_shared<RiemannSelfAttentionImpl>(channels, num_heads, num_kv_heads, causal, bias);
+        .def(py::init([](int64_t channels, int64_t num_heads, int64_t num_kv_heads, bool causal, bool bias,
+                         c10::optional<double> rotary_base, bool qk_norm, c10::optional<int64_t> window, int64_t sinks) {
+               return std::make_shared<RiemannSelfAttentionImpl>(channels, num_heads, num_kv_heads, causal, bias, rotary_base, qk_norm,
+                                                                 window, sinks);
              }),
              py::arg("channels"), py::arg("num_heads"), py::arg("num_kv_heads") = 0, py::arg("causal") = false,
-             py::arg("bias") = true);
+             py::arg("bias") = true, py::arg("rotary_base") = py::none(), py::arg("qk_norm") = false, py::arg("window") = py::none(),
+             py::arg("sinks") = 0);
   }
 
   // the example encoder/decoder of networks.hpp (the network the benchmark trains)

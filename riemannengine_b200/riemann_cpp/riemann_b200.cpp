@@ -1931,6 +1931,12 @@ at::Tensor gradient_rows(const at::Tensor& grad) {
   return whole ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 
+void check_window(const c10::optional<int64_t>& window, int64_t sinks) {
+  TORCH_CHECK(window.has_value() || !sinks, "sinks need a window");
+  TORCH_CHECK(!window.has_value() || (*window >= 1 && *window <= std::numeric_limits<int32_t>::max() && sinks >= 0 && sinks < (1 << 30)),
+              "window must be from 1 to 2^31 - 1, sinks from 0 to 2^30 - 1");
+}
+
 struct AttentionInputs {
   at::Tensor q, k, v, offsets, kv_offsets, kv_lengths;  // an absent one of the last two: undefined or empty
   bool causal;
@@ -2082,9 +2088,7 @@ at::Tensor packed_attention(const at::Tensor& q, const at::Tensor& k, const at::
   TORCH_CHECK(!kv_lengths.defined() || kv_lengths.numel() == n, "kv_lengths must have one entry per sample");
   TORCH_CHECK(kv_offsets.defined() || k.size(0) == q.size(0), "q and k must have the same rows unless kv_offsets are given");
   const double by = scale.value_or(1.0 / std::sqrt(static_cast<double>(q.size(2))));
-  TORCH_CHECK(window.has_value() || !sinks, "sinks need a window");
-  TORCH_CHECK(!window.has_value() || (*window >= 1 && *window <= std::numeric_limits<int32_t>::max() && sinks >= 0 && sinks < (1 << 30)),
-              "window must be from 1 to 2^31 - 1, sinks from 0 to 2^30 - 1");
+  check_window(window, sinks);
   const int64_t width = window.value_or(0);
   if (!wants_gradient({q, k, v}))
     return attention_forward({head_rows(q), head_rows(k), head_rows(v), offsets, kv_offsets, kv_lengths, causal, by,
@@ -2324,23 +2328,63 @@ std::pair<at::Tensor, at::Tensor> qk_norm_rotary(const at::Tensor& q, const at::
   return {out[0], out[1]};
 }
 
-RiemannSelfAttentionImpl::RiemannSelfAttentionImpl(int64_t channels, int64_t num_heads, int64_t num_kv_heads, bool causal,
-                                                   bool bias)
-    : channels_(channels), heads_(num_heads), kv_heads_(num_kv_heads ? num_kv_heads : num_heads), causal_(causal) {
+RiemannSelfAttentionImpl::RiemannSelfAttentionImpl(int64_t channels, int64_t num_heads, int64_t num_kv_heads, bool causal, bool bias,
+                                                   c10::optional<double> rotary_base, bool qk_norm, c10::optional<int64_t> window,
+                                                   int64_t sinks)
+    : channels_(channels), heads_(num_heads), kv_heads_(num_kv_heads ? num_kv_heads : num_heads), causal_(causal),
+      rotary_base_(rotary_base), window_(window), sinks_(sinks) {
   TORCH_CHECK(channels > 0 && num_heads > 0 && channels % num_heads == 0,
               "Attention channels must be a positive multiple of the number of heads");
   TORCH_CHECK(kv_heads_ > 0 && heads_ % kv_heads_ == 0,
               "the number of query heads must be a multiple of the number of key heads");
   dim_ = channels / num_heads;
+  TORCH_CHECK((!rotary_base.has_value() && !qk_norm) || (dim_ % 2 == 0 && dim_ <= 256),
+              "rotary positions and norms of heads take an even number of channels a head, up to 256");
+  TORCH_CHECK(!rotary_base.has_value() || *rotary_base > 0, "the base of rotary positions must be positive");
+  check_window(window, sinks);
   qkv_ = register_module("qkv", torch::nn::Linear(torch::nn::LinearOptions(channels, (heads_ + 2 * kv_heads_) * dim_).bias(bias)));
   projection_ = register_module("projection", torch::nn::Linear(torch::nn::LinearOptions(channels, channels).bias(bias)));
+  if (qk_norm) {
+    q_norm_ = register_parameter("q_norm", at::ones({dim_}));
+    k_norm_ = register_parameter("k_norm", at::ones({dim_}));
+  }
 }
 
 SparseTensor RiemannSelfAttentionImpl::forward(const SparseTensor& input) {
   TORCH_CHECK(input.F().size(1) == channels_, "Input channel count does not match attention");
   auto offsets = input.coordinate_manager()->sample_offsets(input.coordinate_map_key());
-  auto parts = qkv_->forward(input.F()).view({-1, heads_ + 2 * kv_heads_, dim_}).split_with_sizes({heads_, kv_heads_, kv_heads_}, 1);
-  auto out = packed_attention(parts[0], parts[1], parts[2], offsets, {}, {}, causal_);
+  auto heads = qkv_->forward(input.F()).view({-1, heads_ + 2 * kv_heads_, dim_});
+  at::Tensor positions, frequencies, q, k, v;
+  std::vector<int64_t> sections;
+  if (rotary_base_.has_value()) {
+    auto coordinates = input.C();
+    const int64_t axes = coordinates.size(1) - 1;
+    positions = coordinates.narrow(1, 1, axes);
+    sections = rotary_sections(dim_, axes);
+    std::lock_guard<std::mutex> lock(frequencies_mutex_);
+    if (static_cast<int64_t>(frequencies_.size()) <= axes) frequencies_.resize(axes + 1);
+    auto& kept = frequencies_[axes];
+    if (!kept.defined() || kept.device() != positions.device())
+      kept = rotary_frequencies(sections, *rotary_base_).to(positions.device());
+    frequencies = kept;
+  }
+  if (q_norm_.defined()) {
+    auto parts = heads.split_with_sizes({heads_, kv_heads_, kv_heads_}, 1);
+    std::tie(q, k) = qk_norm_rotary(parts[0], parts[1], q_norm_, k_norm_, positions, frequencies, sections);
+    v = parts[2];
+  } else if (rotary_base_.has_value()) {
+    auto parts = heads.split_with_sizes({heads_ + kv_heads_, kv_heads_}, 1);
+    auto turned = rotary_positions(parts[0], positions, frequencies, sections).split_with_sizes({heads_, kv_heads_}, 1);
+    q = turned[0];
+    k = turned[1];
+    v = parts[1];
+  } else {
+    auto parts = heads.split_with_sizes({heads_, kv_heads_, kv_heads_}, 1);
+    q = parts[0];
+    k = parts[1];
+    v = parts[2];
+  }
+  auto out = packed_attention(q, k, v, offsets, {}, {}, causal_, c10::nullopt, window_, sinks_);
   return SparseTensor(projection_->forward(out.reshape({-1, channels_})), input.coordinate_map_key(), input.coordinate_manager());
 }
 

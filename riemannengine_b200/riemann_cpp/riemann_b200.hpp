@@ -16,6 +16,7 @@
 // is no CPU backend.
 #pragma once
 
+#include <mutex>
 #include <torch/torch.h>
 
 #include <map>
@@ -499,10 +500,15 @@ std::pair<at::Tensor, at::Tensor> qk_norm_rotary(const at::Tensor& q, const at::
                                                  double eps = 1e-6, bool interleaved = false);
 
 // Self-attention of the rows of a SparseTensor within their sample: `qkv` projects the features to queries, keys and values,
-// packed_attention runs on CoordinateManager::sample_offsets, `projection` mixes the heads. num_kv_heads 0: as many as heads.
+// packed_attention runs on CoordinateManager::sample_offsets, `projection` mixes the heads. num_kv_heads 0: as many as heads. rotary_base:
+// queries and keys are turned by their rows' coordinates (rotary_positions, the pairs dealt out evenly to the axes); qk_norm: behind a norm
+// of every head with weights of its own, q_norm and k_norm (qk_norm_rotary). window and sinks: of packed_attention, over the rows in
+// their order.
 class RiemannSelfAttentionImpl : public torch::nn::Module {
 public:
-  RiemannSelfAttentionImpl(int64_t channels, int64_t num_heads, int64_t num_kv_heads = 0, bool causal = false, bool bias = true);
+  RiemannSelfAttentionImpl(int64_t channels, int64_t num_heads, int64_t num_kv_heads = 0, bool causal = false, bool bias = true,
+                           c10::optional<double> rotary_base = c10::nullopt, bool qk_norm = false,
+                           c10::optional<int64_t> window = c10::nullopt, int64_t sinks = 0);
   SparseTensor forward(const SparseTensor& input);
   torch::nn::Linear qkv() { return qkv_; }
   torch::nn::Linear projection() { return projection_; }
@@ -510,7 +516,13 @@ public:
 private:
   int64_t channels_, heads_, kv_heads_, dim_;
   bool causal_;
+  c10::optional<double> rotary_base_;
+  c10::optional<int64_t> window_;
+  int64_t sinks_;
   torch::nn::Linear qkv_{nullptr}, projection_{nullptr};
+  at::Tensor q_norm_, k_norm_;   // undefined without norms
+  std::mutex frequencies_mutex_;
+  std::vector<at::Tensor> frequencies_;  // one for each number of axes and device; float64 whatever the layer's type
 };
 TORCH_MODULE(RiemannSelfAttention);
 
