@@ -10,9 +10,9 @@
 // where a turn is full. No bits are lost however far the position is, and no range has to be reduced. What is left of a turn is cut into
 // quarters; sine and cosine of up to an eighth either way are their Taylor polynomials (off by less than 2e-9).
 //
-// Bound by memory: every value is read once and written once. A block works on queries or on keys. A head's channels lie over L lanes (a
-// power of two), each with units of V pairs, 16 bytes a load where sizes and alignment allow; the L lanes are a group. A warp has one or
-// several rows, each with one or several groups that take the row's heads in turn, U at a time. A thread copies what it is going to
+// Bound by memory: every value is read once and written once. A block works on queries or on keys. A head's channels lie over L lanes (with
+// a norm a power of two), each with units of V pairs, 16 bytes a load where sizes and alignment allow; the L lanes are a group. A warp has one
+// or several rows, each with one or several groups that take the row's heads in turn, U at a time. A thread copies what it is going to
 // read into places of its own in shared memory, kStages batches ahead and across rows, so that the copies in flight take no registers and
 // need no barriers; the positions of the rows come the same way. The warp makes the angles of its rows once, every lane a share of them,
 // and hands them on through shared memory. The norm's sums go over the L lanes. dw is summed in registers over the rows that a thread
@@ -42,7 +42,7 @@ struct Heads {  // [rows, heads, dim]
   const void* weight;  // NULL: ones
   void* out;           // no gaps; backward: the gradient of x
   int heads;
-  // layout: groups of a row within a warp (a power of two), warps of a row, blocks
+  // layout: groups of a row within a warp, warps of a row, blocks
   int groups, warps;
   uint32_t blocks;
 };
@@ -50,7 +50,7 @@ struct RotaryArgs {
   Heads part[2];  // queries, keys (0 heads: none)
   uint32_t rows;
   int dim, pairs, lanes, axes;  // lanes of a head
-  int pair_bits;          // of the pairs that these lanes could hold (a power of two)
+  int pair_bits;          // of the angles that a row has room for: pairs that turn, of whole units, and up to a power of two
   const int32_t* positions;
   int64_t position_row, position_axis;
   const double* frequencies;
@@ -195,14 +195,15 @@ struct Lane {
   int turned[NU];              // pairs of the unit that turn
   bool has[NU];
   __device__ __forceinline__ Lane(const RotaryArgs& a, const Heads& p) {
-    const int lane = threadIdx.x & 31;
-    at = lane & (a.lanes - 1);
-    group = lane / a.lanes & (p.groups - 1);
-    row_of_warp = lane / (a.lanes * p.groups);
+    const int lane = threadIdx.x & 31, of_row = a.lanes * p.groups;
+    const bool idle = lane >= 32 / of_row * of_row;
+    at = idle ? 0 : lane % a.lanes;
+    group = idle ? 0 : lane / a.lanes % p.groups;
+    row_of_warp = idle ? 0 : lane / of_row;
 #pragma unroll
     for (int i = 0; i < NU; ++i) {
       const int u = at + i * a.lanes, first = u * V;
-      has[i] = first < a.dim / 2;
+      has[i] = first < a.dim / 2 && !idle;
       turned[i] = min(max(a.pairs - first, 0), V);
       if (!has[i]) {  // (reads what the first lane reads, and stores nothing)
         lo[i] = hi[i] = 0;
@@ -232,7 +233,8 @@ constexpr int kStages = 4;
 // among theirs, for every such position where it is, from the first row's on, and which row it is of; and the ring of copies.
 template <int V, int NU>
 struct alignas(16) Tables {
-  static constexpr int PAIRS = 32 * NU * V;  // of a warp's rows at most
+  // of a warp's rows at most (units of eight pairs come with a norm alone, whose lanes are a power of two)
+  static constexpr int PAIRS = (V == 8 ? 32 : 64) * NU * V;
   float w[2][kMostDim / 2];
   float turns[kWarps][2][PAIRS];
   uint64_t fraction[kMostDim / 2];
@@ -257,8 +259,8 @@ struct alignas(16) Tables {
   __device__ __forceinline__ void begin(const RotaryArgs& a, const Heads& part, bool next, bool norm, int64_t* offset, int* row_of) {
     const void* weight = part.weight;
     const int rows = 32 / (a.lanes * part.groups);
-    for (int p = threadIdx.x; p < 1 << a.pair_bits; p += kThreads) {
-      if (norm) {
+    if (norm) {
+      for (int p = threadIdx.x; p < a.lanes * NU * V; p += kThreads) {
         const int lo = next ? 2 * p : p < a.pairs ? p : p + a.pairs, hi = next ? 2 * p + 1 : p < a.pairs ? p + a.pairs : p + a.dim / 2;
         const bool here = weight && p < a.dim / 2;
         auto of = [&](int c) {
@@ -267,6 +269,8 @@ struct alignas(16) Tables {
         w[0][p] = of(lo);
         w[1][p] = of(hi);
       }
+    }
+    for (int p = threadIdx.x; p < 1 << a.pair_bits; p += kThreads) {
       int ax = 0;
       for (int k = 0; k < kMostAxes - 1; ++k) ax += p >= a.ends[k] && p < a.pairs ? 1 : 0;
       fraction[p] = p < a.pairs ? fraction_of_turn(__ldg(a.frequencies + p)) : 0;
@@ -278,25 +282,45 @@ struct alignas(16) Tables {
     }
     __syncthreads();
   }
+  // Up to 32 pairs a row: a lane makes angles of the same pair, of every few rows.
+  struct Same {
+    uint64_t fraction;
+    int place, step;
+  };
+  __device__ __forceinline__ Same same(const RotaryArgs& a) const {
+    const int lane = threadIdx.x & 31;
+    return {fraction[lane & ((1 << a.pair_bits) - 1)], place[lane], (32 >> a.pair_bits) * a.axes};
+  }
   // the angles of the warp's rows from `positions`, then each lane those of its units
-  __device__ __forceinline__ void angles(const RotaryArgs& a, const Heads& p, const int32_t* positions, int at, int row_of_warp,
+  template <class Lane>
+  __device__ __forceinline__ void angles(const RotaryArgs& a, const Heads& p, const Same& same, const int32_t* positions, const Lane& lane,
                                          Turn<V> (&turn)[NU]) {
-    const int of_row = 1 << a.pair_bits, n = (32 * NU * V) / p.groups;  // (both powers of two)
+    const int of_row = 1 << a.pair_bits, n = 32 / (a.lanes * p.groups) << a.pair_bits;
     float* cosines = turns[threadIdx.x >> 5][0];
     float* sines = turns[threadIdx.x >> 5][1];
     __syncwarp();  // the angles before have been read, and all lanes' copies are here
     const float sign = a.back ? -1.f : 1.f;
-#pragma unroll 4
-    for (int i = threadIdx.x & 31; i < n; i += 32) {
+    auto make = [&](int i, int32_t position, uint64_t f) {
       float c, s;
-      turn_of(positions[place[i]], fraction[i & (of_row - 1)], c, s);
+      turn_of(position, f, c, s);
       cosines[i] = c;
       sines[i] = s * sign;
+    };
+    if (V < 8 && of_row <= 32) {  // (units of eight have no registers left for it)
+      const int32_t* from = positions + same.place;
+#pragma unroll 4
+      for (int i = threadIdx.x & 31; i < n; i += 32) {
+        make(i, *from, same.fraction);
+        from += same.step;
+      }
+    } else {
+#pragma unroll 4
+      for (int i = threadIdx.x & 31; i < n; i += 32) make(i, positions[place[i]], fraction[i & (of_row - 1)]);
     }
     __syncwarp();
 #pragma unroll
     for (int i = 0; i < NU; ++i) {
-      const int first = row_of_warp * of_row + (at + i * a.lanes) * V;
+      const int first = lane.row_of_warp * of_row + (lane.turned[i] > 0 ? (lane.at + i * a.lanes) * V : 0);
       read(cosines + first, turn[i].c);
       read(sines + first, turn[i].s);
 #pragma unroll
@@ -417,6 +441,7 @@ __global__ void __launch_bounds__(kThreads, kNorm ? 2 : 3) k_rotary(const __grid
   const float inv_dim = 1.f / (float)a.dim;
   tables.begin(a, p, kNext, kNorm, ring.offset, ring.row_of);
   Walk now(a, p, blockIdx.x - (keys ? a.part[0].blocks : 0), lane.group), ahead = now;
+  const auto same = tables.same(a);
   const int64_t in_step = p.head * now.next, out_step = (int64_t)a.dim * now.next;
   const Part part = 2 * a.pairs == a.dim ? Part::kAll : a.pairs % V == 0 ? Part::kUnits : Part::kPairs;
   Number<V> w[2][NU][N];
@@ -468,7 +493,7 @@ __global__ void __launch_bounds__(kThreads, kNorm ? 2 : 3) k_rotary(const __grid
   while (now.base < a.rows) {  // (whole warps)
     ask((stage + kStages - 1) % kStages);
     copies_here<kStages - 1>();
-    if (now.done == 0 && a.pairs) tables.angles(a, p, ring.positions_of(stage), lane.at, lane.row_of_warp, turn);
+    if (now.done == 0 && a.pairs) tables.angles(a, p, same, ring.positions_of(stage), lane, turn);
     const int left = (now.base + lane.row_of_warp < a.rows ? now.mine : 0) - now.done;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -525,6 +550,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_rotary_backward(const __grid_co
   const float inv_dim = 1.f / (float)a.dim;
   tables.begin(a, p, kNext, true, ring.offset, ring.row_of);
   Walk now(a, p, blockIdx.x - (keys ? a.part[0].blocks : 0), lane.group), ahead = now;
+  const auto same = tables.same(a);
   const int64_t x_step = p.head * now.next, g_step = p.grad_head * now.next, out_step = (int64_t)a.dim * now.next;
   const Part part = 2 * a.pairs == a.dim ? Part::kAll : a.pairs % V == 0 ? Part::kUnits : Part::kPairs;
   Number<V> w[2][NU][N];
@@ -587,7 +613,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_rotary_backward(const __grid_co
   while (now.base < a.rows) {  // (whole warps)
     ask((stage + kStages - 1) % kStages);
     copies_here<kStages - 1>();
-    if (now.done == 0 && a.pairs) tables.angles(a, p, ring.positions_of(stage), lane.at, lane.row_of_warp, turn);
+    if (now.done == 0 && a.pairs) tables.angles(a, p, same, ring.positions_of(stage), lane, turn);
     const int left = (now.base + lane.row_of_warp < a.rows ? now.mine : 0) - now.done;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -761,18 +787,29 @@ int pairs_a_load(const RotaryArgs& a, int elem, bool next, bool norm) {
   return v;
 }
 
-// Lanes of a head; groups of a row in a warp: as many as leave each two heads (whose loads run together), and as fit; further warps of a
-// row where there are few rows, until there are eight for every SM.
-void lay_out(RotaryArgs* a, int V, int units_a_lane, uint32_t most_blocks) {
-  const int units = a->dim / 2 / V;
-  a->lanes = 1;
-  while (a->lanes * units_a_lane < units) a->lanes *= 2;
+// Lanes of a head, a power of two with a norm (whose sums they join); groups of a row in a warp: those with which the fewest lanes idle, as
+// many as leave each two heads (which are copied together) among equal ones; further warps of a row where there are few rows, until
+// there are eight for every SM. (65536 rows, 16 heads of 80 in bf16, without a norm: 70 us with 10 lanes and 3 rows a warp, 85 with 16.)
+void lay_out(RotaryArgs* a, int V, int units_a_lane, bool norm, bool backward) {
+  const int units = a->dim / 2 / V, at_once = heads_at_once(backward);
+  const uint32_t most_blocks = norm ? kMostBlocks : kMostPlainBlocks;
+  a->lanes = (units + units_a_lane - 1) / units_a_lane;
+  while (norm && (a->lanes & (a->lanes - 1))) ++a->lanes;
+  const int turned = (a->pairs + V - 1) / V * V;
   a->pair_bits = 0;
-  while (1 << a->pair_bits < a->lanes * units_a_lane * V) ++a->pair_bits;
+  while (1 << a->pair_bits < turned) ++a->pair_bits;
   const uint64_t heads = (uint64_t)a->part[0].heads + a->part[1].heads;
   for (Heads& p : a->part) {
     p.groups = p.warps = 1;
-    while (a->lanes * p.groups < 32 && p.groups * 4 <= p.heads) p.groups *= 2;
+    double best = 0;
+    for (int g = 1; g == 1 || (g * a->lanes <= 32 && g * 2 <= p.heads); g = norm ? g * 2 : g + 1) {
+      const int in_turn = ((p.heads + g - 1) / g + at_once - 1) / at_once * at_once;
+      const double busy = (double)(32 / (a->lanes * g) * a->lanes) * p.heads / in_turn;
+      if (busy >= best) {
+        best = busy;
+        p.groups = g;
+      }
+    }
     const uint64_t rows = 32 / (a->lanes * p.groups);  // of a warp
     auto warps = [&] { return ((uint64_t)a->rows + rows - 1) / rows * p.warps; };
     while (p.warps < kWarps && p.groups * p.warps < p.heads && warps() < 148 * 8) p.warps *= 2;
@@ -798,7 +835,7 @@ int launch_as(const RotaryArgs& a, cudaStream_t stream) {
 }
 template <typename T, int V, int NU>
 int launch(RotaryArgs& a, bool next, bool norm, bool backward, cudaStream_t stream) {
-  lay_out(&a, V, NU, norm ? kMostBlocks : kMostPlainBlocks);
+  lay_out(&a, V, NU, norm, backward && norm);
   if (backward) return next ? launch_as<T, V, NU, true, 2>(a, stream) : launch_as<T, V, NU, false, 2>(a, stream);
   if (norm) return next ? launch_as<T, V, NU, true, 1>(a, stream) : launch_as<T, V, NU, false, 1>(a, stream);
   if constexpr (V <= 4) return next ? launch_as<T, V, NU, true, 0>(a, stream) : launch_as<T, V, NU, false, 0>(a, stream);
