@@ -314,10 +314,27 @@ __device__ __forceinline__ bool search_tile(const AttnArgs& a, uint32_t want, in
 // without a tile cost a block each, and the search leaves them among the others. 8 heads of 64, backward, with counts and with the
 // search: 128 samples of 96 rows 81 and 94 us; 256, 512, 1024, 4096 samples of 64 rows 115 and 122, 240 and 238, 523 and 476,
 // 3650 and 1885.
-template <int kThreads, TilesOf kOf>
+// kWarps: up to 30 samples are counted by every warp for itself, which spares a block with few steps two barriers (windowed attention
+// backward, 8 samples of 511 ... 6007 rows, 8 heads of 32: 58 + 73 us, 61 + 73 without; no gain for blocks with many steps).
+template <int kThreads, TilesOf kOf, bool kWarps = false>
 __device__ __forceinline__ bool find_tile(const AttnArgs& a, uint32_t want, int tile_rows, FoundTile* found, int32_t* warp_sums) {
   const uint32_t n = a.sequences + 2;
-  if (a.sequences <= kCountedSamples) {
+  if (kWarps && n <= 32) {
+    const uint32_t lane = threadIdx.x & 31;
+    Segment g = {};
+    if (lane < n) g = segment(a, lane);
+    const int32_t tiles = lane < n ? segment_tiles<kOf>(g, tile_rows) : 0;
+    int32_t upto = tiles;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int32_t v = __shfl_up_sync(0xffffffffu, upto, o);
+      if ((int)lane >= o) upto = add_tiles(upto, v);
+    }
+    const int32_t before = __shfl_up_sync(0xffffffffu, upto, 1);
+    const uint32_t behind = __ballot_sync(0xffffffffu, (uint32_t)upto > want);  // (the sums do not descend)
+    if (behind == 0u) return false;
+    if ((int)threadIdx.x == __ffs((int)behind) - 1) *found = {g, (int32_t)want - (lane ? before : 0), tiles};
+  } else if (a.sequences <= kCountedSamples) {
     const uint32_t per = (n + kThreads - 1) / kThreads;
     const uint32_t lo = min(threadIdx.x * per, n), hi = min(lo + per, n);
     int32_t mine = 0, first, all;

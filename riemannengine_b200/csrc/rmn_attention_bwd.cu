@@ -18,6 +18,10 @@
 // of the formula, causal 892 us; the tensor pipe is active 43 and 50 % of the two kernels' time, the rest is the chain from a product
 // over the arithmetic to the next. P and dS of the second kernel take the places of S and dP, which are made anew once they have been
 // used.
+// With a window eight warps do the arithmetic at all sizes, up to 64 channels each thread with 32 columns: a tile has few steps, cut by
+// the window's edges, and a warp leaves out what no row of its sees. 8 samples of 511 ... 6007 rows, 8 heads of 32, window 65 both ways,
+// four steps a tile: 53 + 73 us, with four warps 63 + 84 (a tile of dQ takes 15500 clocks, 2400 of them to find it, 3000 to 5800 until its
+// first products and statistics are there, 1600 a step; of dK and dV 20800, 3200 a step: from a product over its arithmetic to the next).
 // One warp makes the bulk copies (and fetches the queries' statistics), one issues the products.
 // Where the key tiles alone would leave the GPU waiting for the longest sample's first ones, the query heads that share a key head
 // are dealt out to the blocks of a cluster, whose sums of dK and dV are added up through shared memory in the order of the blocks.
@@ -33,12 +37,14 @@ namespace {
 
 constexpr uint32_t kTailBytes = 2560;  // of BwdTail
 
-template <int DP>
+template <int DP, bool kWindow>
 struct BwdShape {
   static constexpr int ATOMS = DP / 64;
   static constexpr int STEP = DP == 64 ? 64 : 128;               // rows of a step
-  static constexpr int WORK = STEP / 16, HALVES = WORK / 4;      // warps of the arithmetic; groups of four with 64 columns each
+  static constexpr int WORK = kWindow ? 8 : STEP / 16;           // warps of the arithmetic
+  static constexpr int HALVES = WORK / 4, COLS = STEP / HALVES;  // groups of four; columns of each
   static constexpr int THREADS = (WORK + 2) * 32;
+  static constexpr bool SKIP = kWindow && DP == 64;              // warps skip columns that no row of theirs sees
   static constexpr int BLOCKS = DP == 64 ? 2 : 1;                // an SM
   static constexpr uint32_t COLUMNS = DP == 64 ? 256 : 512;      // tensor memory
   static constexpr uint32_t HELD = ATOMS * kAtomBytes;           // a resident tile
@@ -60,9 +66,15 @@ struct BwdTail {
 };
 static_assert(sizeof(BwdTail) <= kTailBytes, "tail");
 
-__device__ __forceinline__ void tc_ld64(uint32_t taddr, uint32_t (&r)[64]) {
+template <int N>  // 32 or 64 columns
+__device__ __forceinline__ void tc_ld_columns(uint32_t taddr, uint32_t (&r)[N]) {
   tc_ld32_at<0>(taddr, r);
-  tc_ld32_at<32>(taddr + 32, r);
+  if constexpr (N == 64) tc_ld32_at<32>(taddr + 32, r);
+}
+template <int N>  // 16 or 32 columns
+__device__ __forceinline__ void tc_st_columns(uint32_t taddr, const uint32_t (&w)[N]) {
+  if constexpr (N == 32) tc_st32<0>(taddr, w);
+  else tc_st16(taddr, w);
 }
 
 // 32 columns of tensor memory times `by` as bf16 to row[c ... c + 31], those below dim; zeros where there are no steps
@@ -84,7 +96,7 @@ __device__ __forceinline__ void store32(uint32_t taddr, float by, __nv_bfloat16*
 }
 
 // the barriers, the same in both kernels
-template <int DP>
+template <int DP, bool kWindow>
 __device__ __forceinline__ void init_barriers(BwdTail* tail) {
   if (threadIdx.x == 0) {
     for (int s = 0; s < 8; ++s) {
@@ -94,10 +106,10 @@ __device__ __forceinline__ void init_barriers(BwdTail* tail) {
     uint64_t* ones[] = {&tail->held, &tail->s_full, &tail->dp_full, &tail->dv_done, &tail->dk_done};
     for (uint64_t* b : ones) mbar_init(b, 1);
     uint64_t* all[] = {&tail->s_free, &tail->p_full, &tail->ds_full};
-    for (uint64_t* b : all) mbar_init(b, BwdShape<DP>::WORK * 32);
+    for (uint64_t* b : all) mbar_init(b, BwdShape<DP, kWindow>::WORK * 32);
     for (int i = 0; i < kStats; ++i) {
       mbar_init(&tail->st_full[i], 32);
-      mbar_init(&tail->st_empty[i], BwdShape<DP>::WORK * 32);
+      mbar_init(&tail->st_empty[i], BwdShape<DP, kWindow>::WORK * 32);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_proxy_async();
@@ -106,16 +118,16 @@ __device__ __forceinline__ void init_barriers(BwdTail* tail) {
 
 // map_q and map_g (the output's gradient) in boxes of 128 rows, map_k and map_v of a step's
 template <int DP, bool kWindow>
-__global__ void __launch_bounds__(BwdShape<DP>::THREADS, BwdShape<DP>::BLOCKS)
+__global__ void __launch_bounds__(BwdShape<DP, kWindow>::THREADS, BwdShape<DP, kWindow>::BLOCKS)
     k_attention_dq(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_g,
                    const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const AttnArgs a) {
-  using C = BwdShape<DP>;
-  constexpr int SLOTS = C::SLOTS, STEP = C::STEP;
+  using C = BwdShape<DP, kWindow>;
+  constexpr int SLOTS = C::SLOTS, STEP = C::STEP, COLS = C::COLS;
   constexpr uint32_t T_S = 0, T_DP = STEP, T_DS = 2 * STEP, T_DQ = DP == 64 ? 192 : 320;
   extern __shared__ __align__(1024) uint8_t smem[];
   BwdTail* tail = reinterpret_cast<BwdTail*>(smem + C::TAIL);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  init_barriers<DP>(tail);
+  init_barriers<DP, kWindow>(tail);
   if (tid == C::WORK * 32) {
     tma_prefetch_map(&map_q);
     tma_prefetch_map(&map_k);
@@ -137,7 +149,7 @@ __global__ void __launch_bounds__(BwdShape<DP>::THREADS, BwdShape<DP>::BLOCKS)
   bool timed_out = false;
 
   const int head = blockIdx.x % a.heads;
-  const bool exists = find_tile<C::THREADS, TilesOf::kQueries>(a, blockIdx.x / a.heads, 128, &tail->found, tail->warp_sums);
+  const bool exists = find_tile<C::THREADS, TilesOf::kQueries, kWindow>(a, blockIdx.x / a.heads, 128, &tail->found, tail->warp_sums);
   const Segment g = tail->found.g;
   const int first = (tail->found.tiles - 1 - tail->found.tile) * 128;  // the tiles that see the most keys first
   const int rows = min(128, g.n_q - first);
@@ -216,76 +228,114 @@ __global__ void __launch_bounds__(BwdShape<DP>::THREADS, BwdShape<DP>::BLOCKS)
     const uint32_t lanes = ((uint32_t)(warp & 3) * 32u) << 16;
     const int r = (warp & 3) * 32 + lane, row = first + r;
     const bool mine = row < g.n_q;
-    const RowKeys seen = mine ? row_keys<kWindow>(a, g, row) : RowKeys{0, 0, 0};
     float lse = 0.f, delta = 0.f;
     const size_t at = ((size_t)(g.q0 + row) * a.heads + head) * a.dim;
-    if (mine) {
-      // (two halves of the warps take every second eight channels)
-      const __nv_bfloat16* grad = static_cast<const __nv_bfloat16*>(a.grad) + (int64_t)(g.q0 + row) * a.grad_row +
-                                  (int64_t)head * a.grad_head;
-      const __nv_bfloat16* out = static_cast<const __nv_bfloat16*>(a.fwd_out) + at;
-      const __nv_bfloat16* low = static_cast<const __nv_bfloat16*>(a.low);
-#pragma unroll 4
-      for (int c = half * 8; c < a.dim; c += 8 * C::HALVES) {
-        const uint4 x = __ldg(reinterpret_cast<const uint4*>(grad + c)), y = __ldg(reinterpret_cast<const uint4*>(out + c));
-        const uint4 z = low ? __ldg(reinterpret_cast<const uint4*>(low + at + c)) : make_uint4(0, 0, 0, 0);
-        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w}, zs[4] = {z.x, z.y, z.z, z.w};
+    const __nv_bfloat16* low = static_cast<const __nv_bfloat16*>(a.low);
+    auto add_eight = [](float sum, const uint4& x, const uint4& y, const uint4& z) {  // of dO, O and what rounding took from it
+      const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w}, zs[4] = {z.x, z.y, z.z, z.w};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          delta = fmaf(__uint_as_float(xs[e] << 16), __uint_as_float(ys[e] << 16) + __uint_as_float(zs[e] << 16), delta);
-          delta = fmaf(__uint_as_float(xs[e] & 0xffff0000u),
-                       __uint_as_float(ys[e] & 0xffff0000u) + __uint_as_float(zs[e] & 0xffff0000u), delta);
+      for (int e = 0; e < 4; ++e) {
+        sum = fmaf(__uint_as_float(xs[e] << 16), __uint_as_float(ys[e] << 16) + __uint_as_float(zs[e] << 16), sum);
+        sum = fmaf(__uint_as_float(xs[e] & 0xffff0000u), __uint_as_float(ys[e] & 0xffff0000u) + __uint_as_float(zs[e] & 0xffff0000u), sum);
+      }
+      return sum;
+    };
+    if (mine) lse = __ldg(a.lse + (size_t)head * a.rows_q + g.q0 + row) * kLog2e;
+    if constexpr (kWindow) {
+      // A row over 4, 8 or 16 lanes, two rows of a thread at a time: with few steps the time to fetch these rows counts (a row a thread took
+      // 9600 of the block's 32000 clocks with 64 channels and a window of 512, so 5900; the first products are there after 3000).
+      const int lanes_of_row = DP == 128 ? 16 : a.dim > 32 ? 8 : 4, rows_at_once = C::WORK * 32 / lanes_of_row;  // (at most 64)
+      const int c = tid % lanes_of_row * 8, here = c < a.dim ? c : 0;
+      for (int r0 = tid / lanes_of_row; r0 < 128; r0 += 2 * rows_at_once) {
+        uint4 x[2], y[2], z[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int64_t q = g.q0 + min(first + r0 + k * rows_at_once, g.n_q - 1);
+          const int64_t from = (q * a.heads + head) * a.dim + here;
+          x[k] = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.grad) + q * a.grad_row + (int64_t)head * a.grad_head + here));
+          y[k] = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.fwd_out) + from));
+          z[k] = low ? __ldg(reinterpret_cast<const uint4*>(low + from)) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          float sum = c < a.dim ? add_eight(0.f, x[k], y[k], z[k]) : 0.f;
+          for (int o = lanes_of_row / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+          if (c == 0) tail->delta[0][r0 + k * rows_at_once] = sum;
         }
       }
-      lse = __ldg(a.lse + (size_t)head * a.rows_q + g.q0 + row) * kLog2e;
-    }
-    if constexpr (C::HALVES == 2) {
-      tail->delta[half][r] = delta;
       asm volatile("bar.sync 1, %0;" ::"n"(C::WORK * 32) : "memory");
-      delta = tail->delta[0][r] + tail->delta[1][r];
+      delta = mine ? tail->delta[0][r] : 0.f;
+    } else {
+      if (mine) {
+        // (two halves of the warps take every second eight channels)
+        const __nv_bfloat16* grad = static_cast<const __nv_bfloat16*>(a.grad) + (int64_t)(g.q0 + row) * a.grad_row +
+                                    (int64_t)head * a.grad_head;
+        const __nv_bfloat16* out = static_cast<const __nv_bfloat16*>(a.fwd_out) + at;
+#pragma unroll 4
+        for (int c = half * 8; c < a.dim; c += 8 * C::HALVES)
+          delta = add_eight(delta, __ldg(reinterpret_cast<const uint4*>(grad + c)), __ldg(reinterpret_cast<const uint4*>(out + c)),
+                            low ? __ldg(reinterpret_cast<const uint4*>(low + at + c)) : make_uint4(0, 0, 0, 0));
+      }
+      if constexpr (C::HALVES == 2) {
+        tail->delta[half][r] = delta;
+        asm volatile("bar.sync 1, %0;" ::"n"(C::WORK * 32) : "memory");
+        delta = tail->delta[0][r] + tail->delta[1][r];
+      }
     }
+    const RowKeys seen = mine ? row_keys<kWindow>(a, g, row) : RowKeys{0, 0, 0};
     if (mine && half == 0) a.delta[(size_t)head * a.rows_q + g.q0 + row] = delta;
     const Pair scale = make_pair(a.scale * kLog2e, a.scale * kLog2e), minus_lse = make_pair(-lse, -lse),
                minus_delta = make_pair(-delta, -delta);
     for (int j = 0; j < steps; ++j) {
       const uint32_t ph = (uint32_t)j & 1u;
-      uint32_t s[64], dp[64];
+      uint32_t s[COLS], dp[COLS];
       if (!wait(&tail->s_full, ph)) break;
       tc_fence_after();
-      tc_ld64(tmem + lanes + T_S + half * 64, s);
+      tc_ld_columns(tmem + lanes + T_S + half * COLS, s);
       if (!wait(&tail->dp_full, ph)) break;
       tc_fence_after();
-      tc_ld64(tmem + lanes + T_DP + half * 64, dp);
+      tc_ld_columns(tmem + lanes + T_DP + half * COLS, dp);
       tc_wait_ld();
       tc_fence_before();
       mbar_arrive(&tail->s_free);
-      uint32_t w[32];
-      const int k0 = walk.key(j) + half * 64, left = seen.end - k0;  // columns that this row sees (with a window: from seen.low on)
-#pragma unroll
-      for (int c = 0; c < 64; c += 2) {
-        float x, y;
-        parts(fma(pair_of(s[c], s[c + 1]), scale, minus_lse), x, y);
-        const Pair p = make_pair(exp2_approx(x), exp2_approx(y));
-        parts(mul(p, add(pair_of(dp[c], dp[c + 1]), minus_delta)), x, y);
-        w[c / 2] = pack_bf16(x, y);
-      }
+      uint32_t w[COLS / 2];
+      const int k0 = walk.key(j) + half * COLS, left = seen.end - k0;  // columns that this row sees (with a window: from seen.low on)
+      uint32_t bits[COLS / 32];
+      bool some = true;
       if constexpr (kWindow) {
-        if (left < 64 || seen.low > k0) {
+        uint32_t any = 0;
 #pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const uint32_t bits = seen_bits(seen, k0, k);
+        for (int k = 0; k < COLS / 32; ++k) any |= bits[k] = seen_bits(seen, k0, k);
+        some = !C::SKIP || __any_sync(0xffffffffu, any != 0u);
+      }
+      if (some) {
+#pragma unroll
+        for (int c = 0; c < COLS; c += 2) {
+          float x, y;
+          parts(fma(pair_of(s[c], s[c + 1]), scale, minus_lse), x, y);
+          const Pair p = make_pair(exp2_approx(x), exp2_approx(y));
+          parts(mul(p, add(pair_of(dp[c], dp[c + 1]), minus_delta)), x, y);
+          w[c / 2] = pack_bf16(x, y);
+        }
+        if constexpr (kWindow) {
+#pragma unroll
+          for (int k = 0; k < COLS / 32; ++k) {
+            if (__all_sync(0xffffffffu, bits[k] == 0xffffffffu)) continue;
 #pragma unroll
             for (int c = 0; c < 16; ++c)
-              w[k * 16 + c] &= (bits >> (2 * c) & 1u ? 0xffffu : 0u) | (bits >> (2 * c + 1) & 1u ? 0xffff0000u : 0u);
+              w[k * 16 + c] &= (bits[k] >> (2 * c) & 1u ? 0xffffu : 0u) | (bits[k] >> (2 * c + 1) & 1u ? 0xffff0000u : 0u);
           }
-        }
-      } else if (left < 64) {
+        } else if (left < COLS) {
 #pragma unroll
-        for (int c = 0; c < 32; ++c) w[c] = 2 * c >= left ? 0u : 2 * c + 1 >= left ? w[c] & 0xffffu : w[c];
+          for (int c = 0; c < COLS / 2; ++c) w[c] = 2 * c >= left ? 0u : 2 * c + 1 >= left ? w[c] & 0xffffu : w[c];
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < COLS / 2; ++c) w[c] = 0u;
       }
       if (j > 0 && !wait(&tail->dk_done, ph ^ 1u)) break;  // dS of the step before has been used
       tc_fence_after();
-      tc_st32<0>(tmem + lanes + T_DS + half * 32, w);
+      tc_st_columns(tmem + lanes + T_DS + half * (COLS / 2), w);
       tc_wait_st();
       tc_fence_before();
       mbar_arrive(&tail->ds_full);
@@ -312,16 +362,16 @@ __global__ void __launch_bounds__(BwdShape<DP>::THREADS, BwdShape<DP>::BLOCKS)
 
 // map_k and map_v in boxes of 128 rows, map_q and map_g of a step's
 template <int DP, bool kWindow>
-__global__ void __launch_bounds__(BwdShape<DP>::THREADS, BwdShape<DP>::BLOCKS)
+__global__ void __launch_bounds__(BwdShape<DP, kWindow>::THREADS, BwdShape<DP, kWindow>::BLOCKS)
     k_attention_dkv(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                     const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_g, const AttnArgs a) {
-  using C = BwdShape<DP>;
-  constexpr int SLOTS = C::SLOTS, STEP = C::STEP;
-  constexpr uint32_t T_S = 0, T_DP = STEP, T_DV = 2 * STEP, T_DK = T_DV + DP;  // P and dS: in the first halves of 64 columns of S, dP
+  using C = BwdShape<DP, kWindow>;
+  constexpr int SLOTS = C::SLOTS, STEP = C::STEP, COLS = C::COLS;
+  constexpr uint32_t T_S = 0, T_DP = STEP, T_DV = 2 * STEP, T_DK = T_DV + DP;  // P and dS: in the first halves of COLS columns of S, dP
   extern __shared__ __align__(1024) uint8_t smem[];
   BwdTail* tail = reinterpret_cast<BwdTail*>(smem + C::TAIL);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  init_barriers<DP>(tail);
+  init_barriers<DP, kWindow>(tail);
   if (tid == C::WORK * 32) {
     tma_prefetch_map(&map_q);
     tma_prefetch_map(&map_k);
@@ -349,14 +399,14 @@ __global__ void __launch_bounds__(BwdShape<DP>::THREADS, BwdShape<DP>::BLOCKS)
   if constexpr (kWindow) {  // first the chunks' tiles of the sinks
     const int sink_tiles = tiles_of(a.sink_most, 128), of_sinks = a.sink_chunks * sink_tiles;
     if (number < of_sinks) {
-      exists = find_tile<C::THREADS, TilesOf::kLongQueries>(a, number / sink_tiles, a.sink_chunk, &tail->found, tail->warp_sums);
+      exists = find_tile<C::THREADS, TilesOf::kLongQueries, kWindow>(a, number / sink_tiles, a.sink_chunk, &tail->found, tail->warp_sums);
       chunk = tail->found.tile;
       at_tile = number % sink_tiles;
     }
     number -= of_sinks;
   }
   if (!kWindow || number >= 0) {
-    exists = find_tile<C::THREADS, TilesOf::kSlots>(a, number, 128, &tail->found, tail->warp_sums);
+    exists = find_tile<C::THREADS, TilesOf::kSlots, kWindow>(a, number, 128, &tail->found, tail->warp_sums);
     at_tile = tail->found.tile;
     chunk = -1;
   }
@@ -466,13 +516,13 @@ __global__ void __launch_bounds__(BwdShape<DP>::THREADS, BwdShape<DP>::BLOCKS)
       const bool more = i + 1 < steps;
       if (!wait(&tail->p_full, ph)) break;
       tc_fence_after();
-      mma_columns<STEP, 64>(tmem + T_DV, tmem + T_S, slot(2u * i + 1u), idesc_o, i > 0);
+      mma_columns<STEP, COLS, COLS>(tmem + T_DV, tmem + T_S, slot(2u * i + 1u), idesc_o, i > 0);
       tc_commit_elect(&tail->dv_done);
       tc_commit_elect(&tail->empty[(2u * i + 1u) % SLOTS]);
       if (more && wait(&tail->dv_done, ph)) make_s(i + 1);  // P has been used
       if (!wait(&tail->ds_full, ph)) break;
       tc_fence_after();
-      mma_columns<STEP, 64>(tmem + T_DK, tmem + T_DP, slot(2u * i), idesc_o, i > 0);
+      mma_columns<STEP, COLS, COLS>(tmem + T_DK, tmem + T_DP, slot(2u * i), idesc_o, i > 0);
       tc_commit_elect(&tail->dk_done);
       tc_commit_elect(&tail->empty[2u * i % SLOTS]);
       if (more && wait(&tail->dk_done, ph)) make_dp(i + 1);  // dS has been used
@@ -489,60 +539,68 @@ __global__ void __launch_bounds__(BwdShape<DP>::THREADS, BwdShape<DP>::BLOCKS)
     for (int i = 0; i < steps; ++i) {
       const uint32_t ph = (uint32_t)i & 1u;
       const int b = i % kStats;
-      const int lo = seen.lo - q0 - half * 64, hi = last - q0 - half * 64;  // columns of the queries that see this key
+      const int lo = seen.lo - q0 - half * COLS, hi = last - q0 - half * COLS;  // columns of the queries that see this key
       q0 = q0 + STEP >= keys.to ? from : q0 + STEP;
-      const ulonglong2* lse = reinterpret_cast<const ulonglong2*>(&tail->lse[b][half * 64]);
-      const ulonglong2* delta = reinterpret_cast<const ulonglong2*>(&tail->delta[b][half * 64]);
-      uint32_t s[64], w[32];
+      const ulonglong2* lse = reinterpret_cast<const ulonglong2*>(&tail->lse[b][half * COLS]);
+      const ulonglong2* delta = reinterpret_cast<const ulonglong2*>(&tail->delta[b][half * COLS]);
+      uint32_t s[COLS], w[COLS / 2];
       if (!wait(&tail->st_full[b], ((uint32_t)i / kStats) & 1u) || !wait(&tail->s_full, ph)) break;
       tc_fence_after();
-      tc_ld64(tmem + lanes + T_S + half * 64, s);
-      tc_wait_ld();
+      const bool some = !C::SKIP || __any_sync(0xffffffffu, max(lo, 0) < min(hi, COLS));
+      if (some) {
+        tc_ld_columns(tmem + lanes + T_S + half * COLS, s);
+        tc_wait_ld();
 #pragma unroll
-      for (int c = 0; c < 64; c += 4) {
-        const ulonglong2 l = lse[c / 4];
+        for (int c = 0; c < COLS; c += 4) {
+          const ulonglong2 l = lse[c / 4];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float x, y;
-          parts(fma(pair_of(s[c + 2 * e], s[c + 2 * e + 1]), scale, Pair{e ? l.y : l.x}), x, y);
-          s[c + 2 * e] = __float_as_uint(exp2_approx(x));
-          s[c + 2 * e + 1] = __float_as_uint(exp2_approx(y));
+          for (int e = 0; e < 2; ++e) {
+            float x, y;
+            parts(fma(pair_of(s[c + 2 * e], s[c + 2 * e + 1]), scale, Pair{e ? l.y : l.x}), x, y);
+            s[c + 2 * e] = __float_as_uint(exp2_approx(x));
+            s[c + 2 * e + 1] = __float_as_uint(exp2_approx(y));
+          }
         }
-      }
-      if (lo > 0 || hi < 64) {
+        if (lo > 0 || hi < COLS) {
 #pragma unroll
-        for (int c = 0; c < 64; ++c)
-          if (c < lo || c >= hi) s[c] = 0u;
-      }
+          for (int c = 0; c < COLS; ++c)
+            if (c < lo || c >= hi) s[c] = 0u;
+        }
 #pragma unroll
-      for (int c = 0; c < 32; ++c) w[c] = pack_bf16(__uint_as_float(s[2 * c]), __uint_as_float(s[2 * c + 1]));
-      tc_st32<0>(tmem + lanes + T_S + half * 64, w);
+        for (int c = 0; c < COLS / 2; ++c) w[c] = pack_bf16(__uint_as_float(s[2 * c]), __uint_as_float(s[2 * c + 1]));
+      } else {
+#pragma unroll
+        for (int c = 0; c < COLS / 2; ++c) w[c] = 0u;
+      }
+      tc_st_columns(tmem + lanes + T_S + half * COLS, w);
       tc_wait_st();
       tc_fence_before();
       mbar_arrive(&tail->p_full);
-      uint32_t dp[64];
+      uint32_t dp[COLS];
       if (!wait(&tail->dp_full, ph)) break;
       tc_fence_after();
-      tc_ld64(tmem + lanes + T_DP + half * 64, dp);
-      tc_wait_ld();
+      if (some) {
+        tc_ld_columns(tmem + lanes + T_DP + half * COLS, dp);
+        tc_wait_ld();
 #pragma unroll
-      for (int c = 0; c < 64; c += 4) {
-        const ulonglong2 d = delta[c / 4];
+        for (int c = 0; c < COLS; c += 4) {
+          const ulonglong2 d = delta[c / 4];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int k = c + 2 * e;
-          float x, y;
-          parts(mul(pair_of(s[k], s[k + 1]), add(pair_of(dp[k], dp[k + 1]), Pair{e ? d.y : d.x})), x, y);
-          w[k / 2] = pack_bf16(x, y);
+          for (int e = 0; e < 2; ++e) {
+            const int k = c + 2 * e;
+            float x, y;
+            parts(mul(pair_of(s[k], s[k + 1]), add(pair_of(dp[k], dp[k + 1]), Pair{e ? d.y : d.x})), x, y);
+            w[k / 2] = pack_bf16(x, y);
+          }
+        }
+        if (lo > 0 || hi < COLS) {  // (zero times what is not finite)
+#pragma unroll
+          for (int c = 0; c < COLS / 2; ++c)
+            w[c] &= (2 * c < lo || 2 * c >= hi ? 0u : 0xffffu) | (2 * c + 1 < lo || 2 * c + 1 >= hi ? 0u : 0xffff0000u);
         }
       }
       mbar_arrive(&tail->st_empty[b]);
-      if (lo > 0 || hi < 64) {  // (zero times what is not finite)
-#pragma unroll
-        for (int c = 0; c < 32; ++c)
-          w[c] &= (2 * c < lo || 2 * c >= hi ? 0u : 0xffffu) | (2 * c + 1 < lo || 2 * c + 1 >= hi ? 0u : 0xffff0000u);
-      }
-      tc_st32<0>(tmem + lanes + T_DP + half * 64, w);
+      tc_st_columns(tmem + lanes + T_DP + half * COLS, w);
       tc_wait_st();
       tc_fence_before();
       mbar_arrive(&tail->ds_full);
@@ -600,14 +658,14 @@ __global__ void __launch_bounds__(BwdShape<DP>::THREADS, BwdShape<DP>::BLOCKS)
   if (blocks > 1) {
     static_assert(2 * DP * 128 * sizeof(float) <= C::TAIL, "parts in the place of the tiles");
     cluster_sync();
-    if (exists && tid < 128) {
+    if (exists && tid < 128 * C::HALVES) {
       // every block sums its share of the eights of channels, over the blocks in their order
-      const int row = first + tid;
+      const int at_row = tid & 127, row = first + at_row;
       const size_t at = ((size_t)(g.k0 + row) * a.kv_heads + kv) * a.dim;
-      for (int e = rank; e < 2 * DP / 8; e += blocks) {
+      for (int e = rank + (tid >> 7) * blocks; e < 2 * DP / 8; e += blocks * C::HALVES) {
         const int which = e / (DP / 8), c = e % (DP / 8) * 8;
         if (c >= a.dim) continue;
-        const uint32_t addr = smem_base + (uint32_t)(e * 2 * 128 + tid) * 16u;
+        const uint32_t addr = smem_base + (uint32_t)(e * 2 * 128 + at_row) * 16u;
         float4 x = load_of_block(addr, 0), y = load_of_block(addr + 128 * 16, 0);
         for (int r = 1; r < blocks; ++r) {
           const float4 u = load_of_block(addr, (uint32_t)r), v = load_of_block(addr + 128 * 16, (uint32_t)r);
@@ -645,7 +703,7 @@ __global__ void __launch_bounds__(BwdShape<DP>::THREADS, BwdShape<DP>::BLOCKS)
 
 template <int DP, bool kWindow>
 int launch_bwd(const AttnArgs& a, cudaStream_t stream) {
-  using C = BwdShape<DP>;
+  using C = BwdShape<DP, kWindow>;
   static SmemOptIn opt_q, opt_kv;
   // [0]: boxes of 128 rows, [1]: of a step's
   CUtensorMap q[2], k[2], v[2], g[2];

@@ -51,6 +51,14 @@ __device__ __forceinline__ void tc_st32(uint32_t taddr, const uint32_t (&r)[N]) 
       RMN_TC_REGS16(r, FIRST), RMN_TC_REGS16(r, FIRST + 16)
       : "memory");
 }
+template <int N>
+__device__ __forceinline__ void tc_st16(uint32_t taddr, const uint32_t (&r)[N]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16};" ::"r"(taddr),
+      RMN_TC_REGS16(r, 0)
+      : "memory");
+}
 #undef RMN_TC_REGS16
 
 // 32 columns into r[FIRST ... FIRST + 31]
@@ -98,14 +106,14 @@ __device__ __forceinline__ void mma_rows(uint32_t d_tmem, uint32_t a_s, uint32_t
                       DESC + desc_address(b_s + (uint32_t)(j >> 2) * (B_ROWS * 128u) + in), idesc, j != 0);
   }
 }
-// D[128, n] (+)= A[128, ROWS] B[ROWS, n]: A in tensor memory, its pieces of 32 columns (64 values) HALF apart, B a tile whose ROWS
-// rows are summed over (MN-major)
-template <int ROWS = 128, int HALF = 32>
+// D[128, n] (+)= A[128, ROWS] B[ROWS, n]: A in tensor memory, its pieces of VALUES values (half as many columns) HALF apart, B a tile whose
+// ROWS rows are summed over (MN-major)
+template <int ROWS = 128, int HALF = 32, int VALUES = 64>
 __device__ __forceinline__ void mma_columns(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_s, uint32_t idesc, bool accumulate) {
   constexpr uint64_t DESC = smem_desc_sw_const(ROWS * 128, 1024, 2u);
 #pragma unroll
   for (int j = 0; j < ROWS / 16; ++j)
-    tc_mma_bf16_ta_elect(d_tmem, a_tmem + (j >> 2) * HALF + (j & 3) * 8, DESC + desc_address(b_s + (uint32_t)j * 2048u), idesc,
+    tc_mma_bf16_ta_elect(d_tmem, a_tmem + j / (VALUES / 16) * HALF + j % (VALUES / 16) * 8, DESC + desc_address(b_s + (uint32_t)j * 2048u), idesc,
                          accumulate || j != 0);
 }
 
