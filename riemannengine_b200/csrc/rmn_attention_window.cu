@@ -3,14 +3,16 @@
 // 128 queries sees are those of the window and the sinks (KeyWalk).
 //
 // Such a tile has few steps over keys, so that what surrounds them (to find it, to fetch its rows, to store its output) takes as long. So
-// blocks stay and take one tile after the other, `gridDim.x` apart, and the steps of all of them run as one chain: the copying warp finds the next tile and fetches
-// its rows while the steps of this one are under way, and the next tile's scores are made while this one's output is stored. Every barrier is
-// waited for phase by phase across tiles: a step's number counts from the block's first one. What a tile is goes from the copying warp to
-// the others through a ring of four places. Of a step's 128 columns those are left out, 32 at a time, that no row of a warp sees.
+// blocks stay and take one tile after the other, `gridDim.x` apart, and the steps of all of them run as one chain: the copying warp finds
+// the next tile and fetches its rows while the steps of this one are under way, and the next tile's scores are made while this one's
+// output is stored. Every barrier is waited for phase by phase across tiles: a step's number counts from the block's first one. What a
+// tile is goes from the copying warp to the others through a ring of four places. Of a step's 128 columns those are left out, 32 at a
+// time, that no row of a warp sees.
 // 8 samples of 511 ... 6007 rows, 8 heads of 32, window 65 both ways (two steps a tile): 47 us with a block a tile, 38 so; 8 samples of
-// 151 ... 4001 rows, 8 heads of 64, window 512: 62 and 59. A chain of latencies all the same: the exponentials are 1024 clocks of the 4700
-// that a step takes, and two blocks an SM, all that tensor memory holds, fill the gaps in part. Steps of 64 keys and three blocks: 47 and 103
-// us. dQ, dK and dV by blocks that stay: 67 and 91 us on the first of these samples, 63 and 85 with a block a tile.
+// 151 ... 4001 rows, 8 heads of 64, window 512: 62 and 59. A chain of latencies all the same: the exponentials are 1024 clocks of the
+// 4700 that a step takes, and two blocks an SM, all that tensor memory holds, fill the gaps in part. Steps of 64 keys and three blocks:
+// 47 and 103 us. Backward kernels whose blocks stay gained nothing (67 and 91 us on the first of these samples, 63 and 85 with a block a
+// tile, before eight warps made it 53 and 73).
 #include "rmn_attention_tc.cuh"
 
 #include <math_constants.h>
