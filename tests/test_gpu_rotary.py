@@ -102,6 +102,29 @@ def test_row_counts(rows, h, hk, d, dtype):
     _check("cpp", q, None, positions, sections, False, gq=gq, norm=False)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("d,sections", [(12, [6]), (20, [3, 4]), (24, [12]), (40, [16]), (48, [8, 8, 8]), (72, [36]), (80, [8, 12, 12]),
+                                        (88, [40]), (112, [20, 20]), (136, [4]), (200, [100]), (240, [64, 3])], ids=lambda v: str(v))
+def test_lanes_and_heads(d, sections, dtype):
+    """Heads over any number of lanes, several of a row and several rows in a warp, some of its lanes idle; what turns ends inside a lane's
+    share, and lanes have nothing that turns. Channels that do not turn are not finite."""
+    t = TYPES[dtype]
+    for rows, h in ((1, 64), (130, 9), (131, 16), (67, 24), (3001, 7)):
+        q, _, _, _, gq, _, g = _data(rows, h, 1, d, t)
+        positions = _positions(rows, len(sections), g)
+        for interleaved in (False, True):
+            _check("cpp", q, None, positions, sections, interleaved, gq=gq, norm=False, what=f"{rows} {h} {interleaved}")
+        turned = 2 * sum(sections)
+        if turned < d:
+            x = q.clone()
+            x[..., turned] = float("inf")
+            x[..., turned + 1:] = float("nan")
+            y = _host("cpp").rotary_positions(x, positions, _frequencies(sections), sections)
+            assert torch.equal(y[..., turned:].nan_to_num(), x[..., turned:].nan_to_num())
+            want = R.rotary(q[..., :turned], None, positions, _frequencies(sections), sections)["q"]
+            check(y[..., :turned], want, "beside what is not finite")
+
+
 @pytest.mark.parametrize("host", ["python", "cpp"])
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_views(host, dtype):

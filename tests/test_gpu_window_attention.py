@@ -173,6 +173,17 @@ def test_many_samples(dtype):
     _check("cpp", q, k, v, grad, _offsets(lens), 70, 0, causal=False)
 
 
+@pytest.mark.parametrize("samples", [29, 30, 31, 33, 383, 385])
+def test_numbers_of_samples(samples):
+    """Up to as many as a warp counts, as a block counts, and beyond; samples of no rows, rows before the first and behind the last, and
+    one sample long enough for parts of its sinks' gradients."""
+    lens = [(7 * i) % 5 * (i % 3) for i in range(samples)]
+    lens[samples // 2] = 700
+    n = sum(lens) + 9
+    q, k, v, grad = _inputs(n, n, 4, 2, 48, torch.bfloat16)
+    _check("cpp", q, k, v, grad, _offsets(lens, 4), 33, 2, causal=True)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("causal", [False, True])
