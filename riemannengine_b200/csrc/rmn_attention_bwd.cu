@@ -722,12 +722,14 @@ int launch_bwd(const AttnArgs& a, cudaStream_t stream) {
   // With fewer than two tiles of keys for each block that fits the GPU (a sample has a tile at least): clusters of as many blocks, up to
   // eight (the portable size), as the query heads of a key head divide into. Backward of 8 samples of 151 ... 5003 rows, 8 / 2 heads of
   // 64, 238 tiles for 296 places: 560 us without, 340 with; of two samples of 3989 and 4600 rows, 16 / 8 heads of 128, 536 tiles for 148
-  // places: 548 and 604; of 4096 samples of 4 rows, 8 / 1 heads of 64: 990 and 2121.
+  // places: 548 and 604; of 4096 samples of 4 rows, 8 / 1 heads of 64: 990 and 2121. With a window the tiles are of even work: fewer tiles
+  // than blocks (forward and backward, without and with clusters: 3 samples, 8 / 4 heads of 128, window 512, 212 tiles for 148 places,
+  // 170 and 189; 4 samples of 2000, 8 / 2 heads of 48, window 129, 128 tiles for 296 places, 111 and 106).
   const int group = a.heads / a.kv_heads;
   int cluster = 1;
   const uint64_t samples = std::max<uint64_t>(1, std::min(a.sequences, a.rows_k));  // (that can have a row)
   const uint64_t tiles = samples * ((a.rows_k / samples + 127) / 128);
-  if (tiles * a.kv_heads < 2 * 148 * C::BLOCKS) {
+  if (tiles * a.kv_heads < (kWindow ? 1 : 2) * 148 * C::BLOCKS) {
     for (int n = 2; n <= 8; ++n)
       if (group % n == 0) cluster = n;
   }
