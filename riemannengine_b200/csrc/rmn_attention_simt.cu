@@ -615,6 +615,9 @@ int launch_simt(Kernel kern, SmemOptIn& opt_in, const AttnArgs& a, uint64_t tile
   return RMN_OK;
 }
 
+// With a window the query tiles are of even work, and gain nothing from pieces that do not fit at once (4 samples of 301 ... 2203 rows, 4 heads
+// of 32, window 128 both ways, dQ: 51 us with a block a tile, 59 with two; dK and dV, whose sinks' tiles are longer, 129 and 111).
+uint64_t least_of_queries(const AttnArgs& a, uint64_t least) { return a.window ? ~0u : least; }
 // The rows of the other side that a tile may see of `rows`: all, or those of the window (and the sinks).
 uint64_t rows_seen(const AttnArgs& a, uint64_t rows, int BM, uint64_t sinks) {
   return a.window ? std::min<uint64_t>(rows, (uint64_t)a.window * (a.causal ? 1 : 2) + BM + sinks) : rows;
@@ -625,7 +628,7 @@ int forward_as(const AttnArgs& a, cudaStream_t stream) {
   static SmemOptIn opt_in;
   const uint64_t samples = a.sequences ? a.sequences : 1;
   return launch_simt(k_attention_simt<T, DP, BM, kWindow>, opt_in, a, most_tiles(a.rows_q, a.sequences, BM) * a.heads,
-                     blocks_a_tile(a.rows_q, a.heads, rows_seen(a, a.rows_k / samples, BM, (uint64_t)a.sinks), BM, 4),
+                     blocks_a_tile(a.rows_q, a.heads, rows_seen(a, a.rows_k / samples, BM, (uint64_t)a.sinks), BM, least_of_queries(a, 4)),
                      2 * S::tile + S::square, stream);
 }
 template <typename T, int DP, int BM, bool kWindow>
@@ -634,7 +637,7 @@ int backward_as(const AttnArgs& a, cudaStream_t stream) {
   static SmemOptIn opt_q, opt_kv;
   const uint64_t samples = a.sequences ? a.sequences : 1, group = a.heads / a.kv_heads;
   const int st = launch_simt(k_attention_simt_dq<T, DP, BM, kWindow>, opt_q, a, most_tiles(a.rows_q, a.sequences, BM) * a.heads,
-                             blocks_a_tile(a.rows_q, a.heads, rows_seen(a, a.rows_k / samples, BM, (uint64_t)a.sinks), BM, 2),
+                             blocks_a_tile(a.rows_q, a.heads, rows_seen(a, a.rows_k / samples, BM, (uint64_t)a.sinks), BM, least_of_queries(a, 2)),
                              4 * S::tile + S::square, stream);
   if (st != RMN_OK) return st;
   const uint64_t of_sinks = (uint64_t)a.sink_chunks * ((a.sink_most + BM - 1) / BM);
