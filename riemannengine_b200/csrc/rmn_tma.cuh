@@ -47,6 +47,16 @@ inline EncodeTiledFn encode_tiled_fn() {
   }();
   return fn;
 }
+// cuTensorMapEncodeTiled; false where it fails. It wants a context, which a thread that has not called the runtime yet lacks (that of a first
+// backward pass whose memory is there already): the thread gets its device's then.
+template <class... Args>
+inline bool encode_tiled(Args... args) {
+  const EncodeTiledFn fn = encode_tiled_fn();
+  if (!fn) return false;
+  if (fn(args...) == CUDA_SUCCESS) return true;
+  int device = 0;
+  return cudaGetDevice(&device) == cudaSuccess && cudaSetDevice(device) == cudaSuccess && fn(args...) == CUDA_SUCCESS;
+}
 
 }  // namespace tc
 }  // namespace rmn
