@@ -789,7 +789,8 @@ int pairs_a_load(const RotaryArgs& a, int elem, bool next, bool norm) {
 
 // Lanes of a head, a power of two with a norm (whose sums they join); groups of a row in a warp: those with which the fewest lanes idle, as
 // many as leave each two heads (which are copied together) among equal ones; further warps of a row where there are few rows, until
-// there are eight for every SM. (65536 rows, 16 heads of 80 in bf16, without a norm: 70 us with 10 lanes and 3 rows a warp, 85 with 16.)
+// there are eight for every SM. (65536 rows, 16 heads of 80 in bf16, without a norm: 70 us with 10 lanes and 3 rows a warp, 85 with 16;
+// 1.2 M rows, 4 heads of 16: 80 us a pass with two groups a row, 106 with one, whose loads touch twice as many rows.)
 void lay_out(RotaryArgs* a, int V, int units_a_lane, bool norm, bool backward) {
   const int units = a->dim / 2 / V, at_once = heads_at_once(backward);
   const uint32_t most_blocks = norm ? kMostBlocks : kMostPlainBlocks;
